@@ -570,6 +570,118 @@ int voom_expert_swiglu(const voom_expert_pages* d_pages, const uint32_t* d_exper
                        const uint16_t* d_h, uint32_t H, uint32_t I, uint32_t gate_tiles, uint32_t down_tiles,
                        uint16_t* d_y, void* d_scratch, uint64_t scratch_bytes, uint32_t* d_status, void* stream);
 
+/* ------------------------------------------- attention around the KV cache */
+/* Element types of the attention entry points. */
+enum { VOOM_BF16 = 0u, VOOM_FP16 = 1u, VOOM_FP32 = 2u };
+
+/* Per-head RMS norm of queries and keys and the position rotation, one pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * w      (w + 1 with zero_centered; no norm
+ *                                            where the weight is NULL)
+ *   (a, b) -> factor * (a cos t - b sin t, a sin t + b cos t)
+ * for the rot / 2 pairs of the first `rot` values of a head: (i, i + rot / 2),
+ * or (2i, 2i + 1) with `interleaved`; values past `rot` are only normed.
+ * t = 2 pi * frac(position * turns_i), turns_i the pair's turns per position
+ * in units of 2^-64: the 64-bit product wraps, so the angle is as exact far
+ * into a context as at its start.  Strides are in elements; a head's D values
+ * are contiguous.  Outputs may be the inputs (not partly overlap them).  fp32
+ * arithmetic, one rounding.
+ * Covers what the reference does with mx.fast.rms_norm + mx.fast.rope around
+ * its KV caches (attention there is outside the ported path). */
+typedef struct voom_qk_norm_rope_args {
+  const void* d_q;    /* T x hq x D */
+  const void* d_k;    /* T x hk x D */
+  void* d_q_out;
+  void* d_k_out;
+  const void* d_q_w;  /* D weights, or NULL */
+  const void* d_k_w;
+  const void* d_pos;  /* T positions, i32 or i64 */
+  const uint64_t* d_turns; /* rot / 2 */
+  int64_t q_token, q_head, k_token, k_head;     /* input strides */
+  int64_t qo_token, qo_head, ko_token, ko_head; /* output strides */
+  uint32_t T, hq, hk, D, rot;
+  uint32_t type;      /* VOOM_BF16 / FP16 / FP32 of q, k and the outputs */
+  uint32_t w_type;    /* of the weights */
+  uint32_t pos64, interleaved, zero_centered;
+  float eps, factor;
+} voom_qk_norm_rope_args;
+int voom_qk_norm_rope(const voom_qk_norm_rope_args* a, void* stream);
+
+/* What the attention reads: keys and values of B requests, hk heads of D
+ * values (a multiple of 8, at most 256; rows 16-byte aligned), in one of
+ *   one piece:     page = capacity; request b starts at b * k_page;
+ *   pages of one pool: d_table[b * table_stride + p] is the page index, its
+ *                  rows start at index * k_page (index outside [0, n_pages)
+ *                  reads as zero keys and values);
+ *   pages anywhere: d_offsets[2 * (b * table_stride + p)] / [.. + 1] are
+ *                  the element offsets of the page's keys / values from d_k / d_v.
+ * Position s of head h lies (s / page)-th page, + h * k_head + (s % page) * k_pos.
+ * d_len[b] positions are valid (clamped to max_len and to what the table holds). */
+typedef struct voom_kv_view {
+  const void* d_k;
+  const void* d_v;
+  const int32_t* d_len;
+  const int32_t* d_table;
+  const int64_t* d_offsets;
+  int64_t k_page, k_head, k_pos, v_page, v_head, v_pos; /* strides, elements */
+  uint32_t B, hk, D, type; /* VOOM_BF16 / VOOM_FP16 */
+  uint32_t page, table_stride, n_pages, max_len;
+} voom_kv_view;
+
+/* Ancestor masks of B trees of n drafted tokens: d_parents[b * n + i] is the
+ * parent's index (< i), -1 for a root, -2 for no token (an empty row).  Word w
+ * of row (b, i), (n + 31) / 32 words, has bit j - 32 w set where token j is i
+ * or an ancestor of i; d_depth[b * n + i] = ancestors of i (0 for a root; -1
+ * for no token).  A parent outside [-1, i), or that is no token, makes the token
+ * a root.  n <= 1024. */
+int voom_tree_mask(const int32_t* d_parents, uint32_t B, uint32_t n, uint32_t* d_mask, int32_t* d_depth, void* stream);
+
+/* Attention of n new tokens of each request over its cache and over one
+ * another: out[b, i, h] = sum_j softmax_j(scale q . k_j) v_j over the cached
+ * positions and the new tokens j that row i of the mask names (d_mask NULL: a
+ * chain, j <= i).  Query head h reads key head h / (hq / hk).  A row that sees
+ * nothing (a -2 token, which sees no cached position either) gives 0 and lse
+ * = -inf.  lse: natural log of the softmax denominator.  d_weights[b, h, s]
+ * (fp32) += the sum over the rows of key head h of their softmax weight at
+ * position s (cached positions first, then the new tokens), each row times
+ * d_token_weight[b, i] if given.  Each sum is made by one thread in a fixed
+ * order: results do not depend on scheduling.  fp32 softmax; scores and outputs
+ * accumulate in fp32; probabilities are rounded to `type` for the value product. */
+typedef struct voom_tree_attention_args {
+  const void* d_q;  /* B x n x hq x D */
+  const void* d_kn; /* B x n x hk x D: the new tokens' keys   */
+  const void* d_vn; /*                 and values             */
+  void* d_out;      /* B x n x hq x D */
+  float* d_lse;     /* B x n x hq contiguous, or NULL */
+  const uint32_t* d_mask;
+  float* d_weights; /* or NULL */
+  const float* d_token_weight; /* B x n contiguous, or NULL */
+  int64_t q_b, q_t, q_h, kn_b, kn_t, kn_h, vn_b, vn_t, vn_h, o_b, o_t, o_h, w_b, w_h; /* strides, elements */
+  uint32_t n, hq;
+  float scale;
+  uint32_t pad;
+} voom_tree_attention_args;
+uint64_t voom_tree_attention_scratch_bytes(const voom_kv_view* c, const voom_tree_attention_args* a);
+int voom_tree_attention(const voom_kv_view* c, const voom_tree_attention_args* a, void* d_scratch,
+                        uint64_t scratch_bytes, void* stream);
+
+/* Eviction: every head of every request keeps its first `sinks` positions, its
+ * newest `recent` and, of the others, the ones with the largest weights (equal
+ * weights: the lower position; NaN counts as the largest) up to `budget`;
+ * a request of at most `budget` positions keeps all.  Kept positions stay in
+ * order: row j of d_k_out / d_v_out (B x hk x budget x D) and of d_w_out is
+ * position d_index[.., j]; rows past d_len_out[b] are 0 and their index -1. */
+typedef struct voom_kv_evict_args {
+  const float* d_weights; /* w_b, w_h strides */
+  int64_t w_b, w_h;
+  void* d_k_out;
+  void* d_v_out;
+  float* d_w_out;
+  int32_t* d_index;
+  int32_t* d_len_out;
+  uint32_t budget, sinks, recent, pad;
+} voom_kv_evict_args;
+int voom_kv_evict(const voom_kv_view* c, const voom_kv_evict_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -29,6 +29,34 @@ def stream_ptr(device: torch.device, stream: torch.cuda.Stream | None = None) ->
     return int(s.cuda_stream)
 
 
+class on_stream:
+    """`with on_stream(device, stream) as ptr`: inside, `device` is current and
+    `stream` (None: the device's current stream) is the current stream, so
+    that tensors made there belong to it; `ptr` is its cudaStream_t.  Costs
+    nothing where both are current already."""
+
+    __slots__ = ("device", "stream", "ctx")
+
+    def __init__(self, device: torch.device, stream: torch.cuda.Stream | None = None):
+        self.device, self.stream, self.ctx = device, stream, None
+
+    def __enter__(self) -> int:
+        if self.stream is not None:
+            if self.stream.device != self.device:
+                raise ValueError(f"a stream of {self.stream.device} for tensors on {self.device}")
+            self.ctx = torch.cuda.stream(self.stream)
+            self.ctx.__enter__()
+            return int(self.stream.cuda_stream)
+        if torch.cuda.current_device() != self.device.index:
+            self.ctx = torch.cuda.device(self.device)
+            self.ctx.__enter__()
+        return torch._C._cuda_getCurrentRawStream(self.device.index)
+
+    def __exit__(self, *exc) -> None:
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+
+
 def as_u8(buf) -> np.ndarray:
     """bytes / bytearray / memoryview / numpy / CPU tensor -> flat uint8 numpy view."""
     if isinstance(buf, np.ndarray):

@@ -11,6 +11,7 @@ import threading
 from pathlib import Path
 
 import numpy as np
+import torch
 
 LIB_PATH = Path(__file__).resolve().with_name("libvoom_b200.so")
 
@@ -71,6 +72,38 @@ class MoeEp(ctypes.Structure):
         ("world", ctypes.c_uint32),
         ("t_pad", ctypes.c_uint32),
     ]
+
+
+# Element types of the attention entry points (VOOM_BF16 / FP16 / FP32)
+ELEMENT_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _fields(*groups: str) -> list:
+    """ctypes fields from "type: name name ..." groups."""
+    types = {"p": ctypes.c_void_p, "i64": ctypes.c_int64, "u32": ctypes.c_uint32, "f32": ctypes.c_float}
+    return [(n, types[t.strip()]) for g in groups for t, names in [g.split(":")] for n in names.split()]
+
+
+class QkNormRopeArgs(ctypes.Structure):
+    _fields_ = _fields("p: q k q_out k_out q_w k_w pos turns",
+                       "i64: q_token q_head k_token k_head qo_token qo_head ko_token ko_head",
+                       "u32: T hq hk D rot type w_type pos64 interleaved zero_centered", "f32: eps factor")
+
+
+class KvViewStruct(ctypes.Structure):
+    _fields_ = _fields("p: k v len table offsets", "i64: k_page k_head k_pos v_page v_head v_pos",
+                       "u32: B hk D type page table_stride n_pages max_len")
+
+
+class TreeAttentionArgs(ctypes.Structure):
+    _fields_ = _fields("p: q kn vn out lse mask weights token_weight",
+                       "i64: q_b q_t q_h kn_b kn_t kn_h vn_b vn_t vn_h o_b o_t o_h w_b w_h", "u32: n hq", "f32: scale",
+                       "u32: pad")
+
+
+class KvEvictArgs(ctypes.Structure):
+    _fields_ = _fields("p: weights", "i64: w_b w_h", "p: k_out v_out w_out index len_out",
+                       "u32: budget sinks recent pad")
 
 
 class RansPlanInfo(ctypes.Structure):
@@ -138,6 +171,11 @@ SIGNATURES: dict[str, tuple] = {
     "voom_nf12_linear": (_i32, [_vp, _u32, _u32, _u32, _vp, _u64, _u64, _u32, _vp, _u64, _vp, _vp, _vp]),
     "voom_nf12_linear_batch_scratch_bytes": (_u64, [_vp, _u32, _u32]),
     "voom_nf12_linear_batch": (_i32, [_vp, _u32, _u32, _vp, _u64, _u64, _vp, _u64, _vp, _vp]),
+    "voom_qk_norm_rope": (_i32, [_vp, _vp]),
+    "voom_tree_mask": (_i32, [_vp, _u32, _u32, _vp, _vp, _vp]),
+    "voom_tree_attention_scratch_bytes": (_u64, [_vp, _vp]),
+    "voom_tree_attention": (_i32, [_vp, _vp, _vp, _u64, _vp]),
+    "voom_kv_evict": (_i32, [_vp, _vp, _vp]),
     "voom_expert_swiglu": (_i32, [_vp, _vp, _u32, _vp, _vp, _u32, _u32, _vp, _u32, _u32, _u32, _u32, _vp, _vp,
                                   _u64, _vp, _vp]),
 }

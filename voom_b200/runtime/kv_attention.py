@@ -1,0 +1,278 @@
+"""Attention over a KV cache: drafted trees, prompts and single tokens, the
+weight each cached position receives, and eviction by it.
+
+  KVView          - where keys and values lie: one piece, pages of a pool, or
+                    pages anywhere (PagedKVCache.view).
+  DraftTree       - the new tokens of a step: a tree of drafts per request, or
+                    a chain (a prompt's chunk; one token).
+  tree_attention  - the new tokens' attention over the cache and one another
+                    (csrc/kv_attn.cu).
+  kv_evict        - keeps a cache's first, newest and most attended positions
+                    (csrc/kv_evict.cu).
+
+New tokens' keys and values are separate tensors, as they come from the
+projection: a drafted token enters a cache only once it is accepted, so a
+rejected one leaves nothing to undo.  Nothing here synchronises with the host.
+
+Counterpart in the reference: the attention around its caches
+(runtime/layer_runner.py `_attention`, runtime/kv_paged.py:143-181).
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple
+
+import numpy as np
+import torch
+
+from .. import _device
+from .._lib import ELEMENT_TYPES, KvEvictArgs, KvViewStruct, TreeAttentionArgs, check, load
+
+MAX_HEAD_DIM = 256
+MAX_TREE = 1024  # tokens of a tree that is not a chain
+_CACHE_TYPES = (torch.bfloat16, torch.float16)
+
+
+def _rows(x: torch.Tensor, name: str) -> None:
+    """Checks what the kernels need of a tensor whose last dimension is a head's values."""
+    if x.stride(-1) != 1 or x.data_ptr() % 16 or any(s % 8 for s in x.stride()[:-1]):
+        raise ValueError(f"{name}: heads must be contiguous and every row must start on 16 bytes")
+
+
+class KVView:
+    """Keys and values of B requests as the attention reads them; holds the
+    tensors.  `lengths` is an int32 device tensor of the B requests' cached
+    positions, read by the kernels when they run (it may change between
+    calls, and a captured graph sees the change); `max_len` bounds them."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, *, batch: int, heads: int,
+                 head_dim: int, page: int, strides: tuple, max_len: int, table: torch.Tensor | None = None,
+                 offsets: torch.Tensor | None = None, table_stride: int = 0, n_pages: int = 0, keep: object = None):
+        if k.dtype not in _CACHE_TYPES or v.dtype != k.dtype:
+            raise ValueError(f"cached keys and values must both be BF16 or FP16, got {k.dtype} and {v.dtype}")
+        if head_dim % 8 or not 0 < head_dim <= MAX_HEAD_DIM:
+            raise ValueError(f"head size {head_dim}: a multiple of 8 up to {MAX_HEAD_DIM}")
+        self.device = _device.require_cuda(k.device)
+        if lengths.dtype != torch.int32 or lengths.shape != (batch,) or not lengths.is_contiguous():
+            raise ValueError(f"lengths: {batch} contiguous int32 wanted, got {tuple(lengths.shape)} {lengths.dtype}")
+        if not (v.device == lengths.device == self.device):
+            raise ValueError("keys, values and lengths must be on one device")
+        capacity = page * table_stride if (table is not None or offsets is not None) else page
+        if not 0 <= max_len <= capacity:
+            raise ValueError(f"max_len {max_len} of a cache that holds {capacity} positions")
+        self.k, self.v, self.lengths, self.table, self.offsets, self.keep = k, v, lengths, table, offsets, keep
+        self.batch, self.heads, self.head_dim, self.max_len = batch, heads, head_dim, max_len
+        self.dtype = k.dtype
+        self.struct = KvViewStruct(k.data_ptr(), v.data_ptr(), lengths.data_ptr(),
+                                   None if table is None else table.data_ptr(),
+                                   None if offsets is None else offsets.data_ptr(), *strides, batch, heads, head_dim,
+                                   ELEMENT_TYPES[k.dtype], page, table_stride, n_pages, max_len)
+        self._scratch: dict[int, torch.Tensor] = {}
+
+    @classmethod
+    def contiguous(cls, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, max_len: int | None = None) -> "KVView":
+        """k, v: (B, heads, capacity, D), any strides that keep rows on 16 bytes."""
+        if k.dim() != 4 or v.shape != k.shape:
+            raise ValueError(f"k and v: (B, heads, capacity, D) wanted, got {tuple(k.shape)} and {tuple(v.shape)}")
+        _rows(k, "k")
+        _rows(v, "v")
+        B, H, cap, D = k.shape
+        return cls(k, v, lengths, batch=B, heads=H, head_dim=D, page=cap, max_len=cap if max_len is None else max_len,
+                   strides=(*k.stride()[:3], *v.stride()[:3]))
+
+    @classmethod
+    def pool(cls, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
+             max_len: int | None = None) -> "KVView":
+        """k, v: (pages, heads, positions, D); table: (B, pages per request)
+        int32, the pool page of each run of positions.  A table entry outside
+        the pool reads as zero keys and values."""
+        if k.dim() != 4 or v.shape != k.shape:
+            raise ValueError(f"k and v: (pages, heads, positions, D) wanted, got {tuple(k.shape)} and {tuple(v.shape)}")
+        if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous() or table.device != k.device:
+            raise ValueError("table: a contiguous int32 (B, pages) tensor on the pool's device wanted")
+        _rows(k, "k")
+        _rows(v, "v")
+        N, H, P, D = k.shape
+        B, per = table.shape
+        return cls(k, v, lengths, batch=B, heads=H, head_dim=D, page=P, table=table, table_stride=per, n_pages=N,
+                   max_len=P * per if max_len is None else max_len, strides=(*k.stride()[:3], *v.stride()[:3]))
+
+    @classmethod
+    def pages(cls, pages: list[list[tuple[torch.Tensor, torch.Tensor]]], lengths: torch.Tensor,
+              max_len: int | None = None) -> "KVView":
+        """One list of (k, v) pages per request, each (1, heads, positions, D)
+        or (heads, positions, D) with the same strides, anywhere on the device."""
+        flat = [p for request in pages for p in request]
+        if not flat:
+            raise ValueError("a view of pages needs at least one page")
+        k0, v0 = flat[0]
+        ks, vs = k0.stride()[-3:], v0.stride()[-3:]
+        for k, v in flat:
+            if k.shape != k0.shape or v.shape != k0.shape or k.stride()[-3:] != ks or v.stride()[-3:] != vs:
+                raise ValueError("all pages must have one shape and one set of strides")
+            if k.dtype != k0.dtype or v.dtype != k0.dtype or k.device != k0.device or v.device != k0.device:
+                raise ValueError("all pages must have one type and lie on one device")
+            _rows(k, "k page")
+            _rows(v, "v page")
+        if k0.dim() not in (3, 4) or (k0.dim() == 4 and k0.shape[0] != 1):
+            raise ValueError(f"pages of (1, heads, positions, D) wanted, got {tuple(k0.shape)}")
+        H, P, D = k0.shape[-3:]
+        per = max(len(request) for request in pages)
+        e = k0.element_size()
+        off = np.zeros((len(pages), per, 2), np.int64)
+        for b, request in enumerate(pages):
+            for p, (k, v) in enumerate(request):
+                off[b, p] = (k.data_ptr() - k0.data_ptr()) // e, (v.data_ptr() - v0.data_ptr()) // e
+        offsets = torch.from_numpy(off).to(k0.device)
+        return cls(k0, v0, lengths, batch=len(pages), heads=H, head_dim=D, page=P, offsets=offsets, table_stride=per,
+                   max_len=P * per if max_len is None else max_len, strides=(0, ks[0], ks[1], 0, vs[0], vs[1]),
+                   keep=flat)
+
+    def scratch(self, n: int, stream_ptr: int) -> torch.Tensor:
+        """Workspace of at least n bytes for calls on one stream, kept with the view."""
+        s = self._scratch.get(stream_ptr)
+        if s is None or s.numel() < n:
+            s = self._scratch[stream_ptr] = torch.zeros(n, dtype=torch.uint8, device=self.device)
+        return s
+
+
+class DraftTree:
+    """The new tokens of one step.  `parents` (B, n) int32: the parent of each
+    drafted token (a lower index), -1 for a root, which follows the last cached
+    position, -2 for no token (requests with fewer drafts than n).  A token sees
+    the whole cache, its ancestors and itself.  The masks and depths are made
+    on the device once and serve every layer of the step."""
+
+    def __init__(self, parents: torch.Tensor, stream: torch.cuda.Stream | None = None):
+        if parents.dim() != 2 or parents.dtype != torch.int32:
+            raise ValueError(f"parents: an int32 (B, n) tensor wanted, got {tuple(parents.shape)} {parents.dtype}")
+        if parents.shape[1] > MAX_TREE:
+            raise ValueError(f"a tree of {parents.shape[1]} tokens: at most {MAX_TREE}")
+        self.device = _device.require_cuda(parents.device)
+        self.batch, self.n = parents.shape
+        with _device.on_stream(self.device, stream) as sp:
+            parents = parents.contiguous()
+            self.mask: torch.Tensor | None = torch.empty((self.batch, self.n, (self.n + 31) // 32), dtype=torch.int32,
+                                                         device=self.device)
+            self.depth = torch.empty((self.batch, self.n), dtype=torch.int32, device=self.device)
+            if parents.numel():
+                check(load().voom_tree_mask(parents.data_ptr(), self.batch, self.n, self.mask.data_ptr(),
+                                            self.depth.data_ptr(), sp), "voom_tree_mask")
+
+    @classmethod
+    def chain(cls, batch: int, n: int, device=None) -> "DraftTree":
+        """n tokens that follow one another in every request: one new token, a
+        prompt or a chunk of one.  Any length; needs no mask."""
+        t = cls.__new__(cls)
+        t.device = _device.require_cuda(device)
+        t.batch, t.n, t.mask = int(batch), int(n), None
+        t.depth = torch.arange(n, dtype=torch.int32, device=t.device).expand(batch, n)
+        return t
+
+    def positions(self, lengths: torch.Tensor) -> torch.Tensor:
+        """Position of every new token, (B, n) int32: cached positions + depth."""
+        return lengths[:, None] + self.depth
+
+
+def _new(x: torch.Tensor, name: str, B: int, n: int, heads: int, cache: KVView) -> None:
+    if x.shape != (B, n, heads, cache.head_dim) or x.dtype != cache.dtype or x.device != cache.device:
+        raise ValueError(f"{name}: ({B}, {n}, {heads}, {cache.head_dim}) {cache.dtype} on {cache.device} wanted, got "
+                         f"{tuple(x.shape)} {x.dtype} on {x.device}")
+    _rows(x, name)
+
+
+def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: DraftTree, cache: KVView, *,
+                   scale: float | None = None, weights: torch.Tensor | None = None,
+                   token_weight: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                   return_lse: bool = False, stream: torch.cuda.Stream | None = None):
+    """Attention of the new tokens (q: (B, n, Hq, D); k, v: (B, n, heads, D),
+    any strides with 16-byte rows) over the cache and over one another, as
+    `tree` says: (B, n, Hq, D) in the cache's type, and with `return_lse` the
+    natural log of each row's softmax denominator, (B, n, Hq) fp32.  Query head
+    h reads key head h // (Hq // heads); `scale` defaults to D ** -0.5.  A row
+    of no token gives zeros and lse -inf.
+
+    `weights` (B, heads, >= max_len + n) fp32: each position's softmax weight,
+    summed over the rows that share its head (each times `token_weight` (B, n)
+    fp32, if given), is added in place: cached positions at their index, new
+    token j at lengths[b] + j.  kv_evict reads these sums."""
+    B, n, hq, D = q.shape
+    heads = cache.heads
+    if B != cache.batch or (B, n) != (tree.batch, tree.n):
+        raise ValueError(f"{B} requests of {n} new tokens in q, {tree.batch} of {tree.n} in the tree, {cache.batch} cached")
+    if hq % heads or not hq:
+        raise ValueError(f"{hq} query heads do not divide into {heads} key heads")
+    _new(q, "q", B, n, hq, cache)
+    _new(k, "k", B, n, heads, cache)
+    _new(v, "v", B, n, heads, cache)
+    if tree.device != cache.device:
+        raise ValueError(f"the tree is on {tree.device}, the cache on {cache.device}")
+    if weights is not None:
+        if weights.dim() != 3 or weights.shape[:2] != (B, heads) or weights.shape[2] < cache.max_len + n or \
+                weights.dtype != torch.float32 or weights.stride(2) != 1 or weights.device != cache.device:
+            raise ValueError(f"weights: fp32 ({B}, {heads}, at least {cache.max_len + n}) on {cache.device} wanted, got "
+                             f"{tuple(weights.shape)} {weights.dtype}")
+    if token_weight is not None:
+        if weights is None:
+            raise ValueError("token_weight goes with weights")
+        if token_weight.shape != (B, n) or token_weight.dtype != torch.float32 or not token_weight.is_contiguous() \
+                or token_weight.device != cache.device:
+            raise ValueError(f"token_weight: contiguous fp32 ({B}, {n}) on {cache.device} wanted")
+    with _device.on_stream(cache.device, stream) as sp:
+        if out is None:
+            out = torch.empty((B, n, hq, D), dtype=q.dtype, device=cache.device)
+        else:
+            _new(out, "out", B, n, hq, cache)
+        lse = torch.empty((B, n, hq), dtype=torch.float32, device=cache.device) if return_lse else None
+        if n:
+            a = TreeAttentionArgs(
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
+                None if tree.mask is None else tree.mask.data_ptr(), None if weights is None else weights.data_ptr(),
+                None if token_weight is None else token_weight.data_ptr(), *q.stride()[:3], *k.stride()[:3],
+                *v.stride()[:3], *out.stride()[:3], *(weights.stride()[:2] if weights is not None else (0, 0)), n, hq,
+                D ** -0.5 if scale is None else scale, 0)
+            lib = load()
+            c, ap = ctypes.byref(cache.struct), ctypes.byref(a)
+            need = lib.voom_tree_attention_scratch_bytes(c, ap)
+            s = cache.scratch(need, sp).data_ptr() if need else None
+            check(lib.voom_tree_attention(c, ap, s, need, sp), "voom_tree_attention")
+    return (out, lse) if return_lse else out
+
+
+class Evicted(NamedTuple):
+    """What kv_evict kept: k, v (B, heads, budget, D), the weights (B, heads,
+    budget) and original positions (int32, -1 past the length) of the kept
+    rows, in order, and the requests' new lengths (B) int32."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    weights: torch.Tensor
+    index: torch.Tensor
+    lengths: torch.Tensor
+
+
+def kv_evict(cache: KVView, weights: torch.Tensor, *, budget: int, sinks: int = 4, recent: int = 0,
+             stream: torch.cuda.Stream | None = None) -> Evicted:
+    """Cuts every request to at most `budget` positions: the first `sinks`, the
+    newest `recent`, and of the others those with the largest `weights` (B,
+    heads, >= max_len) fp32 (equal ones: the lower position), each head by
+    itself.  Rows past a request's new length are zero."""
+    B, H, D = cache.batch, cache.heads, cache.head_dim
+    if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
+        raise ValueError(f"a budget of {budget} positions cannot hold {sinks} first and {recent} newest ones")
+    if weights.dim() != 3 or weights.shape[:2] != (B, H) or weights.shape[2] < cache.max_len or \
+            weights.dtype != torch.float32 or weights.stride(2) != 1 or weights.device != cache.device:
+        raise ValueError(f"weights: fp32 ({B}, {H}, at least {cache.max_len}) on {cache.device} wanted, got "
+                         f"{tuple(weights.shape)} {weights.dtype}")
+    dev = cache.device
+    with _device.on_stream(dev, stream) as sp:
+        k = torch.empty((B, H, budget, D), dtype=cache.dtype, device=dev)
+        v = torch.empty((B, H, budget, D), dtype=cache.dtype, device=dev)
+        w = torch.empty((B, H, budget), dtype=torch.float32, device=dev)
+        index = torch.empty((B, H, budget), dtype=torch.int32, device=dev)
+        lengths = torch.empty(B, dtype=torch.int32, device=dev)
+        a = KvEvictArgs(weights.data_ptr(), weights.stride(0), weights.stride(1), k.data_ptr(), v.data_ptr(),
+                        w.data_ptr(), index.data_ptr(), lengths.data_ptr(), budget, sinks, recent, 0)
+        check(load().voom_kv_evict(ctypes.byref(cache.struct), ctypes.byref(a), sp), "voom_kv_evict")
+    return Evicted(k, v, w, index, lengths)

@@ -1,0 +1,151 @@
+"""Position rotation of queries and keys, with their per-head norms, in one pass.
+
+  Rotary         - the frequencies of a head: size, rotated part, base, pair
+                   layout and long-context scaling.
+  qk_norm_rope   - norm + rotation of q and k (csrc/rope.cu).
+
+Counterpart in the reference: the mx.fast.rms_norm / mx.fast.rope calls of its
+attention layers (runtime/layer_runner.py `_attention`), ahead of the KV caches.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from .. import _device
+from .._lib import ELEMENT_TYPES, QkNormRopeArgs, check, load
+
+LAYOUTS = ("half", "interleaved")
+MAX_HEAD_DIM = 512
+
+
+def _scaled(freqs: list[float], rot_dim: int, theta: float, scaling: dict) -> tuple[list[float], float]:
+    """Frequencies (radians per position) stretched for a longer context, and
+    the factor on the rotated values.  `scaling` uses the names of model
+    configurations: rope_type linear, ntk, yarn or llama3."""
+    kind = scaling.get("rope_type", scaling.get("type"))
+    factor = float(scaling.get("factor", 1.0))
+    if factor < 1.0:
+        raise ValueError(f"rotary scaling factor {factor}: at least 1")
+    if kind == "linear":
+        return [f / factor for f in freqs], 1.0
+    if kind == "ntk":
+        base = theta * factor ** (rot_dim / max(rot_dim - 2, 1))
+        return [base ** (-2.0 * i / rot_dim) for i in range(rot_dim // 2)], 1.0
+    if kind == "yarn":
+        orig = float(scaling["original_max_position_embeddings"])
+
+        def pair_with(turns: float) -> float:  # the pair that makes `turns` turns over the original context
+            return rot_dim * math.log(orig / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+        lo = max(math.floor(pair_with(float(scaling.get("beta_fast", 32.0)))), 0)
+        hi = min(math.ceil(pair_with(float(scaling.get("beta_slow", 1.0)))), rot_dim - 1)
+        out = []
+        for i, f in enumerate(freqs):
+            ramp = min(max((i - lo) / max(hi - lo, 0.001), 0.0), 1.0)
+            out.append(f / factor * ramp + f * (1.0 - ramp))
+        attention = scaling.get("attention_factor")
+        return out, 0.1 * math.log(factor) + 1.0 if attention is None else float(attention)
+    if kind == "llama3":
+        orig = float(scaling["original_max_position_embeddings"])
+        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        out = []
+        for f in freqs:
+            turns = orig * f / (2 * math.pi)  # turns over the original context
+            keep = min(max((turns - low) / (high - low), 0.0), 1.0)
+            out.append(f / factor * (1.0 - keep) + f * keep)
+        return out, 1.0
+    raise ValueError(f"unknown rotary scaling {kind!r} (one of linear, ntk, yarn, llama3)")
+
+
+class Rotary:
+    """The rotation of one head: `rot_dim` of its `head_dim` values (all of
+    them by default) in pairs (i, i + rot_dim / 2) for layout "half" or
+    (2i, 2i + 1) for "interleaved", pair i turning by theta ** (-2 i / rot_dim)
+    radians per position, stretched by `scaling`.
+
+    `turns` holds each pair's turns per position in units of 2^-64, so that
+    angles far into a context keep their precision; `factor` multiplies the
+    rotated values (1 but for yarn)."""
+
+    def __init__(self, head_dim: int, *, rot_dim: int | None = None, theta: float = 10000.0, layout: str = "half",
+                 scaling: dict | None = None, device=None):
+        rot_dim = head_dim if rot_dim is None else rot_dim
+        if not 0 < head_dim <= MAX_HEAD_DIM:
+            raise ValueError(f"head size {head_dim}: 1 to {MAX_HEAD_DIM}")
+        if rot_dim % 2 or not 0 <= rot_dim <= head_dim:
+            raise ValueError(f"rotated part {rot_dim} of a head of {head_dim}: an even number up to the head's size")
+        if layout not in LAYOUTS:
+            raise ValueError(f"unknown rotary layout {layout!r} (one of {LAYOUTS})")
+        self.head_dim, self.rot_dim, self.theta, self.layout = int(head_dim), int(rot_dim), float(theta), layout
+        freqs = [self.theta ** (-2.0 * i / rot_dim) for i in range(rot_dim // 2)]
+        self.factor = 1.0
+        if scaling is not None:
+            freqs, self.factor = _scaled(freqs, rot_dim, self.theta, scaling)
+        self.freqs = freqs
+        turns = [round(f / (2 * math.pi) * 2 ** 64) % 2 ** 64 for f in freqs]
+        self.device = _device.require_cuda(device)
+        self.turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64,
+                                  device=self.device)
+
+
+def _heads(x: torch.Tensor, name: str, D: int) -> None:
+    if x.dim() != 3 or x.shape[2] != D:
+        raise ValueError(f"{name}: (tokens, heads, {D}) wanted, got {tuple(x.shape)}")
+    if x.stride(2) != 1 and x.numel():
+        raise ValueError(f"{name}: the values of a head must be contiguous")
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rotary: Rotary, *,
+                 q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                 zero_centered: bool = False, out_q: torch.Tensor | None = None, out_k: torch.Tensor | None = None,
+                 stream: torch.cuda.Stream | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """q (T, Hq, D) and k (T, Hk, D), normed per head (x rsqrt(mean x^2 + eps)
+    times the weight, or 1 + the weight with `zero_centered`; not normed where
+    the weight is None) and rotated by their tokens' `positions` (T, int32 or
+    int64).  BF16, FP16 or FP32; any token and head strides, so q and k may be
+    views of a fused projection.  `out_q` / `out_k` may be views of a cache, or q
+    and k themselves.  fp32 arithmetic, one rounding."""
+    T, hq, D = q.shape
+    _heads(q, "q", rotary.head_dim)
+    _heads(k, "k", rotary.head_dim)
+    dt = q.dtype
+    if dt not in ELEMENT_TYPES or k.dtype != dt:
+        raise ValueError(f"q and k must both be BF16, FP16 or FP32, got {q.dtype} and {k.dtype}")
+    if k.shape[0] != T or positions.shape != (T,):
+        raise ValueError(f"{T} tokens in q, {k.shape[0]} in k, positions {tuple(positions.shape)}")
+    if positions.dtype not in (torch.int64, torch.int32) or not positions.is_contiguous():
+        raise ValueError("positions must be contiguous int32 or int64")
+    dev = rotary.device
+    w_type = None
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is None:
+            continue
+        if w.shape != (D,) or w.dtype not in ELEMENT_TYPES or not w.is_contiguous() or w.device != dev:
+            raise ValueError(f"{name}: {D} contiguous BF16, FP16 or FP32 weights on {dev} wanted")
+        if w_type is not None and w.dtype != w_type:
+            raise ValueError("q_weight and k_weight must have one type")
+        w_type = w.dtype
+    with _device.on_stream(dev, stream) as sp:
+        if out_q is None:
+            out_q = torch.empty((T, hq, D), dtype=dt, device=dev)
+        if out_k is None:
+            out_k = torch.empty((T, k.shape[1], D), dtype=dt, device=dev)
+        for name, x, like in (("out_q", out_q, q), ("out_k", out_k, k)):
+            if x.shape != like.shape or x.dtype != dt or (x.stride(2) != 1 and x.numel()):
+                raise ValueError(f"{name}: {tuple(like.shape)} {dt} with contiguous heads wanted")
+        if not (q.device == k.device == positions.device == out_q.device == out_k.device == dev):
+            raise ValueError(f"q, k, positions and the outputs must be on the rotary plan's device {dev}")
+        a = QkNormRopeArgs(
+            q.data_ptr(), k.data_ptr(), out_q.data_ptr(), out_k.data_ptr(),
+            None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
+            positions.data_ptr(), rotary.turns.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1),
+            out_q.stride(0), out_q.stride(1), out_k.stride(0), out_k.stride(1), T, hq, k.shape[1], D, rotary.rot_dim,
+            ELEMENT_TYPES[dt], 0 if w_type is None else ELEMENT_TYPES[w_type], positions.dtype == torch.int64,
+            rotary.layout == "interleaved", zero_centered, eps, rotary.factor)
+        if T:
+            check(load().voom_qk_norm_rope(ctypes.byref(a), sp), "voom_qk_norm_rope")
+    return out_q, out_k
