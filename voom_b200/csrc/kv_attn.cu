@@ -1,22 +1,18 @@
 // Attention of drafted tokens over a KV cache, its weight sums, and the tree masks.
+#include <algorithm>
+#include <atomic>
 #include <initializer_list>
+#include <type_traits>
 
-#include "kv_view.cuh"
+#include "kv_rows.cuh"
 
 namespace {
 
-using voom::kv::elem;
-using voom::kv::rounded;
-using voom::kv::View;
+using std::max;
+using std::min;
+using voom::kv::Attn;
 
 constexpr uint32_t kMaxTree = 1024;
-
-struct Attn {
-  View c;
-  voom_tree_attention_args a;
-  float* lse;  // a.d_lse, or scratch
-  uint32_t g, words;
-};
 
 // --------------------------------------------------------------- tree masks
 // One CTA per tree, a warp per row, which walks from its token to the root.
@@ -46,98 +42,143 @@ __global__ void __launch_bounds__(256) tree_mask(const int32_t* __restrict__ par
   }
 }
 
-// ------------------------------------------------------------------- rows
-__device__ __forceinline__ bool sees(const Attn& P, uint32_t b, uint32_t i, uint32_t j) {
-  if (!P.a.d_mask) return j <= i;
-  return P.a.d_mask[(uint64_t(b) * P.a.n + i) * P.words + (j >> 5)] >> (j & 31u) & 1u;
+// ------------------------------------------------------------------- finish
+// Joins the partial sums of units that several blocks shared (blocks below
+// n_merge: one per unit and eight rows), and adds the rows' weights at each
+// position to the running sums (the others: one per key head and kWeightSpan
+// positions), from the scores the attention kept and the rows' denominators.
+// The partial sums are joined in block order, the rows added in row order, so
+// that nothing depends on scheduling.
+constexpr uint32_t kWeightSpan = 1024;
+constexpr uint32_t kMergeRows = 8;
+
+struct Split {
+  uint32_t first, last;  // blocks that hold the unit's partial sums; first > last: none, it is whole
+};
+
+__device__ __forceinline__ Split split_of(const Attn& P, uint32_t b, uint32_t u, uint64_t total, uint64_t before) {
+  Split s{1, 0};
+  if (!P.ctas) return s;
+  const uint32_t steps = voom::kv::cache_steps(P, P.c.length(b)) + voom::kv::new_steps(P);
+  voom::kv::owners(P, total, before + uint64_t(u) * steps, steps, s.first, s.last);
+  if (s.first == s.last) s = Split{1, 0};
+  return s;
 }
 
-// Key and value row of position s (cached, then new); false: a page that is none.
-template <typename T>
-__device__ __forceinline__ bool rows_of(const Attn& P, uint32_t b, uint32_t h, uint32_t len, uint32_t s, const T*& k,
-                                        const T*& v) {
-  if (s < len) {
-    int64_t ko, vo;
-    if (!P.c.row_at(b, h, s, ko, vo)) return false;
-    k = static_cast<const T*>(P.c.v.d_k) + ko;
-    v = static_cast<const T*>(P.c.v.d_v) + vo;
-  } else {
-    const int64_t j = s - len;
-    k = static_cast<const T*>(P.a.d_kn) + int64_t(b) * P.a.kn_b + j * P.a.kn_t + int64_t(h) * P.a.kn_h;
-    v = static_cast<const T*>(P.a.d_vn) + int64_t(b) * P.a.vn_b + j * P.a.vn_t + int64_t(h) * P.a.vn_h;
-  }
-  return true;
+__device__ __forceinline__ const float* part_of(const Attn& P, const Split& s, uint32_t c) {
+  return voom::kv::slot_of(P, 2 * c + (c == s.first ? 1u : 0u));
 }
 
-__device__ __forceinline__ float warp_sum(float x) {
-  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
-  return x;
-}
-
-constexpr uint32_t kPer = voom::kv::kMaxD / 32;  // head values of a lane
-
-// One warp per row (request, new token, query head): running maximum and sum
-// of the softmax over the keys, one at a time.
-template <typename T>
-__global__ void __launch_bounds__(256) attn_rows(const Attn P) {
-  const uint32_t lane = threadIdx.x & 31u, n = P.a.n, hq = P.a.hq, D = P.c.v.D;
-  const uint64_t row = uint64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (row >= uint64_t(P.c.v.B) * n * hq) return;
-  const uint32_t hh = uint32_t(row % hq), i = uint32_t(row / hq % n), b = uint32_t(row / hq / n), h = hh / P.g;
-  const uint32_t len = P.c.length(b);
-  const T* q = static_cast<const T*>(P.a.d_q) + int64_t(b) * P.a.q_b + int64_t(i) * P.a.q_t + int64_t(hh) * P.a.q_h;
-  float x[kPer], o[kPer];
-  for (uint32_t e = 0; e < kPer; e++) {
-    x[e] = lane + 32 * e < D ? elem<T>(q[lane + 32 * e]) * P.a.scale : 0.0f;
-    o[e] = 0.0f;
-  }
+// Maximum and sum of one row over the partial sums (warp-collective).
+__device__ __forceinline__ float2 joined(const Attn& P, const Split& s, uint32_t r) {
+  const uint32_t lane = threadIdx.x & 31u;
   float top = -INFINITY, sum = 0.0f;
-  if (sees(P, b, i, i))
-    for (uint32_t s = 0; s < len + n; s++) {
-      if (s >= len && !sees(P, b, i, s - len)) continue;
-      const T *k, *v;
-      const bool is = rows_of<T>(P, b, h, len, s, k, v);
-      float z = 0.0f;
-      for (uint32_t e = 0; e < kPer; e++)
-        if (is && lane + 32 * e < D) z += x[e] * elem<T>(k[lane + 32 * e]);
-      z = warp_sum(z);
-      const float t = fmaxf(top, z), f = expf(top - t), p = expf(z - t);
-      sum = sum * f + p;
-      for (uint32_t e = 0; e < kPer; e++)
-        o[e] = o[e] * f + (is && lane + 32 * e < D ? p * elem<T>(v[lane + 32 * e]) : 0.0f);
-      top = t;
-    }
-  T* out = static_cast<T*>(P.a.d_out) + int64_t(b) * P.a.o_b + int64_t(i) * P.a.o_t + int64_t(hh) * P.a.o_h;
-  for (uint32_t e = 0; e < kPer; e++)
-    if (lane + 32 * e < D) out[lane + 32 * e] = rounded<T>(sum == 0.0f ? 0.0f : o[e] / sum);
-  if (P.lse && lane == 0) P.lse[row] = top + logf(sum);
+  for (uint32_t c = s.first + lane; c <= s.last; c += 32) {
+    const float2 ml = *reinterpret_cast<const float2*>(part_of(P, s, c) + P.rows * P.ld_o + 2 * r);
+    const float t = fmaxf(top, ml.x), base = t == -INFINITY ? 0.0f : t;
+    sum = sum * voom::kv::exp2_fast(top - base) + ml.y * voom::kv::exp2_fast(ml.x - base);
+    top = t;
+  }
+  for (int o = 16; o; o >>= 1) {
+    const float ot = __shfl_xor_sync(0xFFFFFFFFu, top, o), os = __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    const float t = fmaxf(top, ot), base = t == -INFINITY ? 0.0f : t;
+    // both lanes of a pair add the same two terms in the same order
+    const bool low = (lane & uint32_t(o)) == 0;
+    const float a = (low ? sum : os) * voom::kv::exp2_fast((low ? top : ot) - base);
+    const float c = (low ? os : sum) * voom::kv::exp2_fast((low ? ot : top) - base);
+    sum = a + c;
+    top = t;
+  }
+  return make_float2(top, sum);
 }
 
-// One warp per (request, key head, position): the rows' weights at it, from
-// the scores and the rows' softmax denominators.
 template <typename T>
-__global__ void __launch_bounds__(256) attn_weights(const Attn P) {
-  const uint32_t lane = threadIdx.x & 31u, n = P.a.n, D = P.c.v.D, b = blockIdx.z, h = blockIdx.y;
-  const uint32_t len = P.c.length(b), s = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (s >= len + n) return;
-  const T *k, *v;
-  const bool is = rows_of<T>(P, b, h, len, s, k, v);
-  float x[kPer];
-  for (uint32_t e = 0; e < kPer; e++) x[e] = is && lane + 32 * e < D ? elem<T>(k[lane + 32 * e]) * P.a.scale : 0.0f;
-  float got = 0.0f;
-  for (uint32_t i = 0; i < n; i++) {
-    if (!sees(P, b, i, i) || (s >= len && !sees(P, b, i, s - len))) continue;
-    const float tw = P.a.d_token_weight ? P.a.d_token_weight[uint64_t(b) * n + i] : 1.0f;
-    for (uint32_t hh = h * P.g; hh < (h + 1) * P.g; hh++) {
-      const T* q = static_cast<const T*>(P.a.d_q) + int64_t(b) * P.a.q_b + int64_t(i) * P.a.q_t + int64_t(hh) * P.a.q_h;
-      float z = 0.0f;
-      for (uint32_t e = 0; e < kPer; e++)
-        if (lane + 32 * e < D) z += x[e] * elem<T>(q[lane + 32 * e]);
-      z = warp_sum(z);
-      got += tw * expf(z - P.lse[(uint64_t(b) * n + i) * P.a.hq + hh]);
+__global__ void __launch_bounds__(256) attn_finish(const __grid_constant__ Attn P, uint32_t n_merge) {
+  extern __shared__ float s_row[];  // lse (log2 units) of the key head's rows, then their weights
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, U = voom::kv::units_of(P);
+  const uint64_t total = P.ctas ? voom::kv::steps_before(P, P.c.v.B) : 0;
+  if (blockIdx.x < n_merge) {
+    const uint32_t groups = P.rows / kMergeRows, unit = blockIdx.x / groups, r0 = (blockIdx.x - unit * groups) * kMergeRows;
+    const uint32_t b = unit / U, u = unit - b * U, h = u / P.mblocks, row0 = (u - h * P.mblocks) * P.rows;
+    if (row0 + r0 >= P.R) return;
+    const Split s = split_of(P, b, u, total, voom::kv::steps_before(P, b));
+    if (s.first > s.last) return;
+    if (warp < kMergeRows) {
+      const float2 ml = joined(P, s, r0 + warp);
+      if (lane == 0) {
+        s_row[2 * warp] = ml.x == -INFINITY ? 0.0f : ml.x;
+        s_row[2 * warp + 1] = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
+        const uint32_t row = row0 + r0 + warp;
+        if (P.lse && row < P.R)
+          P.lse[(uint64_t(b) * P.a.n + row / P.g) * P.a.hq + h * P.g + row % P.g] = voom::kv::kLn2 * (s_row[2 * warp] + log2f(ml.y));
+      }
+    }
+    __syncthreads();
+    const uint32_t quads = P.ld_o / 4;
+    for (uint32_t i = tid; i < kMergeRows * quads; i += 256) {
+      const uint32_t k = i / quads, d = 4 * (i - k * quads), r = r0 + k, row = row0 + r;
+      if (row >= P.R || d >= P.c.v.D) continue;
+      const float base = s_row[2 * k], inv = s_row[2 * k + 1];
+      float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+      for (uint32_t c = s.first; c <= s.last; c++) {
+        const float* part = part_of(P, s, c);
+        const float f = voom::kv::exp2_fast(part[P.rows * P.ld_o + 2 * r] - base);
+        const float4 v = *reinterpret_cast<const float4*>(part + r * P.ld_o + d);
+        y.x += f * v.x;
+        y.y += f * v.y;
+        y.z += f * v.z;
+        y.w += f * v.w;
+      }
+      T* out = static_cast<T*>(P.a.d_out) + int64_t(b) * P.a.o_b + int64_t(row / P.g) * P.a.o_t +
+               int64_t(h * P.g + row % P.g) * P.a.o_h + d;
+      uint2 x = make_uint2(voom::kv::pack2(y.x * inv, y.y * inv, T()), voom::kv::pack2(y.z * inv, y.w * inv, T()));
+      if (inv == 0.0f) x = make_uint2(0u, 0u);  // a row that sees nothing
+      *reinterpret_cast<uint2*>(out) = x;
+    }
+    return;
+  }
+  const uint32_t spans = (P.score_ld + kWeightSpan - 1) / kWeightSpan, item = blockIdx.x - n_merge;
+  const uint32_t head = item / spans, b = head / P.c.v.hk, h = head - b * P.c.v.hk, s0 = (item - head * spans) * kWeightSpan;
+  const uint32_t len = P.c.length(b);
+  if (s0 >= len && s0 + kWeightSpan <= P.score_new) return;
+  float* s_w = s_row + P.R;
+  const uint64_t before = P.ctas ? voom::kv::steps_before(P, b) : 0;
+  for (uint32_t r = warp; r < P.R; r += 8) {
+    const uint32_t k = r / P.rows, i = r / P.g, hh = h * P.g + r % P.g;
+    const Split s = split_of(P, b, h * P.mblocks + k, total, before);
+    float lse2;
+    if (s.first <= s.last) {
+      const float2 ml = joined(P, s, r - k * P.rows);
+      lse2 = (ml.x == -INFINITY ? 0.0f : ml.x) + log2f(ml.y);
+    } else {
+      lse2 = P.lse[(uint64_t(b) * P.a.n + i) * P.a.hq + hh] * voom::kv::kLog2e;
+    }
+    if (lane == 0) {
+      s_row[r] = lse2 == -INFINITY ? INFINITY : lse2;  // a row that sees nothing has no weight anywhere
+      s_w[r] = P.a.d_token_weight ? P.a.d_token_weight[uint64_t(b) * P.a.n + i] : 1.0f;
     }
   }
-  if (lane == 0) P.a.d_weights[int64_t(b) * P.a.w_b + int64_t(h) * P.a.w_h + s] += got;
+  __syncthreads();
+  const float* z = P.scores + uint64_t(head) * P.R * P.score_ld;
+  float got[kWeightSpan / 256] = {};
+  const uint32_t end = min(P.score_ld, s0 + kWeightSpan);
+  for (uint32_t r = 0; r < P.R; r++) {
+    const float lse2 = s_row[r], w = s_w[r];
+#pragma unroll
+    for (uint32_t k = 0; k < kWeightSpan / 256; k++) {
+      const uint32_t s = s0 + k * 256 + tid;
+      if (s < end) got[k] += w * voom::kv::exp2_fast(z[uint64_t(r) * P.score_ld + s] - lse2);
+    }
+  }
+  float* sums = P.a.d_weights + int64_t(b) * P.a.w_b + int64_t(h) * P.a.w_h;
+#pragma unroll
+  for (uint32_t k = 0; k < kWeightSpan / 256; k++) {
+    const uint32_t s = s0 + k * 256 + tid;
+    if (s < len) sums[s] += got[k];
+    else if (s >= P.score_new && s - P.score_new < P.a.n) sums[len + s - P.score_new] += got[k];
+  }
 }
 
 bool rows16(const void* p, std::initializer_list<int64_t> strides) {
@@ -147,22 +188,90 @@ bool rows16(const void* p, std::initializer_list<int64_t> strides) {
   return true;
 }
 
+int sm_count() {
+  int dev = 0, n = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n;
+}
+
+// Lets a kernel use `bytes` of shared memory on the current device, once per device.
+bool allow_smem(const void* kernel, uint32_t bytes, std::atomic<uint64_t>& devices) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  if (devices.load(std::memory_order_relaxed) >> (dev & 63) & 1u) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  devices.fetch_or(uint64_t(1) << (dev & 63), std::memory_order_relaxed);
+  return true;
+}
+
+// Tiles, grid and scratch of a call.  Returns the scratch bytes; sets the
+// pointers where `scratch` is given.
 uint64_t plan(Attn& P, void* scratch) {
-  P.g = P.a.hq / P.c.v.hk;
+  const voom_kv_view& c = P.c.v;
+  P.g = P.a.hq / c.hk;
+  P.R = P.a.n * P.g;
   P.words = (P.a.n + 31) / 32;
+  P.scale2 = P.a.scale * voom::kv::kLog2e;
+  P.ld_o = c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256;
+  P.keys = voom::kv::row_keys(P.ld_o);
+  // 32 rows to a block read the cache once where 16 would read it twice; at
+  // head size 256 the output of 32 rows does not fit the registers
+  P.rows = P.R > 16 && P.ld_o <= 128 ? 32 : 16;
+  P.mblocks = (P.R + P.rows - 1) / P.rows;
+  const uint64_t units = uint64_t(c.B) * c.hk * P.mblocks;
+  const uint32_t steps = (c.max_len + P.keys - 1) / P.keys + (P.a.n + P.keys - 1) / P.keys;
+  P.ctas = steps <= 16 ? 0u : uint32_t(min(uint64_t(sm_count()), (units * steps + 7) / 8));
+  uint64_t at = 0;
+  auto take = [&](uint64_t bytes) {
+    const uint64_t o = at;
+    at += (bytes + 255) & ~uint64_t(255);
+    return scratch ? static_cast<uint8_t*>(scratch) + o : nullptr;
+  };
+  P.partial = reinterpret_cast<float*>(take(uint64_t(2) * P.ctas * P.rows * (P.ld_o + 2) * sizeof(float)));
   P.lse = P.a.d_lse;
-  if (!P.a.d_weights || P.lse) return 0;
-  P.lse = static_cast<float*>(scratch);
-  return uint64_t(P.c.v.B) * P.a.n * P.a.hq * sizeof(float);
+  if (P.a.d_weights) {
+    if (!P.lse) P.lse = reinterpret_cast<float*>(take(uint64_t(c.B) * P.a.n * P.a.hq * sizeof(float)));
+    P.score_new = (c.max_len + P.keys - 1) / P.keys * P.keys;
+    P.score_ld = P.score_new + (P.a.n + P.keys - 1) / P.keys * P.keys;
+    P.scores = reinterpret_cast<float*>(take(uint64_t(c.B) * c.hk * P.R * P.score_ld * sizeof(float)));
+  }
+  return at;
+}
+
+template <typename T, int DP, int MT>
+int launch_rows(const Attn& P, cudaStream_t s) {
+  constexpr uint32_t smem = voom::kv::row_smem(DP, MT);
+  static std::atomic<uint64_t> allowed{0};
+  if (!allow_smem(reinterpret_cast<const void*>(voom::kv::attn_rows<T, DP, MT>), smem, allowed)) return VOOM_E_CUDA;
+  const uint64_t grid = P.ctas ? P.ctas : uint64_t(P.c.v.B) * P.c.v.hk * P.mblocks;
+  voom::kv::attn_rows<T, DP, MT><<<uint32_t(grid), 32 * voom::kv::kRowWarps, smem, s>>>(P);
+  return cudaGetLastError() == cudaSuccess ? VOOM_OK : VOOM_E_CUDA;
 }
 
 template <typename T>
 int run(const Attn& P, cudaStream_t s) {
-  const uint64_t rows = uint64_t(P.c.v.B) * P.a.n * P.a.hq;
-  attn_rows<T><<<uint32_t((rows + 7) / 8), 256, 0, s>>>(P);
-  if (P.a.d_weights)
-    attn_weights<T><<<dim3((P.c.v.max_len + P.a.n + 7) / 8, P.c.v.hk, P.c.v.B), 256, 0, s>>>(P);
-  return cudaGetLastError() == cudaSuccess ? VOOM_OK : VOOM_E_CUDA;
+  int rc;
+  if (P.ld_o == 64) rc = P.rows == 16 ? launch_rows<T, 64, 1>(P, s) : launch_rows<T, 64, 2>(P, s);
+  else if (P.ld_o == 128) rc = P.rows == 16 ? launch_rows<T, 128, 1>(P, s) : launch_rows<T, 128, 2>(P, s);
+  else rc = launch_rows<T, 256, 1>(P, s);
+  if (rc != VOOM_OK || (!P.ctas && !P.a.d_weights)) return rc;
+  const uint64_t units = uint64_t(P.c.v.B) * P.c.v.hk * P.mblocks;
+  const uint32_t n_merge = P.ctas ? uint32_t(units * (P.rows / kMergeRows)) : 0u;
+  const uint64_t spans = P.a.d_weights ? uint64_t(P.c.v.B) * P.c.v.hk * ((P.score_ld + kWeightSpan - 1) / kWeightSpan) : 0;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(uint32_t(n_merge + spans));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = max(2u * kMergeRows, 2u * (P.a.d_weights ? P.R : 0u)) * sizeof(float);
+  cfg.stream = s;
+  cudaLaunchAttribute early{};  // its launch overlaps the attention's end; it waits for it before it reads
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attn_finish<T>, P, n_merge) == cudaSuccess ? VOOM_OK : VOOM_E_CUDA;
 }
 
 }  // namespace

@@ -1,0 +1,185 @@
+// Shared pieces of the cache attention kernels: the call, how its work is cut
+// into steps and spread over the blocks, and the partial results.
+#pragma once
+
+#include <type_traits>
+
+#include "kv_view.cuh"
+
+namespace voom {
+namespace kv {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// Rows: the n new tokens of a request times the g query heads that share a key
+// head, row r = token r / g, head h * g + r % g.  A unit is a block of `rows`
+// rows of one key head of one request; its steps are the tiles of `keys`
+// cached positions, then those of the new tokens.  The blocks of the grid
+// either take one unit each (direct), or equal shares of all units' steps in
+// order, so that a long request is spread over many blocks and short ones
+// share a block; a block then leaves at most two units unfinished, its first
+// and its last, as partial sums in its two slots.
+struct Attn {
+  View c;
+  voom_tree_attention_args a;
+  float* lse;       // B x n x hq: the caller's, or scratch, or NULL
+  float* scores;    // scratch, or NULL: unit rows x score_ld, log2 units
+  float* partial;   // scratch: 2 slots per block, each rows x (ld_o + 2)
+  uint32_t g, R, words;      // query heads per key head, rows, mask words of a row
+  uint32_t keys, rows, ld_o; // tile sizes
+  uint32_t mblocks;          // blocks of rows of a key head
+  uint32_t ctas;             // 0: direct
+  uint32_t score_ld, score_new; // score row length; where the new tokens' scores start
+  float scale2;              // scale * log2(e)
+  uint32_t all_split;        // partial sums even for whole units
+};
+
+struct Seg {
+  uint32_t b, u, s0, s1, steps, len;  // request, unit of it, steps [s0, s1) of `steps`
+  uint64_t at, end;                   // this block's place in the list of steps, and its end
+};
+
+__device__ __forceinline__ uint32_t new_steps(const Attn& P) { return (P.a.n + P.keys - 1) / P.keys; }
+__device__ __forceinline__ uint32_t cache_steps(const Attn& P, uint32_t len) { return (len + P.keys - 1) / P.keys; }
+__device__ __forceinline__ uint32_t units_of(const Attn& P) { return P.c.v.hk * P.mblocks; }
+
+// Steps of all units before request b (warp-collective); b = B: of all.
+__device__ __forceinline__ uint64_t steps_before(const Attn& P, uint32_t b) {
+  uint64_t sum = 0;
+  for (uint32_t i = threadIdx.x & 31u; i < b; i += 32) sum += cache_steps(P, P.c.length(i)) + new_steps(P);
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  return sum * units_of(P);
+}
+
+// First segment of grid block `cta` (warp-collective); false: it has none.
+__device__ __forceinline__ bool first_seg(const Attn& P, uint32_t cta, Seg& s) {
+  const uint32_t U = units_of(P), tail = new_steps(P);
+  if (!P.ctas) {
+    s.b = cta / U;
+    s.u = cta - s.b * U;
+    s.len = P.c.length(s.b);
+    s.steps = s.s1 = cache_steps(P, s.len) + tail;
+    s.s0 = 0;
+    s.at = 0;
+    s.end = s.steps;
+    return s.steps != 0;
+  }
+  const uint64_t total = steps_before(P, P.c.v.B);
+  s.at = total * cta / P.ctas;
+  s.end = total * (cta + 1) / P.ctas;
+  if (s.at >= s.end) return false;
+  uint64_t base = 0;
+  const uint32_t lane = threadIdx.x & 31u;
+  for (uint32_t b0 = 0;; b0 += 32) {
+    const uint32_t b = b0 + lane;
+    const uint64_t mine = b < P.c.v.B ? uint64_t(cache_steps(P, P.c.length(b)) + tail) * U : 0;
+    uint64_t upto = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+      if (int(lane) >= o) upto += x;
+    }
+    const uint32_t hit = __ballot_sync(0xFFFFFFFFu, base + upto > s.at);
+    if (hit) {
+      const int k = __ffs(hit) - 1;
+      s.b = b0 + uint32_t(k);
+      base += __shfl_sync(0xFFFFFFFFu, upto - mine, k);
+      break;
+    }
+    base += __shfl_sync(0xFFFFFFFFu, upto, 31);
+    if (b0 + 32 >= P.c.v.B) return false;  // not reached: at < total
+  }
+  s.len = P.c.length(s.b);
+  s.steps = cache_steps(P, s.len) + tail;
+  s.u = uint32_t((s.at - base) / s.steps);
+  s.s0 = uint32_t(s.at - base - uint64_t(s.u) * s.steps);
+  s.s1 = uint32_t(min(uint64_t(s.steps), s.s0 + (s.end - s.at)));
+  return true;
+}
+
+__device__ __forceinline__ bool next_seg(const Attn& P, Seg& s) {
+  s.at += s.s1 - s.s0;
+  if (s.at >= s.end) return false;
+  if (++s.u == units_of(P)) {
+    s.u = 0;
+    s.b++;
+    s.len = P.c.length(s.b);
+    s.steps = cache_steps(P, s.len) + new_steps(P);
+  }
+  s.s0 = 0;
+  s.s1 = uint32_t(min(uint64_t(s.steps), s.end - s.at));
+  return true;
+}
+
+// The blocks that hold partial sums of a unit whose steps are [at, at + steps)
+// of the list: first .. last, and first's slot is its second one.
+__device__ __forceinline__ void owners(const Attn& P, uint64_t total, uint64_t at, uint32_t steps, uint32_t& first,
+                                       uint32_t& last) {
+  // block c covers [total * c / ctas, total * (c + 1) / ctas)
+  auto holder = [&](uint64_t x) {
+    uint32_t c = uint32_t(x * P.ctas / total);
+    while (total * (c + 1) / P.ctas <= x) c++;
+    while (total * c / P.ctas > x) c--;
+    return c;
+  };
+  first = holder(at);
+  last = holder(at + steps - 1);
+}
+
+__device__ __forceinline__ float* slot_of(const Attn& P, uint32_t slot) {
+  return P.partial + uint64_t(slot) * P.rows * (P.ld_o + 2);
+}
+
+__device__ __forceinline__ bool sees(const Attn& P, uint32_t b, uint32_t i, uint32_t j) {
+  if (!P.a.d_mask) return j <= i;
+  return P.a.d_mask[(uint64_t(b) * P.a.n + i) * P.words + (j >> 5)] >> (j & 31u) & 1u;
+}
+
+// Bits [j0, j0 + 32) of row i's mask.
+__device__ __forceinline__ uint32_t sees32(const Attn& P, uint32_t b, uint32_t i, uint32_t j0) {
+  if (i >= P.a.n || j0 >= P.a.n) return 0u;
+  if (P.a.d_mask) {
+    const uint32_t* m = P.a.d_mask + (uint64_t(b) * P.a.n + i) * P.words;
+    const uint32_t w = j0 >> 5, r = j0 & 31u, lo = __ldg(m + w);
+    if (!r) return lo;
+    return __funnelshift_r(lo, w + 1 < P.words ? __ldg(m + w + 1) : 0u, r);
+  }
+  return i < j0 ? 0u : i - j0 >= 31u ? 0xFFFFFFFFu : (2u << (i - j0)) - 1u;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+
+// 16 bytes to shared memory without a register, or 16 zero bytes.
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16u : 0u) : "memory");
+}
+
+// Any of the eight 16-bit values of a chunk infinite or NaN (exponent all ones).
+template <typename T>
+__device__ __forceinline__ bool odd_values(uint4 c) {
+  const uint32_t m = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;
+  bool bad = false;
+  for (uint32_t w : {c.x, c.y, c.z, c.w}) {
+    const uint32_t e = w & m;
+    bad |= (e & 0xFFFFu) == (m & 0xFFFFu) || (e >> 16) == (m >> 16);
+  }
+  return bad;
+}
+
+}  // namespace kv
+}  // namespace voom
