@@ -655,11 +655,14 @@ typedef struct voom_tree_attention_args {
   const uint32_t* d_mask;
   float* d_weights; /* or NULL */
   const float* d_token_weight; /* B x n contiguous, or NULL */
+  uint32_t* d_status; /* bit 0 set if a wait inside the kernel ran out (reported, never observed); or NULL */
   int64_t q_b, q_t, q_h, kn_b, kn_t, kn_h, vn_b, vn_t, vn_h, o_b, o_t, o_h, w_b, w_h; /* strides, elements */
   uint32_t n, hq;
   float scale;
   uint32_t pad;
 } voom_tree_attention_args;
+/* Scratch (16-byte aligned, contents ignored) of a call; with less of it the
+ * call returns VOOM_E_CAPACITY and launches nothing.  scale > 0. */
 uint64_t voom_tree_attention_scratch_bytes(const voom_kv_view* c, const voom_tree_attention_args* a);
 int voom_tree_attention(const voom_kv_view* c, const voom_tree_attention_args* a, void* d_scratch,
                         uint64_t scratch_bytes, void* stream);

@@ -113,7 +113,10 @@ def run_case(B, n, hq, hk, D, lens, dtype, layout="whole", page=16, kind="tree",
                 d[b, j] = math.nan
     out, lse = kva.tree_attention(d[:, :, :hq], d[:, :, hq:hq + hk], d[:, :, hq + hk:], tree, view, scale=scale,
                                   weights=w, token_weight=None if t is None else t.cuda(), return_lse=True)
+    bare, bare_lse = kva.tree_attention(d[:, :, :hq], d[:, :, hq:hq + hk], d[:, :, hq + hk:], tree, view, scale=scale,
+                                        return_lse=True)
     torch.cuda.synchronize()
+    view.check_status()
     f = D ** -0.5 if scale is None else scale
     for b, x in enumerate(lens):
         o, l, s = oa.attention(qkv[b, :, :hq], qkv[b, :, hq:hq + hk], qkv[b, :, hq + hk:], oa.tree_sees(par[b]),
@@ -121,6 +124,8 @@ def run_case(B, n, hq, hk, D, lens, dtype, layout="whole", page=16, kind="tree",
         big = max(float(v[b].abs().max()), float(qkv[b, :, hq + hk:].abs().max()))
         check(out[b], o, 2 * STEP[dtype] * big, ("out", b))
         check(lse[b], l, 3e-5 * max(1.0, sharp), ("lse", b))
+        check(bare[b], o, 2 * STEP[dtype] * big, ("out without weights", b))
+        check(bare_lse[b], l, 3e-5 * max(1.0, sharp), ("lse without weights", b))
         if weights:
             want = w0[b].double()
             want[:, :x + n] += s
@@ -264,6 +269,9 @@ def test_same_bits_again_streams_and_graph():
             return o, l, w
 
         first = once()
+        bare = kva.tree_attention(*args)
+        for _ in range(3):
+            assert torch.equal(kva.tree_attention(*args), bare)
         for s in (None, torch.cuda.Stream(), None):
             for x, y in zip(once(s), first):
                 assert torch.equal(x, y)
@@ -376,7 +384,7 @@ def test_c_entries_refuse_bad_arguments(built_lib):
     def attn(c, **kw):
         a = TreeAttentionArgs()
         a.q = a.kn = a.vn = a.out = 4096
-        a.n, a.hq = 0, 1
+        a.n, a.hq, a.scale = 0, 1, 0.125
         for x, y in kw.items():
             setattr(a, x, y)
         return built_lib.voom_tree_attention(ctypes.byref(c), ctypes.byref(a), None, 0, None)
@@ -391,6 +399,7 @@ def test_c_entries_refuse_bad_arguments(built_lib):
     assert attn(view(table=4096, offsets=4096)) == -1
     assert attn(view(), q=None) == -1 and attn(view(), q=4100) == -1 and attn(view(), q_t=12) == -1
     assert attn(view(hk=2), hq=3) == -1
+    assert attn(view(), scale=0.0) == -1 and attn(view(), scale=-1.0) == -1 and attn(view(), scale=math.nan) == -1
     assert attn(view(), n=2000, mask=4096) == -3
     assert built_lib.voom_tree_mask(None, 1, 1, None, None, None) == -1
     assert built_lib.voom_tree_mask(4096, 1, 1025, 4096, 4096, None) == -3
@@ -437,6 +446,8 @@ def test_refusals():
         kva.tree_attention(q, kn, vn, kva.DraftTree.chain(1, 2, "cuda"), view)
     with pytest.raises(ValueError, match="do not divide"):
         kva.tree_attention(q[:, :, :3], kn, vn, tree, view)
+    with pytest.raises(ValueError, match="scale"):
+        kva.tree_attention(q, kn, vn, tree, view, scale=-1.0)
     with pytest.raises(ValueError, match="k: "):
         kva.tree_attention(q, kn[:, :, :1], vn, tree, view)
     with pytest.raises(ValueError, match="v: "):

@@ -29,13 +29,23 @@ def stream_ptr(device: torch.device, stream: torch.cuda.Stream | None = None) ->
     return int(s.cuda_stream)
 
 
+def current_index() -> int:
+    """Index of the current device."""
+    return torch._C._cuda_getDevice()
+
+
+def raw_stream(index: int) -> int:
+    """cudaStream_t of the current stream of device `index`."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 class on_stream:
     """`with on_stream(device, stream) as ptr`: inside, `device` is current and
     `stream` (None: the device's current stream) is the current stream, so
     that tensors made there belong to it; `ptr` is its cudaStream_t.  Costs
     nothing where both are current already."""
 
-    __slots__ = ("device", "stream", "ctx")
+    __slots__ = ("device", "stream", "ctx")  # a class, not a generator: it is on the path of one-token calls
 
     def __init__(self, device: torch.device, stream: torch.cuda.Stream | None = None):
         self.device, self.stream, self.ctx = device, stream, None
@@ -47,10 +57,10 @@ class on_stream:
             self.ctx = torch.cuda.stream(self.stream)
             self.ctx.__enter__()
             return int(self.stream.cuda_stream)
-        if torch.cuda.current_device() != self.device.index:
+        if current_index() != self.device.index:
             self.ctx = torch.cuda.device(self.device)
             self.ctx.__enter__()
-        return torch._C._cuda_getCurrentRawStream(self.device.index)
+        return raw_stream(self.device.index)
 
     def __exit__(self, *exc) -> None:
         if self.ctx is not None:

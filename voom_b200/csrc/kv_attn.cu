@@ -5,6 +5,7 @@
 #include <type_traits>
 
 #include "kv_rows.cuh"
+#include "kv_tc.cuh"
 
 namespace {
 
@@ -56,11 +57,13 @@ struct Split {
   uint32_t first, last;  // blocks that hold the unit's partial sums; first > last: none, it is whole
 };
 
-__device__ __forceinline__ Split split_of(const Attn& P, uint32_t b, uint32_t u, uint64_t total, uint64_t before) {
+__device__ __forceinline__ Split split_of(const Attn& P, uint32_t b, uint32_t h, uint32_t m, uint64_t total, uint64_t before) {
   Split s{1, 0};
   if (!P.ctas) return s;
-  const uint32_t steps = voom::kv::cache_steps(P, P.c.length(b)) + voom::kv::new_steps(P);
-  voom::kv::owners(P, total, before + uint64_t(u) * steps, steps, s.first, s.last);
+  const uint32_t len = P.c.length(b), cs = voom::kv::cache_steps(P, len);
+  uint64_t at = before + h * voom::kv::head_steps(P, len);
+  for (uint32_t i = 0; i < m; i++) at += cs + voom::kv::tail_of(P, i);
+  voom::kv::owners(P, total, at, cs + voom::kv::tail_of(P, m), s.first, s.last);
   if (s.first == s.last) s = Split{1, 0};
   return s;
 }
@@ -96,13 +99,13 @@ template <typename T>
 __global__ void __launch_bounds__(256) attn_finish(const __grid_constant__ Attn P, uint32_t n_merge) {
   extern __shared__ float s_row[];  // lse (log2 units) of the key head's rows, then their weights
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, U = voom::kv::units_of(P);
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
   const uint64_t total = P.ctas ? voom::kv::steps_before(P, P.c.v.B) : 0;
   if (blockIdx.x < n_merge) {
     const uint32_t groups = P.rows / kMergeRows, unit = blockIdx.x / groups, r0 = (blockIdx.x - unit * groups) * kMergeRows;
-    const uint32_t b = unit / U, u = unit - b * U, h = u / P.mblocks, row0 = (u - h * P.mblocks) * P.rows;
+    const uint32_t m = unit % P.mblocks, head = unit / P.mblocks, b = head / P.c.v.hk, h = head - b * P.c.v.hk, row0 = m * P.rows;
     if (row0 + r0 >= P.R) return;
-    const Split s = split_of(P, b, u, total, voom::kv::steps_before(P, b));
+    const Split s = split_of(P, b, h, m, total, voom::kv::steps_before(P, b));
     if (s.first > s.last) return;
     if (warp < kMergeRows) {
       const float2 ml = joined(P, s, r0 + warp);
@@ -147,7 +150,7 @@ __global__ void __launch_bounds__(256) attn_finish(const __grid_constant__ Attn 
   const uint64_t before = P.ctas ? voom::kv::steps_before(P, b) : 0;
   for (uint32_t r = warp; r < P.R; r += 8) {
     const uint32_t k = r / P.rows, i = r / P.g, hh = h * P.g + r % P.g;
-    const Split s = split_of(P, b, h * P.mblocks + k, total, before);
+    const Split s = split_of(P, b, h, k, total, before);
     float lse2;
     if (s.first <= s.last) {
       const float2 ml = joined(P, s, r - k * P.rows);
@@ -166,10 +169,12 @@ __global__ void __launch_bounds__(256) attn_finish(const __grid_constant__ Attn 
   const uint32_t end = min(P.score_ld, s0 + kWeightSpan);
   for (uint32_t r = 0; r < P.R; r++) {
     const float lse2 = s_row[r], w = s_w[r];
+    // in a chain, tiles past the row's own token have no scores
+    const uint32_t lim = P.a.d_mask ? end : min(end, P.score_new + r / P.g + 1);
 #pragma unroll
     for (uint32_t k = 0; k < kWeightSpan / 256; k++) {
       const uint32_t s = s0 + k * 256 + tid;
-      if (s < end) got[k] += w * voom::kv::exp2_fast(z[uint64_t(r) * P.score_ld + s] - lse2);
+      if (s < lim) got[k] += w * voom::kv::exp2_fast(z[uint64_t(r) * P.score_ld + s] - lse2);
     }
   }
   float* sums = P.a.d_weights + int64_t(b) * P.a.w_b + int64_t(h) * P.a.w_h;
@@ -216,11 +221,20 @@ uint64_t plan(Attn& P, void* scratch) {
   P.words = (P.a.n + 31) / 32;
   P.scale2 = P.a.scale * voom::kv::kLog2e;
   P.ld_o = c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256;
+  P.tc = -1;
+  if (P.R > (P.ld_o == 256 ? 16u : 32u) && !P.a.d_weights) {
+    P.tc = P.ld_o == 256 ? voom::kv::kSingle : P.R > 128 ? voom::kv::kPair : voom::kv::kAlternate;
+    P.keys = P.tc == voom::kv::kSingle ? 64 : 128;
+    P.rows = P.tc == voom::kv::kPair ? 256 : 128;
+  } else {
   P.keys = voom::kv::row_keys(P.ld_o);
   // 32 rows to a block read the cache once where 16 would read it twice; at
   // head size 256 the output of 32 rows does not fit the registers
   P.rows = P.R > 16 && P.ld_o <= 128 ? 32 : 16;
+  }
   P.mblocks = (P.R + P.rows - 1) / P.rows;
+  P.tails = 0;
+  for (uint32_t m = 0; m < P.mblocks; m++) P.tails += voom::kv::tail_of(P, m);
   const uint64_t units = uint64_t(c.B) * c.hk * P.mblocks;
   const uint32_t steps = (c.max_len + P.keys - 1) / P.keys + (P.a.n + P.keys - 1) / P.keys;
   P.ctas = steps <= 16 ? 0u : uint32_t(min(uint64_t(sm_count()), (units * steps + 7) / 8));
@@ -251,10 +265,26 @@ int launch_rows(const Attn& P, cudaStream_t s) {
   return cudaGetLastError() == cudaSuccess ? VOOM_OK : VOOM_E_CUDA;
 }
 
+template <typename T, int DP, int MODE>
+int launch_tc(const Attn& P, cudaStream_t s) {
+  constexpr uint32_t smem = voom::kv::tc_smem<DP, MODE>();
+  static std::atomic<uint64_t> allowed{0};
+  if (!allow_smem(reinterpret_cast<const void*>(voom::kv::attn_tc<T, DP, MODE>), smem, allowed)) return VOOM_E_CUDA;
+  const uint64_t grid = P.ctas ? P.ctas : uint64_t(P.c.v.B) * P.c.v.hk * P.mblocks;
+  voom::kv::attn_tc<T, DP, MODE><<<uint32_t(grid), voom::kv::Tc<DP, MODE>::THREADS, smem, s>>>(P);
+  return cudaGetLastError() == cudaSuccess ? VOOM_OK : VOOM_E_CUDA;
+}
+
 template <typename T>
 int run(const Attn& P, cudaStream_t s) {
+  using voom::kv::kAlternate;
+  using voom::kv::kPair;
+  using voom::kv::kSingle;
   int rc;
-  if (P.ld_o == 64) rc = P.rows == 16 ? launch_rows<T, 64, 1>(P, s) : launch_rows<T, 64, 2>(P, s);
+  if (P.tc == kSingle) rc = launch_tc<T, 256, kSingle>(P, s);
+  else if (P.tc == kPair) rc = P.ld_o == 64 ? launch_tc<T, 64, kPair>(P, s) : launch_tc<T, 128, kPair>(P, s);
+  else if (P.tc == kAlternate) rc = P.ld_o == 64 ? launch_tc<T, 64, kAlternate>(P, s) : launch_tc<T, 128, kAlternate>(P, s);
+  else if (P.ld_o == 64) rc = P.rows == 16 ? launch_rows<T, 64, 1>(P, s) : launch_rows<T, 64, 2>(P, s);
   else if (P.ld_o == 128) rc = P.rows == 16 ? launch_rows<T, 128, 1>(P, s) : launch_rows<T, 128, 2>(P, s);
   else rc = launch_rows<T, 256, 1>(P, s);
   if (rc != VOOM_OK || (!P.ctas && !P.a.d_weights)) return rc;
@@ -291,7 +321,7 @@ int check(const voom_kv_view* c, const voom_tree_attention_args* a, Attn& P) {
   if (!a || !a->d_q || !a->d_kn || !a->d_vn || !a->d_out) return VOOM_E_INVALID_ARG;
   const int rc = voom::kv::make_view(c, P.c);
   if (rc != VOOM_OK) return rc;
-  if (!a->hq || a->hq % c->hk) return VOOM_E_INVALID_ARG;
+  if (!a->hq || a->hq % c->hk || !(a->scale > 0.0f && a->scale <= 3.0e38f)) return VOOM_E_INVALID_ARG;
   if (a->d_mask && a->n > kMaxTree) return VOOM_E_CAPACITY;
   if (uint64_t(c->max_len) + a->n > 0x7FFFFFFFu || uint64_t(c->B) * a->n * a->hq > 0x7FFFFFFFu) return VOOM_E_UNSUPPORTED;
   if (!rows16(a->d_q, {a->q_b, a->q_t, a->q_h}) || !rows16(a->d_kn, {a->kn_b, a->kn_t, a->kn_h}) ||
@@ -316,8 +346,8 @@ VOOM_API int voom_tree_attention(const voom_kv_view* c, const voom_tree_attentio
   if (rc != VOOM_OK) return rc;
   if (!a->n) return VOOM_OK;
   const uint64_t need = plan(P, d_scratch);
-  if (need && (!d_scratch || (reinterpret_cast<uintptr_t>(d_scratch) & 15u))) return VOOM_E_INVALID_ARG;
   if (bytes < need) return VOOM_E_CAPACITY;
+  if (need && (!d_scratch || (reinterpret_cast<uintptr_t>(d_scratch) & 15u))) return VOOM_E_INVALID_ARG;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return c->type == VOOM_BF16 ? run<__nv_bfloat16>(P, s) : run<__half>(P, s);
 }

@@ -25,45 +25,58 @@ struct Attn {
   voom_tree_attention_args a;
   float* lse;       // B x n x hq: the caller's, or scratch, or NULL
   float* scores;    // scratch, or NULL: unit rows x score_ld, log2 units
-  float* partial;   // scratch: 2 slots per block, each rows x (ld_o + 2)
+  float* partial;   // scratch: 2 slots per block, each rows x ld_o sums, rows x (maximum, sum)
   uint32_t g, R, words;      // query heads per key head, rows, mask words of a row
   uint32_t keys, rows, ld_o; // tile sizes
-  uint32_t mblocks;          // blocks of rows of a key head
+  uint32_t mblocks, tails;   // blocks of rows of a key head; their steps over the new tokens
   uint32_t ctas;             // 0: direct
   uint32_t score_ld, score_new; // score row length; where the new tokens' scores start
   float scale2;              // scale * log2(e)
-  uint32_t all_split;        // partial sums even for whole units
+  int32_t tc;                // tensor-core kernel's mode, or -1: attn_rows
 };
 
 struct Seg {
-  uint32_t b, u, s0, s1, steps, len;  // request, unit of it, steps [s0, s1) of `steps`
-  uint64_t at, end;                   // this block's place in the list of steps, and its end
+  uint32_t b, h, m, s0, s1, steps, len;  // unit (request, key head, block of rows), steps [s0, s1) of `steps`
+  uint64_t at, end;                      // this block's place in the list of steps, and its end
 };
 
-__device__ __forceinline__ uint32_t new_steps(const Attn& P) { return (P.a.n + P.keys - 1) / P.keys; }
-__device__ __forceinline__ uint32_t cache_steps(const Attn& P, uint32_t len) { return (len + P.keys - 1) / P.keys; }
-__device__ __forceinline__ uint32_t units_of(const Attn& P) { return P.c.v.hk * P.mblocks; }
+__host__ __device__ __forceinline__ uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
+
+__device__ __forceinline__ uint32_t cache_steps(const Attn& P, uint32_t len) { return ceil_div(len, P.keys); }
+
+// Steps over the new tokens of the m-th block of rows: in a chain, up to its last token.
+__host__ __device__ __forceinline__ uint32_t tail_of(const Attn& P, uint32_t m) {
+  if (P.a.d_mask) return ceil_div(P.a.n, P.keys);
+  const uint32_t rows = (m + 1) * P.rows;
+  return ceil_div(((rows < P.R ? rows : P.R) - 1) / P.g + 1, P.keys);
+}
+
+// Steps of one key head of a request.
+__device__ __forceinline__ uint64_t head_steps(const Attn& P, uint32_t len) {
+  return uint64_t(P.mblocks) * cache_steps(P, len) + P.tails;
+}
 
 // Steps of all units before request b (warp-collective); b = B: of all.
 __device__ __forceinline__ uint64_t steps_before(const Attn& P, uint32_t b) {
   uint64_t sum = 0;
-  for (uint32_t i = threadIdx.x & 31u; i < b; i += 32) sum += cache_steps(P, P.c.length(i)) + new_steps(P);
+  for (uint32_t i = threadIdx.x & 31u; i < b; i += 32) sum += head_steps(P, P.c.length(i));
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-  return sum * units_of(P);
+  return sum * P.c.v.hk;
 }
 
 // First segment of grid block `cta` (warp-collective); false: it has none.
 __device__ __forceinline__ bool first_seg(const Attn& P, uint32_t cta, Seg& s) {
-  const uint32_t U = units_of(P), tail = new_steps(P);
-  if (!P.ctas) {
+  if (!P.ctas) {  // the units of a request with the most steps first
+    const uint32_t hk = P.c.v.hk, U = hk * P.mblocks, r = cta % U;
     s.b = cta / U;
-    s.u = cta - s.b * U;
+    s.h = r % hk;
+    s.m = P.mblocks - 1 - r / hk;
     s.len = P.c.length(s.b);
-    s.steps = s.s1 = cache_steps(P, s.len) + tail;
+    s.steps = s.s1 = cache_steps(P, s.len) + tail_of(P, s.m);
     s.s0 = 0;
     s.at = 0;
     s.end = s.steps;
-    return s.steps != 0;
+    return true;
   }
   const uint64_t total = steps_before(P, P.c.v.B);
   s.at = total * cta / P.ctas;
@@ -72,8 +85,9 @@ __device__ __forceinline__ bool first_seg(const Attn& P, uint32_t cta, Seg& s) {
   uint64_t base = 0;
   const uint32_t lane = threadIdx.x & 31u;
   for (uint32_t b0 = 0;; b0 += 32) {
+    if (b0 >= P.c.v.B) return false;  // not reached: at < total
     const uint32_t b = b0 + lane;
-    const uint64_t mine = b < P.c.v.B ? uint64_t(cache_steps(P, P.c.length(b)) + tail) * U : 0;
+    const uint64_t mine = b < P.c.v.B ? head_steps(P, P.c.length(b)) * P.c.v.hk : 0;
     uint64_t upto = mine;
     for (int o = 1; o < 32; o <<= 1) {
       const uint64_t x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
@@ -87,25 +101,34 @@ __device__ __forceinline__ bool first_seg(const Attn& P, uint32_t cta, Seg& s) {
       break;
     }
     base += __shfl_sync(0xFFFFFFFFu, upto, 31);
-    if (b0 + 32 >= P.c.v.B) return false;  // not reached: at < total
   }
   s.len = P.c.length(s.b);
-  s.steps = cache_steps(P, s.len) + tail;
-  s.u = uint32_t((s.at - base) / s.steps);
-  s.s0 = uint32_t(s.at - base - uint64_t(s.u) * s.steps);
-  s.s1 = uint32_t(min(uint64_t(s.steps), s.s0 + (s.end - s.at)));
+  const uint32_t cs = cache_steps(P, s.len);
+  const uint64_t per = head_steps(P, s.len);
+  uint64_t off = s.at - base;
+  s.h = uint32_t(off / per);
+  off -= s.h * per;
+  s.m = 0;
+  while (off >= (s.steps = cs + tail_of(P, s.m))) {
+    off -= s.steps;
+    s.m++;
+  }
+  s.s0 = uint32_t(off);
+  s.s1 = uint32_t(min(uint64_t(s.steps), off + (s.end - s.at)));
   return true;
 }
 
 __device__ __forceinline__ bool next_seg(const Attn& P, Seg& s) {
   s.at += s.s1 - s.s0;
   if (s.at >= s.end) return false;
-  if (++s.u == units_of(P)) {
-    s.u = 0;
-    s.b++;
-    s.len = P.c.length(s.b);
-    s.steps = cache_steps(P, s.len) + new_steps(P);
+  if (++s.m == P.mblocks) {
+    s.m = 0;
+    if (++s.h == P.c.v.hk) {
+      s.h = 0;
+      s.len = P.c.length(++s.b);
+    }
   }
+  s.steps = cache_steps(P, s.len) + tail_of(P, s.m);
   s.s0 = 0;
   s.s1 = uint32_t(min(uint64_t(s.steps), s.end - s.at));
   return true;

@@ -113,7 +113,7 @@ __device__ __forceinline__ void load_tile(const Attn& P, const Seg& g, uint32_t 
 template <typename T, int DP, int MT>
 __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_constant__ Attn P) {
   constexpr uint32_t KT = row_keys(DP), CH = DP / 8, NT = KT / 8, DT = DP / 8, LDJ = kJoin, ROWS = 16 * MT;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, quad = lane & 3u, oct = lane >> 2;
   const uint32_t stage0 = smem_addr(smem) + warp * kRowStages * 16384u;
   float* s_join = reinterpret_cast<float*>(smem + kRowWarps * kRowStages * 16384u);  // [warp][16][LDJ]
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
       ps = pg.s0 + warp;
     }
     if (more) {
-      load_tile<T, DP>(P, pg, pg.u / P.mblocks, ps, stage0 + slot * 16384u);
+      load_tile<T, DP>(P, pg, pg.h, ps, stage0 + slot * 16384u);
       ps += kRowWarps;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
 
   uint32_t slot = 0;
   do {
-    const uint32_t h = g.u / P.mblocks, row0 = (g.u - h * P.mblocks) * ROWS, nrows = min(ROWS, P.R - row0);
+    const uint32_t h = g.h, row0 = g.m * ROWS, nrows = min(ROWS, P.R - row0);
     const uint32_t cs = cache_steps(P, g.len);
     // the unit's queries
     for (uint32_t i = tid; i < ROWS * CH; i += 32 * kRowWarps) {
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
           s_l[warp * ROWS + r] = token ? l[t][x] : 0.0f;
         }
       }
-    const bool whole = g.s0 == 0 && g.s1 == g.steps && !P.all_split;
+    const bool whole = g.s0 == 0 && g.s1 == g.steps;
     // a unit that starts in this block and goes on goes to the second slot
     float* part = whole ? nullptr : slot_of(P, 2 * blockIdx.x + (g.s0 == 0 ? 1u : 0u));
 #pragma unroll

@@ -21,16 +21,18 @@ Counterpart in the reference: the attention around its caches
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import NamedTuple
 
 import numpy as np
 import torch
 
 from .. import _device
-from .._lib import ELEMENT_TYPES, KvEvictArgs, KvViewStruct, TreeAttentionArgs, check, load
+from .._lib import VOOM_E_CAPACITY, ELEMENT_TYPES, KvEvictArgs, KvViewStruct, TreeAttentionArgs, check, load
 
 MAX_HEAD_DIM = 256
 MAX_TREE = 1024  # tokens of a tree that is not a chain
+_NO_SCRATCH = (None, 0)
 _CACHE_TYPES = (torch.bfloat16, torch.float16)
 
 
@@ -68,7 +70,13 @@ class KVView:
                                    None if table is None else table.data_ptr(),
                                    None if offsets is None else offsets.data_ptr(), *strides, batch, heads, head_dim,
                                    ELEMENT_TYPES[k.dtype], page, table_stride, n_pages, max_len)
+        self.packed = bytes(self.struct)
+        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self.status_ptr = self.status.data_ptr()
+        self.scale = head_dim ** -0.5
+        self.index = self.device.index
         self._scratch: dict[int, torch.Tensor] = {}
+        self.scratch: dict[int, tuple[int, int]] = {}  # stream -> address, bytes
 
     @classmethod
     def contiguous(cls, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, max_len: int | None = None) -> "KVView":
@@ -129,11 +137,20 @@ class KVView:
                    max_len=P * per if max_len is None else max_len, strides=(0, ks[0], ks[1], 0, vs[0], vs[1]),
                    keep=flat)
 
-    def scratch(self, n: int, stream_ptr: int) -> torch.Tensor:
-        """Workspace of at least n bytes for calls on one stream, kept with the view."""
-        s = self._scratch.get(stream_ptr)
-        if s is None or s.numel() < n:
-            s = self._scratch[stream_ptr] = torch.zeros(n, dtype=torch.uint8, device=self.device)
+    def check_status(self) -> None:
+        """Raises RuntimeError if a wait inside an attention kernel ran out since
+        the last check (its outputs are then not valid); clears the status.
+        Synchronises; calls never do, so callers check where they read results."""
+        if int(self.status.item()):
+            self.status.zero_()
+            raise RuntimeError("tree_attention: a wait inside the kernel ran out")
+
+    def more_scratch(self, n: int, stream_ptr: int) -> tuple[int, int]:
+        """(address, bytes) of a workspace of at least n bytes for the calls on
+        one stream, kept with the view."""
+        t = torch.empty(n, dtype=torch.uint8, device=self.device)
+        self._scratch[stream_ptr] = t
+        s = self.scratch[stream_ptr] = (t.data_ptr(), n)
         return s
 
 
@@ -150,6 +167,7 @@ class DraftTree:
         if parents.shape[1] > MAX_TREE:
             raise ValueError(f"a tree of {parents.shape[1]} tokens: at most {MAX_TREE}")
         self.device = _device.require_cuda(parents.device)
+        self.index = self.device.index
         self.batch, self.n = parents.shape
         with _device.on_stream(self.device, stream) as sp:
             parents = parents.contiguous()
@@ -159,6 +177,7 @@ class DraftTree:
             if parents.numel():
                 check(load().voom_tree_mask(parents.data_ptr(), self.batch, self.n, self.mask.data_ptr(),
                                             self.depth.data_ptr(), sp), "voom_tree_mask")
+        self.mask_ptr = self.mask.data_ptr() if parents.numel() else 0
 
     @classmethod
     def chain(cls, batch: int, n: int, device=None) -> "DraftTree":
@@ -166,6 +185,7 @@ class DraftTree:
         prompt or a chunk of one.  Any length; needs no mask."""
         t = cls.__new__(cls)
         t.device = _device.require_cuda(device)
+        t.index, t.mask_ptr = t.device.index, 0
         t.batch, t.n, t.mask = int(batch), int(n), None
         t.depth = torch.arange(n, dtype=torch.int32, device=t.device).expand(batch, n)
         return t
@@ -175,11 +195,32 @@ class DraftTree:
         return lengths[:, None] + self.depth
 
 
-def _new(x: torch.Tensor, name: str, B: int, n: int, heads: int, cache: KVView) -> None:
-    if x.shape != (B, n, heads, cache.head_dim) or x.dtype != cache.dtype or x.device != cache.device:
+# voom_tree_attention_args and voom_kv_evict_args as bytes: cheaper to make than
+# ctypes structures, and one-token calls are bound by the host
+_ATTN = struct.Struct("9Q14q2If4x")
+_EVICT = struct.Struct("Q2q5Q4I")
+assert _ATTN.size == ctypes.sizeof(TreeAttentionArgs) and _EVICT.size == ctypes.sizeof(KvEvictArgs)
+
+
+def _new(x: torch.Tensor, name: str, B: int, n: int, heads: int, cache: KVView) -> tuple:
+    """Checks a (B, n, heads, D) tensor of new tokens; its first three strides."""
+    s = x.stride()
+    if x.shape != (B, n, heads, cache.head_dim) or x.dtype != cache.dtype or x.get_device() != cache.index:
         raise ValueError(f"{name}: ({B}, {n}, {heads}, {cache.head_dim}) {cache.dtype} on {cache.device} wanted, got "
                          f"{tuple(x.shape)} {x.dtype} on {x.device}")
-    _rows(x, name)
+    if s[3] != 1 or (s[0] | s[1] | s[2]) & 7 or x.data_ptr() & 15:
+        raise ValueError(f"{name}: heads must be contiguous and every row must start on 16 bytes")
+    return s
+
+
+def _sums(weights: torch.Tensor, cache: KVView, positions: int) -> tuple:
+    """Checks the positions' weight sums; their strides."""
+    s = weights.stride()
+    if weights.dim() != 3 or weights.shape[:2] != (cache.batch, cache.heads) or weights.shape[2] < positions or \
+            weights.dtype != torch.float32 or s[2] != 1 or weights.get_device() != cache.index:
+        raise ValueError(f"weights: fp32 ({cache.batch}, {cache.heads}, at least {positions}) on {cache.device} wanted, "
+                         f"got {tuple(weights.shape)} {weights.dtype}")
+    return s
 
 
 def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: DraftTree, cache: KVView, *,
@@ -197,46 +238,51 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: Draf
     summed over the rows that share its head (each times `token_weight` (B, n)
     fp32, if given), is added in place: cached positions at their index, new
     token j at lengths[b] + j.  kv_evict reads these sums."""
+    if stream is not None or _device.current_index() != cache.index:
+        with _device.on_stream(cache.device, stream):
+            return tree_attention(q, k, v, tree, cache, scale=scale, weights=weights, token_weight=token_weight,
+                                  out=out, return_lse=return_lse)
+    if q.dim() != 4:
+        raise ValueError(f"q: (B, n, Hq, D) wanted, got {tuple(q.shape)}")
     B, n, hq, D = q.shape
     heads = cache.heads
-    if B != cache.batch or (B, n) != (tree.batch, tree.n):
+    if B != cache.batch or B != tree.batch or n != tree.n:
         raise ValueError(f"{B} requests of {n} new tokens in q, {tree.batch} of {tree.n} in the tree, {cache.batch} cached")
     if hq % heads or not hq:
         raise ValueError(f"{hq} query heads do not divide into {heads} key heads")
-    _new(q, "q", B, n, hq, cache)
-    _new(k, "k", B, n, heads, cache)
-    _new(v, "v", B, n, heads, cache)
-    if tree.device != cache.device:
+    if scale is not None and not 0.0 < scale < 3e38:
+        raise ValueError(f"scale {scale}: a positive number wanted")
+    qs = _new(q, "q", B, n, hq, cache)
+    ks = _new(k, "k", B, n, heads, cache)
+    vs = _new(v, "v", B, n, heads, cache)
+    if tree.index != cache.index:
         raise ValueError(f"the tree is on {tree.device}, the cache on {cache.device}")
+    wp = wb = wh = tw = 0
     if weights is not None:
-        if weights.dim() != 3 or weights.shape[:2] != (B, heads) or weights.shape[2] < cache.max_len + n or \
-                weights.dtype != torch.float32 or weights.stride(2) != 1 or weights.device != cache.device:
-            raise ValueError(f"weights: fp32 ({B}, {heads}, at least {cache.max_len + n}) on {cache.device} wanted, got "
-                             f"{tuple(weights.shape)} {weights.dtype}")
+        wb, wh, _ = _sums(weights, cache, cache.max_len + n)
+        wp = weights.data_ptr()
     if token_weight is not None:
         if weights is None:
             raise ValueError("token_weight goes with weights")
         if token_weight.shape != (B, n) or token_weight.dtype != torch.float32 or not token_weight.is_contiguous() \
-                or token_weight.device != cache.device:
+                or token_weight.get_device() != cache.index:
             raise ValueError(f"token_weight: contiguous fp32 ({B}, {n}) on {cache.device} wanted")
-    with _device.on_stream(cache.device, stream) as sp:
-        if out is None:
-            out = torch.empty((B, n, hq, D), dtype=q.dtype, device=cache.device)
-        else:
-            _new(out, "out", B, n, hq, cache)
-        lse = torch.empty((B, n, hq), dtype=torch.float32, device=cache.device) if return_lse else None
-        if n:
-            a = TreeAttentionArgs(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
-                None if tree.mask is None else tree.mask.data_ptr(), None if weights is None else weights.data_ptr(),
-                None if token_weight is None else token_weight.data_ptr(), *q.stride()[:3], *k.stride()[:3],
-                *v.stride()[:3], *out.stride()[:3], *(weights.stride()[:2] if weights is not None else (0, 0)), n, hq,
-                D ** -0.5 if scale is None else scale, 0)
-            lib = load()
-            c, ap = ctypes.byref(cache.struct), ctypes.byref(a)
-            need = lib.voom_tree_attention_scratch_bytes(c, ap)
-            s = cache.scratch(need, sp).data_ptr() if need else None
-            check(lib.voom_tree_attention(c, ap, s, need, sp), "voom_tree_attention")
+        tw = token_weight.data_ptr()
+    if out is None:
+        out = q.new_empty((B, n, hq, D))
+    os = _new(out, "out", B, n, hq, cache)
+    lse = q.new_empty((B, n, hq), dtype=torch.float32) if return_lse else None
+    if n:
+        a = _ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+                       tree.mask_ptr, wp, tw, cache.status_ptr, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], os[0],
+                       os[1], os[2], wb, wh, n, hq, cache.scale if scale is None else scale)
+        lib, sp = load(), _device.raw_stream(cache.index)
+        ws = cache.scratch.get(sp, _NO_SCRATCH)
+        rc = lib.voom_tree_attention(cache.packed, a, ws[0], ws[1], sp)
+        if rc == VOOM_E_CAPACITY:  # refused before anything was launched
+            ws = cache.more_scratch(lib.voom_tree_attention_scratch_bytes(cache.packed, a), sp)
+            rc = lib.voom_tree_attention(cache.packed, a, ws[0], ws[1], sp)
+        check(rc, "voom_tree_attention")
     return (out, lse) if return_lse else out
 
 
@@ -258,21 +304,18 @@ def kv_evict(cache: KVView, weights: torch.Tensor, *, budget: int, sinks: int = 
     newest `recent`, and of the others those with the largest `weights` (B,
     heads, >= max_len) fp32 (equal ones: the lower position), each head by
     itself.  Rows past a request's new length are zero."""
+    if stream is not None or _device.current_index() != cache.index:
+        with _device.on_stream(cache.device, stream):
+            return kv_evict(cache, weights, budget=budget, sinks=sinks, recent=recent)
     B, H, D = cache.batch, cache.heads, cache.head_dim
     if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
         raise ValueError(f"a budget of {budget} positions cannot hold {sinks} first and {recent} newest ones")
-    if weights.dim() != 3 or weights.shape[:2] != (B, H) or weights.shape[2] < cache.max_len or \
-            weights.dtype != torch.float32 or weights.stride(2) != 1 or weights.device != cache.device:
-        raise ValueError(f"weights: fp32 ({B}, {H}, at least {cache.max_len}) on {cache.device} wanted, got "
-                         f"{tuple(weights.shape)} {weights.dtype}")
-    dev = cache.device
-    with _device.on_stream(dev, stream) as sp:
-        k = torch.empty((B, H, budget, D), dtype=cache.dtype, device=dev)
-        v = torch.empty((B, H, budget, D), dtype=cache.dtype, device=dev)
-        w = torch.empty((B, H, budget), dtype=torch.float32, device=dev)
-        index = torch.empty((B, H, budget), dtype=torch.int32, device=dev)
-        lengths = torch.empty(B, dtype=torch.int32, device=dev)
-        a = KvEvictArgs(weights.data_ptr(), weights.stride(0), weights.stride(1), k.data_ptr(), v.data_ptr(),
-                        w.data_ptr(), index.data_ptr(), lengths.data_ptr(), budget, sinks, recent, 0)
-        check(load().voom_kv_evict(ctypes.byref(cache.struct), ctypes.byref(a), sp), "voom_kv_evict")
+    wb, wh, _ = _sums(weights, cache, cache.max_len)
+    k, v = cache.k.new_empty((2, B, H, budget, D)).unbind(0)
+    w, index = weights.new_empty((2, B, H, budget)).unbind(0)
+    index = index.view(torch.int32)
+    lengths = cache.lengths.new_empty(B)
+    a = _EVICT.pack(weights.data_ptr(), wb, wh, k.data_ptr(), v.data_ptr(), w.data_ptr(), index.data_ptr(),
+                    lengths.data_ptr(), budget, sinks, recent, 0)
+    check(load().voom_kv_evict(cache.packed, a, _device.raw_stream(cache.index)), "voom_kv_evict")
     return Evicted(k, v, w, index, lengths)

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -88,15 +89,39 @@ class Rotary:
         self.freqs = freqs
         turns = [round(f / (2 * math.pi) * 2 ** 64) % 2 ** 64 for f in freqs]
         self.device = _device.require_cuda(device)
+        self.index = self.device.index
+        self.interleaved = layout == "interleaved"
         self.turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64,
                                   device=self.device)
+        self.turns_ptr = self.turns.data_ptr()
 
 
-def _heads(x: torch.Tensor, name: str, D: int) -> None:
-    if x.dim() != 3 or x.shape[2] != D:
-        raise ValueError(f"{name}: (tokens, heads, {D}) wanted, got {tuple(x.shape)}")
-    if x.stride(2) != 1 and x.numel():
-        raise ValueError(f"{name}: the values of a head must be contiguous")
+# voom_qk_norm_rope_args as bytes: a packed call costs a third of filling a
+# ctypes structure, and one-token calls are bound by the host
+_ARGS = struct.Struct("8Q8q10I2f")
+assert _ARGS.size == ctypes.sizeof(QkNormRopeArgs)
+
+
+def _refuse(q, k, positions, rotary, q_weight, k_weight) -> None:
+    """Raises what is wrong with the arguments of qk_norm_rope."""
+    D, dev = rotary.head_dim, rotary.device
+    for name, x in (("q", q), ("k", k)):
+        if x.dim() != 3 or x.shape[2] != D:
+            raise ValueError(f"{name}: (tokens, heads, {D}) wanted, got {tuple(x.shape)}")
+        if x.stride(2) != 1 and x.numel():
+            raise ValueError(f"{name}: the values of a head must be contiguous")
+    if q.dtype not in ELEMENT_TYPES or k.dtype != q.dtype:
+        raise ValueError(f"q and k must both be BF16, FP16 or FP32, got {q.dtype} and {k.dtype}")
+    if k.shape[0] != q.shape[0] or positions.shape != (q.shape[0],):
+        raise ValueError(f"{q.shape[0]} tokens in q, {k.shape[0]} in k, positions {tuple(positions.shape)}")
+    if positions.dtype not in (torch.int64, torch.int32) or not positions.is_contiguous():
+        raise ValueError("positions must be contiguous int32 or int64")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (w.shape != (D,) or w.dtype not in ELEMENT_TYPES or not w.is_contiguous() or w.device != dev):
+            raise ValueError(f"{name}: {D} contiguous BF16, FP16 or FP32 weights on {dev} wanted")
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise ValueError("q_weight and k_weight must have one type")
+    raise ValueError(f"q, k, positions and the outputs must be on the rotary plan's device {dev}")
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rotary: Rotary, *,
@@ -109,43 +134,54 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rota
     int64).  BF16, FP16 or FP32; any token and head strides, so q and k may be
     views of a fused projection.  `out_q` / `out_k` may be views of a cache, or q
     and k themselves.  fp32 arithmetic, one rounding."""
-    T, hq, D = q.shape
-    _heads(q, "q", rotary.head_dim)
-    _heads(k, "k", rotary.head_dim)
-    dt = q.dtype
-    if dt not in ELEMENT_TYPES or k.dtype != dt:
-        raise ValueError(f"q and k must both be BF16, FP16 or FP32, got {q.dtype} and {k.dtype}")
-    if k.shape[0] != T or positions.shape != (T,):
-        raise ValueError(f"{T} tokens in q, {k.shape[0]} in k, positions {tuple(positions.shape)}")
-    if positions.dtype not in (torch.int64, torch.int32) or not positions.is_contiguous():
-        raise ValueError("positions must be contiguous int32 or int64")
-    dev = rotary.device
-    w_type = None
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is None:
-            continue
-        if w.shape != (D,) or w.dtype not in ELEMENT_TYPES or not w.is_contiguous() or w.device != dev:
-            raise ValueError(f"{name}: {D} contiguous BF16, FP16 or FP32 weights on {dev} wanted")
-        if w_type is not None and w.dtype != w_type:
-            raise ValueError("q_weight and k_weight must have one type")
-        w_type = w.dtype
-    with _device.on_stream(dev, stream) as sp:
-        if out_q is None:
-            out_q = torch.empty((T, hq, D), dtype=dt, device=dev)
-        if out_k is None:
-            out_k = torch.empty((T, k.shape[1], D), dtype=dt, device=dev)
-        for name, x, like in (("out_q", out_q, q), ("out_k", out_k, k)):
-            if x.shape != like.shape or x.dtype != dt or (x.stride(2) != 1 and x.numel()):
-                raise ValueError(f"{name}: {tuple(like.shape)} {dt} with contiguous heads wanted")
-        if not (q.device == k.device == positions.device == out_q.device == out_k.device == dev):
-            raise ValueError(f"q, k, positions and the outputs must be on the rotary plan's device {dev}")
-        a = QkNormRopeArgs(
-            q.data_ptr(), k.data_ptr(), out_q.data_ptr(), out_k.data_ptr(),
-            None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
-            positions.data_ptr(), rotary.turns.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1),
-            out_q.stride(0), out_q.stride(1), out_k.stride(0), out_k.stride(1), T, hq, k.shape[1], D, rotary.rot_dim,
-            ELEMENT_TYPES[dt], 0 if w_type is None else ELEMENT_TYPES[w_type], positions.dtype == torch.int64,
-            rotary.layout == "interleaved", zero_centered, eps, rotary.factor)
-        if T:
-            check(load().voom_qk_norm_rope(ctypes.byref(a), sp), "voom_qk_norm_rope")
+    if stream is not None or _device.current_index() != rotary.index:
+        with _device.on_stream(rotary.device, stream):
+            return qk_norm_rope(q, k, positions, rotary, q_weight=q_weight, k_weight=k_weight, eps=eps,
+                                zero_centered=zero_centered, out_q=out_q, out_k=out_k)
+    D, at, dt = rotary.head_dim, rotary.index, q.dtype
+    kind = ELEMENT_TYPES.get(dt)
+    if q.dim() != 3 or k.dim() != 3 or kind is None or k.dtype != dt:
+        _refuse(q, k, positions, rotary, q_weight, k_weight)
+    (T, hq, dq), (tk, hk, dk), (qt, qh, qd), (kt, kh, kd) = q.shape, k.shape, q.stride(), k.stride()
+    pt = positions.dtype
+    if not (dq == dk == D and tk == T and positions.shape == (T,) and positions.is_contiguous()
+            and (pt is torch.int64 or pt is torch.int32) and (qd == kd == 1 or not T * hq * hk)
+            and q.get_device() == k.get_device() == positions.get_device() == at):
+        _refuse(q, k, positions, rotary, q_weight, k_weight)
+    w_type = qw = kw = 0
+    if q_weight is not None or k_weight is not None:
+        for w in (q_weight, k_weight):
+            if w is not None and (w.shape != (D,) or w.dtype not in ELEMENT_TYPES or not w.is_contiguous()
+                                  or w.get_device() != at):
+                _refuse(q, k, positions, rotary, q_weight, k_weight)
+        if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+            _refuse(q, k, positions, rotary, q_weight, k_weight)
+        w_type = ELEMENT_TYPES[(k_weight if q_weight is None else q_weight).dtype]
+        qw = 0 if q_weight is None else q_weight.data_ptr()
+        kw = 0 if k_weight is None else k_weight.data_ptr()
+    if out_q is None:
+        out_q = q.new_empty((T, hq, D))
+        qot, qoh = hq * D, D
+    else:
+        qot, qoh = _output(out_q, q, "out_q", at)
+    if out_k is None:
+        out_k = k.new_empty((T, hk, D))
+        kot, koh = hk * D, D
+    else:
+        kot, koh = _output(out_k, k, "out_k", at)
+    if T:
+        check(load().voom_qk_norm_rope(
+            _ARGS.pack(q.data_ptr(), k.data_ptr(), out_q.data_ptr(), out_k.data_ptr(), qw, kw, positions.data_ptr(),
+                       rotary.turns_ptr, qt, qh, kt, kh, qot, qoh, kot, koh, T, hq, hk, D, rotary.rot_dim, kind,
+                       w_type, pt is torch.int64, rotary.interleaved, zero_centered, eps, rotary.factor),
+            _device.raw_stream(at)), "voom_qk_norm_rope")
     return out_q, out_k
+
+
+def _output(x: torch.Tensor, like: torch.Tensor, name: str, device: int) -> tuple[int, int]:
+    """Token and head strides of a caller's output."""
+    if x.shape != like.shape or x.dtype != like.dtype or (x.stride(2) != 1 and x.numel()):
+        raise ValueError(f"{name}: {tuple(like.shape)} {like.dtype} with contiguous heads wanted")
+    if x.get_device() != device:
+        raise ValueError(f"{name} must be on the rotary plan's device")
+    return x.stride(0), x.stride(1)
