@@ -595,7 +595,7 @@ typedef struct voom_qk_norm_rope_args {
   const void* d_q_w;  /* D weights, or NULL */
   const void* d_k_w;
   const void* d_pos;  /* T positions, i32 or i64 */
-  const uint64_t* d_turns; /* rot / 2 */
+  const uint64_t* d_turns; /* rot / 2, 16-byte aligned */
   int64_t q_token, q_head, k_token, k_head;     /* input strides */
   int64_t qo_token, qo_head, ko_token, ko_head; /* output strides */
   uint32_t T, hq, hk, D, rot;
