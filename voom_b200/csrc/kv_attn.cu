@@ -212,6 +212,50 @@ bool allow_smem(const void* kernel, uint32_t bytes, std::atomic<uint64_t>& devic
   return true;
 }
 
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) != cudaSuccess || r != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      return EncodeTiled(nullptr);
+    }
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+// Tensor maps of the cache, where TMA can read it: in one piece, or pages of a
+// pool whose size is a multiple of 8 positions (a swizzled tile's row groups).
+void map_cache(Attn& P) {
+  const voom_kv_view& c = P.c.v;
+  P.box = 0;
+  if (c.d_offsets) return;
+  uint32_t box = P.keys;
+  if (c.d_table)
+    while (box >= 8 && c.page % box) box /= 2;
+  if (box < 8 || !encode_tiled()) return;
+  const cuuint64_t dims[4] = {c.D, c.page, c.hk, c.d_table ? c.n_pages : c.B};
+  const cuuint32_t size[4] = {64, box, 1, 1}, ones[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType type = c.type == VOOM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  auto one = [&](CUtensorMap& map, const void* base, int64_t pos, int64_t head, int64_t page) {
+    // a stride that is never used may be anything: TMA wants a positive one
+    auto bytes = [](int64_t s, uint64_t n) { return n > 1 ? s * 2 : 16; };
+    for (int64_t s : {bytes(pos, dims[1]), bytes(head, dims[2]), bytes(page, dims[3])})
+      if (s <= 0 || s >= (int64_t(1) << 40)) return false;
+    const cuuint64_t strides[3] = {cuuint64_t(bytes(pos, dims[1])), cuuint64_t(bytes(head, dims[2])), cuuint64_t(bytes(page, dims[3]))};
+    return dims[3] > 0 &&
+           encode_tiled()(&map, type, 4, const_cast<void*>(base), dims, strides, size, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (one(P.k_map, c.d_k, c.k_pos, c.k_head, c.k_page) && one(P.v_map, c.d_v, c.v_pos, c.v_head, c.v_page)) P.box = box;
+}
+
 // Tiles, grid and scratch of a call.  Returns the scratch bytes; sets the
 // pointers where `scratch` is given.
 uint64_t plan(Attn& P, void* scratch) {
@@ -276,11 +320,12 @@ int launch_tc(const Attn& P, cudaStream_t s) {
 }
 
 template <typename T>
-int run(const Attn& P, cudaStream_t s) {
+int run(Attn& P, cudaStream_t s) {
   using voom::kv::kAlternate;
   using voom::kv::kPair;
   using voom::kv::kSingle;
   int rc;
+  if (P.tc >= 0) map_cache(P);
   if (P.tc == kSingle) rc = launch_tc<T, 256, kSingle>(P, s);
   else if (P.tc == kPair) rc = P.ld_o == 64 ? launch_tc<T, 64, kPair>(P, s) : launch_tc<T, 128, kPair>(P, s);
   else if (P.tc == kAlternate) rc = P.ld_o == 64 ? launch_tc<T, 64, kAlternate>(P, s) : launch_tc<T, 128, kAlternate>(P, s);

@@ -2,6 +2,8 @@
 // into steps and spread over the blocks, and the partial results.
 #pragma once
 
+#include <cuda.h>
+
 #include <type_traits>
 
 #include "kv_view.cuh"
@@ -20,7 +22,9 @@ constexpr float kLn2 = 0.6931471805599453f;
 // order, so that a long request is spread over many blocks and short ones
 // share a block; a block then leaves at most two units unfinished, its first
 // and its last, as partial sums in its two slots.
-struct Attn {
+struct alignas(64) Attn {
+  CUtensorMap k_map, v_map;  // the cache (head values, positions, heads, pages or requests), boxes of 64 values x `box` positions
+  uint32_t box;              // 0: the cache cannot be read with TMA
   View c;
   voom_tree_attention_args a;
   float* lse;       // B x n x hq: the caller's, or scratch, or NULL
@@ -174,6 +178,32 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two fp32 values in a register pair: one instruction works on both.
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 make2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void take2(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {

@@ -29,12 +29,14 @@ struct Tc {
   static constexpr uint32_t KT = MODE == kSingle ? 64 : 128;       // keys of a tile
   static constexpr uint32_t ROWS = MODE == kPair ? 256 : 128;      // rows of a unit
   static constexpr uint32_t WGS = MODE == kSingle ? 1 : 2;         // softmax warpgroups
-  static constexpr uint32_t THREADS = WGS * 128 + 128 + 32;
+  // two softmax warpgroups: a full fourth one with the issuing warp, so that
+  // registers can be moved to the softmax, whose threads hold a row of S
+  static constexpr uint32_t THREADS = WGS * 128 + 128 + (WGS == 2 ? 128 : 32);
+  static constexpr uint32_t MORE = 192, LESS = 64;                 // 2 x 128 x 192 + 2 x 128 x 64 = 512 x 128
   static constexpr uint32_t TILE = KT * DP * 2;                    // bytes of a tile of keys or values
   static constexpr uint32_t QTILE = 128 * DP * 2;
   static constexpr uint32_t Q = (ROWS / 128) * QTILE;
   static constexpr uint32_t RING = (224 * 1024 - Q) / TILE;        // tiles in flight or in use
-  static constexpr uint32_t LAG = RING >= 8 ? 4 : 2;               // tiles a loader keeps unfinished
   static constexpr uint32_t O_COL = 256;                           // TMEM columns: S at 0 and S_COL, then O
   static constexpr uint32_t S_COL = 128;
 };
@@ -51,7 +53,7 @@ struct TcShared {
 template <int DP, int MODE>
 constexpr uint32_t tc_smem() {
   constexpr uint32_t n = Tc<DP, MODE>::Q + Tc<DP, MODE>::RING * Tc<DP, MODE>::TILE + uint32_t(sizeof(TcShared));
-  static_assert(n <= 227 * 1024 && Tc<DP, MODE>::RING <= 16 && Tc<DP, MODE>::RING > Tc<DP, MODE>::LAG, "shared memory of a block");
+  static_assert(n <= 227 * 1024 && Tc<DP, MODE>::RING <= 16 && Tc<DP, MODE>::RING >= 3, "shared memory of a block");
   return n;
 }
 
@@ -65,7 +67,7 @@ __device__ __forceinline__ uint32_t sw128(uint32_t r, uint32_t c, uint32_t rows)
 // probability of 0 must not meet them); this adds them back for a row that
 // sees them, one at a time: y[0..32) are the row's sums of values col ..
 template <typename T>
-__device__ __noinline__ void odd_fix(const Attn& P, const Seg& g, uint32_t row, float m2, uint32_t col, float* y) {
+__device__ __forceinline__ void odd_fix(const Attn& P, const Seg& g, uint32_t row, float m2, uint32_t col, float* y) {
   const uint32_t cs = cache_steps(P, g.len), i = row / P.g;
   const uint32_t j0 = (max(g.s0, cs) - cs) * P.keys, j1 = g.s1 > cs ? min(P.a.n, (g.s1 - cs) * P.keys) : 0u;
   const T* q = static_cast<const T*>(P.a.d_q) + int64_t(g.b) * P.a.q_b + int64_t(i) * P.a.q_t +
@@ -79,6 +81,7 @@ __device__ __noinline__ void odd_fix(const Attn& P, const Seg& g, uint32_t row, 
       if (p < 0.0f) {
         const T* k = static_cast<const T*>(P.a.d_kn) + int64_t(g.b) * P.a.kn_b + int64_t(j) * P.a.kn_t + int64_t(g.h) * P.a.kn_h;
         float z = 0.0f;
+        #pragma unroll 1
         for (uint32_t d = 0; d < P.c.v.D; d++) z += elem<T>(q[d]) * elem<T>(k[d]);
         p = exp2_fast(z * P.scale2 - m2);
       }
@@ -90,7 +93,7 @@ __device__ __noinline__ void odd_fix(const Attn& P, const Seg& g, uint32_t row, 
 template <typename T, int DP, int MODE>
 __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid_constant__ Attn P) {
   using C = Tc<DP, MODE>;
-  constexpr uint32_t KT = C::KT, ROWS = C::ROWS, CH = DP / 8, RING = C::RING, LAG = C::LAG;
+  constexpr uint32_t KT = C::KT, ROWS = C::ROWS, CH = DP / 8, RING = C::RING;
   extern __shared__ __align__(1024) uint8_t smem[];
   TcShared& sh = *reinterpret_cast<TcShared*>(smem + C::Q + RING * C::TILE);
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
@@ -127,61 +130,38 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = sh.tmem;
-
   if (any && warp >= LOAD_WARP && warp < MMA_WARP) {
     // ------------------------------------------------------------- loaders
+    if (C::WGS == 2) tc::regs_less<C::LESS>();
     constexpr uint32_t RW = KT / 4;  // rows of a tile to a warp
     const uint32_t pw = warp - LOAD_WARP;
-    uint32_t it = 0, nq = 0, pend = 0;  // tiles issued, query tiles issued, issued and not yet announced
-    uint32_t hist[LAG];                 // what each was: ring place, | 64: queries, | 128: new tokens' values
-#pragma unroll
-    for (uint32_t i = 0; i < LAG; i++) hist[i] = 0;
+    uint32_t it = 0, nq = 0;  // tiles and query tiles asked for
     bool ok = true;
-    // announces a tile whose copies have landed
-    auto announce = [&](uint32_t what) {
-      const uint32_t place = what & 63u;
-      if (what & 128u) {
-        const uint32_t base = C::Q + place * C::TILE;
-        bool found = false;
-        for (uint32_t k = 0; k < RW * CH / 32; k++) {
-          const uint32_t id = k * 32 + lane, r = pw * RW + id / CH;
-          uint4* at = reinterpret_cast<uint4*>(smem + base + sw128(r, id % CH, KT));
-          if (odd_values<T>(*at)) {
-            *at = make_uint4(0, 0, 0, 0);
-            found = true;
-          }
+    // A tile of cached positions that are all valid comes by TMA, one box for
+    // each run of positions in a page: the lanes of the first warp find the
+    // pages.  Others (the end of a cache, new tokens, caches that TMA cannot
+    // read) are gathered through cp.async; their barrier hears of the copies as
+    // they land, and the issuing thread fences them for the tensor cores.  The
+    // gather alone took 1500 cycles to a tile, with a page table 3000, against
+    // 1024 that its matrix products take.
+    // New tokens' values are looked through first: those that are not finite
+    // are taken out, whatever probability they meet.
+    auto look_through = [&](uint32_t place) {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      bool found = false;
+      for (uint32_t k = 0; k < RW * CH / 32; k++) {
+        const uint32_t id = k * 32 + lane, r = pw * RW + id / CH;
+        uint4* at = reinterpret_cast<uint4*>(smem + C::Q + place * C::TILE + sw128(r, id % CH, KT));
+        if (odd_values<T>(*at)) {
+          *at = make_uint4(0, 0, 0, 0);
+          found = true;
         }
-        if (found) sh.odd = 1;
       }
-      tc::fence_async_smem();
-      tc::mbar_arrive(what & 64u ? bar(sh.q_full) : bar(sh.full[place]));
-    };
-    auto issued = [&](uint32_t what) {
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      if (pend == LAG) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(LAG) : "memory");
-        announce(hist[0]);
-#pragma unroll
-        for (uint32_t i = 0; i + 1 < LAG; i++) hist[i] = hist[i + 1];
-        hist[LAG - 1] = what;
-      } else {
-#pragma unroll
-        for (uint32_t i = 0; i < LAG; i++)
-          if (i == pend) hist[i] = what;
-        pend++;
-      }
-    };
-    auto flush = [&]() {
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-#pragma unroll
-      for (uint32_t i = 0; i < LAG; i++)
-        if (i < pend) announce(hist[i]);
-      pend = 0;
+      if (found) sh.odd = 1;
     };
     do {
       const uint32_t row0 = g.m * ROWS, cs = cache_steps(P, g.len), n = g.s1 - g.s0;
       if (nq) {  // the last segment's products of the queries must be done
-        flush();
         if (!(ok = warp_wait(sh.q_empty, (nq - 1) & 1u))) break;
       }
 #pragma unroll 1
@@ -200,7 +180,7 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
         }
       }
       nq++;
-      issued(64u);
+      tc::mbar_arrive_copies(bar(sh.q_full));
       for (uint32_t x = 0; x < 2 * n; x++) {
         // order of use: K0 V0 K1 V1 .. for kPair, K0 K1 V0 K2 V1 .. else
         bool is_v;
@@ -215,6 +195,27 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
         const uint32_t step = g.s0 + j, place = it % RING;
         if (it >= RING && !(ok = warp_wait(sh.empty[place], (it / RING - 1) & 1u))) break;
         const bool fresh = step >= cs;
+        if (P.box && step * KT + KT <= g.len) {
+          if (pw == 0) {
+            if (lane == 0) tc::mbar_arrive_expect(bar(sh.full[place]), C::TILE);
+            else tc::mbar_arrive(bar(sh.full[place]));
+            __syncwarp();
+            if (lane < KT / P.box) {
+              const uint32_t s = step * KT + lane * P.box, pg = P.c.page_of(s);
+              const int32_t w = P.c.v.d_table ? __ldg(P.c.v.d_table + uint64_t(g.b) * P.c.v.table_stride + pg) : int32_t(g.b);
+              const uint32_t y = P.c.v.d_table ? s - pg * P.c.v.page : s;
+              const void* map = is_v ? &P.v_map : &P.k_map;
+#pragma unroll
+              for (uint32_t x = 0; x < DP; x += 64)
+                tc::tma_load4(ring_s + place * C::TILE + (x / 64) * (KT * 128u) + lane * P.box * 128u, map, bar(sh.full[place]),
+                              int32_t(x), int32_t(y), int32_t(g.h), w);
+            }
+          } else {
+            tc::mbar_arrive(bar(sh.full[place]));
+          }
+          it++;
+          continue;
+        }
         uint64_t a = 0;
         if (lane < RW) {
           const uint32_t r = pw * RW + lane;
@@ -242,66 +243,87 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
           cp16(dst + sw128(pw * RW + r, c, KT), in ? reinterpret_cast<const void*>(y + 16 * c) : P.c.v.d_k, in);
         }
         it++;
-        issued(place | (fresh && is_v ? 128u : 0u));
+        if (fresh && is_v) {
+          look_through(place);
+          tc::mbar_arrive(bar(sh.full[place]));
+        } else {
+          tc::mbar_arrive_copies(bar(sh.full[place]));
+        }
       }
     } while (ok && next_seg(P, g));
-    flush();
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (!ok) sh.failed = 1;
-  } else if (any && warp == MMA_WARP && lane == 0) {
+  } else if (any && warp >= MMA_WARP) {
     // ------------------------------------------------ the tensor cores' orders
+    if (C::WGS == 2) tc::regs_less<C::LESS>();
+    if (warp == MMA_WARP) {
     constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     constexpr uint32_t base = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 4) << 24);
     constexpr uint32_t id_qk = base | ((KT >> 3) << 17), id_pv = base | ((uint32_t(DP) >> 3) << 17) | (1u << 16);
     uint32_t it = 0, nq = 0, np[2] = {0, 0};  // tiles, query tiles and probabilities used so far
     bool ok = true;
+    const bool one = tc::elect_one();  // the whole warp goes along; one lane issues
+    const uint32_t tm = tc::uniform(tmem), q_lo = (q_s >> 4) | (1u << 16), ring_lo = (ring_s >> 4);
     auto wait = [&](const uint64_t& b, uint32_t parity) {
-      if (ok && !tc::mbar_wait(bar(b), parity)) ok = false;
+      if (ok) ok = warp_wait(b, parity);
       tc::tc_fence_after();
     };
-    auto wait_tile = [&](uint32_t i) { wait(sh.full[i % RING], (i / RING) & 1u); };
-    auto tile_at = [&](uint32_t i) { return ring_s + (i % RING) * C::TILE; };
+    auto wait_tile = [&](uint32_t i) {
+      wait(sh.full[i % RING], (i / RING) & 1u);
+      tc::fence_async_smem();  // what the loaders copied, for the tensor cores
+    };
+    auto commit = [&](const uint64_t& b) {
+      if (one) tc::umma_commit(bar(b));
+    };
+    auto tile_at = [&](uint32_t i) { return ring_lo + (i % RING) * (C::TILE >> 4); };  // in 16-byte units
     auto qk = [&](uint32_t slot, uint32_t qt, uint32_t k_at) {
+      const uint32_t a = q_lo + qt * (C::QTILE >> 4), b = k_at | (1u << 16), d = tm + slot * C::S_COL;
+      if (one) {
 #pragma unroll
-      for (uint32_t k = 0; k < DP / 16; k++)
-        tc::umma_bf16(tmem + slot * C::S_COL, tc::umma_desc_sw128(q_s + qt * C::QTILE + (k / 4) * 16384u + (k % 4) * 32u, 16u),
-                      tc::umma_desc_sw128(k_at + (k / 4) * (KT * 128u) + (k % 4) * 32u, 16u), id_qk, k > 0);
-      tc::umma_commit(bar(sh.s_full[slot]));
+        for (uint32_t k = 0; k < DP / 16; k++)
+          tc::umma_bf16(d, tc::umma_desc_at(a + (k / 4) * 1024u + (k % 4) * 2u, tc::kDescHiSw128),
+                        tc::umma_desc_at(b + (k / 4) * (KT * 8u) + (k % 4) * 2u, tc::kDescHiSw128), id_qk, k > 0);
+        tc::umma_commit(bar(sh.s_full[slot]));
+      }
     };
     auto pv = [&](uint32_t slot, uint32_t o_col, uint32_t v_at, bool first) {
       wait(sh.p_ready[slot], np[slot]++ & 1u);
       if (!ok) return;
+      const uint32_t b = v_at | (KT * 8u) << 16, d = tm + o_col, a = tm + slot * C::S_COL;
+      if (one) {
 #pragma unroll
-      for (uint32_t k = 0; k < KT / 16; k++)
-        tc::umma_f16_ts(tmem + o_col, tmem + slot * C::S_COL + k * 8u, tc::umma_desc_sw128(v_at + k * 2048u, KT * 128u), id_pv,
-                        !first || k > 0);
+        for (uint32_t k = 0; k < KT / 16; k++)
+          tc::umma_f16_ts(d, a + k * 8u, tc::umma_desc_at(b + k * 128u, tc::kDescHiSw128), id_pv, !first || k > 0);
+      }
     };
     do {
-      const uint32_t n = g.s1 - g.s0, i0 = it;
+      const uint32_t n = tc::uniform(g.s1 - g.s0), i0 = it;
       wait(sh.q_full, nq++ & 1u);
+      tc::fence_async_smem();
       if (MODE == kPair) {
         wait_tile(i0);
         if (!ok) break;
         qk(0, 0, tile_at(i0));
         qk(1, 1, tile_at(i0));
-        tc::umma_commit(bar(sh.empty[i0 % RING]));
-        if (n == 1) tc::umma_commit(bar(sh.q_empty));
+        commit(sh.empty[i0 % RING]);
+        if (n == 1) commit(sh.q_empty);
         for (uint32_t j = 0; j < n && ok; j++) {
           const uint32_t v = i0 + 2 * j + 1, k = v + 1;
           for (uint32_t t = 0; t < 2; t++) {
             if (t == 0) wait_tile(v);
             pv(t, C::O_COL + t * DP, tile_at(v), j == 0);
             if (!ok) break;
-            if (t == 1) tc::umma_commit(bar(sh.empty[v % RING]));
+            if (t == 1) commit(sh.empty[v % RING]);
             if (j + 1 < n) {
               if (t == 0) wait_tile(k);
               if (!ok) break;
               qk(t, t, tile_at(k));
               if (t == 1) {
-                tc::umma_commit(bar(sh.empty[k % RING]));
-                if (j + 2 == n) tc::umma_commit(bar(sh.q_empty));
+                commit(sh.empty[k % RING]);
+                if (j + 2 == n) commit(sh.q_empty);
               }
             } else {
-              tc::umma_commit(bar(sh.o_full[t]));
+              commit(sh.o_full[t]);
             }
           }
         }
@@ -312,34 +334,36 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
           wait_tile(k);
           if (!ok) break;
           qk(i, 0, tile_at(k));
-          tc::umma_commit(bar(sh.empty[k % RING]));
-          if (i + 1 == n) tc::umma_commit(bar(sh.q_empty));
+          commit(sh.empty[k % RING]);
+          if (i + 1 == n) commit(sh.q_empty);
         }
         for (uint32_t i = 0; i < n && ok; i++) {
           const uint32_t t = i & 1u, v = i0 + (i + 1 == n ? 2 * n - 1 : 2 * i + 2);
           wait_tile(v);
           pv(t, C::O_COL + (MODE == kAlternate ? t * DP : 0u), tile_at(v), MODE == kAlternate ? i < 2 : i == 0);
           if (!ok) break;
-          tc::umma_commit(bar(sh.empty[v % RING]));
-          if (MODE == kSingle) tc::umma_commit(bar(sh.pv_done));
+          commit(sh.empty[v % RING]);
+          if (MODE == kSingle) commit(sh.pv_done);
           if (i + 2 < n) {
             const uint32_t k = i0 + 2 * (i + 2) - 1;
             wait_tile(k);
             if (!ok) break;
             qk(t, 0, tile_at(k));
-            tc::umma_commit(bar(sh.empty[k % RING]));
-            if (i + 3 == n) tc::umma_commit(bar(sh.q_empty));
+            commit(sh.empty[k % RING]);
+            if (i + 3 == n) commit(sh.q_empty);
           }
-          if (MODE == kAlternate ? i + 2 >= n : i + 1 == n) tc::umma_commit(bar(sh.o_full[MODE == kAlternate ? t : 0]));
+          if (MODE == kAlternate ? i + 2 >= n : i + 1 == n) commit(sh.o_full[MODE == kAlternate ? t : 0]);
         }
       }
       it += 2 * n;
     } while (ok && next_seg(P, g));
-    tc::umma_commit(bar(sh.drained));  // nothing may be under way when TMEM is given back
-    if (!tc::mbar_wait(bar(sh.drained), 0)) ok = false;
+    commit(sh.drained);  // nothing may be under way when TMEM is given back
+    if (!warp_wait(sh.drained, 0)) ok = false;
     if (!ok) sh.failed = 1;
+    }
   } else if (any && warp < LOAD_WARP) {
     // ------------------------------------------------------------- softmax
+    if (C::WGS == 2) tc::regs_more<C::MORE>();
     const uint32_t w = warp >> 2, tr = tid & 127u, lanes = (warp & 3u) << 21;  // TMEM lane 32 * (warp % 4)
     uint32_t ns[2] = {0, 0}, no[2] = {0, 0}, done = 0, nj = 0;  // S tiles, finished outputs, steps, joins so far
     bool ok = true;
@@ -366,20 +390,25 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
             }
           }
         }
-        float top = -INFINITY;
+        uint32_t s[KT / 32][32];
 #pragma unroll
-        for (uint32_t c = 0; c < KT / 32; c++) {
-          uint32_t s[32];
-          tc::tmem_ld32(s_at + 32 * c, s);
-          tc::tmem_wait_ld();
-          if (masked) {
+        for (uint32_t c = 0; c < KT / 32; c++) tc::tmem_ld32(s_at + 32 * c, s[c]);
+        tc::tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; e++) top = fmaxf(top, see[c] >> e & 1u ? __uint_as_float(s[e]) : -INFINITY);
-          } else {
+        for (uint32_t c = 0; c < KT / 32; c++) tc::tmem_hold(s[c]);
+        if (masked) {
 #pragma unroll
-            for (int e = 0; e < 32; e++) top = fmaxf(top, __uint_as_float(s[e]));
-          }
+          for (uint32_t c = 0; c < KT / 32; c++)
+#pragma unroll
+            for (int e = 0; e < 32; e++) s[c][e] = see[c] >> e & 1u ? s[c][e] : 0xFF800000u;
         }
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (uint32_t c = 0; c < KT / 32; c++)
+#pragma unroll
+          for (int e = 0; e < 32; e += 2)
+            tops[(e >> 1) & 3] = max3(tops[(e >> 1) & 3], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         const bool grow = m != -INFINITY && (top - m) * P.scale2 > 8.0f;
         if (__any_sync(0xFFFFFFFFu, grow)) {
           const float f = grow ? exp2_fast((m - top) * P.scale2) : 1.0f;
@@ -401,24 +430,26 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
         }
         if (m == -INFINITY) m = top;
         const float base = m == -INFINITY ? 0.0f : m * P.scale2;
+        const F2 sc = make2(P.scale2, P.scale2), nb = make2(-base, -base);
+        F2 sum[2] = {make2(0.0f, 0.0f), make2(0.0f, 0.0f)};
 #pragma unroll
         for (uint32_t c = 0; c < KT / 32; c++) {
-          uint32_t s[32], p[16];
-          tc::tmem_ld32(s_at + 32 * c, s);
-          tc::tmem_wait_ld();
-          float sum[4] = {};
+          uint32_t p[16];
 #pragma unroll
-          for (int e = 0; e < 32; e++) {
-            float x = exp2_fast(fmaf(__uint_as_float(s[e]), P.scale2, -base));
-            if (masked) x = see[c] >> e & 1u ? x : 0.0f;
-            sum[e & 3] += x;
-            s[e] = __float_as_uint(x);
+          for (int e = 0; e < 16; e++) {
+            float x, y;
+            take2(fma2(make2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])), sc, nb), x, y);
+            x = exp2_fast(x);
+            y = exp2_fast(y);
+            sum[e & 1] = add2(sum[e & 1], make2(x, y));
+            p[e] = pack2(x, y, T());
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-          for (int e = 0; e < 16; e++) p[e] = pack2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]), T());
           tc::tmem_st16(s_at + 16 * c, p);
         }
+        float s0, s1, s2, s3;
+        take2(sum[0], s0, s1);
+        take2(sum[1], s2, s3);
+        l += (s0 + s1) + (s2 + s3);
         tc::tmem_wait_st();
         tc::tc_fence_before();
         tc::mbar_arrive(bar(sh.p_ready[slot]));
