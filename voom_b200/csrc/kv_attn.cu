@@ -5,6 +5,7 @@
 #include <type_traits>
 
 #include "kv_rows.cuh"
+#include "kv_sums.cuh"
 #include "kv_tc.cuh"
 
 namespace {
@@ -45,13 +46,13 @@ __global__ void __launch_bounds__(256) tree_mask(const int32_t* __restrict__ par
 
 // ------------------------------------------------------------------- finish
 // Joins the partial sums of units that several blocks shared (blocks below
-// n_merge: one per unit and eight rows), and adds the rows' weights at each
+// n_merge: one per unit and 32 rows), and adds the rows' weights at each
 // position to the running sums (the others: one per key head and kWeightSpan
 // positions), from the scores the attention kept and the rows' denominators.
 // The partial sums are joined in block order, the rows added in row order, so
 // that nothing depends on scheduling.
 constexpr uint32_t kWeightSpan = 1024;
-constexpr uint32_t kMergeRows = 8;
+constexpr uint32_t kMergeRows = 32;
 
 struct Split {
   uint32_t first, last;  // blocks that hold the unit's partial sums; first > last: none, it is whole
@@ -61,8 +62,7 @@ __device__ __forceinline__ Split split_of(const Attn& P, uint32_t b, uint32_t h,
   Split s{1, 0};
   if (!P.ctas) return s;
   const uint32_t len = P.c.length(b), cs = voom::kv::cache_steps(P, len);
-  uint64_t at = before + h * voom::kv::head_steps(P, len);
-  for (uint32_t i = 0; i < m; i++) at += cs + voom::kv::tail_of(P, i);
+  const uint64_t at = before + h * voom::kv::head_steps(P, len) + uint64_t(m) * cs + voom::kv::tails_before(P, m);
   voom::kv::owners(P, total, at, cs + voom::kv::tail_of(P, m), s.first, s.last);
   if (s.first == s.last) s = Split{1, 0};
   return s;
@@ -100,28 +100,34 @@ __global__ void __launch_bounds__(256) attn_finish(const __grid_constant__ Attn 
   extern __shared__ float s_row[];  // lse (log2 units) of the key head's rows, then their weights
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
-  const uint64_t total = P.ctas ? voom::kv::steps_before(P, P.c.v.B) : 0;
+  __shared__ Split s_split;
   if (blockIdx.x < n_merge) {
-    const uint32_t groups = P.rows / kMergeRows, unit = blockIdx.x / groups, r0 = (blockIdx.x - unit * groups) * kMergeRows;
+    const uint32_t groups = (P.rows + kMergeRows - 1) / kMergeRows, unit = blockIdx.x / groups, r0 = (blockIdx.x - unit * groups) * kMergeRows;
     const uint32_t m = unit % P.mblocks, head = unit / P.mblocks, b = head / P.c.v.hk, h = head - b * P.c.v.hk, row0 = m * P.rows;
     if (row0 + r0 >= P.R) return;
-    const Split s = split_of(P, b, h, m, total, voom::kv::steps_before(P, b));
+    if (warp == 0) {
+      const uint64_t total = voom::kv::steps_before(P, P.c.v.B), before = voom::kv::steps_before(P, b);
+      if (lane == 0) s_split = split_of(P, b, h, m, total, before);
+    }
+    __syncthreads();
+    const Split s = s_split;
     if (s.first > s.last) return;
-    if (warp < kMergeRows) {
-      const float2 ml = joined(P, s, r0 + warp);
+    const uint32_t rows = min(min(uint32_t(kMergeRows), P.rows - r0), P.R - row0 - r0);
+    for (uint32_t k = warp; k < rows; k += 8) {
+      const float2 ml = joined(P, s, r0 + k);
       if (lane == 0) {
-        s_row[2 * warp] = ml.x == -INFINITY ? 0.0f : ml.x;
-        s_row[2 * warp + 1] = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
-        const uint32_t row = row0 + r0 + warp;
-        if (P.lse && row < P.R)
-          P.lse[(uint64_t(b) * P.a.n + row / P.g) * P.a.hq + h * P.g + row % P.g] = voom::kv::kLn2 * (s_row[2 * warp] + log2f(ml.y));
+        const uint32_t row = row0 + r0 + k;
+        s_row[2 * k] = ml.x == -INFINITY ? 0.0f : ml.x;
+        s_row[2 * k + 1] = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
+        if (P.lse)
+          P.lse[(uint64_t(b) * P.a.n + row / P.g) * P.a.hq + h * P.g + row % P.g] = voom::kv::kLn2 * (s_row[2 * k] + log2f(ml.y));
       }
     }
     __syncthreads();
     const uint32_t quads = P.ld_o / 4;
-    for (uint32_t i = tid; i < kMergeRows * quads; i += 256) {
+    for (uint32_t i = tid; i < rows * quads; i += 256) {
       const uint32_t k = i / quads, d = 4 * (i - k * quads), r = r0 + k, row = row0 + r;
-      if (row >= P.R || d >= P.c.v.D) continue;
+      if (d >= P.c.v.D) continue;
       const float base = s_row[2 * k], inv = s_row[2 * k + 1];
       float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
@@ -147,13 +153,20 @@ __global__ void __launch_bounds__(256) attn_finish(const __grid_constant__ Attn 
   const uint32_t len = P.c.length(b);
   if (s0 >= len && s0 + kWeightSpan <= P.score_new) return;
   float* s_w = s_row + P.R;
-  const uint64_t before = P.ctas ? voom::kv::steps_before(P, b) : 0;
+  // (the scores are kept for one block of rows only)
+  if (P.ctas && warp == 0) {
+    const uint64_t total = voom::kv::steps_before(P, P.c.v.B), before = voom::kv::steps_before(P, b);
+    if (lane == 0) s_split = split_of(P, b, h, 0, total, before);
+  } else if (!P.ctas && tid == 0) {
+    s_split = Split{1, 0};
+  }
+  __syncthreads();
+  const Split s = s_split;
   for (uint32_t r = warp; r < P.R; r += 8) {
-    const uint32_t k = r / P.rows, i = r / P.g, hh = h * P.g + r % P.g;
-    const Split s = split_of(P, b, h, k, total, before);
+    const uint32_t i = r / P.g, hh = h * P.g + r % P.g;
     float lse2;
     if (s.first <= s.last) {
-      const float2 ml = joined(P, s, r - k * P.rows);
+      const float2 ml = joined(P, s, r);
       lse2 = (ml.x == -INFINITY ? 0.0f : ml.x) + log2f(ml.y);
     } else {
       lse2 = P.lse[(uint64_t(b) * P.a.n + i) * P.a.hq + hh] * voom::kv::kLog2e;
@@ -266,7 +279,7 @@ uint64_t plan(Attn& P, void* scratch) {
   P.scale2 = P.a.scale * voom::kv::kLog2e;
   P.ld_o = c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256;
   P.tc = -1;
-  if (P.R > (P.ld_o == 256 ? 16u : 32u) && !P.a.d_weights) {
+  if (P.R > (P.ld_o == 256 ? 16u : 32u)) {
     P.tc = P.ld_o == 256 ? voom::kv::kSingle : P.R > 128 ? voom::kv::kPair : voom::kv::kAlternate;
     P.keys = P.tc == voom::kv::kSingle ? 64 : 128;
     P.rows = P.tc == voom::kv::kPair ? 256 : 128;
@@ -277,8 +290,7 @@ uint64_t plan(Attn& P, void* scratch) {
   P.rows = P.R > 16 && P.ld_o <= 128 ? 32 : 16;
   }
   P.mblocks = (P.R + P.rows - 1) / P.rows;
-  P.tails = 0;
-  for (uint32_t m = 0; m < P.mblocks; m++) P.tails += voom::kv::tail_of(P, m);
+  P.tails = uint32_t(voom::kv::tails_before(P, P.mblocks - 1)) + voom::kv::tail_of(P, P.mblocks - 1);
   const uint64_t units = uint64_t(c.B) * c.hk * P.mblocks;
   const uint32_t steps = (c.max_len + P.keys - 1) / P.keys + (P.a.n + P.keys - 1) / P.keys;
   P.ctas = steps <= 16 ? 0u : uint32_t(min(uint64_t(sm_count()), (units * steps + 7) / 8));
@@ -292,6 +304,7 @@ uint64_t plan(Attn& P, void* scratch) {
   P.lse = P.a.d_lse;
   if (P.a.d_weights) {
     if (!P.lse) P.lse = reinterpret_cast<float*>(take(uint64_t(c.B) * P.a.n * P.a.hq * sizeof(float)));
+    if (P.R > 16) return at;  // attn_sums goes over the keys again
     P.score_new = (c.max_len + P.keys - 1) / P.keys * P.keys;
     P.score_ld = P.score_new + (P.a.n + P.keys - 1) / P.keys * P.keys;
     P.scores = reinterpret_cast<float*>(take(uint64_t(c.B) * c.hk * P.R * P.score_ld * sizeof(float)));
@@ -319,6 +332,33 @@ int launch_tc(const Attn& P, cudaStream_t s) {
   return cudaGetLastError() == cudaSuccess ? VOOM_OK : VOOM_E_CUDA;
 }
 
+template <typename T, int DP>
+int launch_sums(const Attn& P, cudaStream_t s) {
+  constexpr uint32_t smem = voom::kv::sums_smem<DP>();
+  static std::atomic<uint64_t> allowed{0};
+  if (!allow_smem(reinterpret_cast<const void*>(voom::kv::attn_sums<T, DP>), smem, allowed)) return VOOM_E_CUDA;
+  voom::kv::attn_sums<T, DP><<<P.ctas, voom::kv::Sums<DP>::THREADS, smem, s>>>(P);
+  return cudaGetLastError() == cudaSuccess ? VOOM_OK : VOOM_E_CUDA;
+}
+
+template <typename T>
+int finish(const Attn& P, cudaStream_t s) {
+  const uint64_t units = uint64_t(P.c.v.B) * P.c.v.hk * P.mblocks;
+  const uint32_t n_merge = P.ctas ? uint32_t(units * ((P.rows + kMergeRows - 1) / kMergeRows)) : 0u;
+  const uint64_t spans = P.scores ? uint64_t(P.c.v.B) * P.c.v.hk * ((P.score_ld + kWeightSpan - 1) / kWeightSpan) : 0;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(uint32_t(n_merge + spans));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = max(2u * kMergeRows, 2u * (P.scores ? P.R : 0u)) * sizeof(float);
+  cfg.stream = s;
+  cudaLaunchAttribute early{};  // its launch overlaps the attention's end; it waits for it before it reads
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attn_finish<T>, P, n_merge) == cudaSuccess ? VOOM_OK : VOOM_E_CUDA;
+}
+
 template <typename T>
 int run(Attn& P, cudaStream_t s) {
   using voom::kv::kAlternate;
@@ -332,22 +372,20 @@ int run(Attn& P, cudaStream_t s) {
   else if (P.ld_o == 64) rc = P.rows == 16 ? launch_rows<T, 64, 1>(P, s) : launch_rows<T, 64, 2>(P, s);
   else if (P.ld_o == 128) rc = P.rows == 16 ? launch_rows<T, 128, 1>(P, s) : launch_rows<T, 128, 2>(P, s);
   else rc = launch_rows<T, 256, 1>(P, s);
-  if (rc != VOOM_OK || (!P.ctas && !P.a.d_weights)) return rc;
-  const uint64_t units = uint64_t(P.c.v.B) * P.c.v.hk * P.mblocks;
-  const uint32_t n_merge = P.ctas ? uint32_t(units * (P.rows / kMergeRows)) : 0u;
-  const uint64_t spans = P.a.d_weights ? uint64_t(P.c.v.B) * P.c.v.hk * ((P.score_ld + kWeightSpan - 1) / kWeightSpan) : 0;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(uint32_t(n_merge + spans));
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = max(2u * kMergeRows, 2u * (P.a.d_weights ? P.R : 0u)) * sizeof(float);
-  cfg.stream = s;
-  cudaLaunchAttribute early{};  // its launch overlaps the attention's end; it waits for it before it reads
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &early;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attn_finish<T>, P, n_merge) == cudaSuccess ? VOOM_OK : VOOM_E_CUDA;
+  if (rc != VOOM_OK) return rc;
+  if (P.ctas || P.scores) rc = finish<T>(P, s);
+  if (rc != VOOM_OK || !P.a.d_weights || P.scores) return rc;
+  // the rows' weights from the keys again: all rows of a key head as one unit, tiles of 128 keys
+  P.keys = 128;
+  P.rows = P.R;
+  P.mblocks = 1;
+  P.tails = voom::kv::tail_of(P, 0);
+  const uint64_t steps = uint64_t(P.c.v.B) * P.c.v.hk * ((P.c.v.max_len + 127) / 128 + P.tails);
+  P.ctas = uint32_t(min(uint64_t(sm_count()), steps));
+  map_cache(P);
+  return P.ld_o == 64 ? launch_sums<T, 64>(P, s) : P.ld_o == 128 ? launch_sums<T, 128>(P, s) : launch_sums<T, 256>(P, s);
 }
+
 
 }  // namespace
 

@@ -55,6 +55,28 @@ __host__ __device__ __forceinline__ uint32_t tail_of(const Attn& P, uint32_t m) 
   return ceil_div(((rows < P.R ? rows : P.R) - 1) / P.g + 1, P.keys);
 }
 
+// Those of the first m blocks (m < mblocks, or all but the last of them).  In a
+// chain block i takes floor(((i + 1) rows - 1) / (g keys)) + 1 steps: a sum of
+// floors of an arithmetic progression, by the reciprocity that swaps slope and
+// modulus as Euclid's algorithm does.
+__host__ __device__ __forceinline__ uint64_t tails_before(const Attn& P, uint32_t m) {
+  if (P.a.d_mask) return uint64_t(m) * ceil_div(P.a.n, P.keys);
+  uint64_t sum = m, n = m, a = P.rows, b = P.rows - 1, q = uint64_t(P.g) * P.keys;
+  if (!m) return 0;
+  for (;;) {  // sum of floor((a i + b) / q) over i < n
+    sum += n * (n - 1) / 2 * (a / q) + n * (b / q);
+    a %= q;
+    b %= q;
+    const uint64_t top = a * n + b;
+    if (top < q) return sum;
+    n = top / q;
+    b = top % q;
+    const uint64_t t = q;
+    q = a;
+    a = t;
+  }
+}
+
 // Steps of one key head of a request.
 __device__ __forceinline__ uint64_t head_steps(const Attn& P, uint32_t len) {
   return uint64_t(P.mblocks) * cache_steps(P, len) + P.tails;
@@ -112,11 +134,15 @@ __device__ __forceinline__ bool first_seg(const Attn& P, uint32_t cta, Seg& s) {
   uint64_t off = s.at - base;
   s.h = uint32_t(off / per);
   off -= s.h * per;
-  s.m = 0;
-  while (off >= (s.steps = cs + tail_of(P, s.m))) {
-    off -= s.steps;
-    s.m++;
+  uint32_t lo = 0, hi = P.mblocks - 1;  // the last block of rows that starts at off or before
+  while (lo < hi) {
+    const uint32_t mid = (lo + hi + 1) / 2;
+    if (uint64_t(mid) * cs + tails_before(P, mid) <= off) lo = mid;
+    else hi = mid - 1;
   }
+  s.m = lo;
+  off -= uint64_t(lo) * cs + tails_before(P, lo);
+  s.steps = cs + tail_of(P, lo);
   s.s0 = uint32_t(off);
   s.s1 = uint32_t(min(uint64_t(s.steps), off + (s.end - s.at)));
   return true;

@@ -90,6 +90,73 @@ __device__ __forceinline__ void odd_fix(const Attn& P, const Seg& g, uint32_t ro
   }
 }
 
+// One of four warps' part (128 threads) of bringing a tile of keys or values to
+// shared memory; its barrier gets 128 arrivals.  A tile of cached positions
+// that are all valid comes by TMA, one box for each run of positions in a page:
+// the lanes of the first warp find the pages.  Others (the end of a cache, new
+// tokens, caches that TMA cannot read) are gathered through cp.async; their
+// barrier hears of the copies as they land, and the issuing thread fences them
+// for the tensor cores.  With `hold` nothing is announced: the caller waits
+// for the copies, and arrives; true then.
+template <typename T, int DP, int KT>
+__device__ __forceinline__ bool load_tile_sw128(const Attn& P, const Seg& g, uint32_t step, uint32_t cs, bool is_v, uint32_t pw,
+                                                uint32_t lane, uint32_t dst, uint32_t full, bool hold) {
+  constexpr uint32_t CH = DP / 8, RW = KT / 4;
+  const bool fresh = step >= cs;
+  if (P.box && step * KT + KT <= g.len) {
+    if (pw == 0) {
+      if (lane == 0) tc::mbar_arrive_expect(full, KT * DP * 2);
+      else tc::mbar_arrive(full);
+      __syncwarp();
+      if (lane < KT / P.box) {
+        const uint32_t s = step * KT + lane * P.box, pg = P.c.page_of(s);
+        const int32_t w = P.c.v.d_table ? __ldg(P.c.v.d_table + uint64_t(g.b) * P.c.v.table_stride + pg) : int32_t(g.b);
+        const uint32_t y = P.c.v.d_table ? s - pg * P.c.v.page : s;
+        const void* map = is_v ? &P.v_map : &P.k_map;
+#pragma unroll
+        for (uint32_t x = 0; x < DP; x += 64)
+          tc::tma_load4(dst + (x / 64) * (KT * 128u) + lane * P.box * 128u, map, full, int32_t(x), int32_t(y), int32_t(g.h), w);
+      }
+    } else {
+      tc::mbar_arrive(full);
+    }
+    return false;
+  }
+  uint64_t a = 0;
+  if (lane < RW) {
+    const uint32_t r = pw * RW + lane;
+    if (!fresh) {
+      const uint32_t s = step * KT + r;
+      int64_t ko, vo;
+      if (s < g.len && P.c.row_at(g.b, g.h, s, ko, vo))
+        a = is_v ? reinterpret_cast<uint64_t>(static_cast<const T*>(P.c.v.d_v) + vo)
+                 : reinterpret_cast<uint64_t>(static_cast<const T*>(P.c.v.d_k) + ko);
+    } else {
+      const uint32_t s = (step - cs) * KT + r;
+      if (s < P.a.n && sees(P, g.b, s, s))
+        a = is_v ? reinterpret_cast<uint64_t>(static_cast<const T*>(P.a.d_vn) + int64_t(g.b) * P.a.vn_b + int64_t(s) * P.a.vn_t +
+                                              int64_t(g.h) * P.a.vn_h)
+                 : reinterpret_cast<uint64_t>(static_cast<const T*>(P.a.d_kn) + int64_t(g.b) * P.a.kn_b + int64_t(s) * P.a.kn_t +
+                                              int64_t(g.h) * P.a.kn_h);
+    }
+  }
+#pragma unroll
+  for (uint32_t k = 0; k < RW * CH / 32; k++) {
+    const uint32_t id = k * 32 + lane, r = id / CH, c = id % CH;
+    const uint64_t y = __shfl_sync(0xFFFFFFFFu, a, r);
+    const bool in = y && c * 8 < P.c.v.D;
+    cp16(dst + sw128(pw * RW + r, c, KT), in ? reinterpret_cast<const void*>(y + 16 * c) : P.c.v.d_k, in);
+  }
+  if (!hold) tc::mbar_arrive_copies(full);
+  return hold;
+}
+
+template <typename T, int DP, int KT>
+__device__ __forceinline__ void load_keys(const Attn& P, const Seg& g, uint32_t step, uint32_t cs, uint32_t pw, uint32_t lane,
+                                          uint32_t dst, uint32_t full) {
+  load_tile_sw128<T, DP, KT>(P, g, step, cs, false, pw, lane, dst, full, false);
+}
+
 template <typename T, int DP, int MODE>
 __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid_constant__ Attn P) {
   using C = Tc<DP, MODE>;
@@ -137,13 +204,6 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
     const uint32_t pw = warp - LOAD_WARP;
     uint32_t it = 0, nq = 0;  // tiles and query tiles asked for
     bool ok = true;
-    // A tile of cached positions that are all valid comes by TMA, one box for
-    // each run of positions in a page: the lanes of the first warp find the
-    // pages.  Others (the end of a cache, new tokens, caches that TMA cannot
-    // read) are gathered through cp.async; their barrier hears of the copies as
-    // they land, and the issuing thread fences them for the tensor cores.  The
-    // gather alone took 1500 cycles to a tile, with a page table 3000, against
-    // 1024 that its matrix products take.
     // New tokens' values are looked through first: those that are not finite
     // are taken out, whatever probability they meet.
     auto look_through = [&](uint32_t place) {
@@ -194,60 +254,10 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
         }
         const uint32_t step = g.s0 + j, place = it % RING;
         if (it >= RING && !(ok = warp_wait(sh.empty[place], (it / RING - 1) & 1u))) break;
-        const bool fresh = step >= cs;
-        if (P.box && step * KT + KT <= g.len) {
-          if (pw == 0) {
-            if (lane == 0) tc::mbar_arrive_expect(bar(sh.full[place]), C::TILE);
-            else tc::mbar_arrive(bar(sh.full[place]));
-            __syncwarp();
-            if (lane < KT / P.box) {
-              const uint32_t s = step * KT + lane * P.box, pg = P.c.page_of(s);
-              const int32_t w = P.c.v.d_table ? __ldg(P.c.v.d_table + uint64_t(g.b) * P.c.v.table_stride + pg) : int32_t(g.b);
-              const uint32_t y = P.c.v.d_table ? s - pg * P.c.v.page : s;
-              const void* map = is_v ? &P.v_map : &P.k_map;
-#pragma unroll
-              for (uint32_t x = 0; x < DP; x += 64)
-                tc::tma_load4(ring_s + place * C::TILE + (x / 64) * (KT * 128u) + lane * P.box * 128u, map, bar(sh.full[place]),
-                              int32_t(x), int32_t(y), int32_t(g.h), w);
-            }
-          } else {
-            tc::mbar_arrive(bar(sh.full[place]));
-          }
-          it++;
-          continue;
-        }
-        uint64_t a = 0;
-        if (lane < RW) {
-          const uint32_t r = pw * RW + lane;
-          if (!fresh) {
-            const uint32_t s = step * KT + r;
-            int64_t ko, vo;
-            if (s < g.len && P.c.row_at(g.b, g.h, s, ko, vo))
-              a = is_v ? reinterpret_cast<uint64_t>(static_cast<const T*>(P.c.v.d_v) + vo)
-                       : reinterpret_cast<uint64_t>(static_cast<const T*>(P.c.v.d_k) + ko);
-          } else {
-            const uint32_t s = (step - cs) * KT + r;
-            if (s < P.a.n && sees(P, g.b, s, s))
-              a = is_v ? reinterpret_cast<uint64_t>(static_cast<const T*>(P.a.d_vn) + int64_t(g.b) * P.a.vn_b +
-                                                    int64_t(s) * P.a.vn_t + int64_t(g.h) * P.a.vn_h)
-                       : reinterpret_cast<uint64_t>(static_cast<const T*>(P.a.d_kn) + int64_t(g.b) * P.a.kn_b +
-                                                    int64_t(s) * P.a.kn_t + int64_t(g.h) * P.a.kn_h);
-          }
-        }
-        const uint32_t dst = ring_s + place * C::TILE;
-#pragma unroll
-        for (uint32_t k = 0; k < RW * CH / 32; k++) {
-          const uint32_t id = k * 32 + lane, r = id / CH, c = id % CH;
-          const uint64_t y = __shfl_sync(0xFFFFFFFFu, a, r);
-          const bool in = y && c * 8 < P.c.v.D;
-          cp16(dst + sw128(pw * RW + r, c, KT), in ? reinterpret_cast<const void*>(y + 16 * c) : P.c.v.d_k, in);
-        }
         it++;
-        if (fresh && is_v) {
+        if (load_tile_sw128<T, DP, KT>(P, g, step, cs, is_v, pw, lane, ring_s + place * C::TILE, bar(sh.full[place]), step >= cs && is_v)) {
           look_through(place);
           tc::mbar_arrive(bar(sh.full[place]));
-        } else {
-          tc::mbar_arrive_copies(bar(sh.full[place]));
         }
       }
     } while (ok && next_seg(P, g));
