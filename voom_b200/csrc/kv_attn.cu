@@ -46,13 +46,13 @@ __global__ void __launch_bounds__(256) tree_mask(const int32_t* __restrict__ par
 
 // ------------------------------------------------------------------- finish
 // Joins the partial sums of units that several blocks shared (blocks below
-// n_merge: one per unit and 32 rows), and adds the rows' weights at each
+// n_merge: one per unit and 8 rows), and adds the rows' weights at each
 // position to the running sums (the others: one per key head and kWeightSpan
 // positions), from the scores the attention kept and the rows' denominators.
 // The partial sums are joined in block order, the rows added in row order, so
 // that nothing depends on scheduling.
 constexpr uint32_t kWeightSpan = 1024;
-constexpr uint32_t kMergeRows = 32;
+constexpr uint32_t kMergeRows = 8;
 
 struct Split {
   uint32_t first, last;  // blocks that hold the unit's partial sums; first > last: none, it is whole
@@ -293,7 +293,10 @@ uint64_t plan(Attn& P, void* scratch) {
   P.tails = uint32_t(voom::kv::tails_before(P, P.mblocks - 1)) + voom::kv::tail_of(P, P.mblocks - 1);
   const uint64_t units = uint64_t(c.B) * c.hk * P.mblocks;
   const uint32_t steps = (c.max_len + P.keys - 1) / P.keys + (P.a.n + P.keys - 1) / P.keys;
-  P.ctas = steps <= 16 ? 0u : uint32_t(min(uint64_t(sm_count()), (units * steps + 7) / 8));
+  // a block takes at least two tiles for each of its warps (rows), or a few of
+  // the larger ones (tensor cores), before the work is spread further
+  const uint32_t least = P.tc >= 0 ? 3 : 8;
+  P.ctas = steps <= (P.tc >= 0 ? 4u : 16u) ? 0u : uint32_t(min(uint64_t(sm_count()), (units * steps + least - 1) / least));
   uint64_t at = 0;
   auto take = [&](uint64_t bytes) {
     const uint64_t o = at;

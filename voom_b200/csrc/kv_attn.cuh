@@ -105,8 +105,9 @@ __device__ __forceinline__ bool first_seg(const Attn& P, uint32_t cta, Seg& s) {
     return true;
   }
   const uint64_t total = steps_before(P, P.c.v.B);
-  s.at = total * cta / P.ctas;
-  s.end = total * (cta + 1) / P.ctas;
+  const uint64_t top = total * (cta + 1);
+  s.at = top >> 32 ? (top - total) / P.ctas : uint32_t(top - total) / P.ctas;
+  s.end = top >> 32 ? top / P.ctas : uint32_t(top) / P.ctas;
   if (s.at >= s.end) return false;
   uint64_t base = 0;
   const uint32_t lane = threadIdx.x & 31u;
@@ -168,12 +169,11 @@ __device__ __forceinline__ bool next_seg(const Attn& P, Seg& s) {
 // of the list: first .. last, and first's slot is its second one.
 __device__ __forceinline__ void owners(const Attn& P, uint64_t total, uint64_t at, uint32_t steps, uint32_t& first,
                                        uint32_t& last) {
-  // block c covers [total * c / ctas, total * (c + 1) / ctas)
+  // block c covers [total * c / ctas, total * (c + 1) / ctas): x is in the
+  // largest c with total * c / ctas <= x, that is total * c < ctas * (x + 1)
   auto holder = [&](uint64_t x) {
-    uint32_t c = uint32_t(x * P.ctas / total);
-    while (total * (c + 1) / P.ctas <= x) c++;
-    while (total * c / P.ctas > x) c--;
-    return c;
+    const uint64_t top = uint64_t(P.ctas) * (x + 1) - 1;
+    return top >> 32 ? uint32_t(top / total) : uint32_t(top) / uint32_t(total);
   };
   first = holder(at);
   last = holder(at + steps - 1);

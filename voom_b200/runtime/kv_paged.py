@@ -272,7 +272,15 @@ class PagedKVCache:
         self.stats = KVStats()
         self._pool = ThreadPoolExecutor(max_workers=max(1, spill_threads))
 
-    def update(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        """update() without its result: the new positions are stored (and the
+        byte budget enforced after the last layer), nothing is put together."""
+        self._extend(layer, k, v)
+        if layer == self.num_layers - 1:
+            self._offset += k.shape[2]
+            self._enforce_budget()
+
+    def _extend(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
         if self._tail_k[layer] is None:
             self._tail_k[layer], self._tail_v[layer] = k, v
         else:
@@ -284,20 +292,67 @@ class PagedKVCache:
             self._pages[layer].append(_Page(pk, pv))
             self._tail_k[layer] = self._tail_k[layer][:, :, self.page_positions:, :].contiguous()
             self._tail_v[layer] = self._tail_v[layer][:, :, self.page_positions:, :].contiguous()
-        if layer == self.num_layers - 1:
-            self._offset += k.shape[2]
-            self._enforce_budget()
+
+    def _loaded(self, layer: int) -> list[tuple[torch.Tensor, torch.Tensor]]:
+        """Keys and values of the layer's closed pages, spilled ones reloaded."""
         pages = self._pages[layer]
         spilled = [p for p in pages if not p.resident]
-        if spilled:
-            t0 = time.perf_counter()
-            loaded = load_pages(spilled)
-            self.stats.reloads += len(spilled)
-            self.stats.reload_s += time.perf_counter() - t0
-            it = iter(loaded)
-            parts = [(p.k, p.v) if p.resident else next(it) for p in pages]
-        else:
-            parts = [(p.k, p.v) for p in pages]
+        if not spilled:
+            return [(p.k, p.v) for p in pages]
+        t0 = time.perf_counter()
+        loaded = load_pages(spilled)
+        self.stats.reloads += len(spilled)
+        self.stats.reload_s += time.perf_counter() - t0
+        it = iter(loaded)
+        return [(p.k, p.v) if p.resident else next(it) for p in pages]
+
+    def length(self, layer: int) -> int:
+        """Positions the layer holds (fewer than `offset` after an eviction)."""
+        tail = self._tail_k[layer]
+        return len(self._pages[layer]) * self.page_positions + (0 if tail is None else int(tail.shape[2]))
+
+    def view(self, layer: int):
+        """The layer's positions for kv_attention.tree_attention: pages are read
+        where they are (spilled ones reloaded for the view's life), only the
+        open page is copied, into a page of its own; update() would copy every
+        position instead."""
+        from .kv_attention import KVView
+
+        tail = self._tail_k[layer]
+        if tail is None:
+            raise ValueError(f"layer {layer} holds no positions yet")
+        pages = self._loaded(layer)
+        t = int(tail.shape[2])
+        if t or not pages:
+            shape = (*tail.shape[:2], self.page_positions, tail.shape[3])
+            k, v = tail.new_zeros(shape), tail.new_zeros(shape)
+            k[:, :, :t], v[:, :, :t] = tail, self._tail_v[layer]
+            pages = [*pages, (k, v)]
+        n = self.length(layer)
+        return KVView.pages([pages], torch.tensor([n], dtype=torch.int32, device=tail.device), max_len=n)
+
+    def evict(self, layer: int, weights: torch.Tensor, *, budget: int, sinks: int = 4, recent: int = 0):
+        """Cuts the layer to its first `sinks`, newest `recent` and most attended
+        positions, `budget` in all (kv_attention.kv_evict; `weights` are the
+        running sums of tree_attention).  Returns what kv_evict returned: the
+        kept positions' weights and original indexes among it.  `offset` still
+        counts all positions seen."""
+        from .kv_attention import kv_evict
+
+        n = self.length(layer)
+        e = kv_evict(self.view(layer), weights, budget=budget, sinks=sinks, recent=recent)
+        files = {pg.path for pg in self._pages[layer] if pg.path is not None}
+        self._pages[layer] = []
+        self._tail_k[layer] = self._tail_v[layer] = None
+        m = min(n, budget)
+        self._extend(layer, e.k[:, :, :m].contiguous(), e.v[:, :, :m].contiguous())
+        for f in files:
+            f.unlink(missing_ok=True)
+        return e
+
+    def update(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        self.append(layer, k, v)
+        parts = self._loaded(layer)
         parts_k = [a for a, _ in parts]
         parts_v = [b for _, b in parts]
         if self._tail_k[layer].shape[2] > 0 or not parts_k:
