@@ -180,14 +180,26 @@ __global__ void __launch_bounds__(256) attn_finish(const __grid_constant__ Attn 
   const float* z = P.scores + uint64_t(head) * P.R * P.score_ld;
   float got[kWeightSpan / 256] = {};
   const uint32_t end = min(P.score_ld, s0 + kWeightSpan);
-  for (uint32_t r = 0; r < P.R; r++) {
-    const float lse2 = s_row[r], w = s_w[r];
-    // in a chain, tiles past the row's own token have no scores
-    const uint32_t lim = P.a.d_mask ? end : min(end, P.score_new + r / P.g + 1);
+  // four rows' scores under way at a time (up to 16 loads a thread)
+  for (uint32_t r0 = 0; r0 < P.R; r0 += 4) {
+    float x[4][kWeightSpan / 256];
 #pragma unroll
-    for (uint32_t k = 0; k < kWeightSpan / 256; k++) {
-      const uint32_t s = s0 + k * 256 + tid;
-      if (s < lim) got[k] += w * voom::kv::exp2_fast(z[uint64_t(r) * P.score_ld + s] - lse2);
+    for (uint32_t q = 0; q < 4; q++) {
+      const uint32_t r = r0 + q;
+      // in a chain, tiles past the row's own token have no scores
+      const uint32_t lim = r >= P.R ? 0u : P.a.d_mask ? end : min(end, P.score_new + r / P.g + 1);
+#pragma unroll
+      for (uint32_t k = 0; k < kWeightSpan / 256; k++) {
+        const uint32_t s = s0 + k * 256 + tid;
+        x[q][k] = s < lim ? z[uint64_t(r) * P.score_ld + s] : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (uint32_t q = 0; q < 4; q++) {
+      const uint32_t r = min(r0 + q, P.R - 1);
+      const float lse2 = s_row[r], w = s_w[r];
+#pragma unroll
+      for (uint32_t k = 0; k < kWeightSpan / 256; k++) got[k] += w * voom::kv::exp2_fast(x[q][k] - lse2);
     }
   }
   float* sums = P.a.d_weights + int64_t(b) * P.a.w_b + int64_t(h) * P.a.w_h;

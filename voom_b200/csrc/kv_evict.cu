@@ -44,6 +44,11 @@ __device__ __forceinline__ uint32_t key_of(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// The weight of a key (a NaN comes back as the canonical one, -0 as 0).
+__device__ __forceinline__ float weight_of(uint32_t k) {
+  return __uint_as_float(k == 0xFFFFFFFFu ? 0x7FFFFFFFu : k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+
 // Sum of x over the threads after this one (by index); every thread gets `total`.
 __device__ __forceinline__ uint32_t sum_after(uint32_t x, uint32_t* s_warp, uint32_t& total) {
   const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
@@ -104,8 +109,17 @@ __global__ void __launch_bounds__(kSelThreads) evict_select(const __grid_constan
   const uint32_t per = (m + ranks - 1) / ranks, begin = min(m, rank * per), n = min(m, begin + per) - begin;
   w += lo + begin;  // this block's slice
   const bool held = P.held;
-  if (held)
-    for (uint32_t i = tid; i < n; i += kSelThreads) s_keys[i] = key_of(w[i]);
+  if (held) {
+    constexpr uint32_t kDeep = 8;  // loads of a thread under way
+    for (uint32_t i0 = tid; i0 < n; i0 += kDeep * kSelThreads) {
+      float x[kDeep];
+#pragma unroll
+      for (uint32_t k = 0; k < kDeep; k++) x[k] = i0 + k * kSelThreads < n ? w[i0 + k * kSelThreads] : 0.0f;
+#pragma unroll
+      for (uint32_t k = 0; k < kDeep; k++)
+        if (i0 + k * kSelThreads < n) s_keys[i0 + k * kSelThreads] = key_of(x[k]);
+    }
+  }
   auto key = [&](uint32_t i) { return held ? s_keys[i] : key_of(w[i]); };
   uint32_t prefix = 0, mask = 0;
 #pragma unroll 1
@@ -188,7 +202,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select(const __grid_constan
     const uint32_t keeps = __ballot_sync(0xFFFFFFFFu, keep);
     if (keep) {
       index[at + __popc(keeps & below)] = int32_t(lo + begin + i);
-      w_out[at + __popc(keeps & below)] = w[i];
+      w_out[at + __popc(keeps & below)] = weight_of(k);
     }
     at += __popc(keeps);
     tie0 += __popc(ties);

@@ -33,6 +33,7 @@ struct SumsShared {
   uint64_t q_full, q_empty, s_full[2], s_empty[2], ready[2], drained;
   uint32_t tmem, failed;
   float2 row[2][256];  // for each softmax warpgroup: minus the row's denominator (log2), its weight
+  uint32_t tok[2][256];  // and its token
 };
 
 template <int DP>
@@ -171,6 +172,7 @@ __global__ void __launch_bounds__(Sums<DP>::THREADS, 1) attn_sums(const __grid_c
             x.y = P.a.d_token_weight ? P.a.d_token_weight[uint64_t(g.b) * P.a.n + i] : 1.0f;
           }
           sh.row[w][r] = x;
+          sh.tok[w][r] = row < P.R ? i : P.a.n;
         }
         if (!(ok = together())) break;
         for (uint32_t t = w; t < n; t += 2) {
@@ -192,9 +194,9 @@ __global__ void __launch_bounds__(Sums<DP>::THREADS, 1) attn_sums(const __grid_c
               float p = exp2_fast(fmaf(__uint_as_float(s[e]), P.scale2, x.x));
               float q = exp2_fast(fmaf(__uint_as_float(s[e + 1]), P.scale2, x.z));
               if (fresh) {
-                const uint32_t r = row0 + c + e;
-                if (r >= P.R || j >= P.a.n || !sees(P, g.b, r / P.g, j)) p = 0.0f;
-                if (r + 1 >= P.R || j >= P.a.n || !sees(P, g.b, (r + 1) / P.g, j)) q = 0.0f;
+                const uint32_t i0 = sh.tok[w][c + e], i1 = sh.tok[w][c + e + 1];
+                if (i0 >= P.a.n || j >= P.a.n || !sees(P, g.b, i0, j)) p = 0.0f;
+                if (i1 >= P.a.n || j >= P.a.n || !sees(P, g.b, i1, j)) q = 0.0f;
               }
               acc[0] = fmaf(x.y, p, acc[0]);
               acc[1] = fmaf(x.w, q, acc[1]);
