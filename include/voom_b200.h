@@ -585,8 +585,8 @@ enum { VOOM_BF16 = 0u, VOOM_FP16 = 1u, VOOM_FP32 = 2u };
  * into a context as at its start.  Strides are in elements; a head's D values
  * are contiguous.  Outputs may be the inputs (not partly overlap them).  fp32
  * arithmetic, one rounding.
- * Covers what the reference does with mx.fast.rms_norm + mx.fast.rope around
- * its KV caches (attention there is outside the ported path). */
+ * Replaces: the norm and rotation calls of the reference's attention layers
+ * (runtime/layer_runner.py _attention), outside its ported path. */
 typedef struct voom_qk_norm_rope_args {
   const void* d_q;    /* T x hq x D */
   const void* d_k;    /* T x hk x D */

@@ -87,12 +87,5 @@ template <>
 __device__ __forceinline__ float elem<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <>
 __device__ __forceinline__ float elem<__half>(__half v) { return __half2float(v); }
-template <typename T>
-__device__ __forceinline__ T rounded(float v);
-template <>
-__device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <>
-__device__ __forceinline__ __half rounded<__half>(float v) { return __float2half_rn(v); }
-
 }  // namespace kv
 }  // namespace voom

@@ -115,16 +115,10 @@ __device__ __forceinline__ void tma_load4(uint32_t dst, const void* map, uint32_
 }
 
 // Shared-memory matrix descriptor of a tile whose rows are 128 bytes, swizzled
-// in groups of eight rows (1024 bytes, the stride byte offset): K-major tiles
-// ignore the leading offset; in MN-major ones it is the distance between
-// blocks of 64 values of the M or N dimension.
-__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t saddr, uint32_t lbo) {
-  return uint64_t((saddr >> 4) & 0x3FFFu) | (uint64_t((lbo >> 4) & 0x3FFFu) << 16) |
-         (uint64_t(1024u >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
-}
-
-// The low word of a matrix descriptor moves through a tile by whole 16-byte
-// units; the high word is the tile's layout.
+// in groups of eight rows (1024 bytes, the stride byte offset).  Its low word is
+// the address in 16-byte units and, from bit 16, the leading byte offset:
+// ignored by K-major tiles, in MN-major ones the distance between blocks of 64
+// values of the M or N dimension.  Its high word is the layout.
 __device__ __forceinline__ uint64_t umma_desc_at(uint32_t lo, uint32_t hi) {
   uint64_t d;
   asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));

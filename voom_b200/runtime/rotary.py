@@ -4,8 +4,8 @@
                    layout and long-context scaling.
   qk_norm_rope   - norm + rotation of q and k (csrc/rope.cu).
 
-Counterpart in the reference: the mx.fast.rms_norm / mx.fast.rope calls of its
-attention layers (runtime/layer_runner.py `_attention`), ahead of the KV caches.
+Counterpart in the reference: the norm and rotation calls of its attention
+layers (runtime/layer_runner.py `_attention`), ahead of the KV caches.
 """
 
 from __future__ import annotations
