@@ -1,0 +1,50 @@
+"""Cache attention and eviction where lengths, pages, masks and workspaces are at
+their edges, against the definitions in 64 bits.  Tolerances as in
+test_kv_attention.py; those that are tighter or exact say why."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from oracle import attention as oa
+from tests.test_kv_attention import STEP, check, inputs, place
+
+
+def poison(view):
+    """The view's workspaces filled with NaN: whatever a call does not write, it must not read."""
+    for t in view._scratch.values():
+        t.fill_(255)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[100], [1], [0], [33, 0, 5], [700, 64]])
+@pytest.mark.parametrize("n,g,D", [(1, 1, 64), (1, 4, 128), (2, 2, 256), (12, 2, 64), (40, 4, 128), (20, 2, 256), (300, 1, 64)])
+def test_lengths_far_below_the_bound(lens, n, g, D):
+    """The blocks are laid out for max_len; with fewer steps than blocks, those without one leave nothing to join."""
+    from voom_b200.runtime import kv_attention as kva
+
+    cap = 24000
+    B = len(lens)
+    qkv, _, _ = inputs(B, n, g, 1, D, [1], torch.bfloat16)
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    k, v = (torch.randn((B, 1, cap, D), device="cuda", generator=gen).to(torch.bfloat16) for _ in range(2))
+    view = kva.KVView.contiguous(k, v, torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    tree = kva.DraftTree.chain(B, n, "cuda")
+    d = qkv.cuda()
+    for call in range(2):
+        w = torch.zeros((B, 1, cap + n), device="cuda")
+        poison(view)  # the second call's workspace
+        out, lse = kva.tree_attention(d[:, :, :g], d[:, :, g:g + 1], d[:, :, g + 1:], tree, view, weights=w,
+                                      return_lse=True)
+    sees = oa.tree_sees(list(range(-1, n - 1)))
+    for b, x in enumerate(lens):
+        o, l, s = oa.attention(qkv[b, :, :g], qkv[b, :, g:g + 1], qkv[b, :, g + 1:], sees, k[b, :, :x].cpu(),
+                               v[b, :, :x].cpu(), D ** -0.5)
+        big = max(float(qkv[b, :, g + 1:].abs().max()), float(v[b, :, :max(x, 1)].abs().max()))
+        check(out[b], o, 2 * STEP[torch.bfloat16] * big, ("out", b))
+        check(lse[b], l, 3e-5, ("lse", b))
+        check(w[b, :, :x + n], s, 5e-5 * (n * g) ** 0.5 + 1e-6, ("weights", b))
+        assert not w[b, :, x + n:].any()

@@ -90,6 +90,14 @@ __device__ __forceinline__ uint64_t steps_before(const Attn& P, uint32_t b) {
   return sum * P.c.v.hk;
 }
 
+// Blocks that share `total` steps.  The grid is laid out for max_len; where the
+// lengths on the device leave fewer steps than blocks, the blocks past the last
+// step take none, so that every block between a unit's first and last has left
+// a partial sum.
+__device__ __forceinline__ uint32_t sharers(const Attn& P, uint64_t total) {
+  return total < P.ctas ? uint32_t(total) : P.ctas;
+}
+
 // First segment of grid block `cta` (warp-collective); false: it has none.
 __device__ __forceinline__ bool first_seg(const Attn& P, uint32_t cta, Seg& s) {
   if (!P.ctas) {  // the units of a request with the most steps first
@@ -105,10 +113,11 @@ __device__ __forceinline__ bool first_seg(const Attn& P, uint32_t cta, Seg& s) {
     return true;
   }
   const uint64_t total = steps_before(P, P.c.v.B);
+  const uint32_t ctas = sharers(P, total);
+  if (cta >= ctas) return false;
   const uint64_t top = total * (cta + 1);
-  s.at = top >> 32 ? (top - total) / P.ctas : uint32_t(top - total) / P.ctas;
-  s.end = top >> 32 ? top / P.ctas : uint32_t(top) / P.ctas;
-  if (s.at >= s.end) return false;
+  s.at = top >> 32 ? (top - total) / ctas : uint32_t(top - total) / ctas;
+  s.end = top >> 32 ? top / ctas : uint32_t(top) / ctas;
   uint64_t base = 0;
   const uint32_t lane = threadIdx.x & 31u;
   for (uint32_t b0 = 0;; b0 += 32) {
@@ -169,10 +178,11 @@ __device__ __forceinline__ bool next_seg(const Attn& P, Seg& s) {
 // of the list: first .. last, and first's slot is its second one.
 __device__ __forceinline__ void owners(const Attn& P, uint64_t total, uint64_t at, uint32_t steps, uint32_t& first,
                                        uint32_t& last) {
-  // block c covers [total * c / ctas, total * (c + 1) / ctas): x is in the
-  // largest c with total * c / ctas <= x, that is total * c < ctas * (x + 1)
+  // block c covers [total * c / ctas, total * (c + 1) / ctas), one step at least:
+  // x is in the largest c with total * c / ctas <= x, that is total * c < ctas * (x + 1)
+  const uint32_t ctas = sharers(P, total);
   auto holder = [&](uint64_t x) {
-    const uint64_t top = uint64_t(P.ctas) * (x + 1) - 1;
+    const uint64_t top = uint64_t(ctas) * (x + 1) - 1;
     return top >> 32 ? uint32_t(top / total) : uint32_t(top) / uint32_t(total);
   };
   first = holder(at);
