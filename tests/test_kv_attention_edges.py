@@ -48,3 +48,42 @@ def test_lengths_far_below_the_bound(lens, n, g, D):
         check(lse[b], l, 3e-5, ("lse", b))
         check(w[b, :, :x + n], s, 5e-5 * (n * g) ** 0.5 + 1e-6, ("weights", b))
         assert not w[b, :, x + n:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,g", [(1, 2), (40, 4)])
+def test_a_captured_graph_keeps_its_workspace(n, g):
+    """A larger call on the same stream and view must not give a captured call's workspace to other tensors."""
+    from voom_b200.runtime import kv_attention as kva
+
+    qkv, k, v = inputs(1, 90, g, 1, 128, [6000], torch.bfloat16)
+    d = qkv.cuda()
+    view = place(k, v, [6000], "whole", 0)
+
+    def call(m, **kw):
+        x = d[:, :m]
+        return kva.tree_attention(x[:, :, :g], x[:, :, g:g + 1], x[:, :, g + 1:], kva.DraftTree.chain(1, m, "cuda"), view,
+                                  **kw)
+
+    want = call(n)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(n)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = call(n)
+    with torch.cuda.stream(side):
+        w = torch.zeros((1, 1, view.max_len + 90), device="cuda")
+        call(90, weights=w)
+        call(3, weights=w)
+        others = [torch.full((size,), 7, dtype=torch.uint8, device="cuda")
+                  for size in (1 << 12, 1 << 16, 1 << 18, 1 << 20, 1 << 21, 1 << 22, 1 << 23, 1 << 24, 1 << 25) for _ in range(4)]
+    torch.cuda.synchronize()
+    out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    for t in others:
+        assert bool((t == 7).all())

@@ -39,6 +39,11 @@ def raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+def capturing() -> bool:
+    """The current stream is being captured into a graph."""
+    return torch._C._cuda_isCurrentStreamCapturing()
+
+
 class on_stream:
     """`with on_stream(device, stream) as ptr`: inside, `device` is current and
     `stream` (None: the device's current stream) is the current stream, so

@@ -147,7 +147,8 @@ class KVView:
 
     def more_scratch(self, n: int, stream_ptr: int) -> tuple[int, int]:
         """(address, bytes) of a workspace of at least n bytes for the calls on
-        one stream, kept with the view."""
+        one stream, kept with the view until a call needs more.  Calls that are
+        captured do not use it: a graph keeps the address that it was given."""
         t = torch.empty(n, dtype=torch.uint8, device=self.device)
         self._scratch[stream_ptr] = t
         s = self.scratch[stream_ptr] = (t.data_ptr(), n)
@@ -277,11 +278,16 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: Draf
                        tree.mask_ptr, wp, tw, cache.status_ptr, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], os[0],
                        os[1], os[2], wb, wh, n, hq, cache.scale if scale is None else scale)
         lib, sp = load(), _device.raw_stream(cache.index)
-        ws = cache.scratch.get(sp, _NO_SCRATCH)
-        rc = lib.voom_tree_attention(cache.packed, a, ws[0], ws[1], sp)
-        if rc == VOOM_E_CAPACITY:  # refused before anything was launched
-            ws = cache.more_scratch(lib.voom_tree_attention_scratch_bytes(cache.packed, a), sp)
+        if _device.capturing():
+            # a workspace from the graph's own pool, which no tensor outside the graph gets for as long as it lives
+            ws = q.new_empty(lib.voom_tree_attention_scratch_bytes(cache.packed, a), dtype=torch.uint8)
+            rc = lib.voom_tree_attention(cache.packed, a, ws.data_ptr(), ws.numel(), sp)
+        else:
+            ws = cache.scratch.get(sp, _NO_SCRATCH)
             rc = lib.voom_tree_attention(cache.packed, a, ws[0], ws[1], sp)
+            if rc == VOOM_E_CAPACITY:  # refused before anything was launched
+                ws = cache.more_scratch(lib.voom_tree_attention_scratch_bytes(cache.packed, a), sp)
+                rc = lib.voom_tree_attention(cache.packed, a, ws[0], ws[1], sp)
         check(rc, "voom_tree_attention")
     return (out, lse) if return_lse else out
 
