@@ -87,3 +87,38 @@ def test_a_captured_graph_keeps_its_workspace(n, g):
     assert torch.equal(out, want)
     for t in others:
         assert bool((t == 7).all())
+
+
+@pytest.mark.gpu
+def test_threads_on_one_stream_do_not_mix_their_calls():
+    """Two host threads, one stream, one view: the launches of a call stay together."""
+    import threading
+
+    from voom_b200.runtime import kv_attention as kva
+
+    qkv, k, v = inputs(1, 2, 8, 2, 128, [9000], torch.bfloat16)
+    d = qkv.cuda()
+    view = place(k, v, [9000], "whole", 0)
+    tree = kva.DraftTree.chain(1, 1, "cuda")
+    stream = torch.cuda.current_stream()
+
+    def call(i):
+        x = d[:, i:i + 1]
+        return kva.tree_attention(x[:, :, :8], x[:, :, 8:10], x[:, :, 10:], tree, view)
+
+    want = [call(0), call(1)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(stream):
+            got = [call(i) for _ in range(300)]
+            torch.cuda.synchronize()
+            wrong.extend(i for x in got if not torch.equal(x, want[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

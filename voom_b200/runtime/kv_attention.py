@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
+import threading
 from typing import NamedTuple
 
 import numpy as np
@@ -77,6 +78,7 @@ class KVView:
         self.index = self.device.index
         self._scratch: dict[int, torch.Tensor] = {}
         self.scratch: dict[int, tuple[int, int]] = {}  # stream -> address, bytes
+        self.lock = threading.Lock()  # a call's launches share the stream's workspace: they stay together
 
     @classmethod
     def contiguous(cls, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, max_len: int | None = None) -> "KVView":
@@ -283,11 +285,12 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: Draf
             ws = q.new_empty(lib.voom_tree_attention_scratch_bytes(cache.packed, a), dtype=torch.uint8)
             rc = lib.voom_tree_attention(cache.packed, a, ws.data_ptr(), ws.numel(), sp)
         else:
-            ws = cache.scratch.get(sp, _NO_SCRATCH)
-            rc = lib.voom_tree_attention(cache.packed, a, ws[0], ws[1], sp)
-            if rc == VOOM_E_CAPACITY:  # refused before anything was launched
-                ws = cache.more_scratch(lib.voom_tree_attention_scratch_bytes(cache.packed, a), sp)
+            with cache.lock:
+                ws = cache.scratch.get(sp, _NO_SCRATCH)
                 rc = lib.voom_tree_attention(cache.packed, a, ws[0], ws[1], sp)
+                if rc == VOOM_E_CAPACITY:  # refused before anything was launched
+                    ws = cache.more_scratch(lib.voom_tree_attention_scratch_bytes(cache.packed, a), sp)
+                    rc = lib.voom_tree_attention(cache.packed, a, ws[0], ws[1], sp)
         check(rc, "voom_tree_attention")
     return (out, lse) if return_lse else out
 
