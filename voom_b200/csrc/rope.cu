@@ -206,7 +206,8 @@ __device__ __forceinline__ void load_weights(const Rope& P, const void* w, uint3
 // w the weights and c, s the pair's cosine and sine, a task's two chunks x, y
 // become  r (x A + y B),  r (x C + y D)  in the half layout (A = w_x c, B =
 // -w_y s, C = w_x s, D = w_y c), and each of them  r (x P + swapped x Q)  in the
-// interleaved one; values that are not rotated have c = 1, s = 0.
+// interleaved one.  Values that are not rotated take their own weight alone: a
+// neighbour that is not finite must not reach them, not even times 0.
 template <typename T, int VEC, int KT, bool INTER>
 __global__ void __launch_bounds__(kThreads, KT * VEC == 8 ? 6 : 4) qk_norm_rope(const __grid_constant__ Rope P) {
   constexpr int N = VEC > 1 ? VEC / 2 : 1;        // register pairs of a chunk
@@ -379,19 +380,29 @@ __global__ void __launch_bounds__(kThreads, KT * VEC == 8 ? 6 : 4) qk_norm_rope(
     for (int k = 0; k < KT; k++) {
       if (!c[k].has) continue;
       if constexpr (VEC == 1) {  // (x C + y D, x A + y B) at once
-        F2 o = fma2(make2(y[k][0], y[k][0]), cb[k][0], mul2(make2(x[k][0], x[k][0]), ca[k][0]));
+        F2 o;
+        if (c[k].rotated) {
+          o = fma2(make2(y[k][0], y[k][0]), cb[k][0], mul2(make2(x[k][0], x[k][0]), ca[k][0]));
+        } else {
+          float a0, a1, b0, b1;
+          take2(ca[k][0], a0, a1);
+          take2(cb[k][0], b0, b1);
+          o = mul2(make2(x[k][0], y[k][0]), make2(a0, b1));
+        }
         take2(mul2(o, rr), x[k][0], y[k][0]);
       } else {
 #pragma unroll
         for (int i = 0; i < N; i++) {
           const F2 u = mul2(make2(x[k][2 * i], x[k][2 * i + 1]), rr), v = mul2(make2(y[k][2 * i], y[k][2 * i + 1]), rr);
-          F2 p, q;
-          if constexpr (SWAP) {
-            p = fma2(swap2(u), cb[k][i], mul2(u, ca[k][i]));
-            q = fma2(swap2(v), cd[k][i], mul2(v, cc[k][i]));
-          } else {
-            p = fma2(v, cb[k][i], mul2(u, ca[k][i]));
-            q = fma2(v, cd[k][i], mul2(u, cc[k][i]));
+          F2 p = mul2(u, ca[k][i]), q = mul2(v, SWAP ? cc[k][i] : cd[k][i]);
+          if (c[k].rotated) {
+            if constexpr (SWAP) {
+              p = fma2(swap2(u), cb[k][i], p);
+              q = fma2(swap2(v), cd[k][i], q);
+            } else {
+              p = fma2(v, cb[k][i], p);
+              q = fma2(v, cd[k][i], mul2(u, cc[k][i]));
+            }
           }
           take2(p, x[k][2 * i], x[k][2 * i + 1]);
           take2(q, y[k][2 * i], y[k][2 * i + 1]);
