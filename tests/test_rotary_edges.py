@@ -53,3 +53,50 @@ def test_an_infinity_in_a_normed_head(layout, offset):
     other[70] = False
     assert bool(got[0, 0, 70].isnan()) and bool((got[0, 0].cpu()[other] == 0).all())
     assert bool(torch.isfinite(got[0, 1]).all())
+
+
+def _base(r=64, theta=10000.0):
+    return [theta ** (-2.0 * i / r) for i in range(r // 2)]
+
+
+def test_yarn_keys_of_model_configurations():
+    from voom_b200.runtime.rotary import _scaled
+
+    r, theta, factor, orig = 64, 10000.0, 40.0, 4096
+    yarn = {"rope_type": "yarn", "factor": factor, "original_max_position_embeddings": orig}
+    f, a = _scaled(_base(), r, theta, yarn)
+
+    def gain(m):
+        return 0.1 * m * math.log(factor) + 1.0
+
+    assert math.isclose(a, gain(1.0))
+    assert math.isclose(_scaled(_base(), r, theta, {**yarn, "mscale": 1.0, "mscale_all_dim": 1.0})[1], 1.0)
+    assert math.isclose(_scaled(_base(), r, theta, {**yarn, "mscale": 0.707, "mscale_all_dim": 0.5})[1], gain(0.707) / gain(0.5))
+    assert _scaled(_base(), r, theta, {**yarn, "mscale": 0.707, "mscale_all_dim": 0.5, "attention_factor": 1.5})[1] == 1.5
+    with pytest.raises(ValueError, match="together"):
+        _scaled(_base(), r, theta, {**yarn, "mscale": 0.707})
+    # the ramp between the pairs that make 32 turns and 1 turn over the original context, not rounded to whole pairs
+    g, _ = _scaled(_base(), r, theta, {**yarn, "truncate": False})
+    ends = [r * math.log(orig / (t * 2 * math.pi)) / (2 * math.log(theta)) for t in (32.0, 1.0)]
+    for i, (x, y) in enumerate(zip(g, _base())):
+        ramp = min(max((i - ends[0]) / (ends[1] - ends[0]), 0.0), 1.0)
+        assert math.isclose(x, y / factor * ramp + y * (1.0 - ramp), rel_tol=1e-12)
+    assert g != f and _scaled(_base(), r, theta, {**yarn, "truncate": True})[0] == f
+
+
+def test_default_scaling_and_keys_that_would_be_ignored():
+    from voom_b200.runtime.rotary import _scaled
+
+    assert _scaled(_base(), 64, 10000.0, {"rope_type": "default"}) == (_base(), 1.0)
+    assert _scaled(_base(), 64, 10000.0, {"rope_type": "default", "rope_theta": 10000.0}) == (_base(), 1.0)
+    assert _scaled(_base(), 64, 10000.0, {"type": "linear", "factor": 2, "truncate": None})[1] == 1.0
+    for scaling in ({"rope_type": "default", "factor": 2.0}, {"rope_type": "default", "rope_theta": 5e5},
+                    {"rope_type": "linear", "factor": 2.0, "mscale": 1.0},
+                    {"rope_type": "llama3", "factor": 2.0, "beta_fast": 32},
+                    {"rope_type": "yarn", "factor": 2.0, "original_max_position_embeddings": 4096, "other": 1}):
+        with pytest.raises(ValueError, match="rotary scaling"):
+            _scaled(_base(), 64, 10000.0, scaling)
+    half = {"rope_type": "default", "partial_rotary_factor": 0.5}
+    assert _scaled(_base(), 64, 10000.0, half, 128) == (_base(), 1.0)
+    with pytest.raises(ValueError, match="rotary scaling"):
+        _scaled(_base(), 64, 10000.0, half, 64)

@@ -23,43 +23,83 @@ LAYOUTS = ("half", "interleaved")
 MAX_HEAD_DIM = 512
 
 
-def _scaled(freqs: list[float], rot_dim: int, theta: float, scaling: dict) -> tuple[list[float], float]:
+_COMMON_KEYS = {"rope_type", "type", "factor", "rope_theta", "partial_rotary_factor"}
+_SCALING_KEYS = {
+    "default": set(),
+    "linear": set(),
+    "ntk": set(),
+    "yarn": {"original_max_position_embeddings", "beta_fast", "beta_slow", "attention_factor", "mscale",
+             "mscale_all_dim", "truncate"},
+    "llama3": {"original_max_position_embeddings", "low_freq_factor", "high_freq_factor"},
+}
+
+
+def _scaled(freqs: list[float], rot_dim: int, theta: float, scaling: dict,
+            head_dim: int | None = None) -> tuple[list[float], float]:
     """Frequencies (radians per position) stretched for a longer context, and
     the factor on the rotated values.  `scaling` uses the names of model
-    configurations: rope_type linear, ntk, yarn or llama3."""
+    configurations: rope_type default (no stretching), linear, ntk, yarn or
+    llama3.  A key that is not known for its type is refused, and so is one
+    (rope_theta, partial_rotary_factor) that contradicts the arguments: each may
+    change the angles."""
     kind = scaling.get("rope_type", scaling.get("type"))
-    factor = float(scaling.get("factor", 1.0))
+    if kind not in _SCALING_KEYS:
+        raise ValueError(f"unknown rotary scaling {kind!r} (one of {', '.join(_SCALING_KEYS)})")
+    given = {k: v for k, v in scaling.items() if v is not None}
+    unknown = sorted(set(given) - _COMMON_KEYS - _SCALING_KEYS[kind])
+    if unknown:
+        raise ValueError(f"rotary scaling {kind!r} does not take {', '.join(map(repr, unknown))}")
+    if float(given.get("rope_theta", theta)) != theta:
+        raise ValueError(f"rotary scaling says rope_theta {given['rope_theta']}, the argument theta is {theta}")
+    if head_dim and "partial_rotary_factor" in given and \
+            abs(head_dim * float(given["partial_rotary_factor"]) - rot_dim) >= 1.0:
+        raise ValueError(f"rotary scaling rotates {given['partial_rotary_factor']} of a head of {head_dim}, the argument "
+                         f"rot_dim is {rot_dim}")
+    factor = float(given.get("factor", 1.0))
     if factor < 1.0:
         raise ValueError(f"rotary scaling factor {factor}: at least 1")
+    if kind == "default":
+        if factor != 1.0:
+            raise ValueError(f"rotary scaling 'default' does not stretch, got factor {factor}")
+        return freqs, 1.0
     if kind == "linear":
         return [f / factor for f in freqs], 1.0
     if kind == "ntk":
         base = theta * factor ** (rot_dim / max(rot_dim - 2, 1))
         return [base ** (-2.0 * i / rot_dim) for i in range(rot_dim // 2)], 1.0
     if kind == "yarn":
-        orig = float(scaling["original_max_position_embeddings"])
+        orig = float(given["original_max_position_embeddings"])
 
         def pair_with(turns: float) -> float:  # the pair that makes `turns` turns over the original context
             return rot_dim * math.log(orig / (turns * 2 * math.pi)) / (2 * math.log(theta))
 
-        lo = max(math.floor(pair_with(float(scaling.get("beta_fast", 32.0)))), 0)
-        hi = min(math.ceil(pair_with(float(scaling.get("beta_slow", 1.0)))), rot_dim - 1)
+        lo, hi = pair_with(float(given.get("beta_fast", 32.0))), pair_with(float(given.get("beta_slow", 1.0)))
+        if given.get("truncate", True):  # the ramp starts and ends on whole pairs
+            lo, hi = math.floor(lo), math.ceil(hi)
+        lo, hi = max(lo, 0), min(hi, rot_dim - 1)
         out = []
         for i, f in enumerate(freqs):
             ramp = min(max((i - lo) / max(hi - lo, 0.001), 0.0), 1.0)
             out.append(f / factor * ramp + f * (1.0 - ramp))
-        attention = scaling.get("attention_factor")
-        return out, 0.1 * math.log(factor) + 1.0 if attention is None else float(attention)
-    if kind == "llama3":
-        orig = float(scaling["original_max_position_embeddings"])
-        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
-        out = []
-        for f in freqs:
-            turns = orig * f / (2 * math.pi)  # turns over the original context
-            keep = min(max((turns - low) / (high - low), 0.0), 1.0)
-            out.append(f / factor * (1.0 - keep) + f * keep)
-        return out, 1.0
-    raise ValueError(f"unknown rotary scaling {kind!r} (one of linear, ntk, yarn, llama3)")
+        if "attention_factor" in given:
+            return out, float(given["attention_factor"])
+        if "mscale" in given or "mscale_all_dim" in given:
+            if not ("mscale" in given and "mscale_all_dim" in given):
+                raise ValueError("rotary scaling 'yarn' takes mscale and mscale_all_dim together")
+
+            def gain(m: float) -> float:
+                return 0.1 * m * math.log(factor) + 1.0
+
+            return out, gain(float(given["mscale"])) / gain(float(given["mscale_all_dim"]))
+        return out, 0.1 * math.log(factor) + 1.0
+    orig = float(given["original_max_position_embeddings"])
+    low, high = float(given["low_freq_factor"]), float(given["high_freq_factor"])
+    out = []
+    for f in freqs:
+        turns = orig * f / (2 * math.pi)  # turns over the original context
+        keep = min(max((turns - low) / (high - low), 0.0), 1.0)
+        out.append(f / factor * (1.0 - keep) + f * keep)
+    return out, 1.0
 
 
 class Rotary:
@@ -85,7 +125,7 @@ class Rotary:
         freqs = [self.theta ** (-2.0 * i / rot_dim) for i in range(rot_dim // 2)]
         self.factor = 1.0
         if scaling is not None:
-            freqs, self.factor = _scaled(freqs, rot_dim, self.theta, scaling)
+            freqs, self.factor = _scaled(freqs, rot_dim, self.theta, scaling, head_dim)
         self.freqs = freqs
         turns = [round(f / (2 * math.pi) * 2 ** 64) % 2 ** 64 for f in freqs]
         self.device = _device.require_cuda(device)
