@@ -613,9 +613,12 @@ int voom_qk_norm_rope(const voom_qk_norm_rope_args* a, void* stream);
  *                  rows start at index * k_page (index outside [0, n_pages)
  *                  reads as zero keys and values);
  *   pages anywhere: d_offsets[2 * (b * table_stride + p)] / [.. + 1] are
- *                  the element offsets of the page's keys / values from d_k / d_v.
+ *                  the element offsets of the page's keys / values from d_k / d_v;
+ *                  VOOM_NO_PAGE as the first reads as zero keys and values.
  * Position s of head h lies (s / page)-th page, + h * k_head + (s % page) * k_pos.
- * d_len[b] positions are valid (clamped to max_len and to what the table holds). */
+ * d_len[b] positions are valid (clamped to 0 .. max_len, which the table's
+ * table_stride pages must hold; a request with fewer pages says so in its entries). */
+#define VOOM_NO_PAGE INT64_MIN
 typedef struct voom_kv_view {
   const void* d_k;
   const void* d_v;

@@ -122,3 +122,68 @@ def test_threads_on_one_stream_do_not_mix_their_calls():
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,g,D", [(1, 4, 64), (40, 4, 128), (20, 2, 256)])
+def test_a_length_past_a_requests_own_pages_reads_zeros(n, g, D):
+    """Requests of unequal page lists: what a request has no page for is zero keys and values, never another's."""
+    from voom_b200.runtime import kv_attention as kva
+
+    page, lists = 16, [9, 2, 0]
+    gen = torch.Generator().manual_seed(5)
+    k, v = (torch.randn((3, 9 * page, D), generator=gen).to(torch.bfloat16) for _ in range(2))
+    for b, m in enumerate(lists):
+        k[b, m * page:] = 0
+        v[b, m * page:] = 0
+
+    def cut(x, b, p):
+        return x[b, p * page:(p + 1) * page].cuda()[None, None]
+
+    view = kva.KVView.pages([[(cut(k, b, p), cut(v, b, p)) for p in range(m)] for b, m in enumerate(lists)],
+                            torch.tensor([140, 140, 20], dtype=torch.int32, device="cuda"))
+    qkv, _, _ = inputs(3, n, g, 1, D, [1], torch.bfloat16)
+    d = qkv.cuda()
+    out, lse = kva.tree_attention(d[:, :, :g], d[:, :, g:g + 1], d[:, :, g + 1:], kva.DraftTree.chain(3, n, "cuda"), view,
+                                  return_lse=True)
+    sees = oa.tree_sees(list(range(-1, n - 1)))
+    for b, x in enumerate([140, 140, 20]):
+        o, l, _ = oa.attention(qkv[b, :, :g], qkv[b, :, g:g + 1], qkv[b, :, g + 1:], sees, k[b:b + 1, :x], v[b:b + 1, :x],
+                               D ** -0.5)
+        check(out[b], o, 2 * STEP[torch.bfloat16] * 6.0, ("out", b))
+        check(lse[b], l, 3e-5, ("lse", b))
+    w = torch.rand((3, 1, 9 * page), generator=gen)
+    e = kva.kv_evict(view, w.cuda(), budget=50, sinks=2, recent=3)
+    for b, x in enumerate([140, 140, 20]):
+        want = oa.kept(w[b, 0].tolist(), x, 50, 2, 3)
+        assert torch.equal(e.k[b, 0, :len(want)].cpu(), k[b, want]) and torch.equal(e.v[b, 0, :len(want)].cpu(), v[b, want])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 5])  # through TMA, and gathered
+@pytest.mark.parametrize("n,g", [(1, 4), (40, 4)])
+def test_a_pool_entry_that_is_no_page_reads_zeros(page, n, g):
+    from voom_b200.runtime import kv_attention as kva
+
+    L, D = 400, 64
+    per = L // page
+    gen = torch.Generator().manual_seed(6)
+    kp, vp = (torch.randn((per, 1, page, D), generator=gen).to(torch.bfloat16) for _ in range(2))
+    table = torch.arange(per, dtype=torch.int32)
+    for at, entry in ((1, -1), (per // 2, per), (per - 1, -7)):
+        table[at] = entry
+        kp[at] = 0
+        vp[at] = 0
+    kd, vd = kp.cuda(), vp.cuda()
+    for at in (1, per // 2, per - 1):  # no entry names them
+        kd[at] = math.nan
+        vd[at] = math.nan
+    view = kva.KVView.pool(kd, vd, table[None].cuda(), torch.tensor([L], dtype=torch.int32, device="cuda"))
+    qkv, _, _ = inputs(1, n, g, 1, D, [1], torch.bfloat16)
+    d = qkv.cuda()
+    out = kva.tree_attention(d[:, :, :g], d[:, :, g:g + 1], d[:, :, g + 1:], kva.DraftTree.chain(1, n, "cuda"), view)
+    o, _, _ = oa.attention(qkv[0, :, :g], qkv[0, :, g:g + 1], qkv[0, :, g + 1:], oa.tree_sees(list(range(-1, n - 1))),
+                           kp.reshape(1, L, D), vp.reshape(1, L, D), D ** -0.5)
+    check(out[0], o, 2 * STEP[torch.bfloat16] * 6.0, "out")
+    e = kva.kv_evict(view, torch.zeros((1, 1, L), device="cuda"), budget=L - 1, sinks=0, recent=L - 1)
+    assert torch.equal(e.k[0, 0].cpu(), kp.reshape(L, D)[1:]) and torch.equal(e.v[0, 0].cpu(), vp.reshape(L, D)[1:])

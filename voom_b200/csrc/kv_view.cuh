@@ -36,6 +36,7 @@ struct View {
       w = int64_t(i) * v.v_page;
     } else if (v.d_offsets) {
       const longlong2 o = __ldg(reinterpret_cast<const longlong2*>(v.d_offsets) + uint64_t(b) * v.table_stride + p);
+      if (o.x == VOOM_NO_PAGE) return false;
       k = o.x;
       w = o.y;
     } else {

@@ -33,6 +33,7 @@ from .._lib import VOOM_E_CAPACITY, ELEMENT_TYPES, KvEvictArgs, KvViewStruct, Tr
 
 MAX_HEAD_DIM = 256
 MAX_TREE = 1024  # tokens of a tree that is not a chain
+NO_PAGE = -2 ** 63  # VOOM_NO_PAGE
 _NO_SCRATCH = (None, 0)
 _CACHE_TYPES = (torch.bfloat16, torch.float16)
 
@@ -112,7 +113,8 @@ class KVView:
     def pages(cls, pages: list[list[tuple[torch.Tensor, torch.Tensor]]], lengths: torch.Tensor,
               max_len: int | None = None) -> "KVView":
         """One list of (k, v) pages per request, each (1, heads, positions, D)
-        or (heads, positions, D) with the same strides, anywhere on the device."""
+        or (heads, positions, D) with the same strides, anywhere on the device.
+        Positions past a request's own pages read as zero keys and values."""
         flat = [p for request in pages for p in request]
         if not flat:
             raise ValueError("a view of pages needs at least one page")
@@ -130,7 +132,7 @@ class KVView:
         H, P, D = k0.shape[-3:]
         per = max(len(request) for request in pages)
         e = k0.element_size()
-        off = np.zeros((len(pages), per, 2), np.int64)
+        off = np.full((len(pages), per, 2), NO_PAGE, np.int64)
         for b, request in enumerate(pages):
             for p, (k, v) in enumerate(request):
                 off[b, p] = (k.data_ptr() - k0.data_ptr()) // e, (v.data_ptr() - v0.data_ptr()) // e
