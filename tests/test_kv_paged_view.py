@@ -1,0 +1,56 @@
+"""PagedKVCache as the attention and the eviction read and write it: pages of
+their own, one key head, spilled pages, evictions that leave many pages."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+
+def _plain(t):
+    return t.stride() == torch.empty(t.shape, device="meta").stride() and \
+        t.untyped_storage().nbytes() == t.numel() * t.element_size()
+
+
+@pytest.mark.parametrize("hk", [1, 2])
+@pytest.mark.parametrize("sizes", [(53,), (16,), (5, 30, 16, 1), (15, 1, 64)])
+def test_pages_are_pieces_of_their_own(tmp_path, hk, sizes):
+    """Plain strides, and no page holds the bytes of its neighbours."""
+    from voom_b200.runtime.kv_paged import PagedKVCache
+
+    kv = PagedKVCache(1, 1 << 40, tmp_path, page_positions=16)
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn((1, hk, sum(sizes), 64), generator=g).to(torch.bfloat16) for _ in range(2))
+    at = 0
+    for n in sizes:
+        K, V = kv.update(0, k[:, :, at:at + n].clone(), v[:, :, at:at + n].clone())
+        at += n
+        assert torch.equal(K, k[:, :, :at]) and torch.equal(V, v[:, :, :at])
+        assert kv.length(0) == at == kv.offset and len(kv._pages[0]) == at // 16
+    assert all(_plain(x) for p in kv._pages[0] for x in (p.k, p.v))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("compress", [False, True])
+@pytest.mark.parametrize("hk,n", [(1, 53), (1, 16), (2, 160)])
+def test_pages_of_one_key_head_in_place_and_evicted(tmp_path, compress, hk, n):
+    """One key head, a prompt longer than a page, spilled pages, and an eviction that leaves many pages."""
+    from voom_b200.runtime.kv_attention import DraftTree, KVView, tree_attention
+    from voom_b200.runtime.kv_paged import PagedKVCache
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    kv = PagedKVCache(1, 20000, tmp_path / "a", page_positions=16, compress_spill=compress)
+    k, v = (torch.randn((1, hk, n, 64), device="cuda", generator=g).to(torch.bfloat16) for _ in range(2))
+    K, V = kv.update(0, k, v)
+    assert torch.equal(K, k) and torch.equal(V, v)
+    q = torch.randn((1, 3, 4, 64), device="cuda", generator=g).to(torch.bfloat16)
+    kn, vn = (torch.randn((1, 3, hk, 64), device="cuda", generator=g).to(torch.bfloat16) for _ in range(2))
+    tree = DraftTree.chain(1, 3, "cuda")
+    whole = KVView.contiguous(K, V, torch.tensor([n], dtype=torch.int32, device="cuda"))
+    assert torch.equal(tree_attention(q, kn, vn, tree, kv.view(0)), tree_attention(q, kn, vn, tree, whole))
+    w = torch.rand((1, hk, n), device="cuda", generator=g)
+    m = n - 5
+    e = kv.evict(0, w, budget=m, sinks=2, recent=4)
+    assert kv.length(0) == m
+    K2, V2 = kv.update(0, k[:, :, :3], v[:, :, :3])
+    assert torch.equal(K2[:, :, :m], e.k) and torch.equal(V2[:, :, :m], e.v) and torch.equal(K2[:, :, m:], k[:, :, :3])

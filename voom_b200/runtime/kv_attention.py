@@ -44,6 +44,11 @@ def _rows(x: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name}: heads must be contiguous and every row must start on 16 bytes")
 
 
+def _steps(x: torch.Tensor) -> tuple:
+    """Strides of a (.., heads, positions, D) page; 0 where there is one of a kind and any stride will do."""
+    return tuple(s if n > 1 else 0 for s, n in zip(x.stride()[-3:], x.shape[-3:]))
+
+
 class KVView:
     """Keys and values of B requests as the attention reads them; holds the
     tensors.  `lengths` is an int32 device tensor of the B requests' cached
@@ -119,9 +124,9 @@ class KVView:
         if not flat:
             raise ValueError("a view of pages needs at least one page")
         k0, v0 = flat[0]
-        ks, vs = k0.stride()[-3:], v0.stride()[-3:]
+        ks, vs = _steps(k0), _steps(v0)
         for k, v in flat:
-            if k.shape != k0.shape or v.shape != k0.shape or k.stride()[-3:] != ks or v.stride()[-3:] != vs:
+            if k.shape != k0.shape or v.shape != k0.shape or _steps(k) != ks or _steps(v) != vs:
                 raise ValueError("all pages must have one shape and one set of strides")
             if k.dtype != k0.dtype or v.dtype != k0.dtype or k.device != k0.device or v.device != k0.device:
                 raise ValueError("all pages must have one type and lie on one device")

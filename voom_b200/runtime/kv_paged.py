@@ -97,6 +97,17 @@ def _read_safetensors(path: Path, device) -> dict[str, torch.Tensor]:
     return out
 
 
+def _piece(t: torch.Tensor, a: int, b: int) -> torch.Tensor:
+    """Positions [a, b) of (1, H, n, D) with a storage and plain strides of their
+    own, so that dropping the piece frees its bytes (`.contiguous()` alone takes
+    a slice of a single head for contiguous as it is)."""
+    piece = t[:, :, a:b]
+    plain = torch.empty(piece.shape, dtype=t.dtype, device=t.device)
+    if piece.stride() == plain.stride() and piece.untyped_storage().nbytes() == plain.untyped_storage().nbytes():
+        return piece
+    return plain.copy_(piece)
+
+
 class _Page:
     __slots__ = ("k", "v", "path", "nbytes", "_compressed", "shape", "device")
 
@@ -286,12 +297,13 @@ class PagedKVCache:
         else:
             self._tail_k[layer] = torch.cat([self._tail_k[layer], k], dim=2)
             self._tail_v[layer] = torch.cat([self._tail_v[layer], v], dim=2)
-        while self._tail_k[layer].shape[2] >= self.page_positions:
-            pk = self._tail_k[layer][:, :, : self.page_positions, :].contiguous()
-            pv = self._tail_v[layer][:, :, : self.page_positions, :].contiguous()
-            self._pages[layer].append(_Page(pk, pv))
-            self._tail_k[layer] = self._tail_k[layer][:, :, self.page_positions:, :].contiguous()
-            self._tail_v[layer] = self._tail_v[layer][:, :, self.page_positions:, :].contiguous()
+        n, P = int(self._tail_k[layer].shape[2]), self.page_positions
+        if n < P:
+            return
+        k, v = self._tail_k[layer], self._tail_v[layer]
+        for at in range(0, n - P + 1, P):
+            self._pages[layer].append(_Page(_piece(k, at, at + P), _piece(v, at, at + P)))
+        self._tail_k[layer], self._tail_v[layer] = _piece(k, n - n % P, n), _piece(v, n - n % P, n)
 
     def _loaded(self, layer: int) -> list[tuple[torch.Tensor, torch.Tensor]]:
         """Keys and values of the layer's closed pages, spilled ones reloaded."""
@@ -345,7 +357,9 @@ class PagedKVCache:
         self._pages[layer] = []
         self._tail_k[layer] = self._tail_v[layer] = None
         m = min(n, budget)
-        self._extend(layer, e.k[:, :, :m].contiguous(), e.v[:, :, :m].contiguous())
+        # closed pages are copies already; a tail alone must be one too, as the caller has e
+        k, v = (x[:, :, :m] if m >= self.page_positions else _piece(x, 0, m) for x in (e.k, e.v))
+        self._extend(layer, k, v)
         for f in files:
             f.unlink(missing_ok=True)
         return e
