@@ -54,3 +54,51 @@ def test_pages_of_one_key_head_in_place_and_evicted(tmp_path, compress, hk, n):
     assert kv.length(0) == m
     K2, V2 = kv.update(0, k[:, :, :3], v[:, :, :3])
     assert torch.equal(K2[:, :, :m], e.k) and torch.equal(V2[:, :, :m], e.v) and torch.equal(K2[:, :, m:], k[:, :, :3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("compress", [False, True])
+def test_evict_keeps_the_byte_budget(tmp_path, compress):
+    """Pages that were reloaded for the eviction do not stay beyond the budget."""
+    from voom_b200.runtime.kv_paged import PagedKVCache
+
+    g = torch.Generator(device="cuda").manual_seed(2)
+    limit = 60000
+    kv = PagedKVCache(2, limit, tmp_path / "a", page_positions=16, compress_spill=compress)
+    k, v = (torch.randn((1, 2, 300, 64), device="cuda", generator=g).to(torch.bfloat16) for _ in range(2))
+    for layer in range(2):
+        kv.append(layer, k, v)
+    assert kv.nbytes() <= limit
+    w = torch.rand((1, 2, 300), device="cuda", generator=g)
+    kept = []
+    for layer in range(2):
+        kept.append(kv.evict(layer, w, budget=250, sinks=2, recent=4))
+        assert kv.nbytes() <= limit, layer
+    for layer in range(2):  # what was spilled again comes back, and later files are not the deleted ones
+        K, V = kv.update(layer, k[:, :, :1], v[:, :, :1])
+        assert torch.equal(K[:, :, :250], kept[layer].k) and torch.equal(V[:, :, :250], kept[layer].v)
+        assert torch.equal(K[:, :, 250:], k[:, :, :1])
+    kv.release()
+    assert not list((tmp_path / "a").iterdir())
+
+
+def test_evict_keeps_the_byte_budget_on_the_host(tmp_path, monkeypatch):
+    """The same bookkeeping without a GPU: the eviction itself is a stand-in that keeps the first positions."""
+    from voom_b200.runtime import kv_attention
+    from voom_b200.runtime.kv_paged import PagedKVCache
+
+    kv = PagedKVCache(1, 20000, tmp_path, page_positions=16)
+    k = torch.randn((1, 2, 100, 64)).to(torch.bfloat16)
+    kv.append(0, k, k)
+    assert kv.nbytes() <= 20000
+
+    def evict(view, weights, *, budget, sinks, recent):
+        n = torch.arange(budget, dtype=torch.int32).expand(1, 2, -1)
+        return kv_attention.Evicted(k[:, :, :budget], k[:, :, :budget], weights[..., :budget], n, torch.tensor([budget]))
+
+    monkeypatch.setattr(kv_attention, "kv_evict", evict)
+    monkeypatch.setattr(PagedKVCache, "view", lambda self, layer: None)
+    kv.evict(0, torch.zeros((1, 2, 100)), budget=90)
+    assert kv.length(0) == 90 and kv.nbytes() <= 20000
+    K, _ = kv.update(0, k[:, :, :1], k[:, :, :1])
+    assert torch.equal(K, torch.cat((k[:, :, :90], k[:, :, :1]), 2))

@@ -348,7 +348,8 @@ class PagedKVCache:
         positions, `budget` in all (kv_attention.kv_evict; `weights` are the
         running sums of tree_attention).  Returns what kv_evict returned: the
         kept positions' weights and original indexes among it.  `offset` still
-        counts all positions seen."""
+        counts all positions seen.  The byte budget holds afterwards, as after an
+        append to the last layer."""
         from .kv_attention import kv_evict
 
         n = self.length(layer)
@@ -360,8 +361,9 @@ class PagedKVCache:
         # closed pages are copies already; a tail alone must be one too, as the caller has e
         k, v = (x[:, :, :m] if m >= self.page_positions else _piece(x, 0, m) for x in (e.k, e.v))
         self._extend(layer, k, v)
-        for f in files:
+        for f in files:  # before new spills, which may take their names again
             f.unlink(missing_ok=True)
+        self._enforce_budget()
         return e
 
     def update(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
