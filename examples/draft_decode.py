@@ -43,6 +43,8 @@ class AttentionStack:
         self.q_norm = [1 + w(head_dim, std=0.1) for _ in range(layers)]
         self.k_norm = [1 + w(head_dim, std=0.1) for _ in range(layers)]
         self.rotary = Rotary(head_dim, device=device)
+        e = torch.zeros((1, kv_heads, 1, head_dim), dtype=torch.bfloat16, device=device)
+        self.empty = KVView.contiguous(e, e, torch.zeros(1, dtype=torch.int32, device=device), max_len=0)
 
     def __len__(self) -> int:
         return len(self.qkv)
@@ -58,15 +60,11 @@ class AttentionStack:
             qkv = (h @ self.qkv[i].T).view(n, self.hq + 2 * self.hk, self.D)
             q, k, v = qkv.split((self.hq, self.hk, self.hk), dim=1)
             qk_norm_rope(q, k, pos, self.rotary, q_weight=self.q_norm[i], k_weight=self.k_norm[i], out_q=q, out_k=k)
-            view = kv.view(i) if kv.length(i) else self.empty_view()
+            view = kv.view(i) if kv.length(i) else self.empty
             o = tree_attention(q[None], k[None], v[None], tree, view, weights=sums[i][None])
             x = x + o.view(n, -1) @ self.out[i].T
             new.append((k, v))
         return x, new
-
-    def empty_view(self) -> KVView:
-        e = torch.zeros((1, self.hk, 1, self.D), dtype=torch.bfloat16, device=self.device)
-        return KVView.contiguous(e, e, torch.zeros(1, dtype=torch.int32, device=self.device), max_len=0)
 
     def commit(self, new, path: torch.Tensor, kv: PagedKVCache, sums: list[torch.Tensor]) -> None:
         """Appends the accepted tokens (indexes of the tree, root first) to every
@@ -120,6 +118,8 @@ def run(layers: int = 4, prompt: int = 700, steps: int = 20, budget: int = 512, 
             stack.commit(new, torch.tensor(path[::-1], device=dev), kv, sums)
             accepted += len(path)
         torch.cuda.synchronize()
+        stack.empty.check_status()
+        kv.check_status()  # no wait inside a kernel ran out in any layer of any step
         return {"accepted": accepted, "steps": steps, "seconds": time.perf_counter() - t0, "offset": kv.offset,
                 "lengths": [kv.length(i) for i in range(layers)], "hidden": x, "sums": sums}
 

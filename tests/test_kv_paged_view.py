@@ -102,3 +102,41 @@ def test_evict_keeps_the_byte_budget_on_the_host(tmp_path, monkeypatch):
     assert kv.length(0) == 90 and kv.nbytes() <= 20000
     K, _ = kv.update(0, k[:, :, :1], k[:, :, :1])
     assert torch.equal(K, torch.cat((k[:, :, :90], k[:, :, :1]), 2))
+
+
+def test_a_wait_that_ran_out_is_reported_by_the_cache(tmp_path, monkeypatch):
+    """All views share the cache's status word; a kernel's report (here: the test's) reaches check_status()."""
+    from voom_b200.runtime import kv_attention
+    from voom_b200.runtime.kv_paged import PagedKVCache
+
+    words = []
+    monkeypatch.setattr(kv_attention.KVView, "pages", classmethod(lambda cls, *a, status=None, **kw: words.append(status)))
+    kv = PagedKVCache(2, 1 << 40, tmp_path, page_positions=16)
+    kv.check_status()  # no view yet
+    k = torch.zeros((1, 2, 20, 64), dtype=torch.bfloat16)
+    for layer in range(2):
+        kv.append(layer, k, k)
+        kv.view(layer)
+    kv.check_status()
+    words[0].fill_(1)  # a view that is gone by now
+    kv.view(1)
+    assert all(w is words[0] for w in words)
+    with pytest.raises(RuntimeError, match="ran out"):
+        kv.check_status()
+    kv.check_status()
+
+
+@pytest.mark.gpu
+def test_views_of_a_cache_report_to_one_word(tmp_path):
+    from voom_b200.runtime.kv_paged import PagedKVCache
+
+    kv = PagedKVCache(1, 1 << 40, tmp_path, page_positions=16)
+    k = torch.zeros((1, 2, 20, 64), dtype=torch.bfloat16, device="cuda")
+    kv.append(0, k, k)
+    a, b = kv.view(0), kv.view(0)
+    assert a.status_ptr == b.status_ptr == kv._status.data_ptr()
+    assert a.struct.k is not None and a.status.dtype == torch.int32
+    a.status.fill_(1)
+    with pytest.raises(RuntimeError, match="ran out"):
+        kv.check_status()
+    b.check_status()

@@ -49,6 +49,13 @@ def _steps(x: torch.Tensor) -> tuple:
     return tuple(s if n > 1 else 0 for s, n in zip(x.stride()[-3:], x.shape[-3:]))
 
 
+def check_wait_status(status: torch.Tensor) -> None:
+    """Raises RuntimeError if an attention kernel has set the status word; clears it.  Synchronises."""
+    if int(status.item()):
+        status.zero_()
+        raise RuntimeError("tree_attention: a wait inside the kernel ran out")
+
+
 class KVView:
     """Keys and values of B requests as the attention reads them; holds the
     tensors.  `lengths` is an int32 device tensor of the B requests' cached
@@ -57,7 +64,8 @@ class KVView:
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, *, batch: int, heads: int,
                  head_dim: int, page: int, strides: tuple, max_len: int, table: torch.Tensor | None = None,
-                 offsets: torch.Tensor | None = None, table_stride: int = 0, n_pages: int = 0, keep: object = None):
+                 offsets: torch.Tensor | None = None, table_stride: int = 0, n_pages: int = 0, keep: object = None,
+                 status: torch.Tensor | None = None):
         if k.dtype not in _CACHE_TYPES or v.dtype != k.dtype:
             raise ValueError(f"cached keys and values must both be BF16 or FP16, got {k.dtype} and {v.dtype}")
         if head_dim % 8 or not 0 < head_dim <= MAX_HEAD_DIM:
@@ -78,7 +86,7 @@ class KVView:
                                    None if offsets is None else offsets.data_ptr(), *strides, batch, heads, head_dim,
                                    ELEMENT_TYPES[k.dtype], page, table_stride, n_pages, max_len)
         self.packed = bytes(self.struct)
-        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=self.device) if status is None else status
         self.status_ptr = self.status.data_ptr()
         self.scale = head_dim ** -0.5
         self.index = self.device.index
@@ -116,10 +124,11 @@ class KVView:
 
     @classmethod
     def pages(cls, pages: list[list[tuple[torch.Tensor, torch.Tensor]]], lengths: torch.Tensor,
-              max_len: int | None = None) -> "KVView":
+              max_len: int | None = None, status: torch.Tensor | None = None) -> "KVView":
         """One list of (k, v) pages per request, each (1, heads, positions, D)
         or (heads, positions, D) with the same strides, anywhere on the device.
-        Positions past a request's own pages read as zero keys and values."""
+        Positions past a request's own pages read as zero keys and values.
+        `status`: an int32 word on the device that several views share."""
         flat = [p for request in pages for p in request]
         if not flat:
             raise ValueError("a view of pages needs at least one page")
@@ -144,15 +153,13 @@ class KVView:
         offsets = torch.from_numpy(off).to(k0.device)
         return cls(k0, v0, lengths, batch=len(pages), heads=H, head_dim=D, page=P, offsets=offsets, table_stride=per,
                    max_len=P * per if max_len is None else max_len, strides=(0, ks[0], ks[1], 0, vs[0], vs[1]),
-                   keep=flat)
+                   keep=flat, status=status)
 
     def check_status(self) -> None:
         """Raises RuntimeError if a wait inside an attention kernel ran out since
         the last check (its outputs are then not valid); clears the status.
         Synchronises; calls never do, so callers check where they read results."""
-        if int(self.status.item()):
-            self.status.zero_()
-            raise RuntimeError("tree_attention: a wait inside the kernel ran out")
+        check_wait_status(self.status)
 
     def more_scratch(self, n: int, stream_ptr: int) -> tuple[int, int]:
         """(address, bytes) of a workspace of at least n bytes for the calls on

@@ -281,6 +281,7 @@ class PagedKVCache:
         self._tail_v: list[torch.Tensor | None] = []
         self._reset()
         self.stats = KVStats()
+        self._status: torch.Tensor | None = None  # of the attention over every view()
         self._pool = ThreadPoolExecutor(max_workers=max(1, spill_threads))
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
@@ -341,7 +342,20 @@ class PagedKVCache:
             k[:, :, :t], v[:, :, :t] = tail, self._tail_v[layer]
             pages = [*pages, (k, v)]
         n = self.length(layer)
-        return KVView.pages([pages], torch.tensor([n], dtype=torch.int32, device=tail.device), max_len=n)
+        if self._status is None or self._status.device != tail.device:
+            self._status = torch.zeros(1, dtype=torch.int32, device=tail.device)
+        return KVView.pages([pages], torch.tensor([n], dtype=torch.int32, device=tail.device), max_len=n,
+                            status=self._status)
+
+    def check_status(self) -> None:
+        """Raises RuntimeError if a wait inside an attention kernel ran out, over
+        any view of this cache, since the last check: hidden states, cached
+        positions and weight sums since then are not valid.  Synchronises; call
+        it where results are read."""
+        from .kv_attention import check_wait_status
+
+        if self._status is not None:
+            check_wait_status(self._status)
 
     def evict(self, layer: int, weights: torch.Tensor, *, budget: int, sinks: int = 4, recent: int = 0):
         """Cuts the layer to its first `sinks`, newest `recent` and most attended
