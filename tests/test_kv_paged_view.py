@@ -140,3 +140,23 @@ def test_views_of_a_cache_report_to_one_word(tmp_path):
     with pytest.raises(RuntimeError, match="ran out"):
         kv.check_status()
     b.check_status()
+
+
+@pytest.mark.gpu
+def test_view_of_resident_pages_does_not_wait(tmp_path):
+    from voom_b200.runtime.kv_attention import DraftTree, tree_attention
+    from voom_b200.runtime.kv_paged import PagedKVCache
+
+    kv = PagedKVCache(1, 1 << 40, tmp_path / "a", page_positions=16)
+    k = torch.randn((1, 2, 53, 64), device="cuda").to(torch.bfloat16)
+    kv.append(0, k, k)
+    q = torch.randn((1, 1, 4, 64), device="cuda").to(torch.bfloat16)
+    tree = DraftTree.chain(1, 1, "cuda")
+    tree_attention(q, k[:, :, :1].transpose(1, 2), k[:, :, :1].transpose(1, 2), tree, kv.view(0))
+    torch.cuda.synchronize()
+    mode = torch.cuda.get_sync_debug_mode()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        tree_attention(q, k[:, :, :1].transpose(1, 2), k[:, :, :1].transpose(1, 2), tree, kv.view(0))
+    finally:
+        torch.cuda.set_sync_debug_mode(mode)

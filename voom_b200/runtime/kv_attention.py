@@ -12,7 +12,9 @@ weight each cached position receives, and eviction by it.
 
 New tokens' keys and values are separate tensors, as they come from the
 projection: a drafted token enters a cache only once it is accepted, so a
-rejected one leaves nothing to undo.  Nothing here synchronises with the host.
+rejected one leaves nothing to undo.  Only check_status synchronises with the
+host.  A view's own tensors belong to the stream that was current when it was
+made: calls on another stream need it kept until they have run.
 
 Counterpart in the reference: the attention around its caches
 (runtime/layer_runner.py `_attention`, runtime/kv_paged.py:143-181).
@@ -133,9 +135,10 @@ class KVView:
         if not flat:
             raise ValueError("a view of pages needs at least one page")
         k0, v0 = flat[0]
-        ks, vs = _steps(k0), _steps(v0)
+        kw, vw, ks, vs = k0.stride(), v0.stride(), _steps(k0), _steps(v0)
         for k, v in flat:
-            if k.shape != k0.shape or v.shape != k0.shape or _steps(k) != ks or _steps(v) != vs:
+            if k.shape != k0.shape or v.shape != k0.shape or (k.stride() != kw and _steps(k) != ks) or \
+                    (v.stride() != vw and _steps(v) != vs):
                 raise ValueError("all pages must have one shape and one set of strides")
             if k.dtype != k0.dtype or v.dtype != k0.dtype or k.device != k0.device or v.device != k0.device:
                 raise ValueError("all pages must have one type and lie on one device")
@@ -150,7 +153,8 @@ class KVView:
         for b, request in enumerate(pages):
             for p, (k, v) in enumerate(request):
                 off[b, p] = (k.data_ptr() - k0.data_ptr()) // e, (v.data_ptr() - v0.data_ptr()) // e
-        offsets = torch.from_numpy(off).to(k0.device)
+        # from pinned memory: a copy from pageable memory waits for all that the stream has to do
+        offsets = torch.from_numpy(off).pin_memory().to(k0.device, non_blocking=True)
         return cls(k0, v0, lengths, batch=len(pages), heads=H, head_dim=D, page=P, offsets=offsets, table_stride=per,
                    max_len=P * per if max_len is None else max_len, strides=(0, ks[0], ks[1], 0, vs[0], vs[1]),
                    keep=flat, status=status)

@@ -328,7 +328,7 @@ class PagedKVCache:
         """The layer's positions for kv_attention.tree_attention: pages are read
         where they are (spilled ones reloaded for the view's life), only the
         open page is copied, into a page of its own; update() would copy every
-        position instead."""
+        position instead.  The host waits for the device only to reload pages."""
         from .kv_attention import KVView
 
         tail = self._tail_k[layer]
@@ -344,8 +344,8 @@ class PagedKVCache:
         n = self.length(layer)
         if self._status is None or self._status.device != tail.device:
             self._status = torch.zeros(1, dtype=torch.int32, device=tail.device)
-        return KVView.pages([pages], torch.tensor([n], dtype=torch.int32, device=tail.device), max_len=n,
-                            status=self._status)
+        length = torch.full((1,), n, dtype=torch.int32, device=tail.device)  # (a tensor from a list waits for the device)
+        return KVView.pages([pages], length, max_len=n, status=self._status)
 
     def check_status(self) -> None:
         """Raises RuntimeError if a wait inside an attention kernel ran out, over
