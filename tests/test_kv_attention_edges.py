@@ -187,3 +187,26 @@ def test_a_pool_entry_that_is_no_page_reads_zeros(page, n, g):
     check(out[0], o, 2 * STEP[torch.bfloat16] * 6.0, "out")
     e = kva.kv_evict(view, torch.zeros((1, 1, L), device="cuda"), budget=L - 1, sinks=0, recent=L - 1)
     assert torch.equal(e.k[0, 0].cpu(), kp.reshape(L, D)[1:]) and torch.equal(e.v[0, 0].cpu(), vp.reshape(L, D)[1:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,g,D", [(1, 1, 64), (1, 8, 128), (24, 1, 64), (40, 4, 64), (80, 4, 64), (20, 1, 256)])
+def test_denominator_of_many_small_weights_beside_a_large_one(dtype, n, g, D):
+    """Half a million positions of 2^-25 each of the row's largest, 2^-6 of the row together: added to it one by
+    one in fp32 they would not count.  160 requests read one cache, so that a block has a whole unit."""
+    from voom_b200.runtime import kv_attention as kva
+
+    B, page, L = 160, 1 << 13, 1 << 19
+    k, v = (torch.zeros((L // page, 1, page, D), dtype=dtype, device="cuda") for _ in range(2))
+    k[0, 0, 0, 0] = 25.1 * math.log(2.0)
+    table = torch.arange(L // page, dtype=torch.int32, device="cuda").expand(B, -1).contiguous()
+    view = kva.KVView.pool(k, v, table, torch.full((B,), L, dtype=torch.int32, device="cuda"))
+    q = torch.zeros((B, n, g, D), dtype=dtype, device="cuda")
+    q[..., 0] = 1.0
+    new = torch.zeros((B, n, 1, D), dtype=dtype, device="cuda")
+    _, lse = kva.tree_attention(q, new, new, kva.DraftTree.chain(B, n, "cuda"), view, scale=1.0, return_lse=True)
+    top = math.exp(float(k[0, 0, 0, 0]))
+    for i in (0, n - 1):
+        want = math.log(top + (L - 1) + (i + 1))
+        assert float((lse[:, i].double() - want).abs().max()) <= 3e-5, i

@@ -216,6 +216,15 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// sum += x with what the addition lost kept in `rest`: beside one large term, a
+// long cache's small ones would be lost one by one (2^-25 of a row's largest
+// does not change a 1 at all).  Both are at least 0.
+__device__ __forceinline__ void add_kept(float& sum, float& rest, float x) {
+  const float t = sum + x;
+  rest += fminf(sum, x) - (t - fmaxf(sum, x));
+  sum = t;
+}
+
 // Two fp32 values in a register pair: one instruction works on both.
 struct F2 {
   uint64_t v;

@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
       *reinterpret_cast<uint4*>(s_q + row_off<DP>(r, c)) = x;
     }
     __syncthreads();
-    float o[MT][DT][4], m[MT][2], l[MT][2];
+    float o[MT][DT][4], m[MT][2], l[MT][2], rest[MT][2];  // l + rest: the denominator
 #pragma unroll
     for (int t = 0; t < MT; t++) {
 #pragma unroll
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
 #pragma unroll
         for (int e = 0; e < 4; e++) o[t][d][e] = 0.0f;
       m[t][0] = m[t][1] = -INFINITY;
-      l[t][0] = l[t][1] = 0.0f;
+      l[t][0] = l[t][1] = rest[t][0] = rest[t][1] = 0.0f;
     }
     for (uint32_t step = g.s0 + warp; step < g.s1; step += kRowWarps) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kRowStages - 2) : "memory");
@@ -270,6 +270,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
           f[x] = top[x] == m[t][x] ? 1.0f : exp2_fast(m[t][x] - top[x]);  // (nothing seen yet: -inf both)
           m[t][x] = top[x];
           l[t][x] *= f[x];
+          rest[t][x] *= f[x];
         }
         if (__any_sync(0xFFFFFFFFu, f[0] != 1.0f || f[1] != 1.0f)) {
 #pragma unroll
@@ -280,14 +281,16 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
 #pragma unroll
         for (int x = 0; x < 2; x++) {
           const float base = m[t][x] == -INFINITY ? 0.0f : m[t][x];
+          float sum = 0.0f;  // of the tile
 #pragma unroll
           for (uint32_t j = 0; j < NT; j++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
               const float p = exp2_fast(z[t][j][2 * x + e] - base);
               z[t][j][2 * x + e] = p;
-              l[t][x] += p;
+              sum += p;
             }
+          add_kept(l[t][x], rest[t][x], sum);
         }
       }
       // o += p v
@@ -348,6 +351,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
     for (int t = 0; t < MT; t++)
 #pragma unroll
       for (int x = 0; x < 2; x++) {
+        l[t][x] += rest[t][x];
         l[t][x] += __shfl_xor_sync(0xFFFFFFFFu, l[t][x], 1);
         l[t][x] += __shfl_xor_sync(0xFFFFFFFFu, l[t][x], 2);
         if (quad == 0) {

@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
     do {
       const uint32_t row = g.m * ROWS + (MODE == kPair ? w * 128 : 0) + tr, tok = row / P.g, cs = cache_steps(P, g.len);
       const uint32_t n = g.s1 - g.s0;
-      float m = -INFINITY, l = 0.0f;
+      float m = -INFINITY, l = 0.0f, rest = 0.0f;  // l + rest: the denominator
       for (uint32_t i = MODE == kAlternate ? w : 0; i < n; i += MODE == kAlternate ? 2 : 1) {
         const uint32_t slot = MODE == kSingle ? i & 1u : w, step = g.s0 + i;
         const uint32_t o_col = C::O_COL + (MODE == kSingle ? 0u : w * DP);
@@ -442,6 +442,7 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
             tc::tmem_st32(tmem + lanes + o_col + c, o);
           }
           l *= f;
+          rest *= f;
           if (grow) m = top;
         }
         if (m == -INFINITY) m = top;
@@ -465,7 +466,7 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
         float s0, s1, s2, s3;
         take2(sum[0], s0, s1);
         take2(sum[1], s2, s3);
-        l += (s0 + s1) + (s2 + s3);
+        add_kept(l, rest, (s0 + s1) + (s2 + s3));
         tc::tmem_wait_st();
         tc::tc_fence_before();
         tc::mbar_arrive(bar(sh.p_ready[slot]));
@@ -473,6 +474,7 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
       }
       if (!ok) break;
       // the segment's sums
+      l += rest;
       float m2 = m == -INFINITY ? -INFINITY : m * P.scale2, f0 = 1.0f, f1 = 0.0f;
       uint32_t c0 = 0, c1 = DP;
       if (MODE == kAlternate) {
