@@ -210,3 +210,28 @@ def test_denominator_of_many_small_weights_beside_a_large_one(dtype, n, g, D):
     for i in (0, n - 1):
         want = math.log(top + (L - 1) + (i + 1))
         assert float((lse[:, i].double() - want).abs().max()) <= 3e-5, i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,g,D,L", [(1, 1, 64, 1 << 19), (40, 4, 64, 1 << 17), (80, 4, 64, 1 << 17), (20, 1, 256, 1 << 17)])
+def test_fp16_many_small_probabilities_beside_a_large_one(n, g, D, L):
+    """One position takes nearly all of a row's weight, the others 2^-25 of it each: too small for FP16 by
+    themselves, 2^-6 or 2^-8 of the row together.  160 requests read one cache, so that a block has a whole unit."""
+    from voom_b200.runtime import kv_attention as kva
+
+    B, page = 160, 1 << 13
+    k, v = (torch.zeros((L // page, 1, page, D), dtype=torch.float16, device="cuda") for _ in range(2))
+    v[..., 0] = 1.0
+    k[0, 0, 0, 0], v[0, 0, 0, 0] = 25.1 * math.log(2.0), 0.0
+    table = torch.arange(L // page, dtype=torch.int32, device="cuda").expand(B, -1).contiguous()
+    view = kva.KVView.pool(k, v, table, torch.full((B,), L, dtype=torch.int32, device="cuda"))
+    q = torch.zeros((B, n, g, D), dtype=torch.float16, device="cuda")
+    q[..., 0] = 1.0
+    new = torch.zeros((B, n, 1, D), dtype=torch.float16, device="cuda")
+    out, lse = kva.tree_attention(q, new, new, kva.DraftTree.chain(B, n, "cuda"), view, scale=1.0, return_lse=True)
+    top = math.exp(float(k[0, 0, 0, 0]))
+    for i in (0, n - 1):
+        total = top + (L - 1) + (i + 1)
+        err = (out[:, i, :, 0].double() - (L - 1) / total).abs().max()
+        assert float(err) <= 2 * STEP[torch.float16], (i, float(err), (L - 1) / total)
+        assert float((lse[:, i].double() - math.log(total)).abs().max()) <= 3e-5

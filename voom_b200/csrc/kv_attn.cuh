@@ -251,6 +251,16 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// Probabilities are rounded to the cache's type for the value product (the tensor
+// cores want both operands in one), half a unit each of a sum that is rounded
+// to that type anyway; the denominator adds them up unrounded.  What is rounded
+// is 2^kLift p.  FP16 ends at 2^-24: beside a position that takes nearly all of a
+// row's weight, a long cache's many small ones would vanish, or lose up to half,
+// one by one.  Lifted, with p at most 2^SLACK, they are at most 2^14 and keep 11
+// bits down to 2^-14 / 2^kLift.  BF16 has fp32's range.
+template <typename T, int SLACK>
+constexpr float kLift = std::is_same<T, __half>::value ? 14.0f - SLACK : 0.0f;
+
 __device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);

@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
           for (uint32_t j = 0; j < NT; j++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-              const float p = exp2_fast(z[t][j][2 * x + e] - base);
+              const float p = exp2_fast((z[t][j][2 * x + e] - base) + kLift<T, 0>);
               z[t][j][2 * x + e] = p;
               sum += p;
             }
@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
         if (quad == 0) {
           const uint32_t r = 16 * t + oct + 8 * x, i = (row0 + r) / P.g;
           const bool token = r < nrows && sees(P, g.b, i, i);  // else it has seen nothing
-          s_m[warp * ROWS + r] = token ? m[t][x] : -INFINITY;
+          s_m[warp * ROWS + r] = token ? m[t][x] - kLift<T, 0> : -INFINITY;  // what o and l are relative to
           s_l[warp * ROWS + r] = token ? l[t][x] : 0.0f;
         }
       }

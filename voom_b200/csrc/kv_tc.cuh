@@ -13,7 +13,7 @@
 //               the slots are two S buffers.
 // A row's maximum is raised only when it grows by more than 2^8: O is rescaled
 // then, which is rare; until then probabilities are at most 2^8, which 16-bit
-// types hold as precisely as 1.
+// types hold as precisely as 1 (kLift: what that leaves of FP16's range).
 //
 // Bound by the softmax beside the products (kPair: both take about 2000 cycles
 // of the 4200 that a tile of keys takes), kSingle by the tiles' way from L2 and
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
           if (grow) m = top;
         }
         if (m == -INFINITY) m = top;
-        const float base = m == -INFINITY ? 0.0f : m * P.scale2;
+        const float base = m == -INFINITY ? 0.0f : m * P.scale2 - kLift<T, 8>;
         const F2 sc = make2(P.scale2, P.scale2), nb = make2(-base, -base);
         F2 sum[2] = {make2(0.0f, 0.0f), make2(0.0f, 0.0f)};
 #pragma unroll
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
       if (!ok) break;
       // the segment's sums
       l += rest;
-      float m2 = m == -INFINITY ? -INFINITY : m * P.scale2, f0 = 1.0f, f1 = 0.0f;
+      float m2 = m == -INFINITY ? -INFINITY : m * P.scale2 - kLift<T, 8>, f0 = 1.0f, f1 = 0.0f;  // what O and l are relative to
       uint32_t c0 = 0, c1 = DP;
       if (MODE == kAlternate) {
         sh.ml[w][tr] = make_float2(m2, l);
