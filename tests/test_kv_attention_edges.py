@@ -235,3 +235,25 @@ def test_fp16_many_small_probabilities_beside_a_large_one(n, g, D, L):
         err = (out[:, i, :, 0].double() - (L - 1) / total).abs().max()
         assert float(err) <= 2 * STEP[torch.float16], (i, float(err), (L - 1) / total)
         assert float((lse[:, i].double() - math.log(total)).abs().max()) <= 3e-5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,g", [(3, 2), (20, 2)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_token_weight_of_no_token_counts_for_nothing(n, g, bad):
+    from voom_b200.runtime import kv_attention as kva
+
+    par = [-1] * n
+    par[1] = -2
+    qkv, k, v = inputs(1, n, g, 1, 64, [50], torch.bfloat16)
+    d = qkv.cuda()
+    view = place(k, v, [50], "whole", 0)
+    tree = kva.DraftTree(torch.tensor([par], dtype=torch.int32, device="cuda"))
+    sums = []
+    for x in (0.0, bad):
+        tw = torch.ones((1, n), device="cuda")
+        tw[0, 1] = x
+        w = torch.zeros((1, 1, 50 + n), device="cuda")
+        kva.tree_attention(d[:, :, :g], d[:, :, g:g + 1], d[:, :, g + 1:], tree, view, weights=w, token_weight=tw)
+        sums.append(w)
+    assert bool(torch.isfinite(sums[0]).all()) and torch.equal(sums[0], sums[1])

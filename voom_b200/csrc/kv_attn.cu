@@ -172,8 +172,10 @@ __global__ void __launch_bounds__(256) attn_finish(const __grid_constant__ Attn 
       lse2 = P.lse[(uint64_t(b) * P.a.n + i) * P.a.hq + hh] * voom::kv::kLog2e;
     }
     if (lane == 0) {
-      s_row[r] = lse2 == -INFINITY ? INFINITY : lse2;  // a row that sees nothing has no weight anywhere
-      s_w[r] = P.a.d_token_weight ? P.a.d_token_weight[uint64_t(b) * P.a.n + i] : 1.0f;
+      // a row that sees nothing has no weight anywhere, whatever its factor and its scores are
+      const bool none = lse2 == -INFINITY;
+      s_row[r] = none ? INFINITY : lse2;
+      s_w[r] = none ? 0.0f : P.a.d_token_weight ? P.a.d_token_weight[uint64_t(b) * P.a.n + i] : 1.0f;
     }
   }
   __syncthreads();
@@ -187,7 +189,7 @@ __global__ void __launch_bounds__(256) attn_finish(const __grid_constant__ Attn 
     for (uint32_t q = 0; q < 4; q++) {
       const uint32_t r = r0 + q;
       // in a chain, tiles past the row's own token have no scores
-      const uint32_t lim = r >= P.R ? 0u : P.a.d_mask ? end : min(end, P.score_new + r / P.g + 1);
+      const uint32_t lim = r >= P.R || s_row[r] == INFINITY ? 0u : P.a.d_mask ? end : min(end, P.score_new + r / P.g + 1);
 #pragma unroll
       for (uint32_t k = 0; k < kWeightSpan / 256; k++) {
         const uint32_t s = s0 + k * 256 + tid;
