@@ -37,6 +37,7 @@ enum {
   VOOM_E_CUDA = -2,        /* a CUDA launch or runtime call failed            */
   VOOM_E_CAPACITY = -3,    /* caller-provided array or buffer is too small    */
   VOOM_E_UNSUPPORTED = -4, /* a valid input outside what this build decodes   */
+  VOOM_E_OVERLAP = -5,     /* an output overlaps itself or what it may not    */
 
   /* formats/bf16_rans.py decode() ValueError messages, in the order the
    * reference checks them (bf16_rans.py:97-130, 180-222). */
@@ -583,7 +584,8 @@ enum { VOOM_BF16 = 0u, VOOM_FP16 = 1u, VOOM_FP32 = 2u };
  * t = 2 pi * frac(position * turns_i), turns_i the pair's turns per position
  * in units of 2^-64: the 64-bit product wraps, so the angle is as exact far
  * into a context as at its start.  Strides are in elements; a head's D values
- * are contiguous.  Outputs may be the inputs (not partly overlap them).  fp32
+ * are contiguous.  Each output may be its input, or share memory with none
+ * (else VOOM_E_OVERLAP; an output whose rows overlap one another too).  fp32
  * arithmetic, one rounding.
  * Replaces: the norm and rotation calls of the reference's attention layers
  * (runtime/layer_runner.py _attention), outside its ported path. */
@@ -648,7 +650,9 @@ int voom_tree_mask(const int32_t* d_parents, uint32_t B, uint32_t n, uint32_t* d
  * position s (cached positions first, then the new tokens), each row times
  * d_token_weight[b, i] if given.  Each sum is made by one thread in a fixed
  * order: results do not depend on scheduling.  fp32 softmax; scores and outputs
- * accumulate in fp32; probabilities are rounded to `type` for the value product. */
+ * accumulate in fp32; probabilities are rounded to `type` for the value product.
+ * Rows of d_out, or of d_weights, that overlap one another, and a d_out that
+ * shares memory with d_q, d_kn or d_vn, are refused (VOOM_E_OVERLAP). */
 typedef struct voom_tree_attention_args {
   const void* d_q;  /* B x n x hq x D */
   const void* d_kn; /* B x n x hk x D: the new tokens' keys   */

@@ -21,6 +21,7 @@ VOOM_E_INVALID_ARG = -1
 VOOM_E_CUDA = -2
 VOOM_E_CAPACITY = -3
 VOOM_E_UNSUPPORTED = -4
+VOOM_E_OVERLAP = -5
 
 RANS_MESSAGES = {
     101: "truncated rANS frame",
@@ -212,7 +213,8 @@ def check(rc: int, what: str) -> None:
     if rc == VOOM_OK:
         return
     names = {VOOM_E_INVALID_ARG: "invalid argument", VOOM_E_CUDA: "CUDA launch/runtime failure",
-             VOOM_E_CAPACITY: "capacity exceeded", VOOM_E_UNSUPPORTED: "unsupported input"}
+             VOOM_E_CAPACITY: "capacity exceeded", VOOM_E_UNSUPPORTED: "unsupported input",
+             VOOM_E_OVERLAP: "overlapping output"}
     raise VoomError(f"{what} failed: {names.get(rc, rc)}")
 
 

@@ -7,6 +7,7 @@
 #include "kv_rows.cuh"
 #include "kv_sums.cuh"
 #include "kv_tc.cuh"
+#include "rows.h"
 
 namespace {
 
@@ -428,6 +429,15 @@ int check(const voom_kv_view* c, const voom_tree_attention_args* a, Attn& P) {
   if (!rows16(a->d_q, {a->q_b, a->q_t, a->q_h}) || !rows16(a->d_kn, {a->kn_b, a->kn_t, a->kn_h}) ||
       !rows16(a->d_vn, {a->vn_b, a->vn_t, a->vn_h}) || !rows16(a->d_out, {a->o_b, a->o_t, a->o_h}))
     return VOOM_E_INVALID_ARG;
+  // blocks write out while others still read the new tokens, and add to the weights without atomics
+  const int64_t B = c->B, n = a->n, hq = a->hq, hk = c->hk, D = c->D;
+  const voom::Rows out{a->d_out, {B, n, hq}, {a->o_b, a->o_t, a->o_h}, D, 2};
+  if (!voom::separate(out) || !voom::disjoint(out, {a->d_q, {B, n, hq}, {a->q_b, a->q_t, a->q_h}, D, 2}) ||
+      !voom::disjoint(out, {a->d_kn, {B, n, hk}, {a->kn_b, a->kn_t, a->kn_h}, D, 2}) ||
+      !voom::disjoint(out, {a->d_vn, {B, n, hk}, {a->vn_b, a->vn_t, a->vn_h}, D, 2}))
+    return VOOM_E_OVERLAP;
+  if (a->d_weights && !voom::separate({a->d_weights, {B, hk, 1}, {a->w_b, a->w_h, 0}, int64_t(c->max_len) + n, 4}))
+    return VOOM_E_OVERLAP;
   P.a = *a;
   return VOOM_OK;
 }

@@ -27,6 +27,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "rows.h"
 
 namespace {
 
@@ -476,6 +477,12 @@ VOOM_API int voom_qk_norm_rope(const voom_qk_norm_rope_args* a, void* stream) {
   if (a->type > VOOM_FP32 || a->w_type > VOOM_FP32) return VOOM_E_INVALID_ARG;
   if (uint64_t(a->hq) + a->hk > 65536u) return VOOM_E_UNSUPPORTED;
   if (!a->T || a->hq + a->hk == 0) return VOOM_OK;
+  const int64_t T = a->T, D = a->D, e = a->type == VOOM_FP32 ? 4 : 2;
+  const voom::Rows q{a->d_q, {T, a->hq, 1}, {a->q_token, a->q_head, 0}, D, e}, k{a->d_k, {T, a->hk, 1}, {a->k_token, a->k_head, 0}, D, e};
+  const voom::Rows qo{a->d_q_out, {T, a->hq, 1}, {a->qo_token, a->qo_head, 0}, D, e}, ko{a->d_k_out, {T, a->hk, 1}, {a->ko_token, a->ko_head, 0}, D, e};
+  if (!voom::separate(qo) || !voom::separate(ko) || !voom::disjoint(qo, ko) || !voom::disjoint(qo, k) || !voom::disjoint(ko, q) ||
+      !(voom::same_place(qo, q) || voom::disjoint(qo, q)) || !(voom::same_place(ko, k) || voom::disjoint(ko, k)))
+    return VOOM_E_OVERLAP;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a->type == VOOM_BF16) return dispatch<__nv_bfloat16>(*a, s);
   if (a->type == VOOM_FP16) return dispatch<__half>(*a, s);

@@ -31,7 +31,7 @@ import numpy as np
 import torch
 
 from .. import _device
-from .._lib import VOOM_E_CAPACITY, ELEMENT_TYPES, KvEvictArgs, KvViewStruct, TreeAttentionArgs, check, load
+from .._lib import VOOM_E_CAPACITY, VOOM_E_OVERLAP, ELEMENT_TYPES, KvEvictArgs, KvViewStruct, TreeAttentionArgs, check, load
 
 MAX_HEAD_DIM = 256
 MAX_TREE = 1024  # tokens of a tree that is not a chain
@@ -253,7 +253,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: Draf
     `tree` says: (B, n, Hq, D) in the cache's type, and with `return_lse` the
     natural log of each row's softmax denominator, (B, n, Hq) fp32.  Query head
     h reads key head h // (Hq // heads); `scale` defaults to D ** -0.5.  A row
-    of no token gives zeros and lse -inf.
+    of no token gives zeros and lse -inf.  `out` must not share memory with q, k
+    or v, nor rows of `out` or `weights` with one another.
 
     `weights` (B, heads, >= max_len + n) fp32: each position's softmax weight,
     summed over the rows that share its head (each times `token_weight` (B, n)
@@ -309,6 +310,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: Draf
                 if rc == VOOM_E_CAPACITY:  # refused before anything was launched
                     ws = cache.more_scratch(lib.voom_tree_attention_scratch_bytes(cache.packed, a), sp)
                     rc = lib.voom_tree_attention(cache.packed, a, ws[0], ws[1], sp)
+        if rc == VOOM_E_OVERLAP:
+            raise ValueError("rows of out or of weights overlap one another, or out shares memory with q, k or v")
         check(rc, "voom_tree_attention")
     return (out, lse) if return_lse else out
 

@@ -17,7 +17,7 @@ import struct
 import torch
 
 from .. import _device
-from .._lib import ELEMENT_TYPES, QkNormRopeArgs, check, load
+from .._lib import VOOM_E_OVERLAP, ELEMENT_TYPES, QkNormRopeArgs, check, load
 
 LAYOUTS = ("half", "interleaved")
 MAX_HEAD_DIM = 512
@@ -173,7 +173,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rota
     the weight is None) and rotated by their tokens' `positions` (T, int32 or
     int64).  BF16, FP16 or FP32; any token and head strides, so q and k may be
     views of a fused projection.  `out_q` / `out_k` may be views of a cache, or q
-    and k themselves.  fp32 arithmetic, one rounding."""
+    and k themselves (each its own, else no memory of either).  fp32 arithmetic,
+    one rounding."""
     if stream is not None or _device.current_index() != rotary.index:
         with _device.on_stream(rotary.device, stream):
             return qk_norm_rope(q, k, positions, rotary, q_weight=q_weight, k_weight=k_weight, eps=eps,
@@ -210,11 +211,14 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rota
     else:
         kot, koh = _output(out_k, k, "out_k", at)
     if T:
-        check(load().voom_qk_norm_rope(
+        rc = load().voom_qk_norm_rope(
             _ARGS.pack(q.data_ptr(), k.data_ptr(), out_q.data_ptr(), out_k.data_ptr(), qw, kw, positions.data_ptr(),
                        rotary.turns_ptr, qt, qh, kt, kh, qot, qoh, kot, koh, T, hq, hk, D, rotary.rot_dim, kind,
                        w_type, pt is torch.int64, rotary.interleaved, zero_centered, eps, rotary.factor),
-            _device.raw_stream(at)), "voom_qk_norm_rope")
+            _device.raw_stream(at))
+        if rc == VOOM_E_OVERLAP:
+            raise ValueError("rows of out_q or out_k overlap one another, or memory of q and k that is not their own")
+        check(rc, "voom_qk_norm_rope")
     return out_q, out_k
 
 
