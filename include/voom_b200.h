@@ -585,8 +585,9 @@ enum { VOOM_BF16 = 0u, VOOM_FP16 = 1u, VOOM_FP32 = 2u };
  * in units of 2^-64: the 64-bit product wraps, so the angle is as exact far
  * into a context as at its start.  Strides are in elements; a head's D values
  * are contiguous.  Each output may be its input, or share memory with none
- * (else VOOM_E_OVERLAP; an output whose rows overlap one another too).  fp32
- * arithmetic, one rounding.
+ * (else VOOM_E_OVERLAP; an output whose rows overlap one another too).  With no
+ * query heads, or no key heads, their pointers may be NULL.  fp32 arithmetic, one
+ * rounding.
  * Replaces: the norm and rotation calls of the reference's attention layers
  * (runtime/layer_runner.py _attention), outside its ported path. */
 typedef struct voom_qk_norm_rope_args {

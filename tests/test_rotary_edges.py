@@ -100,3 +100,36 @@ def test_default_scaling_and_keys_that_would_be_ignored():
     assert _scaled(_base(), 64, 10000.0, half, 128) == (_base(), 1.0)
     with pytest.raises(ValueError, match="rotary scaling"):
         _scaled(_base(), 64, 10000.0, half, 64)
+
+
+def test_c_entry_takes_one_side_alone(built_lib):
+    import ctypes
+
+    from voom_b200._lib import QkNormRopeArgs
+
+    a = QkNormRopeArgs()
+    for f in ("q", "q_out", "pos", "turns"):
+        setattr(a, f, 4096)
+    a.T, a.hq, a.hk, a.D, a.rot = 0, 1, 0, 64, 64
+    assert built_lib.voom_qk_norm_rope(ctypes.byref(a), None) == 0  # no key heads: no keys
+    a.hk = 1
+    assert built_lib.voom_qk_norm_rope(ctypes.byref(a), None) == -1
+    a.hq, a.k, a.k_out, a.q, a.q_out = 0, 4096, 4096, None, None
+    assert built_lib.voom_qk_norm_rope(ctypes.byref(a), None) == 0  # no query heads: no queries
+
+
+@pytest.mark.gpu
+def test_queries_or_keys_alone():
+    from voom_b200.runtime import rotary
+
+    x = torch.randn((4, 3, 64), generator=torch.Generator().manual_seed(3))
+    pos = torch.arange(4)
+    plan = rotary.Rotary(64, device="cuda")
+    d = x.cuda()
+    want = oa.norm_rope(x, pos, plan.freqs, rot=64)
+    q, k = rotary.qk_norm_rope(d, d[:, :0], pos.cuda(), plan)
+    close(q, want, torch.float32)
+    assert k.shape == (4, 0, 64)
+    q, k = rotary.qk_norm_rope(d[:, :0], d, pos.cuda(), plan)
+    close(k, want, torch.float32)
+    assert q.shape == (4, 0, 64)

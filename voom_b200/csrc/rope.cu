@@ -470,7 +470,7 @@ int dispatch(const voom_qk_norm_rope_args& a, cudaStream_t s) {
 }  // namespace
 
 VOOM_API int voom_qk_norm_rope(const voom_qk_norm_rope_args* a, void* stream) {
-  if (!a || !a->d_q || !a->d_k || !a->d_q_out || !a->d_k_out || !a->d_pos) return VOOM_E_INVALID_ARG;
+  if (!a || (a->hq && (!a->d_q || !a->d_q_out)) || (a->hk && (!a->d_k || !a->d_k_out)) || (a->T && !a->d_pos)) return VOOM_E_INVALID_ARG;
   if (!a->D || a->rot > a->D || a->rot % 2 || (a->rot && !a->d_turns)) return VOOM_E_INVALID_ARG;
   if (reinterpret_cast<uintptr_t>(a->d_turns) & 15u) return VOOM_E_INVALID_ARG;
   if (a->D > kMaxD) return VOOM_E_UNSUPPORTED;
