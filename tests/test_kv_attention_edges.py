@@ -257,3 +257,45 @@ def test_token_weight_of_no_token_counts_for_nothing(n, g, bad):
         kva.tree_attention(d[:, :, :g], d[:, :, g:g + 1], d[:, :, g + 1:], tree, view, weights=w, token_weight=tw)
         sums.append(w)
     assert bool(torch.isfinite(sums[0]).all()) and torch.equal(sums[0], sums[1])
+
+
+@pytest.mark.gpu
+def test_evict_more_positions_than_shared_memory_holds():
+    """Past 8 x 40960 positions of a head, the weights are read again in every pass."""
+    from voom_b200.runtime import kv_attention as kva
+
+    L, budget, sinks, recent = 330001, 5000, 3, 77
+    gen = torch.Generator().manual_seed(2)
+    w = torch.round(torch.rand((1, 1, L), generator=gen) * 1000) / 8
+    k = torch.arange(L).remainder(251).to(torch.bfloat16)[None, None, :, None].expand(1, 1, L, 8).contiguous()
+    view = kva.KVView.contiguous(k.cuda(), (-k).cuda(), torch.tensor([L], dtype=torch.int32, device="cuda"))
+    e = kva.kv_evict(view, w.cuda(), budget=budget, sinks=sinks, recent=recent)
+    want = oa.kept(w[0, 0].tolist(), L, budget, sinks, recent)
+    assert e.index[0, 0].tolist() == want
+    assert torch.equal(e.k[0, 0].cpu(), k[0, 0, want]) and torch.equal(e.weights[0, 0].cpu(), w[0, 0, want])
+
+
+@pytest.mark.gpu
+def test_a_graph_follows_lengths_far_below_its_bound():
+    """A captured call over a cache laid out for 20000 positions, replayed as its lengths change."""
+    from voom_b200.runtime import kv_attention as kva
+
+    for n, g in ((1, 4), (40, 4)):
+        qkv, k, v = inputs(2, n, g, 1, 64, [20000, 20000], torch.bfloat16)
+        d, kd, vd = qkv.cuda(), k.cuda(), v.cuda()
+        length = torch.tensor([20000, 3], dtype=torch.int32, device="cuda")
+        view = kva.KVView.contiguous(kd, vd, length)
+        tree = kva.DraftTree.chain(2, n, "cuda")
+        args = (d[:, :, :g], d[:, :, g:g + 1], d[:, :, g + 1:], tree)
+        kva.tree_attention(*args, view)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = kva.tree_attention(*args, view)
+        for lens in ([20000, 3], [0, 0], [1, 70], [5, 20000]):
+            length.copy_(torch.tensor(lens, dtype=torch.int32))
+            graph.replay()
+            tight = kva.KVView.contiguous(kd, vd, length.clone(), max_len=max(lens))
+            want = kva.tree_attention(*args, tight).float()
+            big = max(float(v.abs().max()), float(qkv.abs().max()))
+            assert float((out.float() - want).abs().max()) <= 4 * STEP[torch.bfloat16] * big, lens  # two roundings

@@ -324,7 +324,10 @@ uint64_t plan(Attn& P, void* scratch) {
   P.lse = P.a.d_lse;
   if (P.a.d_weights) {
     if (!P.lse) P.lse = reinterpret_cast<float*>(take(uint64_t(c.B) * P.a.n * P.a.hq * sizeof(float)));
-    if (P.R > 16) return at;  // attn_sums goes over the keys again
+    // beyond one block of 16 rows attn_sums goes over the keys again: 2 D bytes a
+    // position against 8 a row kept here, which is fewer up to D / 4 rows (16 for
+    // heads of 64; 32 and 64 rows of larger heads are not measured this way)
+    if (P.R > 16) return at;
     P.score_new = (c.max_len + P.keys - 1) / P.keys * P.keys;
     P.score_ld = P.score_new + (P.a.n + P.keys - 1) / P.keys * P.keys;
     P.scores = reinterpret_cast<float*>(take(uint64_t(c.B) * c.hk * P.R * P.score_ld * sizeof(float)));
@@ -371,7 +374,9 @@ int finish(const Attn& P, cudaStream_t s) {
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = max(2u * kMergeRows, 2u * (P.scores ? P.R : 0u)) * sizeof(float);
   cfg.stream = s;
-  cudaLaunchAttribute early{};  // its launch overlaps the attention's end; it waits for it before it reads
+  // the launch itself is over by the time the attention ends; its blocks start when
+  // the last of the attention's has (none releases them earlier) and wait for its writes
+  cudaLaunchAttribute early{};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &early;

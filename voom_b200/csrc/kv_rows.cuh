@@ -9,9 +9,10 @@
 // three tiles in flight through cp.async into its own shared memory, and keeps
 // its own running maximum, sum and output in registers.  No warp waits for
 // another until a unit ends and the four join.  192 KB in flight per SM.
-// Measured: one token over 131072 positions, 8 key heads of 128: 96 us, 5.6
-// TB/s (86 % of what a copy reaches); 32 requests of up to 16000 positions in
-// pages of 16: 190 us, 5.4 TB/s.
+// Measured: one token over 131072 positions, 8 key heads of 128, with weight sums:
+// 119 us a call, 84 % of it here, 5.4 TB/s (82 % of what a copy reaches); 32 requests
+// of up to 16000 positions in pages of 16: 197 us, 96 % of it here.  At 255
+// registers a thread some values spill (32 rows, or heads of 256: 92-152 bytes).
 #pragma once
 
 #include "kv_attn.cuh"

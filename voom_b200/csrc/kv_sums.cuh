@@ -7,8 +7,9 @@
 // thread has one position's scores in its TMEM lane and adds them up by
 // itself, row after row: no exchange, no atomics, one order.  It reads the keys
 // once more, 2 D bytes a position; keeping the attention's scores instead
-// writes and reads 8 bytes per row and position, which is less up to 16 rows
-// (attn_finish does that then).  Bound by the exponentials: 16 a clock and SM.
+// writes and reads 8 bytes per row and position (attn_finish, up to 16 rows).
+// Bound by the exponentials with many rows, 16 a clock and SM; by its set-up with
+// few tiles a block (26 drafts x 32 heads over 8191 positions: 44 % of the call's 60 us).
 #pragma once
 
 #include "kv_attn.cuh"

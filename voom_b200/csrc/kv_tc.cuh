@@ -17,9 +17,13 @@
 //
 // Bound by the softmax beside the products (kPair: both take about 2000 cycles
 // of the 4200 that a tile of keys takes), kSingle by the tiles' way from L2 and
-// the operands' from shared memory.  Measured: 64 tokens x 32 heads of 128 over
-// up to 16384 positions, 8 requests: 88 us, 740 TFLOP/s; 1023 tokens x 16 heads
-// of 256 over 6145: 150 us, 740 TFLOP/s (45 % of a large matrix product's rate).
+// the operands' from shared memory.  Measured: 64 tokens x 32 heads of 128
+// over up to 16384 positions, 8 requests: 114 us a call, 80 % of it here, 710
+// TFLOP/s; 1023 tokens x 16 heads of 256 over 6145: 179 us, 83 % of it here, 750
+// TFLOP/s (46 % of a large matrix product's rate); the tensor pipe is busy for a
+// third of the time in both.  kPair and kAlternate
+// compile to the 128 registers a thread that the split below starts from, and spill
+// about 290 bytes; a softmax thread holds a row of S, 128 registers of its 192.
 #pragma once
 
 #include "kv_attn.cuh"

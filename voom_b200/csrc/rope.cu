@@ -6,7 +6,9 @@
 // The angle: `turns` holds the pair's turns per position as a 64-bit fraction,
 // so position * turns modulo 2^64 is the fraction of a turn whatever the
 // position (fp32 position * frequency is off by 0.01 rad at 10^5 already).
-// Its top 32 bits, as a signed half-turn count in [-1, 1), go to sincospif.
+// Its top 32 bits are a signed half-turn count in [-1, 1): FP32 values take
+// sincospif of it, 16-bit ones __sincosf of pi times it (exact to 2^-21, far
+// below their rounding).
 //
 // Bound by HBM: every value is read and written once (2 bytes each way in
 // BF16), about ten instructions per value.  A group of lanes takes a few heads
@@ -16,7 +18,7 @@
 // for all its heads, so cosines, sines and weights are made once and stay in
 // registers.  What keeps HBM busy is the next three heads' values on their way
 // into shared memory, where each lane reads back what it asked for itself.
-// Measured: 16384 tokens x 40 heads of 128 in BF16, 57 us, 5.9 TB/s (90 % of
+// Measured: 16384 tokens x 40 heads of 128 in BF16, 57 us, 5.8 TB/s (89 % of
 // what a copy reaches); without the read-ahead 94 us, with cosines, sines and
 // weights in shared memory 84 us.
 #include <cuda_bf16.h>
@@ -303,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, KT * VEC == 8 ? 6 : 4) qk_norm_rope(
         for (int i = 0; i < VEC; i++) {
           const float x = float(int32_t((uint64_t(pos) * turns[i]) >> 32)) * (1.0f / 2147483648.0f);
           if (sizeof(T) == 4) sincospif(x, &si[i], &co[i]);
-          else __sincosf(x * 3.14159265358979f, &si[i], &co[i]);  // to 2^-21 in [-pi, pi]: far below a 16-bit rounding
+          else __sincosf(x * 3.14159265358979f, &si[i], &co[i]);
           co[i] *= a.factor;
           si[i] *= a.factor;
         }

@@ -212,7 +212,9 @@ class DraftTree:
         return t
 
     def positions(self, lengths: torch.Tensor) -> torch.Tensor:
-        """Position of every new token, (B, n) int32: cached positions + depth."""
+        """Cached positions + depth of every new token, (B, n) int32: its rotary
+        position only where nothing was evicted.  After an eviction add the depth
+        to the count of all positions seen (PagedKVCache.offset)."""
         return lengths[:, None] + self.depth
 
 
@@ -259,7 +261,9 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: Draf
     `weights` (B, heads, >= max_len + n) fp32: each position's softmax weight,
     summed over the rows that share its head (each times `token_weight` (B, n)
     fp32, if given), is added in place: cached positions at their index, new
-    token j at lengths[b] + j.  kv_evict reads these sums."""
+    token j at lengths[b] + j.  kv_evict reads these sums.  Up to 16 rows (tokens
+    x query heads) per key head, the workspace holds their scores: 4 bytes a row
+    and position, for max_len positions of every request."""
     if stream is not None or _device.current_index() != cache.index:
         with _device.on_stream(cache.device, stream):
             return tree_attention(q, k, v, tree, cache, scale=scale, weights=weights, token_weight=token_weight,
