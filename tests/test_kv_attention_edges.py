@@ -299,3 +299,25 @@ def test_a_graph_follows_lengths_far_below_its_bound():
             want = kva.tree_attention(*args, tight).float()
             big = max(float(v.abs().max()), float(qkv.abs().max()))
             assert float((out.float() - want).abs().max()) <= 4 * STEP[torch.bfloat16] * big, lens  # two roundings
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,g", [(3, 2), (20, 2), (37, 8)])
+def test_weights_at_an_infinite_key(n, g):
+    """A key whose score is -inf for every row gets no weight, and rows that are no token change nothing."""
+    from voom_b200.runtime import kv_attention as kva
+
+    qkv, k, v = inputs(2, n, g, 1, 64, [50, 50], torch.bfloat16)
+    qkv[:, :, :g, 0] = qkv[:, :, :g, 0].abs() + 0.5
+    k[:, 0, 7, 0] = -math.inf
+    d = qkv.cuda()
+    view = place(k, v, [50, 50], "whole", 0)
+    tree = kva.DraftTree(torch.tensor([[-1] * n, [-2] * n], dtype=torch.int32, device="cuda"))  # the second: no tokens at all
+    w = torch.ones((2, 1, 50 + n), device="cuda")
+    out, lse = kva.tree_attention(d[:, :, :g], d[:, :, g:g + 1], d[:, :, g + 1:], tree, view, weights=w, return_lse=True)
+    assert bool((w[1] == 1).all()) and not out[1].any() and bool(torch.isneginf(lse[1]).all())
+    o, l, s = oa.attention(qkv[0, :, :g], qkv[0, :, g:g + 1], qkv[0, :, g + 1:], oa.tree_sees([-1] * n), k[0], v[0], 64 ** -0.5)
+    assert float(w[0, 0, 7]) == 1.0
+    check(out[0], o, 2 * STEP[torch.bfloat16] * float(v.abs().max() + 1), "out")
+    check(lse[0], l, 3e-5, "lse")
+    check(w[0], 1.0 + s, 5e-5 * (n * g) ** 0.5 + 1e-6, "weights")

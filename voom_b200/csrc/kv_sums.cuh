@@ -199,8 +199,9 @@ __global__ void __launch_bounds__(Sums<DP>::THREADS, 1) attn_sums(const __grid_c
                 if (i0 >= P.a.n || j >= P.a.n || !sees(P, g.b, i0, j)) p = 0.0f;
                 if (i1 >= P.a.n || j >= P.a.n || !sees(P, g.b, i1, j)) q = 0.0f;
               }
-              acc[0] = fmaf(x.y, p, acc[0]);
-              acc[1] = fmaf(x.w, q, acc[1]);
+              // rows that are none have queries of 0, whose score at an infinite key is NaN: not even times 0
+              if (x.y != 0.0f) acc[0] = fmaf(x.y, p, acc[0]);
+              if (x.w != 0.0f) acc[1] = fmaf(x.w, q, acc[1]);
             }
           }
           tc::tc_fence_before();
