@@ -644,7 +644,12 @@ int voom_tree_mask(const int32_t* d_parents, uint32_t B, uint32_t n, uint32_t* d
 /* Attention of n new tokens of each request over its cache and over one
  * another: out[b, i, h] = sum_j softmax_j(scale q . k_j) v_j over the cached
  * positions and the new tokens j that row i of the mask names (d_mask NULL: a
- * chain, j <= i).  Query head h reads key head h / (hq / hk).  A row that sees
+ * chain, j <= i).  With cap > 0 a score becomes cap tanh(score / cap); with
+ * d_slopes, slopes[h] times (key's position - query's) is added to it (after
+ * the cap); with window > 0 a row sees the positions less than `window` before
+ * its own only.  A cached position is its index, a new token's d_len[b] + its
+ * depth (d_depth as voom_tree_mask gives it; NULL in a chain, where it is i).
+ * Query head h reads key head h / (hq / hk).  A row that sees
  * nothing (a -2 token, which sees no cached position either) gives 0 and lse
  * = -inf.  lse: natural log of the softmax denominator.  d_weights[b, h, s]
  * (fp32) += the sum over the rows of key head h of their softmax weight at
@@ -664,13 +669,17 @@ typedef struct voom_tree_attention_args {
   float* d_weights; /* or NULL */
   const float* d_token_weight; /* B x n contiguous, or NULL */
   uint32_t* d_status; /* bit 0 set if a wait inside the kernel ran out (reported, never observed); or NULL */
+  const float* d_slopes;  /* hq, or NULL */
+  const int32_t* d_depth; /* B x n contiguous: wanted with d_mask and (d_slopes or window); else ignored */
   int64_t q_b, q_t, q_h, kn_b, kn_t, kn_h, vn_b, vn_t, vn_h, o_b, o_t, o_h, w_b, w_h; /* strides, elements */
   uint32_t n, hq;
   float scale;
+  float cap;       /* 0: scores are not capped */
+  uint32_t window; /* 0: none */
   uint32_t pad;
 } voom_tree_attention_args;
 /* Scratch (16-byte aligned, contents ignored) of a call; with less of it the
- * call returns VOOM_E_CAPACITY and launches nothing.  scale > 0. */
+ * call returns VOOM_E_CAPACITY and launches nothing.  scale > 0, cap >= 0. */
 uint64_t voom_tree_attention_scratch_bytes(const voom_kv_view* c, const voom_tree_attention_args* a);
 int voom_tree_attention(const voom_kv_view* c, const voom_tree_attention_args* a, void* d_scratch,
                         uint64_t scratch_bytes, void* stream);
@@ -692,6 +701,101 @@ typedef struct voom_kv_evict_args {
   uint32_t budget, sinks, recent, pad;
 } voom_kv_evict_args;
 int voom_kv_evict(const voom_kv_view* c, const voom_kv_evict_args* a, void* stream);
+
+/* New tokens enter the cache: position d_len[b] + j of request b takes the keys
+ * and values of its new token j, or d_index[b * m + j] if given (an entry outside
+ * [0, n): nothing is written), j < m.  Positions past the view's pages, and
+ * pages that are none, take nothing.  The lengths stay.  The view's keys and
+ * values are written although the view names them const; a cache whose rows
+ * overlap one another, or the new tokens, is refused (VOOM_E_OVERLAP; pages
+ * anywhere are checked page by page, not against one another).
+ * Replaces: the concatenation of the reference's caches (runtime/kv_paged.py:143-181). */
+typedef struct voom_kv_append_args {
+  const void* d_kn; /* B x n x hk x D, rows 16-byte aligned */
+  const void* d_vn;
+  const int32_t* d_index; /* B x m contiguous, or NULL: m = n */
+  int64_t kn_b, kn_t, kn_h, vn_b, vn_t, vn_h; /* strides, elements */
+  uint32_t n, m;
+} voom_kv_append_args;
+int voom_kv_append(const voom_kv_view* c, const voom_kv_append_args* a, void* stream);
+
+/* Rows of a page table become continuations of others.  Row r takes over row
+ * p = d_parents[r] (NULL: itself; outside [0, rows): the row ends and is empty):
+ * its length, and its ceil(length / page) pages, which the two then share.  Where
+ * grow positions follow (d_grow[r], or grow), pages for them are made ready:
+ *   - an open page (the last one, not full) that the row may not write on in is
+ *     replaced by a fresh one with a copy of its filled positions in every
+ *     layer.  Of the rows that hold a page one may: the longest, and of equal
+ *     ones the first, unless a row holds the page full;
+ *   - fresh pages for the positions past the open page.
+ * Fresh pages are those that no row holds any more, the lowest first, given out in
+ * the order of rows and positions; those that are not to be had, or that a table
+ * row has no room for, are counted in d_missing and their entries are -1.  Entries
+ * past the pages of length + grow are -1, and so are entries outside the pool.
+ * d_refs counts each page's rows in the new table.  d_table_out / d_lengths_out
+ * may be d_table / d_lengths (both or neither).  A row names a page once.
+ * page <= 32768, rows <= 65535.  Nothing depends on scheduling.
+ * Counterpart in the reference: the block table of its paged pool
+ * (runtime/kv_cache.py:255-810), outside its ported path. */
+typedef struct voom_kv_fork_args {
+  void* d_k; /* layers x n_pages x hk x page x D of 16-bit values, rows 16-byte aligned */
+  void* d_v;
+  const int32_t* d_table; /* rows x per */
+  const int32_t* d_lengths;
+  const int32_t* d_parents; /* or NULL */
+  const int32_t* d_grow;    /* or NULL */
+  int32_t* d_table_out;
+  int32_t* d_lengths_out;
+  int32_t* d_refs;    /* n_pages */
+  int32_t* d_missing; /* one; set, or added to */
+  int64_t k_layer, k_page, k_head, k_pos, v_layer, v_page, v_head, v_pos; /* strides, elements */
+  uint32_t layers, n_pages, hk, page, D, rows, per, grow, add_missing, pad;
+} voom_kv_fork_args;
+uint64_t voom_kv_fork_scratch_bytes(const voom_kv_fork_args* a); /* 16-byte aligned, contents ignored */
+int voom_kv_fork(const voom_kv_fork_args* a, void* d_scratch, uint64_t scratch_bytes, void* stream);
+
+/* The pages that the rows hold (the first ceil(length / page) entries of each)
+ * move to the front of the pool: with L of them, the i-th one past L, in the
+ * pool's order, goes to the i-th page below L that no row holds, in all layers.
+ * The table follows (entries past a row's pages, and outside the pool: -1);
+ * d_live = L.  d_table_out may be d_table. */
+typedef struct voom_kv_compact_args {
+  void* d_k; /* as above */
+  void* d_v;
+  const int32_t* d_table;
+  const int32_t* d_lengths;
+  int32_t* d_table_out;
+  int32_t* d_live;
+  int64_t k_layer, k_page, k_head, k_pos, v_layer, v_page, v_head, v_pos;
+  uint32_t layers, n_pages, hk, page, D, rows, per, pad;
+} voom_kv_compact_args;
+uint64_t voom_kv_compact_scratch_bytes(const voom_kv_compact_args* a);
+int voom_kv_compact(const voom_kv_compact_args* a, void* d_scratch, uint64_t scratch_bytes, void* stream);
+
+/* ------------------------------------------------------------ beam selection */
+/* The `width` best continuations of each of B requests over its beams and the
+ * vocabulary: candidates (beam i, token t) have the score
+ *   d_scores[b, i] + x - log(sum over t' of exp(x_t')),   x = d_logits[b, i, t],
+ * and come largest first, equal ones by beam, then token.  Scores that are NaN or
+ * -inf are never chosen: a logit of -inf takes a token out, a score of -inf a
+ * beam, and a row with a NaN or an infinite logit has none.  Candidates are
+ * compared in 64 bits; the denominators' sums keep what fp32 addition rounds
+ * away.  d_parents: b * beams + i, d_tokens: t, d_scores_out rounded to fp32; where
+ * there are fewer candidates: -1, -1, -inf.  width <= 64, beams <= 64,
+ * beams * V < 2^31. */
+typedef struct voom_beam_select_args {
+  const void* d_logits;  /* B x beams x V, l_b and l_i strides (elements), any alignment */
+  const float* d_scores; /* B x beams contiguous */
+  float* d_scores_out;   /* B x width contiguous */
+  int32_t* d_parents;
+  int32_t* d_tokens;
+  int64_t l_b, l_i;
+  uint32_t B, beams, V, width;
+  uint32_t type; /* VOOM_BF16 / FP16 / FP32 */
+  uint32_t pad;
+} voom_beam_select_args;
+uint64_t voom_beam_select_scratch_bytes(const voom_beam_select_args* a); /* 16-byte aligned, contents ignored */
+int voom_beam_select(const voom_beam_select_args* a, void* d_scratch, uint64_t scratch_bytes, void* stream);
 
 #ifdef __cplusplus
 }

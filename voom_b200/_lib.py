@@ -97,14 +97,33 @@ class KvViewStruct(ctypes.Structure):
 
 
 class TreeAttentionArgs(ctypes.Structure):
-    _fields_ = _fields("p: q kn vn out lse mask weights token_weight status",
-                       "i64: q_b q_t q_h kn_b kn_t kn_h vn_b vn_t vn_h o_b o_t o_h w_b w_h", "u32: n hq", "f32: scale",
-                       "u32: pad")
+    _fields_ = _fields("p: q kn vn out lse mask weights token_weight status slopes depth",
+                       "i64: q_b q_t q_h kn_b kn_t kn_h vn_b vn_t vn_h o_b o_t o_h w_b w_h", "u32: n hq", "f32: scale cap",
+                       "u32: window pad")
 
 
 class KvEvictArgs(ctypes.Structure):
     _fields_ = _fields("p: weights", "i64: w_b w_h", "p: k_out v_out w_out index len_out",
                        "u32: budget sinks recent pad")
+
+
+class KvAppendArgs(ctypes.Structure):
+    _fields_ = _fields("p: kn vn index", "i64: kn_b kn_t kn_h vn_b vn_t vn_h", "u32: n m")
+
+
+class KvForkArgs(ctypes.Structure):
+    _fields_ = _fields("p: k v table lengths parents grow_rows table_out lengths_out refs missing",
+                       "i64: k_layer k_page k_head k_pos v_layer v_page v_head v_pos",
+                       "u32: layers n_pages hk page D rows per grow add_missing pad")
+
+
+class KvCompactArgs(ctypes.Structure):
+    _fields_ = _fields("p: k v table lengths table_out live", "i64: k_layer k_page k_head k_pos v_layer v_page v_head v_pos",
+                       "u32: layers n_pages hk page D rows per pad")
+
+
+class BeamSelectArgs(ctypes.Structure):
+    _fields_ = _fields("p: logits scores scores_out parents tokens", "i64: l_b l_i", "u32: B beams V width type pad")
 
 
 class RansPlanInfo(ctypes.Structure):
@@ -177,6 +196,13 @@ SIGNATURES: dict[str, tuple] = {
     "voom_tree_attention_scratch_bytes": (_u64, [_vp, _vp]),
     "voom_tree_attention": (_i32, [_vp, _vp, _vp, _u64, _vp]),
     "voom_kv_evict": (_i32, [_vp, _vp, _vp]),
+    "voom_kv_append": (_i32, [_vp, _vp, _vp]),
+    "voom_kv_fork_scratch_bytes": (_u64, [_vp]),
+    "voom_kv_fork": (_i32, [_vp, _vp, _u64, _vp]),
+    "voom_kv_compact_scratch_bytes": (_u64, [_vp]),
+    "voom_kv_compact": (_i32, [_vp, _vp, _u64, _vp]),
+    "voom_beam_select_scratch_bytes": (_u64, [_vp]),
+    "voom_beam_select": (_i32, [_vp, _vp, _u64, _vp]),
     "voom_expert_swiglu": (_i32, [_vp, _vp, _u32, _vp, _vp, _u32, _u32, _vp, _u32, _u32, _u32, _u32, _vp, _vp,
                                   _u64, _vp, _vp]),
 }

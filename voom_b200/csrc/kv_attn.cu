@@ -4,9 +4,8 @@
 #include <initializer_list>
 #include <type_traits>
 
-#include "kv_rows.cuh"
-#include "kv_sums.cuh"
-#include "kv_tc.cuh"
+#include "kv_attn.cuh"
+#include "kv_modes.cuh"
 #include "rows.h"
 
 namespace {
@@ -181,6 +180,7 @@ __global__ void __launch_bounds__(256) attn_finish(const __grid_constant__ Attn 
   }
   __syncthreads();
   const float* z = P.scores + uint64_t(head) * P.R * P.score_ld;
+  const uint32_t begin = voom::kv::first_tile(P, len) * P.keys;  // no row sees what lies before: it has no scores
   float got[kWeightSpan / 256] = {};
   const uint32_t end = min(P.score_ld, s0 + kWeightSpan);
   // four rows' scores under way at a time (up to 16 loads a thread)
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(256) attn_finish(const __grid_constant__ Attn 
 #pragma unroll
       for (uint32_t k = 0; k < kWeightSpan / 256; k++) {
         const uint32_t s = s0 + k * 256 + tid;
-        x[q][k] = s < lim ? z[uint64_t(r) * P.score_ld + s] : -INFINITY;
+        x[q][k] = s >= begin && s < lim ? z[uint64_t(r) * P.score_ld + s] : -INFINITY;
       }
     }
 #pragma unroll
@@ -225,19 +225,6 @@ int sm_count() {
   int dev = 0, n = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
   return n;
-}
-
-// Lets a kernel use `bytes` of shared memory on the current device, once per device.
-bool allow_smem(const void* kernel, uint32_t bytes, std::atomic<uint64_t>& devices) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return false;
-  if (devices.load(std::memory_order_relaxed) >> (dev & 63) & 1u) return true;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)) != cudaSuccess) {
-    cudaGetLastError();
-    return false;
-  }
-  devices.fetch_or(uint64_t(1) << (dev & 63), std::memory_order_relaxed);
-  return true;
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -292,6 +279,10 @@ uint64_t plan(Attn& P, void* scratch) {
   P.R = P.a.n * P.g;
   P.words = (P.a.n + 31) / 32;
   P.scale2 = P.a.scale * voom::kv::kLog2e;
+  if (P.a.cap > 0.0f) {
+    P.cap_in = 2.0f * P.scale2 / P.a.cap;
+    P.cap_out = P.a.cap * voom::kv::kLog2e;
+  }
   P.ld_o = c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256;
   P.tc = -1;
   // attn_rows up to the rows whose output its registers hold in one block; it
@@ -309,7 +300,9 @@ uint64_t plan(Attn& P, void* scratch) {
   P.mblocks = (P.R + P.rows - 1) / P.rows;
   P.tails = uint32_t(voom::kv::tails_before(P, P.mblocks - 1)) + voom::kv::tail_of(P, P.mblocks - 1);
   const uint64_t units = uint64_t(c.B) * c.hk * P.mblocks;
-  const uint32_t steps = (c.max_len + P.keys - 1) / P.keys + (P.a.n + P.keys - 1) / P.keys;
+  uint32_t cached = (c.max_len + P.keys - 1) / P.keys;
+  if (P.a.window) cached = min(cached, P.a.window / P.keys + 2);  // (a window ends inside a tile at either side)
+  const uint32_t steps = cached + (P.a.n + P.keys - 1) / P.keys;
   // a block takes at least two tiles for each of its warps (rows), or a few of
   // the larger ones (tensor cores), before the work is spread further
   const uint32_t least = P.tc >= 0 ? 3 : 8;
@@ -335,35 +328,6 @@ uint64_t plan(Attn& P, void* scratch) {
   return at;
 }
 
-template <typename T, int DP, int MT>
-int launch_rows(const Attn& P, cudaStream_t s) {
-  constexpr uint32_t smem = voom::kv::row_smem(DP, MT);
-  static std::atomic<uint64_t> allowed{0};
-  if (!allow_smem(reinterpret_cast<const void*>(voom::kv::attn_rows<T, DP, MT>), smem, allowed)) return VOOM_E_CUDA;
-  const uint64_t grid = P.ctas ? P.ctas : uint64_t(P.c.v.B) * P.c.v.hk * P.mblocks;
-  voom::kv::attn_rows<T, DP, MT><<<uint32_t(grid), 32 * voom::kv::kRowWarps, smem, s>>>(P);
-  return cudaGetLastError() == cudaSuccess ? VOOM_OK : VOOM_E_CUDA;
-}
-
-template <typename T, int DP, int MODE>
-int launch_tc(const Attn& P, cudaStream_t s) {
-  constexpr uint32_t smem = voom::kv::tc_smem<DP, MODE>();
-  static std::atomic<uint64_t> allowed{0};
-  if (!allow_smem(reinterpret_cast<const void*>(voom::kv::attn_tc<T, DP, MODE>), smem, allowed)) return VOOM_E_CUDA;
-  const uint64_t grid = P.ctas ? P.ctas : uint64_t(P.c.v.B) * P.c.v.hk * P.mblocks;
-  voom::kv::attn_tc<T, DP, MODE><<<uint32_t(grid), voom::kv::Tc<DP, MODE>::THREADS, smem, s>>>(P);
-  return cudaGetLastError() == cudaSuccess ? VOOM_OK : VOOM_E_CUDA;
-}
-
-template <typename T, int DP>
-int launch_sums(const Attn& P, cudaStream_t s) {
-  constexpr uint32_t smem = voom::kv::sums_smem<DP>();
-  static std::atomic<uint64_t> allowed{0};
-  if (!allow_smem(reinterpret_cast<const void*>(voom::kv::attn_sums<T, DP>), smem, allowed)) return VOOM_E_CUDA;
-  voom::kv::attn_sums<T, DP><<<P.ctas, voom::kv::Sums<DP>::THREADS, smem, s>>>(P);
-  return cudaGetLastError() == cudaSuccess ? VOOM_OK : VOOM_E_CUDA;
-}
-
 template <typename T>
 int finish(const Attn& P, cudaStream_t s) {
   const uint64_t units = uint64_t(P.c.v.B) * P.c.v.hk * P.mblocks;
@@ -386,17 +350,9 @@ int finish(const Attn& P, cudaStream_t s) {
 
 template <typename T>
 int run(Attn& P, cudaStream_t s) {
-  using voom::kv::kAlternate;
-  using voom::kv::kPair;
-  using voom::kv::kSingle;
-  int rc;
+  const bool scored = P.a.cap > 0.0f || P.a.d_slopes || P.a.window;
   if (P.tc >= 0) map_cache(P);
-  if (P.tc == kSingle) rc = launch_tc<T, 256, kSingle>(P, s);
-  else if (P.tc == kPair) rc = P.ld_o == 64 ? launch_tc<T, 64, kPair>(P, s) : launch_tc<T, 128, kPair>(P, s);
-  else if (P.tc == kAlternate) rc = P.ld_o == 64 ? launch_tc<T, 64, kAlternate>(P, s) : launch_tc<T, 128, kAlternate>(P, s);
-  else if (P.ld_o == 64) rc = P.rows == 16 ? launch_rows<T, 64, 1>(P, s) : launch_rows<T, 64, 2>(P, s);
-  else if (P.ld_o == 128) rc = P.rows == 16 ? launch_rows<T, 128, 1>(P, s) : launch_rows<T, 128, 2>(P, s);
-  else rc = launch_rows<T, 256, 1>(P, s);
+  int rc = scored ? voom::kv::launch_attention<T, true>(P, s) : voom::kv::launch_attention<T, false>(P, s);
   if (rc != VOOM_OK) return rc;
   if (P.ctas || P.scores) rc = finish<T>(P, s);
   if (rc != VOOM_OK || !P.a.d_weights || P.scores) return rc;
@@ -405,10 +361,12 @@ int run(Attn& P, cudaStream_t s) {
   P.rows = P.R;
   P.mblocks = 1;
   P.tails = voom::kv::tail_of(P, 0);
-  const uint64_t steps = uint64_t(P.c.v.B) * P.c.v.hk * ((P.c.v.max_len + 127) / 128 + P.tails);
+  uint32_t cached = (P.c.v.max_len + 127) / 128;
+  if (P.a.window) cached = min(cached, P.a.window / 128 + 2);
+  const uint64_t steps = uint64_t(P.c.v.B) * P.c.v.hk * (cached + P.tails);
   P.ctas = uint32_t(min(uint64_t(sm_count()), steps));
   map_cache(P);
-  return P.ld_o == 64 ? launch_sums<T, 64>(P, s) : P.ld_o == 128 ? launch_sums<T, 128>(P, s) : launch_sums<T, 256>(P, s);
+  return scored ? voom::kv::launch_sums<T, true>(P, s) : voom::kv::launch_sums<T, false>(P, s);
 }
 
 }  // namespace
@@ -429,6 +387,8 @@ int check(const voom_kv_view* c, const voom_tree_attention_args* a, Attn& P) {
   const int rc = voom::kv::make_view(c, P.c);
   if (rc != VOOM_OK) return rc;
   if (!a->hq || a->hq % c->hk || !(a->scale > 0.0f && a->scale <= 3.0e38f)) return VOOM_E_INVALID_ARG;
+  if (!(a->cap >= 0.0f && a->cap <= 3.0e38f)) return VOOM_E_INVALID_ARG;
+  if (a->d_mask && (a->d_slopes || a->window) && !a->d_depth) return VOOM_E_INVALID_ARG;
   if (a->d_mask && a->n > kMaxTree) return VOOM_E_CAPACITY;
   if (uint64_t(c->max_len) + a->n > 0x7FFFFFFFu || uint64_t(c->B) * a->n * a->hq > 0x7FFFFFFFu) return VOOM_E_UNSUPPORTED;
   if (!rows16(a->d_q, {a->q_b, a->q_t, a->q_h}) || !rows16(a->d_kn, {a->kn_b, a->kn_t, a->kn_h}) ||

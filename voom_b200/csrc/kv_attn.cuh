@@ -36,6 +36,7 @@ struct alignas(64) Attn {
   uint32_t ctas;             // 0: direct
   uint32_t score_ld, score_new; // score row length; where the new tokens' scores start
   float scale2;              // scale * log2(e)
+  float cap_in, cap_out;     // of capped scores: 2 scale log2(e) / cap, and cap log2(e); 0: not capped
   int32_t tc;                // tensor-core kernel's mode, or -1: attn_rows
 };
 
@@ -46,7 +47,24 @@ struct Seg {
 
 __host__ __device__ __forceinline__ uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
 
-__device__ __forceinline__ uint32_t cache_steps(const Attn& P, uint32_t len) { return ceil_div(len, P.keys); }
+// The first tile of cached positions that any of a request's rows sees: a window
+// ends `window` positions before the row, and no row stands before position len.
+__device__ __forceinline__ uint32_t first_tile(const Attn& P, uint32_t len) {
+  return P.a.window && len >= P.a.window ? (len - P.a.window + 1) / P.keys : 0u;
+}
+
+// A window's edge moves with the rows: no row sees a cached position below
+// `none`, all see those from `all` on (the last of n rows stands at len + n - 1 at
+// most).  Values between must not reach the rows that do not see them, not even
+// times 0: tiles below `all` are looked through for values that are not finite.
+__device__ __forceinline__ uint32_t window_none(const Attn& P, uint32_t len) {
+  return P.a.window && len >= P.a.window ? len - P.a.window + 1 : 0u;
+}
+__device__ __forceinline__ uint32_t window_all(const Attn& P, uint32_t len) {
+  return P.a.window && len + P.a.n > P.a.window ? len + P.a.n - P.a.window : 0u;
+}
+
+__device__ __forceinline__ uint32_t cache_steps(const Attn& P, uint32_t len) { return ceil_div(len, P.keys) - first_tile(P, len); }
 
 // Steps over the new tokens of the m-th block of rows: in a chain, up to its last token.
 __host__ __device__ __forceinline__ uint32_t tail_of(const Attn& P, uint32_t m) {
@@ -210,10 +228,47 @@ __device__ __forceinline__ uint32_t sees32(const Attn& P, uint32_t b, uint32_t i
   return i < j0 ? 0u : i - j0 >= 31u ? 0xFFFFFFFFu : (2u << (i - j0)) - 1u;
 }
 
+// How far behind the cache new token i stands: its depth in the tree.
+__device__ __forceinline__ int32_t depth_of(const Attn& P, uint32_t b, uint32_t i) {
+  return P.a.d_mask && P.a.d_depth && i < P.a.n ? __ldg(P.a.d_depth + uint64_t(b) * P.a.n + i) : int32_t(i);
+}
+
+// Of 32 keys from distance `ahead` of a row on (key position - row position, one
+// more for each), those inside the window, at distances above -window.
+__device__ __forceinline__ uint32_t window32(const Attn& P, int32_t ahead) {
+  if (!P.a.window) return 0xFFFFFFFFu;
+  const int64_t out = -int64_t(P.a.window) - ahead + 1;  // keys before the window
+  return out <= 0 ? 0xFFFFFFFFu : out >= 32 ? 0u : 0xFFFFFFFFu << out;
+}
+
+__device__ __forceinline__ bool in_window(const Attn& P, int32_t ahead) {
+  return !P.a.window || -int64_t(ahead) < int64_t(P.a.window);
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// A product q . k as a score in log2 units, for calls whose scores are capped,
+// biased or windowed ("scored").  cap tanh(z / cap) as cap - 2 cap / (1 + e^(2 z / cap)):
+// off by a few 2^-23 of the cap, absolutely, and no further at either end.
+__device__ __forceinline__ float scored(const Attn& P, float x, float slope2, float ahead) {
+  float y;
+  if (P.cap_in != 0.0f) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + exp2_fast(x * P.cap_in)));
+    y = fmaf(-2.0f * P.cap_out, r, P.cap_out);
+  } else {
+    y = x * P.scale2;
+  }
+  return fmaf(slope2, ahead, y);
+}
+
+// A query head's slope in log2 units.
+__device__ __forceinline__ float slope2_of(const Attn& P, uint32_t head) {
+  return P.a.d_slopes ? kLog2e * __ldg(P.a.d_slopes + head) : 0.0f;
 }
 
 // sum += x with what the addition lost kept in `rest`: beside one large term, a
@@ -288,6 +343,13 @@ __device__ __forceinline__ bool odd_values(uint4 c) {
   }
   return bad;
 }
+
+// The attention's kernel, and the rows' weights from the keys again, for caches
+// of type T; SCORED: scores are capped, biased or windowed (kv_launch.cuh).
+template <typename T, bool SCORED>
+int launch_attention(const Attn& P, cudaStream_t s);
+template <typename T, bool SCORED>
+int launch_sums(const Attn& P, cudaStream_t s);
 
 }  // namespace kv
 }  // namespace voom

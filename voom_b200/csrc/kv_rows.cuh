@@ -16,6 +16,7 @@
 #pragma once
 
 #include "kv_attn.cuh"
+#include "kv_modes.cuh"
 
 namespace voom {
 namespace kv {
@@ -24,8 +25,6 @@ constexpr uint32_t kRowWarps = 4;
 constexpr uint32_t kRowStages = 3;
 constexpr uint32_t kJoin = 64;  // values of a head that the warps join at a time
 
-// Keys of a tile: 8 KB of keys and 8 KB of values.
-__host__ __device__ constexpr uint32_t row_keys(uint32_t dp) { return 4096u / dp; }
 // Shared memory: the warps' stages, the joining buffer, the rows' maxima and
 // sums, and the queries.
 __host__ __device__ constexpr uint32_t row_smem(uint32_t dp, uint32_t mt) {
@@ -74,7 +73,8 @@ __device__ __forceinline__ uint32_t row_off(uint32_t r, uint32_t c) {
 template <typename T, int DP>
 __device__ __forceinline__ void load_tile(const Attn& P, const Seg& g, uint32_t h, uint32_t step, uint32_t dst) {
   constexpr uint32_t KT = row_keys(DP), CH = DP / 8, per = (KT + 31) / 32;
-  const uint32_t lane = threadIdx.x & 31u, cs = cache_steps(P, g.len);
+  const uint32_t lane = threadIdx.x & 31u, cs = cache_steps(P, g.len), w0 = first_tile(P, g.len),
+                 none = window_none(P, g.len);
   // a lane finds the rows lane, lane + 32; the loads take them by shuffles
   uint64_t ka[per], va[per];
 #pragma unroll
@@ -83,9 +83,9 @@ __device__ __forceinline__ void load_tile(const Attn& P, const Seg& g, uint32_t 
     ka[i] = va[i] = 0;
     if (r < KT) {
       if (step < cs) {
-        const uint32_t s = step * KT + r;
+        const uint32_t s = (w0 + step) * KT + r;
         int64_t ko, vo;
-        if (s < g.len && P.c.row_at(g.b, h, s, ko, vo)) {
+        if (s >= none && s < g.len && P.c.row_at(g.b, h, s, ko, vo)) {
           ka[i] = reinterpret_cast<uint64_t>(static_cast<const T*>(P.c.v.d_k) + ko);
           va[i] = reinterpret_cast<uint64_t>(static_cast<const T*>(P.c.v.d_v) + vo);
         }
@@ -114,7 +114,7 @@ __device__ __forceinline__ void load_tile(const Attn& P, const Seg& g, uint32_t 
 }
 
 // DP: head size rounded up to 64, 128 or 256.  MT: blocks of 16 rows.
-template <typename T, int DP, int MT>
+template <typename T, int DP, int MT, bool SCORED>
 __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_constant__ Attn P) {
   constexpr uint32_t KT = row_keys(DP), CH = DP / 8, NT = KT / 8, DT = DP / 8, LDJ = kJoin, ROWS = 16 * MT;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -148,7 +148,19 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
   uint32_t slot = 0;
   do {
     const uint32_t h = g.h, row0 = g.m * ROWS, nrows = min(ROWS, P.R - row0);
-    const uint32_t cs = cache_steps(P, g.len);
+    const uint32_t cs = cache_steps(P, g.len), w0 = SCORED ? first_tile(P, g.len) : 0u;
+    float slope2[MT][2];  // of the lane's rows, and how far behind the cache they stand
+    int32_t behind[MT][2];
+    if constexpr (SCORED) {
+#pragma unroll
+      for (int t = 0; t < MT; t++)
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+          const uint32_t row = min(row0 + 16 * t + oct + 8 * x, P.R - 1);
+          slope2[t][x] = slope2_of(P, h * P.g + row % P.g);
+          behind[t][x] = depth_of(P, g.b, row / P.g);
+        }
+    }
     // the unit's queries
     for (uint32_t i = tid; i < ROWS * CH; i += 32 * kRowWarps) {
       const uint32_t r = i / CH, c = i % CH, row = row0 + r;
@@ -201,11 +213,29 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
           }
         }
       }
-      // masks: positions past the length, and the new tokens that a row does not see
       const bool fresh = step >= cs;
-      uint32_t odd = 0, odd_hi = 0;  // new tokens of the tile whose values are not all finite
-      if (fresh || step * KT + KT > g.len) {
-        const uint32_t j0 = fresh ? (step - cs) * KT : 0u, valid = fresh ? 0u : g.len - step * KT;
+      const uint32_t p0 = (w0 + step) * KT;  // of a cached tile: its first position
+      if constexpr (SCORED) {
+#pragma unroll
+        for (uint32_t j = 0; j < NT; j++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const uint32_t k = 8 * j + 2 * quad + e;
+            const int32_t key = fresh ? depth_of(P, g.b, (step - cs) * KT + k) : int32_t(p0 + k) - int32_t(g.len);
+#pragma unroll
+            for (int t = 0; t < MT; t++)
+#pragma unroll
+              for (int x = 0; x < 2; x++) {
+                const int32_t ahead = key - behind[t][x];
+                float& y = z[t][j][2 * x + e];
+                y = in_window(P, ahead) ? scored(P, y, slope2[t][x], float(ahead)) : -INFINITY;
+              }
+          }
+      }
+      // masks: positions past the length, and the new tokens that a row does not see
+      uint32_t odd = 0, odd_hi = 0;  // keys of the tile that some rows do not see and whose values are not all finite
+      if (fresh || p0 + KT > g.len) {
+        const uint32_t j0 = fresh ? (step - cs) * KT : 0u, valid = fresh ? 0u : g.len - p0;
 #pragma unroll
         for (int t = 0; t < MT; t++)
 #pragma unroll
@@ -221,23 +251,24 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
                 if (!((k < 32 ? lo : hi) >> (k & 31u) & 1u)) z[t][j][2 * x + e] = -INFINITY;
               }
           }
-        if (fresh) {  // a probability of 0 must not meet an infinite or NaN value: take those out here
-          bool found = false;
-          for (uint32_t id = lane; id < KT * CH; id += 32) {
-            const uint32_t r = id / CH, at = vs - smem_addr(smem) + row_off<DP>(r, id % CH);
-            if (odd_values<T>(*reinterpret_cast<const uint4*>(smem + at))) {
-              *reinterpret_cast<uint4*>(smem + at) = make_uint4(0, 0, 0, 0);
-              if (r < 32) odd |= 1u << r;
-              else odd_hi |= 1u << (r - 32);
-              found = true;
-            }
+      }
+      const bool ragged = SCORED && !fresh && p0 < window_all(P, g.len) && P.a.n > 1;
+      if (fresh || ragged) {  // a probability of 0 must not meet an infinite or NaN value: take those out here
+        bool found = false;
+        for (uint32_t id = lane; id < KT * CH; id += 32) {
+          const uint32_t r = id / CH, at = vs - smem_addr(smem) + row_off<DP>(r, id % CH);
+          if (odd_values<T>(*reinterpret_cast<const uint4*>(smem + at))) {
+            *reinterpret_cast<uint4*>(smem + at) = make_uint4(0, 0, 0, 0);
+            if (r < 32) odd |= 1u << r;
+            else odd_hi |= 1u << (r - 32);
+            found = true;
           }
-          if (__any_sync(0xFFFFFFFFu, found)) {
-            odd = __reduce_or_sync(0xFFFFFFFFu, odd);
-            odd_hi = __reduce_or_sync(0xFFFFFFFFu, odd_hi);
-          }
-          __syncwarp();
         }
+        if (__any_sync(0xFFFFFFFFu, found)) {
+          odd = __reduce_or_sync(0xFFFFFFFFu, odd);
+          odd_hi = __reduce_or_sync(0xFFFFFFFFu, odd_hi);
+        }
+        __syncwarp();
       }
 #pragma unroll
       for (int t = 0; t < MT; t++) {
@@ -246,11 +277,11 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
         for (uint32_t j = 0; j < NT; j++)
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            z[t][j][e] *= P.scale2;
+            if (!SCORED) z[t][j][e] *= P.scale2;
             top[e >> 1] = fmaxf(top[e >> 1], z[t][j][e]);
           }
         if (P.scores) {
-          const uint32_t at = fresh ? P.score_new + (step - cs) * KT : step * KT;
+          const uint32_t at = fresh ? P.score_new + (step - cs) * KT : p0;
 #pragma unroll
           for (int x = 0; x < 2; x++) {
             const uint32_t r = 16 * t + oct + 8 * x;
@@ -326,13 +357,23 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
               if (!((k < 32 ? odd : odd_hi) >> (k & 31u) & 1u)) continue;
               const T* v = static_cast<const T*>(P.a.d_vn) + int64_t(g.b) * P.a.vn_b + int64_t(tok) * P.a.vn_t +
                            int64_t(h) * P.a.vn_h;
+              int32_t key = 0;  // where it stands, from the cache's end
+              if constexpr (SCORED) {
+                key = fresh ? depth_of(P, g.b, tok) : int32_t(p0 + k) - int32_t(g.len);
+                int64_t ko, vo;
+                if (!fresh) {
+                  if (!P.c.row_at(g.b, h, p0 + k, ko, vo)) continue;  // (was zeros)
+                  v = static_cast<const T*>(P.c.v.d_v) + vo;
+                }
+              }
 #pragma unroll
               for (int t = 0; t < MT; t++)
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
                   const float p = __shfl_sync(0xFFFFFFFFu, z[t][j][2 * x + e], (lane & ~3u) | s);
                   const uint32_t i = (row0 + 16 * t + oct + 8 * x) / P.g;
-                  if (i >= P.a.n || !sees(P, g.b, i, tok)) continue;
+                  if (i >= P.a.n || ((!SCORED || fresh) && !sees(P, g.b, i, tok))) continue;
+                  if (SCORED && !in_window(P, key - behind[t][x])) continue;
 #pragma unroll
                   for (uint32_t d = 0; d < DT; d++)
 #pragma unroll

@@ -35,6 +35,8 @@ struct SumsShared {
   uint32_t tmem, failed;
   float2 row[2][256];  // for each softmax warpgroup: minus the row's denominator (log2), its weight
   uint32_t tok[2][256];  // and its token
+  float slope2[2][256];  // scored: its slope, and how far behind the cache it stands
+  int32_t behind[2][256];
 };
 
 template <int DP>
@@ -45,7 +47,7 @@ constexpr uint32_t sums_smem() {
 }
 
 // P: units of all rows of a key head (mblocks = 1), keys = 128.
-template <typename T, int DP>
+template <typename T, int DP, bool SCORED>
 __global__ void __launch_bounds__(Sums<DP>::THREADS, 1) attn_sums(const __grid_constant__ Attn P) {
   using C = Sums<DP>;
   constexpr uint32_t KT = C::KT, NB = C::NB, CH = DP / 8, RING = C::RING, LOAD_WARP = 8, MMA_WARP = 12;
@@ -160,7 +162,7 @@ __global__ void __launch_bounds__(Sums<DP>::THREADS, 1) attn_sums(const __grid_c
       return warp_wait(sh.ready[w], nr++ & 1u);
     };
     do {
-      const uint32_t cs = cache_steps(P, g.len), n = g.s1 - g.s0;
+      const uint32_t cs = cache_steps(P, g.len), n = g.s1 - g.s0, w0 = SCORED ? first_tile(P, g.len) : 0u;
       float* sums = P.a.d_weights + int64_t(g.b) * P.a.w_b + int64_t(g.h) * P.a.w_h;
       for (uint32_t m = 0; m < blocks && ok; m++) {
         const uint32_t row0 = m * NB, nrows = min(NB, P.R - row0), cols = (nrows + 31u) & ~31u;
@@ -174,6 +176,10 @@ __global__ void __launch_bounds__(Sums<DP>::THREADS, 1) attn_sums(const __grid_c
           }
           sh.row[w][r] = x;
           sh.tok[w][r] = row < P.R ? i : P.a.n;
+          if constexpr (SCORED) {
+            sh.slope2[w][r] = slope2_of(P, g.h * P.g + row % P.g);
+            sh.behind[w][r] = depth_of(P, g.b, i);
+          }
         }
         if (!(ok = together())) break;
         for (uint32_t t = w; t < n; t += 2) {
@@ -181,7 +187,8 @@ __global__ void __launch_bounds__(Sums<DP>::THREADS, 1) attn_sums(const __grid_c
           if (!(ok = warp_wait(sh.s_full[w], ns++ & 1u))) break;
           tc::tc_fence_after();
           const bool fresh = step >= cs;
-          const uint32_t j = (fresh ? step - cs : step) * KT + tr;
+          const uint32_t j = (fresh ? step - cs : w0 + step) * KT + tr;
+          const int32_t key = !SCORED ? 0 : fresh ? depth_of(P, g.b, j) : int32_t(j) - int32_t(g.len);  // from the cache's end
           float acc[2] = {0.0f, 0.0f};
           for (uint32_t c = 0; c < cols; c += 32) {
             uint32_t s[32];
@@ -192,8 +199,17 @@ __global__ void __launch_bounds__(Sums<DP>::THREADS, 1) attn_sums(const __grid_c
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
               const float4 x = row[e / 2];
-              float p = exp2_fast(fmaf(__uint_as_float(s[e]), P.scale2, x.x));
-              float q = exp2_fast(fmaf(__uint_as_float(s[e + 1]), P.scale2, x.z));
+              float p, q;
+              if constexpr (SCORED) {
+                const int32_t d0 = key - sh.behind[w][c + e], d1 = key - sh.behind[w][c + e + 1];
+                p = exp2_fast(scored(P, __uint_as_float(s[e]), sh.slope2[w][c + e], float(d0)) + x.x);
+                q = exp2_fast(scored(P, __uint_as_float(s[e + 1]), sh.slope2[w][c + e + 1], float(d1)) + x.z);
+                if (P.a.window && -int64_t(d0) >= int64_t(P.a.window)) p = 0.0f;
+                if (P.a.window && -int64_t(d1) >= int64_t(P.a.window)) q = 0.0f;
+              } else {
+                p = exp2_fast(fmaf(__uint_as_float(s[e]), P.scale2, x.x));
+                q = exp2_fast(fmaf(__uint_as_float(s[e + 1]), P.scale2, x.z));
+              }
               if (fresh) {
                 const uint32_t i0 = sh.tok[w][c + e], i1 = sh.tok[w][c + e + 1];
                 if (i0 >= P.a.n || j >= P.a.n || !sees(P, g.b, i0, j)) p = 0.0f;

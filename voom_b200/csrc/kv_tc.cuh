@@ -27,12 +27,11 @@
 #pragma once
 
 #include "kv_attn.cuh"
+#include "kv_modes.cuh"
 #include "tcgen05.cuh"
 
 namespace voom {
 namespace kv {
-
-constexpr int kPair = 0, kAlternate = 1, kSingle = 2;
 
 template <int DP, int MODE>
 struct Tc {
@@ -76,33 +75,52 @@ __device__ __forceinline__ uint32_t sw128(uint32_t r, uint32_t c, uint32_t rows)
 // Values of new tokens that are not finite were taken out of their tiles (a
 // probability of 0 must not meet them); this adds them back for a row that
 // sees them, one at a time: y[0..32) are the row's sums of values col ..
-template <typename T>
+template <typename T, bool SCORED>
 __device__ __forceinline__ void odd_fix(const Attn& P, const Seg& g, uint32_t row, float m2, uint32_t col, float* y) {
   const uint32_t cs = cache_steps(P, g.len), i = row / P.g;
-  const uint32_t j0 = (max(g.s0, cs) - cs) * P.keys, j1 = g.s1 > cs ? min(P.a.n, (g.s1 - cs) * P.keys) : 0u;
   const T* q = static_cast<const T*>(P.a.d_q) + int64_t(g.b) * P.a.q_b + int64_t(i) * P.a.q_t +
                int64_t(g.h * P.g + row % P.g) * P.a.q_h;
-  for (uint32_t j = j0; j < j1; j++) {
-    if (!sees(P, g.b, i, j)) continue;
-    const T* v = static_cast<const T*>(P.a.d_vn) + int64_t(g.b) * P.a.vn_b + int64_t(j) * P.a.vn_t + int64_t(g.h) * P.a.vn_h;
+  // one key's part; `ahead`: from the row to it
+  auto add = [&](const T* k, const T* v, int32_t ahead) {
     float p = -1.0f;
     for (uint32_t c = 0; c < 32 && col + c < P.c.v.D; c += 8) {
       if (!odd_values<T>(*reinterpret_cast<const uint4*>(v + col + c))) continue;
       if (p < 0.0f) {
-        const T* k = static_cast<const T*>(P.a.d_kn) + int64_t(g.b) * P.a.kn_b + int64_t(j) * P.a.kn_t + int64_t(g.h) * P.a.kn_h;
         float z = 0.0f;
         #pragma unroll 1
         for (uint32_t d = 0; d < P.c.v.D; d++) z += elem<T>(q[d]) * elem<T>(k[d]);
-        p = exp2_fast(z * P.scale2 - m2);
+        if constexpr (SCORED) p = exp2_fast(scored(P, z, slope2_of(P, g.h * P.g + row % P.g), float(ahead)) - m2);
+        else p = exp2_fast(z * P.scale2 - m2);
       }
       for (uint32_t e = 0; e < 8; e++) y[c + e] += p * elem<T>(v[col + c + e]);
     }
+  };
+  const int32_t behind = SCORED ? depth_of(P, g.b, i) : 0;
+  if constexpr (SCORED) {  // cached positions that the window's edge passes
+    const uint32_t w0 = first_tile(P, g.len);
+    const uint32_t edge = ceil_div(window_all(P, g.len), P.keys) * P.keys;  // (whole tiles are looked through)
+    const uint32_t s0 = max(window_none(P, g.len), (w0 + g.s0) * P.keys), s1 = min(min(edge, g.len), (w0 + g.s1) * P.keys);
+    if (P.a.n > 1)
+      for (uint32_t s = s0; s < s1; s++) {
+        const int32_t ahead = int32_t(s) - int32_t(g.len) - behind;
+        int64_t ko, vo;
+        if (in_window(P, ahead) && P.c.row_at(g.b, g.h, s, ko, vo))
+          add(static_cast<const T*>(P.c.v.d_k) + ko, static_cast<const T*>(P.c.v.d_v) + vo, ahead);
+      }
+  }
+  const uint32_t j0 = (max(g.s0, cs) - cs) * P.keys, j1 = g.s1 > cs ? min(P.a.n, (g.s1 - cs) * P.keys) : 0u;
+  for (uint32_t j = j0; j < j1; j++) {
+    if (!sees(P, g.b, i, j)) continue;
+    const int32_t ahead = SCORED ? depth_of(P, g.b, j) - behind : 0;
+    if (SCORED && !in_window(P, ahead)) continue;
+    add(static_cast<const T*>(P.a.d_kn) + int64_t(g.b) * P.a.kn_b + int64_t(j) * P.a.kn_t + int64_t(g.h) * P.a.kn_h,
+        static_cast<const T*>(P.a.d_vn) + int64_t(g.b) * P.a.vn_b + int64_t(j) * P.a.vn_t + int64_t(g.h) * P.a.vn_h, ahead);
   }
 }
 
 // One of four warps' part (128 threads) of bringing a tile of keys or values to
 // shared memory; its barrier gets 128 arrivals.  A tile of cached positions
-// that are all valid comes by TMA, one box for each run of positions in a page:
+// that are all valid and seen comes by TMA, one box for each run of positions in a page:
 // the lanes of the first warp find the pages.  Others (the end of a cache, new
 // tokens, caches that TMA cannot read) are gathered through cp.async; their
 // barrier hears of the copies as they land, and the issuing thread fences them
@@ -113,13 +131,15 @@ __device__ __forceinline__ bool load_tile_sw128(const Attn& P, const Seg& g, uin
                                                 uint32_t lane, uint32_t dst, uint32_t full, bool hold) {
   constexpr uint32_t CH = DP / 8, RW = KT / 4;
   const bool fresh = step >= cs;
-  if (P.box && step * KT + KT <= g.len) {
+  const uint32_t p0 = (first_tile(P, g.len) + step) * KT;  // of a cached tile: its first position
+  const uint32_t none = window_none(P, g.len);  // what no row sees comes as zeros
+  if (P.box && !fresh && p0 + KT <= g.len && p0 >= none && !hold) {
     if (pw == 0) {
       if (lane == 0) tc::mbar_arrive_expect(full, KT * DP * 2);
       else tc::mbar_arrive(full);
       __syncwarp();
       if (lane < KT / P.box) {
-        const uint32_t s = step * KT + lane * P.box, pg = P.c.page_of(s);
+        const uint32_t s = p0 + lane * P.box, pg = P.c.page_of(s);
         const int32_t w = P.c.v.d_table ? __ldg(P.c.v.d_table + uint64_t(g.b) * P.c.v.table_stride + pg) : int32_t(g.b);
         const uint32_t y = P.c.v.d_table ? s - pg * P.c.v.page : s;
         const void* map = is_v ? &P.v_map : &P.k_map;
@@ -136,9 +156,9 @@ __device__ __forceinline__ bool load_tile_sw128(const Attn& P, const Seg& g, uin
   if (lane < RW) {
     const uint32_t r = pw * RW + lane;
     if (!fresh) {
-      const uint32_t s = step * KT + r;
+      const uint32_t s = p0 + r;
       int64_t ko, vo;
-      if (s < g.len && P.c.row_at(g.b, g.h, s, ko, vo))
+      if (s >= none && s < g.len && P.c.row_at(g.b, g.h, s, ko, vo))
         a = is_v ? reinterpret_cast<uint64_t>(static_cast<const T*>(P.c.v.d_v) + vo)
                  : reinterpret_cast<uint64_t>(static_cast<const T*>(P.c.v.d_k) + ko);
     } else {
@@ -167,7 +187,7 @@ __device__ __forceinline__ void load_keys(const Attn& P, const Seg& g, uint32_t 
   load_tile_sw128<T, DP, KT>(P, g, step, cs, false, pw, lane, dst, full, false);
 }
 
-template <typename T, int DP, int MODE>
+template <typename T, int DP, int MODE, bool SCORED>
 __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid_constant__ Attn P) {
   using C = Tc<DP, MODE>;
   constexpr uint32_t KT = C::KT, ROWS = C::ROWS, CH = DP / 8, RING = C::RING;
@@ -231,6 +251,8 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
     };
     do {
       const uint32_t row0 = g.m * ROWS, cs = cache_steps(P, g.len), n = g.s1 - g.s0;
+      // tiles of values below it are looked through, as those of the new tokens are
+      const uint32_t edge = SCORED && P.a.n > 1 ? window_all(P, g.len) : 0u, w0 = SCORED ? first_tile(P, g.len) : 0u;
       if (nq) {  // the last segment's products of the queries must be done
         if (!(ok = warp_wait(sh.q_empty, (nq - 1) & 1u))) break;
       }
@@ -265,7 +287,8 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
         const uint32_t step = g.s0 + j, place = it % RING;
         if (it >= RING && !(ok = warp_wait(sh.empty[place], (it / RING - 1) & 1u))) break;
         it++;
-        if (load_tile_sw128<T, DP, KT>(P, g, step, cs, is_v, pw, lane, ring_s + place * C::TILE, bar(sh.full[place]), step >= cs && is_v)) {
+        if (load_tile_sw128<T, DP, KT>(P, g, step, cs, is_v, pw, lane, ring_s + place * C::TILE, bar(sh.full[place]),
+                                           is_v && (step >= cs || (SCORED && (w0 + step) * KT < edge)))) {
           look_through(place);
           tc::mbar_arrive(bar(sh.full[place]));
         }
@@ -389,24 +412,41 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
     bool ok = true;
     do {
       const uint32_t row = g.m * ROWS + (MODE == kPair ? w * 128 : 0) + tr, tok = row / P.g, cs = cache_steps(P, g.len);
-      const uint32_t n = g.s1 - g.s0;
+      const uint32_t n = g.s1 - g.s0, w0 = SCORED ? first_tile(P, g.len) : 0u;
       float m = -INFINITY, l = 0.0f, rest = 0.0f;  // l + rest: the denominator
+      const float to_log2 = SCORED ? 1.0f : P.scale2;
+      const float slope2 = SCORED ? slope2_of(P, g.h * P.g + row % P.g) : 0.0f;
+      const int32_t behind = SCORED ? depth_of(P, g.b, tok) : 0;  // how far behind the cache the row stands
       for (uint32_t i = MODE == kAlternate ? w : 0; i < n; i += MODE == kAlternate ? 2 : 1) {
         const uint32_t slot = MODE == kSingle ? i & 1u : w, step = g.s0 + i;
         const uint32_t o_col = C::O_COL + (MODE == kSingle ? 0u : w * DP);
         if (!(ok = warp_wait(sh.s_full[slot], ns[slot]++ & 1u))) break;
         tc::tc_fence_after();
         const uint32_t s_at = tmem + lanes + slot * C::S_COL;
-        const bool masked = step >= cs || step * KT + KT > g.len;
+        const uint32_t p0 = (w0 + step) * KT;  // of a cached tile: its first position
+        const bool fresh = step >= cs;
+        // of the tile's first key, in a cached tile or a chain
+        const int32_t ahead = (fresh ? int32_t((step - cs) * KT) : int32_t(p0) - int32_t(g.len)) - behind;
+        const bool masked = fresh || p0 + KT > g.len || (SCORED && P.a.window && -int64_t(ahead) >= int64_t(P.a.window));
         uint32_t see[KT / 32];
         if (masked) {
 #pragma unroll
           for (uint32_t c = 0; c < KT / 32; c++) {
-            if (step >= cs) {
+            if (fresh) {
               see[c] = sees32(P, g.b, tok, (step - cs) * KT + 32 * c);
             } else {
-              const uint32_t valid = g.len - step * KT;
+              const uint32_t valid = g.len - p0;
               see[c] = valid >= 32 * c + 32 ? 0xFFFFFFFFu : valid <= 32 * c ? 0u : (1u << (valid - 32 * c)) - 1u;
+            }
+            if constexpr (SCORED) {
+              if (!fresh || !P.a.d_mask) {
+                see[c] &= window32(P, ahead + int32_t(32 * c));
+              } else if (P.a.window) {  // a tree's tokens stand at their depths
+                for (uint32_t left = see[c]; left; left &= left - 1) {
+                  const uint32_t e = __ffs(left) - 1;
+                  if (int64_t(behind) - depth_of(P, g.b, (step - cs) * KT + 32 * c + e) >= int64_t(P.a.window)) see[c] &= ~(1u << e);
+                }
+              }
             }
           }
         }
@@ -416,6 +456,16 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
         tc::tmem_wait_ld();
 #pragma unroll
         for (uint32_t c = 0; c < KT / 32; c++) tc::tmem_hold(s[c]);
+        if constexpr (SCORED) {
+#pragma unroll
+          for (uint32_t c = 0; c < KT / 32; c++)
+#pragma unroll
+            for (int e = 0; e < 32; e++) {
+              const int32_t k = int32_t(32 * c) + e;
+              const int32_t d = fresh && P.a.d_mask && P.a.d_slopes ? depth_of(P, g.b, (step - cs) * KT + k) - behind : ahead + k;
+              s[c][e] = __float_as_uint(scored(P, __uint_as_float(s[c][e]), slope2, float(d)));
+            }
+        }
         if (masked) {
 #pragma unroll
           for (uint32_t c = 0; c < KT / 32; c++)
@@ -429,9 +479,9 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
           for (int e = 0; e < 32; e += 2)
             tops[(e >> 1) & 3] = max3(tops[(e >> 1) & 3], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
         const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-        const bool grow = m != -INFINITY && (top - m) * P.scale2 > 8.0f;
+        const bool grow = m != -INFINITY && (top - m) * to_log2 > 8.0f;
         if (__any_sync(0xFFFFFFFFu, grow)) {
-          const float f = grow ? exp2_fast((m - top) * P.scale2) : 1.0f;
+          const float f = grow ? exp2_fast((m - top) * to_log2) : 1.0f;
           if (MODE == kSingle && done) {
             if (!(ok = warp_wait(sh.pv_done, (done - 1) & 1u))) break;
             tc::tc_fence_after();
@@ -450,8 +500,8 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
           if (grow) m = top;
         }
         if (m == -INFINITY) m = top;
-        const float base = m == -INFINITY ? 0.0f : m * P.scale2 - kLift<T, 8>;
-        const F2 sc = make2(P.scale2, P.scale2), nb = make2(-base, -base);
+        const float base = m == -INFINITY ? 0.0f : m * to_log2 - kLift<T, 8>;
+        const F2 sc = make2(to_log2, to_log2), nb = make2(-base, -base);
         F2 sum[2] = {make2(0.0f, 0.0f), make2(0.0f, 0.0f)};
 #pragma unroll
         for (uint32_t c = 0; c < KT / 32; c++) {
@@ -479,7 +529,7 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
       if (!ok) break;
       // the segment's sums
       l += rest;
-      float m2 = m == -INFINITY ? -INFINITY : m * P.scale2 - kLift<T, 8>, f0 = 1.0f, f1 = 0.0f;  // what O and l are relative to
+      float m2 = m == -INFINITY ? -INFINITY : m * to_log2 - kLift<T, 8>, f0 = 1.0f, f1 = 0.0f;  // what O and l are relative to
       uint32_t c0 = 0, c1 = DP;
       if (MODE == kAlternate) {
         sh.ml[w][tr] = make_float2(m2, l);
@@ -530,7 +580,7 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
           float z[32];
 #pragma unroll
           for (int e = 0; e < 32; e++) z[e] = y[e];
-          odd_fix<T>(P, g, row, m2, c, z);
+          odd_fix<T, SCORED>(P, g, row, m2, c, z);
 #pragma unroll
           for (int e = 0; e < 32; e++) y[e] = z[e];
         }

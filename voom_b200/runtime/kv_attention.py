@@ -220,7 +220,7 @@ class DraftTree:
 
 # voom_tree_attention_args and voom_kv_evict_args as bytes: cheaper to make than
 # ctypes structures, and one-token calls are bound by the host
-_ATTN = struct.Struct("9Q14q2If4x")
+_ATTN = struct.Struct("11Q14q2I2fI4x")
 _EVICT = struct.Struct("Q2q5Q4I")
 assert _ATTN.size == ctypes.sizeof(TreeAttentionArgs) and _EVICT.size == ctypes.sizeof(KvEvictArgs)
 
@@ -249,7 +249,8 @@ def _sums(weights: torch.Tensor, cache: KVView, positions: int) -> tuple:
 def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: DraftTree, cache: KVView, *,
                    scale: float | None = None, weights: torch.Tensor | None = None,
                    token_weight: torch.Tensor | None = None, out: torch.Tensor | None = None,
-                   return_lse: bool = False, stream: torch.cuda.Stream | None = None):
+                   return_lse: bool = False, cap: float | None = None, slopes: torch.Tensor | None = None,
+                   window: int | None = None, stream: torch.cuda.Stream | None = None):
     """Attention of the new tokens (q: (B, n, Hq, D); k, v: (B, n, heads, D),
     any strides with 16-byte rows) over the cache and over one another, as
     `tree` says: (B, n, Hq, D) in the cache's type, and with `return_lse` the
@@ -257,6 +258,12 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: Draf
     h reads key head h // (Hq // heads); `scale` defaults to D ** -0.5.  A row
     of no token gives zeros and lse -inf.  `out` must not share memory with q, k
     or v, nor rows of `out` or `weights` with one another.
+
+    With `cap` a score z becomes cap tanh(z / cap); with `slopes` (Hq) fp32,
+    slopes[h] (p_k - p_q) is added to it, after the cap; with `window` a row sees
+    only positions with p_q - p_k < window, itself among them (its tiles before
+    are not read).  A cached position is its index, a new token's lengths[b] + its
+    depth in the tree.
 
     `weights` (B, heads, >= max_len + n) fp32: each position's softmax weight,
     summed over the rows that share its head (each times `token_weight` (B, n)
@@ -267,7 +274,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: Draf
     if stream is not None or _device.current_index() != cache.index:
         with _device.on_stream(cache.device, stream):
             return tree_attention(q, k, v, tree, cache, scale=scale, weights=weights, token_weight=token_weight,
-                                  out=out, return_lse=return_lse)
+                                  out=out, return_lse=return_lse, cap=cap, slopes=slopes, window=window)
     if q.dim() != 4:
         raise ValueError(f"q: (B, n, Hq, D) wanted, got {tuple(q.shape)}")
     B, n, hq, D = q.shape
@@ -294,14 +301,26 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: Draf
                 or token_weight.get_device() != cache.index:
             raise ValueError(f"token_weight: contiguous fp32 ({B}, {n}) on {cache.device} wanted")
         tw = token_weight.data_ptr()
+    sl = depth = 0
+    if cap is not None and not 0.0 < cap < 3e38:
+        raise ValueError(f"cap {cap}: a positive number wanted")
+    if window is not None and window < 1:
+        raise ValueError(f"a window of {window} positions: at least 1, the row itself")
+    if slopes is not None:
+        if slopes.shape != (hq,) or slopes.dtype != torch.float32 or not slopes.is_contiguous() or slopes.get_device() != cache.index:
+            raise ValueError(f"slopes: contiguous fp32 ({hq},) on {cache.device} wanted, got {tuple(slopes.shape)} {slopes.dtype}")
+        sl = slopes.data_ptr()
+    if tree.mask_ptr and (slopes is not None or window is not None):
+        depth = tree.depth.data_ptr()
     if out is None:
         out = q.new_empty((B, n, hq, D))
     os = _new(out, "out", B, n, hq, cache)
     lse = q.new_empty((B, n, hq), dtype=torch.float32) if return_lse else None
     if n:
         a = _ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-                       tree.mask_ptr, wp, tw, cache.status_ptr, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], os[0],
-                       os[1], os[2], wb, wh, n, hq, cache.scale if scale is None else scale)
+                       tree.mask_ptr, wp, tw, cache.status_ptr, sl, depth, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0],
+                       vs[1], vs[2], os[0], os[1], os[2], wb, wh, n, hq, cache.scale if scale is None else scale, cap or 0.0,
+                       0 if window is None or window >= 2 ** 31 else window)
         lib, sp = load(), _device.raw_stream(cache.index)
         if _device.capturing():
             # a workspace from the graph's own pool, which no tensor outside the graph gets for as long as it lives
