@@ -3,14 +3,15 @@
 //   score(i, t) = s_i + x_t - log sum exp x,   the `width` largest of a request
 //
 // Within a beam the order is the logits' own, so one pass over a row gives both
-// what the denominator needs and the row's best `width`: beam_rows.  Each lane
-// keeps a running maximum and sum; a warp keeps the best values it has met in a
-// short list in shared memory and compares with the worst of them.  After the
-// first values hardly any gets past that comparison, one vote for 32 values a
-// lane, so the pass is bound by reading.  beam_join, a block per request, makes
-// the beams' denominators and sorts what their rows kept.
+// what the denominator needs and where the row's best are: beam_rows.  A thread
+// keeps a running maximum and sum and notes the largest of every 32 (FP32: 16)
+// values.  The width-th largest of the block's 256 running maxima is a bar that
+// `width` values reach at least, and hardly more do; only the groups whose largest
+// reaches it are read again, and what reaches it there is put in order by
+// counting.  beam_join, a block per request, makes the beams' denominators and
+// finds the best of what their rows kept in the same way.
 //
-// A list entry is one number: the value's bits in unsigned order, then the token
+// An entry is one number: the value's bits in unsigned order, then the token
 // counted from the end, so that no two are equal and the larger one is the better.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -21,6 +22,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -28,9 +30,14 @@ namespace {
 
 constexpr uint32_t kThreads = 256, kWarps = kThreads / 32;
 constexpr uint32_t kMaxWidth = 64, kMaxBeams = 64;
-constexpr uint32_t kList = 128;      // entries of a warp's list, 32 of them for what one step may add
-constexpr uint32_t kChunks = 4;      // 16-byte chunks of a lane under way
+constexpr uint32_t kChunks = 4;      // 16-byte chunks of a thread under way
+constexpr uint32_t kSteps = 16;      // steps of a thread between two looks at the groups' maxima
+constexpr uint32_t kStages = 2;      // steps of a thread under way, the one at work included
+constexpr uint32_t kPerSm = 4;       // blocks to an SM: 57 KB of shared memory each
+constexpr uint32_t kSlots = 148 * kPerSm;
+constexpr uint32_t kFound = 512;     // groups, and entries, that a block holds
 constexpr uint32_t kMaxSort = 8192;  // entries that beam_join sorts
+constexpr uint32_t kMaxCount = 512;  // entries that it puts in order by counting instead
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Beam {
@@ -84,6 +91,36 @@ __device__ __forceinline__ void unpack<__half>(uint4 c, float* x) {
     x[2 * i + 1] = f.y;
   }
 }
+// The largest of 16 bytes' values (not a NaN, if there is another).
+template <typename T>
+__device__ __forceinline__ float largest(const uint4 (&c)[kChunks]) {
+  if constexpr (sizeof(T) == 4) {
+    float m = -INFINITY;
+#pragma unroll
+    for (uint32_t u = 0; u < kChunks; u++)
+      m = fmaxf(fmaxf(m, fmaxf(__uint_as_float(c[u].x), __uint_as_float(c[u].y))), fmaxf(__uint_as_float(c[u].z), __uint_as_float(c[u].w)));
+    return m;
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    auto two = [](uint32_t w) { return *reinterpret_cast<const T2*>(&w); };
+    T2 m = two(c[0].x);
+#pragma unroll
+    for (uint32_t u = 0; u < kChunks; u++) {
+      if (u) m = __hmax2(m, two(c[u].x));
+      m = __hmax2(__hmax2(m, two(c[u].y)), __hmax2(two(c[u].z), two(c[u].w)));
+    }
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+}
+
+__device__ __forceinline__ void copy16(void* smem, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(smem))), "l"(from) : "memory");
+}
+
+// Two bits patterns of -infinity, or one.
+template <typename T>
+constexpr uint32_t kNone = std::is_same<T, float>::value ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
+
 __device__ __forceinline__ float value(float x) { return x; }
 __device__ __forceinline__ float value(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float value(__half x) { return __half2float(x); }
@@ -95,176 +132,255 @@ __device__ __forceinline__ void add_kept(float& sum, float& rest, float x) {
   sum = t;
 }
 
-// The n entries of a warp's list put in order, the first `width` kept.
-__device__ __forceinline__ uint32_t prune(uint64_t* list, uint32_t n, uint32_t width) {
-  const uint32_t lane = threadIdx.x & 31u;
-  uint64_t mine[kList / 32];
-  uint32_t rank[kList / 32] = {};
-  __syncwarp();
+// Two fp32 values in a register pair: one instruction works on both.
+__device__ __forceinline__ uint64_t make2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void take2(uint64_t x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+struct Bar {
+  float tops[kWarps][32];  // the warps' values, falling
+  float at;
+};
+
+struct RowShared {
+  uint4 raw[kStages][kChunks][kThreads];  // a thread's values on their way; it reads its own alone
+  float best[kSteps][kThreads];  // the groups' largest values
+  Bar bar;
+  uint64_t found[kFound];        // entries that reached the bar
+  uint32_t groups[kFound];       // step, thread
+  uint64_t most[kWarps];
+  double sum[kWarps];
+  float top[kWarps];
+  uint32_t n_groups, n;
+};
+
+// The largest of the block's x; all threads call it.
+__device__ __forceinline__ uint64_t block_max(RowShared& sh, uint64_t x) {
+  for (int o = 16; o; o >>= 1) x = max(x, uint64_t(__shfl_xor_sync(0xFFFFFFFFu, static_cast<unsigned long long>(x), o)));
+  __syncthreads();
+  if ((threadIdx.x & 31u) == 0) sh.most[threadIdx.x >> 5] = x;
+  __syncthreads();
+  for (uint32_t w = 0; w < kWarps; w++) x = max(x, sh.most[w]);
+  return x;
+}
+
+// The width-th largest of the threads' values (of equal ones, each counts).  Every warp sorts its own; a value's rank among the others' is
+// found by halving.
+__device__ __forceinline__ float find_bar(Bar& sh, float y, uint32_t width) {
+  const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
 #pragma unroll
-  for (uint32_t i = 0; i < kList / 32; i++) mine[i] = lane + 32 * i < n ? list[lane + 32 * i] : 0;
-  for (uint32_t j = 0; j < n; j++) {
-    const uint64_t x = list[j];
+  for (uint32_t k = 2; k <= 32; k <<= 1)
 #pragma unroll
-    for (uint32_t i = 0; i < kList / 32; i++) rank[i] += x > mine[i];
+    for (uint32_t d = k >> 1; d; d >>= 1) {
+      const float o = __shfl_xor_sync(0xFFFFFFFFu, y, d);
+      const bool up = (lane & k) != 0, low = (lane & d) == 0;  // falling where not up
+      y = low != up ? fmaxf(y, o) : fminf(y, o);
+    }
+  sh.tops[warp][lane] = y;
+  __syncthreads();
+  uint32_t rank = lane;
+#pragma unroll
+  for (uint32_t v = 0; v < kWarps; v++) {
+    if (v == warp) continue;
+    uint32_t at = 0;  // values of warp v that come before y
+#pragma unroll
+    for (uint32_t d = 16; d; d >>= 1) {
+      const float o = sh.tops[v][at + d - 1];
+      if (o > y || (o == y && v < warp)) at += d;
+    }
+    if (at == 31) {
+      const float o = sh.tops[v][31];
+      at += o > y || (o == y && v < warp);
+    }
+    rank += at;
   }
-  __syncwarp();
-#pragma unroll
-  for (uint32_t i = 0; i < kList / 32; i++)
-    if (lane + 32 * i < n && rank[i] < width) list[rank[i]] = mine[i];
-  __syncwarp();
-  return min(n, width);
+  if (rank == width - 1) sh.at = y;
+  __syncthreads();
+  return sh.at;
 }
 
 // Block: part `part` of a row.  The row's 16-byte chunks are counted from the
 // aligned address at or before its start; those at its ends are read value by value.
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) beam_rows(const __grid_constant__ Beam P) {
-  constexpr uint32_t VEC = 16 / sizeof(T);
-  __shared__ uint64_t s_list[kWarps][kList];
-  __shared__ unsigned long long s_least;  // an entry that `width` of the block's are at least as good as
-  __shared__ double s_sum[kWarps];
-  __shared__ float s_top[kWarps];
-  __shared__ uint32_t s_count[kWarps];
+__global__ void __launch_bounds__(kThreads, kPerSm) beam_rows(const __grid_constant__ Beam P) {
+  constexpr uint32_t VEC = 16 / sizeof(T), GROUP = kChunks * VEC;
+  extern __shared__ __align__(16) uint8_t smem[];
+  RowShared& sh = *reinterpret_cast<RowShared*>(smem);
   const uint32_t row = blockIdx.x / P.parts, part = blockIdx.x - row * P.parts;
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, width = P.a.width, V = P.a.V;
   const uint32_t b = row / P.a.beams, i = row - b * P.a.beams;
-  // a logit of -inf is never chosen
-  constexpr uint64_t kNothing = uint64_t(0x007FFFFFu) << 32 | 0xFFFFFFFFu;
-  if (tid == 0) s_least = kNothing;
-  const bool alive = P.a.d_scores[row] > -INFINITY;  // (nor is anything of a beam that has no score)
+  const uint64_t out = uint64_t(row) * P.parts + part;
+  if (!(P.a.d_scores[row] > -INFINITY)) {  // nothing of a beam that has no score is chosen
+    for (uint32_t k = tid; k < width; k += kThreads) P.best[out * width + k] = 0;
+    if (tid == 0) {
+      P.tops[out] = -INFINITY;
+      P.sums[out] = 0.0;
+    }
+    return;
+  }
+  if (tid == 0) sh.n = 0;
   const T* x0 = static_cast<const T*>(P.a.d_logits) + int64_t(b) * P.a.l_b + int64_t(i) * P.a.l_i;
   const uint32_t skew = uint32_t(reinterpret_cast<uintptr_t>(x0) & 15u) / uint32_t(sizeof(T));
-  const uint32_t chunks = alive ? (V + skew + VEC - 1) / VEC : 0u;
-  const uint32_t steps = (chunks + 32 * kChunks - 1) / (32 * kChunks);  // of a warp
+  const uint32_t steps = ((V + skew + VEC - 1) / VEC + 32 * kChunks - 1) / (32 * kChunks);  // of a warp
   const uint32_t first = uint32_t(uint64_t(steps) * part / P.parts), last = uint32_t(uint64_t(steps) * (part + 1) / P.parts);
-  uint64_t* list = s_list[warp];
-  uint32_t n = 0;
-  uint64_t least = kNothing;
+  // value `at - skew` is the first of the chunk at `at`
+  auto whole = [&](uint32_t at) { return at >= skew && at + VEC <= V + skew; };
+  auto fetch = [&](uint32_t step, uint32_t slot) {
+    if (step < last) {
+#pragma unroll
+      for (uint32_t u = 0; u < kChunks; u++) {
+        const uint32_t at = (step * 32 * kChunks + lane + 32 * u) * VEC;
+        if (whole(at)) {
+          copy16(&sh.raw[slot][u][tid], x0 - skew + at);
+        } else {  // at the row's ends: value by value, and -inf for what is not the row's
+          T x[VEC];
+#pragma unroll
+          for (uint32_t e = 0; e < VEC; e++) {
+            const uint32_t t = at + e - skew;  // (before the row: wraps to a large number)
+            const uint32_t none = kNone<T>;
+            x[e] = t < V ? x0[t] : *reinterpret_cast<const T*>(&none);
+          }
+          sh.raw[slot][u][tid] = *reinterpret_cast<const uint4*>(x);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
   float top = -INFINITY, sum = 0.0f, rest = 0.0f;  // sum + rest: of exp(x - top)
-  bool begun = false;
-  __syncthreads();
-  for (uint32_t step = first + warp; step < last; step += kWarps) {
-    float x[kChunks][VEC];
-    uint4 raw[kChunks];
-    const uint32_t c0 = step * 32 * kChunks + lane;
+  bool many = false;
+  uint32_t slot = 0;
 #pragma unroll
-    for (uint32_t u = 0; u < kChunks; u++) {
-      const uint32_t c = c0 + 32 * u, at = c * VEC;  // value `at - skew` is the chunk's first
-      if (at >= skew && at + VEC <= V + skew) raw[u] = __ldcs(reinterpret_cast<const uint4*>(x0 - skew + at));
-    }
-    float best = -INFINITY;
+  for (uint32_t k = 0; k + 1 < kStages; k++) fetch(first + k * kWarps + warp, k);
+  __syncthreads();  // sh.n is set
+  for (uint32_t step0 = first; step0 < last; step0 += kSteps * kWarps) {
+#pragma unroll 1
+    for (uint32_t k = 0; k < kSteps && step0 + k * kWarps < last; k++) {
+      const uint32_t step = step0 + k * kWarps + warp;
+      float best = -INFINITY;
+      if (step < last) {
+        fetch(step + (kStages - 1) * kWarps, slot == 0 ? kStages - 1 : slot - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+        uint4 raw[kChunks];
 #pragma unroll
-    for (uint32_t u = 0; u < kChunks; u++) {
-      const uint32_t c = c0 + 32 * u, at = c * VEC;
-      if (at >= skew && at + VEC <= V + skew) {
-        unpack<T>(raw[u], x[u]);
-      } else {
-#pragma unroll
-        for (uint32_t e = 0; e < VEC; e++) {
-          const uint32_t t = at + e - skew;  // (before the row: wraps to a large number)
-          x[u][e] = t < V ? value(x0[t]) : -INFINITY;
+        for (uint32_t u = 0; u < kChunks; u++) raw[u] = sh.raw[slot][u][tid];
+        slot = slot + 1 == kStages ? 0 : slot + 1;
+        best = largest<T>(raw);
+        if (best > top) {
+          const float f = exp2_fast((top - best) * kLog2e);
+          sum *= f;
+          rest *= f;
+          top = best;
         }
-      }
+        const float base = top == -INFINITY ? 0.0f : top;
+        const uint64_t nb = make2(-base, -base), l2 = make2(kLog2e, kLog2e);
+        uint64_t acc[2] = {0, 0};
 #pragma unroll
-      for (uint32_t e = 0; e < VEC; e++) best = fmaxf(best, x[u][e]);
-    }
-    if (best > top) {
-      const float f = exp2_fast((top - best) * kLog2e);
-      sum *= f;
-      rest *= f;
-      top = best;
-    }
-    const float base = top == -INFINITY ? 0.0f : top;
-    float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t u = 0; u < kChunks; u++) {
+          float x[VEC];
+          unpack<T>(raw[u], x);
 #pragma unroll
-    for (uint32_t u = 0; u < kChunks; u++)
-#pragma unroll
-      for (uint32_t e = 0; e < VEC; e++) s4[e & 3u] += exp2_fast((x[u][e] - base) * kLog2e);
-    add_kept(sum, rest, (s4[0] + s4[1]) + (s4[2] + s4[3]));
-    // the list
-    if (!begun) {
-      begun = true;
-      if (width <= 32) {  // as many lanes have a value at least as large as the width-th of their largest ones
-        float y = best;
-#pragma unroll
-        for (uint32_t k = 2; k <= 32; k <<= 1)
-#pragma unroll
-          for (uint32_t d = k >> 1; d; d >>= 1) {
-            const float o = __shfl_xor_sync(0xFFFFFFFFu, y, d);
-            const bool up = (lane & k) != 0, low = (lane & d) == 0;  // descending where not up
-            y = (low != up) ? fmaxf(y, o) : fminf(y, o);
-          }
-        const float w = __shfl_sync(0xFFFFFFFFu, y, width - 1);
-        if (w > -INFINITY) {
-          least = max(least, uint64_t(ordered(w)) << 32);
-          if (lane == 0) atomicMax(&s_least, static_cast<unsigned long long>(least));
-        }
-      }
-    }
-    least = max(least, uint64_t(*const_cast<volatile unsigned long long*>(&s_least)));
-    const float bar = fmaxf(unordered(uint32_t(least >> 32)), -FLT_MAX);
-    if (__any_sync(0xFFFFFFFFu, best >= bar)) {
-      uint32_t hits = 0;
-#pragma unroll
-      for (uint32_t u = 0; u < kChunks; u++)
-#pragma unroll
-        for (uint32_t e = 0; e < VEC; e++) hits |= uint32_t(x[u][e] >= bar) << (u * VEC + e);
-      while (__any_sync(0xFFFFFFFFu, hits != 0)) {
-        uint64_t mine = 0;
-        if (hits) {
-          const uint32_t k = __ffs(hits) - 1, t = (c0 + 32 * (k / VEC)) * VEC + k % VEC - skew;
-          hits &= hits - 1;
-          if (t < V) mine = entry_of(value(x0[t]), t);
-        }
-        const uint32_t takes = __ballot_sync(0xFFFFFFFFu, mine > least);
-        if (mine > least) list[n + __popc(takes & ((1u << lane) - 1u))] = mine;
-        n += __popc(takes);
-        if (n > kList - 32) {
-          n = prune(list, n, width);
-          if (n == width) {
-            least = max(least, list[width - 1]);
-            if (lane == 0) atomicMax(&s_least, static_cast<unsigned long long>(least));
+          for (uint32_t e = 0; e < VEC; e += 2) {
+            float p, q;
+            take2(mul2(add2(make2(x[e], x[e + 1]), nb), l2), p, q);
+            acc[e >> 1 & 1] = add2(acc[e >> 1 & 1], make2(exp2_fast(p), exp2_fast(q)));
           }
         }
+        float s0, s1;
+        take2(add2(acc[0], acc[1]), s0, s1);
+        add_kept(sum, rest, s0 + s1);
+      }
+      sh.best[k][tid] = best;
+    }
+    if (tid == 0) sh.n_groups = 0;
+    const float bar = fmaxf(find_bar(sh.bar, top, width), -FLT_MAX);  // (a logit of -inf is never chosen)
+    const uint32_t rounds = min(kSteps, (last - step0 + kWarps - 1) / kWarps);
+#pragma unroll 4
+    for (uint32_t k = 0; k < rounds; k++)
+      if (sh.best[k][tid] >= bar) {
+        const uint32_t g = atomicAdd(&sh.n_groups, 1u);
+        if (g < kFound) sh.groups[g] = (step0 + k * kWarps + warp) * 32 + lane;
+      }
+    __syncthreads();
+    many |= sh.n_groups > kFound;
+    const uint32_t groups = min(sh.n_groups, kFound);
+    for (uint32_t q = warp * (32 / GROUP); q < groups; q += kWarps * (32 / GROUP)) {
+      const uint32_t mine = q + lane / GROUP, e = lane % GROUP;
+      if (mine >= groups) continue;
+      const uint32_t g = sh.groups[mine], t = ((g >> 5) * 32 * kChunks + (g & 31u) + 32 * (e / VEC)) * VEC + e % VEC - skew;
+      if (t >= V) continue;
+      const float x = value(x0[t]);
+      if (x >= bar) {
+        const uint32_t at = atomicAdd(&sh.n, 1u);
+        if (at < kFound) sh.found[at] = entry_of(x, t);
       }
     }
+    __syncthreads();
   }
-  n = prune(list, n, width);
-  // the warp's and the block's sums
+  many |= sh.n > kFound;
+  if (many) {  // values that tie, or lie under few threads: one after another, each the best after the last
+    uint64_t last_one = ~0ull;
+    uint32_t k = 0;
+    const uint64_t t0 = uint64_t(first) * 32 * kChunks * VEC, t1 = uint64_t(last) * 32 * kChunks * VEC;
+    for (; k < width; k++) {
+      uint64_t mine = 0;
+      for (uint64_t at = t0 + tid; at < t1; at += kThreads) {
+        const uint32_t t = uint32_t(at) - skew;
+        if (t >= V) continue;
+        const float x = value(x0[t]);
+        const uint64_t y = x > -INFINITY ? entry_of(x, t) : 0;
+        if (y < last_one) mine = max(mine, y);
+      }
+      last_one = block_max(sh, mine);
+      if (!last_one) break;
+      if (tid == 0) sh.found[k] = last_one;
+    }
+    if (tid == 0) sh.n = k;
+    __syncthreads();
+  }
+  // the warps' sums
   float all = top;
   for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xFFFFFFFFu, all, o));
   // (a NaN value is not a maximum, but it is in the sum)
   double s = top == -INFINITY ? double(sum) : (double(sum) + double(rest)) * exp(double(top) - double(all));
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
   if (lane == 0) {
-    s_top[warp] = all;
-    s_sum[warp] = s;
-    s_count[warp] = n;
+    sh.top[warp] = all;
+    sh.sum[warp] = s;
   }
   __syncthreads();
-  const uint64_t out = uint64_t(row) * P.parts + part;
-  if (tid == 0) {
-    float m = -INFINITY;
-    for (uint32_t w = 0; w < kWarps; w++) m = fmaxf(m, s_top[w]);
-    double t = 0.0;
-    for (uint32_t w = 0; w < kWarps; w++) t += s_top[w] == -INFINITY ? s_sum[w] : s_sum[w] * exp(double(s_top[w]) - double(m));
-    P.tops[out] = m;
-    P.sums[out] = t;
+  if (warp == 0) {
+    const float t = lane < kWarps ? sh.top[lane] : -INFINITY;
+    float m = t;
+    for (int o = kWarps / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    double y = lane < kWarps ? sh.sum[lane] : 0.0;
+    if (t > -INFINITY) y *= exp(double(t) - double(m));
+    for (int o = kWarps / 2; o; o >>= 1) y += __shfl_xor_sync(0xFFFFFFFFu, y, o);
+    if (lane == 0) {
+      P.tops[out] = m;
+      P.sums[out] = y;
+    }
   }
-  // the best of the warps' lists: an entry's rank is the number of better ones
-  uint32_t total = 0;
-  for (uint32_t w = 0; w < kWarps; w++) total += s_count[w];
-  for (uint32_t k = tid; k < kWarps * width; k += kThreads) {
-    const uint32_t w = k / width, j = k - w * width;
-    if (j >= s_count[w]) continue;
-    const uint64_t mine = s_list[w][j];
+  const uint32_t n = sh.n;
+  for (uint32_t k = tid; k < n; k += kThreads) {
+    const uint64_t mine = sh.found[k];
     uint32_t rank = 0;
-    for (uint32_t v = 0; v < kWarps; v++)
-      for (uint32_t q = 0; q < s_count[v] && s_list[v][q] > mine; q++) rank++;
+    for (uint32_t q = 0; q < n; q++) rank += sh.found[q] > mine;
     if (rank < width) P.best[out * width + rank] = mine;
   }
-  for (uint32_t k = total + tid; k < width; k += kThreads) P.best[out * width + k] = 0;
+  for (uint32_t k = n + tid; k < width; k += kThreads) P.best[out * width + k] = 0;
 }
 
 __device__ __forceinline__ uint64_t ordered(double x) {
@@ -277,47 +393,93 @@ __device__ __forceinline__ double unordered(uint64_t k) {
 
 __global__ void __launch_bounds__(kThreads) beam_join(const __grid_constant__ Beam P) {
   extern __shared__ uint64_t s_key[];  // the scores in unsigned order, 0: none; then the candidates' indexes
-  __shared__ double s_lse[kMaxBeams];
+  __shared__ double s_lse[kMaxBeams];  // NaN: the beam has no candidates
+  __shared__ float s_score[kMaxBeams];
+  __shared__ Bar s_bar;
+  __shared__ uint32_t s_n;
   uint32_t* s_at = reinterpret_cast<uint32_t*>(s_key + P.sorted);
   const uint32_t b = blockIdx.x, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-  const uint32_t beams = P.a.beams, width = P.a.width, parts = P.parts;
+  const uint32_t beams = P.a.beams, width = P.a.width, parts = P.parts, per = parts * width, all = beams * per;
+  if (tid == 0) s_n = 0;
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const uint64_t* best = P.best + uint64_t(b) * all;
+  uint64_t ahead = tid < all ? best[tid] : 0;  // on its way while the denominators are made
   for (uint32_t i = warp; i < beams; i += kWarps) {
     const uint64_t at = (uint64_t(b) * beams + i) * parts;
+    const float score = P.a.d_scores[b * beams + i];
     float m = -INFINITY;
-    for (uint32_t p = lane; p < parts; p += 32) m = fmaxf(m, P.tops[at + p]);
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
     double s = 0.0;
     for (uint32_t p = lane; p < parts; p += 32) {
       const float t = P.tops[at + p];
-      s += t == -INFINITY ? P.sums[at + p] : P.sums[at + p] * exp(double(t) - double(m));
-    }
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-    if (lane == 0) s_lse[i] = double(m) + log(s);
-  }
-  __syncthreads();
-  const uint32_t per = parts * width;
-  for (uint32_t k = tid; k < P.sorted; k += kThreads) {
-    uint64_t key = 0;
-    uint32_t at = 0xFFFFFFFFu;
-    if (k < beams * per) {
-      const uint32_t i = k / per;
-      const uint64_t x = P.best[uint64_t(b) * beams * per + k];
-      if (x) {
-        const double z = double(P.a.d_scores[b * beams + i]) + (double(unordered(uint32_t(x >> 32))) - s_lse[i]);
-        if (z > -INFINITY) {  // (not NaN)
-          key = ordered(z);
-          at = i * P.a.V + ~uint32_t(x);
-        }
+      const double y = P.sums[at + p];
+      if (t > m) {
+        s = s * exp(double(m) - double(t)) + y;
+        m = t;
+      } else {
+        s += t == -INFINITY ? y : y * exp(double(t) - double(m));
       }
     }
-    s_key[k] = key;
-    s_at[k] = at;
+    float top = m;
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    if (m > -INFINITY && m != top) s *= exp(double(m) - double(top));
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+    if (lane == 0) {
+      s_lse[i] = top > -INFINITY ? double(top) + log(s) : double(NAN);
+      s_score[i] = score;
+    }
   }
   __syncthreads();
-  for (uint32_t k = 2; k <= P.sorted; k <<= 1)
+  // a candidate's score; NaN: it is none
+  auto score_of = [&](uint32_t k, uint64_t x) {
+    const uint32_t i = k / per;
+    return x ? double(s_score[i]) + (double(unordered(uint32_t(x >> 32))) - s_lse[i]) : double(NAN);
+  };
+  float most = -INFINITY;
+  for (uint32_t k = tid; k < all; k += kThreads) most = fmaxf(most, float(score_of(k, k == tid ? ahead : best[k])));
+  const float bar = find_bar(s_bar, most, width);  // `width` candidates reach it, if there are as many
+  for (uint32_t k = tid; k < all; k += kThreads) {
+    const uint64_t x = k == tid ? ahead : best[k];
+    const double z = score_of(k, x);
+    if (z > -INFINITY && float(z) >= bar) {
+      const uint32_t at = atomicAdd(&s_n, 1u);
+      s_key[at] = ordered(z);
+      s_at[at] = k / per * P.a.V + ~uint32_t(x);
+    }
+  }
+  auto put = [&](uint32_t k, uint64_t key, uint32_t at) {
+    const uint64_t out = uint64_t(b) * width + k;
+    const uint32_t i = key ? at / P.a.V : 0u;
+    P.a.d_scores_out[out] = key ? float(unordered(key)) : -INFINITY;
+    P.a.d_parents[out] = key ? int32_t(b * beams + i) : -1;
+    P.a.d_tokens[out] = key ? int32_t(at - i * P.a.V) : -1;
+  };
+  __syncthreads();
+  const uint32_t n = s_n;
+  if (n <= kMaxCount) {  // a candidate's place is the number of better ones
+    for (uint32_t k = tid; k < n; k += kThreads) {
+      const uint64_t key = s_key[k];
+      const uint32_t at = s_at[k];
+      uint32_t rank = 0;
+#pragma unroll 4
+      for (uint32_t q = 0; q < n; q++) {
+        const uint64_t x = s_key[q];
+        rank += (x > key) | ((x == key) & (s_at[q] < at));
+      }
+      if (rank < width) put(rank, key, at);
+    }
+    for (uint32_t k = n + tid; k < width; k += kThreads) put(k, 0, 0);
+    return;
+  }
+  uint32_t sorted = 2;
+  while (sorted < n) sorted *= 2;
+  for (uint32_t k = n + tid; k < sorted; k += kThreads) {
+    s_key[k] = 0;
+    s_at[k] = 0xFFFFFFFFu;
+  }
+  __syncthreads();
+  for (uint32_t k = 2; k <= sorted; k <<= 1)
     for (uint32_t d = k >> 1; d; d >>= 1) {
-      for (uint32_t q = tid; q < P.sorted / 2; q += kThreads) {
+      for (uint32_t q = tid; q < sorted / 2; q += kThreads) {
         const uint32_t lo = 2 * q - (q & (d - 1)), hi = lo + d;
         const uint64_t x = s_key[lo], y = s_key[hi];
         const uint32_t xa = s_at[lo], ya = s_at[hi];
@@ -331,14 +493,7 @@ __global__ void __launch_bounds__(kThreads) beam_join(const __grid_constant__ Be
       }
       __syncthreads();
     }
-  for (uint32_t k = tid; k < width; k += kThreads) {
-    const uint64_t out = uint64_t(b) * width + k;
-    const bool any = k < P.sorted && s_key[k] != 0;
-    const uint32_t at = any ? s_at[k] : 0u, i = at / P.a.V;
-    P.a.d_scores_out[out] = any ? float(unordered(s_key[k])) : -INFINITY;
-    P.a.d_parents[out] = any ? int32_t(b * beams + i) : -1;
-    P.a.d_tokens[out] = any ? int32_t(at - i * P.a.V) : -1;
-  }
+  for (uint32_t k = tid; k < width; k += kThreads) put(k, s_key[k], s_at[k]);  // (n > kMaxCount >= width)
 }
 
 int check(const voom_beam_select_args* a) {
@@ -354,8 +509,9 @@ uint64_t plan(Beam& P, void* scratch) {
   const voom_beam_select_args& a = P.a;
   const uint32_t step = 32 * kChunks * (a.type == VOOM_FP32 ? 4 : 8);
   const uint64_t rows = uint64_t(a.B) * a.beams, steps = (a.V + step - 1) / step + 1;
-  // enough blocks for four to an SM, a step to each of a block's warps at least
-  uint64_t parts = (592 + rows - 1) / std::max<uint64_t>(rows, 1);
+  // as many blocks as the SMs hold at once (a second wave of them, with half the
+  // row each: 39 us against 32), a step to each of a block's warps at least
+  uint64_t parts = std::max<uint64_t>(1, kSlots / std::max<uint64_t>(rows, 1));
   parts = std::min(parts, (steps + kWarps - 1) / kWarps);
   parts = std::min<uint64_t>(parts, std::max(1u, kMaxSort / (a.beams * a.width)));
   P.parts = uint32_t(std::max<uint64_t>(parts, 1));
@@ -387,26 +543,29 @@ VOOM_API int voom_beam_select(const voom_beam_select_args* a, void* d_scratch, u
   if (plan(P, d_scratch) > bytes) return VOOM_E_CAPACITY;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const uint32_t grid = a->B * a->beams * P.parts;
-  if (a->type == VOOM_BF16) beam_rows<__nv_bfloat16><<<grid, kThreads, 0, s>>>(P);
-  else if (a->type == VOOM_FP16) beam_rows<__half><<<grid, kThreads, 0, s>>>(P);
-  else beam_rows<float><<<grid, kThreads, 0, s>>>(P);
-  if (cudaGetLastError() != cudaSuccess) return VOOM_E_CUDA;
-  const uint32_t smem = P.sorted * 12;
   static std::atomic<uint64_t> allowed{0};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return VOOM_E_CUDA;
   if (!(allowed.load(std::memory_order_relaxed) >> (dev & 63) & 1u)) {
-    if (cudaFuncSetAttribute(beam_join, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSort * 12) != cudaSuccess) {
+    const auto allow = [](const void* kernel, int n) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, n) == cudaSuccess; };
+    if (!allow(reinterpret_cast<const void*>(beam_join), kMaxSort * 12) ||
+        !allow(reinterpret_cast<const void*>(beam_rows<__nv_bfloat16>), sizeof(RowShared)) ||
+        !allow(reinterpret_cast<const void*>(beam_rows<__half>), sizeof(RowShared)) ||
+        !allow(reinterpret_cast<const void*>(beam_rows<float>), sizeof(RowShared))) {
       cudaGetLastError();
       return VOOM_E_CUDA;
     }
     allowed.fetch_or(uint64_t(1) << (dev & 63), std::memory_order_relaxed);
   }
+  if (a->type == VOOM_BF16) beam_rows<__nv_bfloat16><<<grid, kThreads, sizeof(RowShared), s>>>(P);
+  else if (a->type == VOOM_FP16) beam_rows<__half><<<grid, kThreads, sizeof(RowShared), s>>>(P);
+  else beam_rows<float><<<grid, kThreads, sizeof(RowShared), s>>>(P);
+  if (cudaGetLastError() != cudaSuccess) return VOOM_E_CUDA;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute early{};
   cfg.gridDim = dim3(a->B);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = P.sorted * 12;
   cfg.stream = s;
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;

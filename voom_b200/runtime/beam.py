@@ -57,7 +57,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: int, *,
     if logits.dim() != 3 or kind is None or (logits.stride(2) != 1 and logits.shape[2] > 1):
         raise ValueError(f"logits: (B, beams, V) BF16, FP16 or FP32 with adjacent values wanted, got {tuple(logits.shape)} "
                          f"{logits.dtype}, strides {logits.stride()}")
-    B, beams, V = logits.shape
+    (B, beams, V), (sb, si, _) = logits.shape, logits.stride()
     if scores.shape != (B, beams) or scores.dtype != torch.float32 or not scores.is_contiguous() or scores.get_device() != index:
         raise ValueError(f"scores: contiguous fp32 ({B}, {beams}) on {logits.device} wanted, got {tuple(scores.shape)} "
                          f"{scores.dtype} on {scores.device}")
@@ -66,14 +66,12 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: int, *,
                          "continuations, one token at least")
     if beams * V >= 2 ** 31 or B * beams >= 2 ** 31:
         raise ValueError(f"{B} requests of {beams} beams over {V} tokens: fewer than 2^31 candidates each wanted")
-    out = scores.new_empty((3, B, width))
-    chosen = out.view(torch.int32)
-    result = BeamChoice(out[0], chosen[1], chosen[2])
+    best = scores.new_empty((B, width))
+    parents, tokens = scores.new_empty((2, B, width), dtype=torch.int32).unbind(0)
     if B:
-        at, step = out.data_ptr(), 4 * B * width
-        a = _ARGS.pack(logits.data_ptr(), scores.data_ptr(), at, at + step, at + 2 * step, logits.stride(0), logits.stride(1),
-                       B, beams, V, width, kind, 0)
+        a = _ARGS.pack(logits.data_ptr(), scores.data_ptr(), best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), sb, si, B,
+                       beams, V, width, kind, 0)
         lib = load()
         ws = scores.new_empty(lib.voom_beam_select_scratch_bytes(a), dtype=torch.uint8)
         check(lib.voom_beam_select(a, ws.data_ptr(), ws.numel(), _device.raw_stream(index)), "voom_beam_select")
-    return result
+    return BeamChoice(best, parents, tokens)
