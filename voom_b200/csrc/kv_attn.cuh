@@ -251,35 +251,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// A product q . k as a score in log2 units, for calls whose scores are capped,
-// biased or windowed ("scored").  cap tanh(z / cap) as cap - 2 cap / (1 + e^(2 z / cap)):
-// off by a few 2^-23 of the cap, absolutely, and no further at either end.
-__device__ __forceinline__ float scored(const Attn& P, float x, float slope2, float ahead) {
-  float y;
-  if (P.cap_in != 0.0f) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + exp2_fast(x * P.cap_in)));
-    y = fmaf(-2.0f * P.cap_out, r, P.cap_out);
-  } else {
-    y = x * P.scale2;
-  }
-  return fmaf(slope2, ahead, y);
-}
-
-// A query head's slope in log2 units.
-__device__ __forceinline__ float slope2_of(const Attn& P, uint32_t head) {
-  return P.a.d_slopes ? kLog2e * __ldg(P.a.d_slopes + head) : 0.0f;
-}
-
-// sum += x with what the addition lost kept in `rest`: beside one large term, a
-// long cache's small ones would be lost one by one (2^-25 of a row's largest
-// does not change a 1 at all).  Both are at least 0.
-__device__ __forceinline__ void add_kept(float& sum, float& rest, float x) {
-  const float t = sum + x;
-  rest += fminf(sum, x) - (t - fmaxf(sum, x));
-  sum = t;
-}
-
 // Two fp32 values in a register pair: one instruction works on both.
 struct F2 {
   uint64_t v;
@@ -300,6 +271,50 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
   return r;
 }
+// Products q . k as scores in log2 units, for calls whose scores are capped,
+// biased or windowed ("scored"): two at a time, whose biases are `bias`.
+// cap tanh(z / cap) as cap - 2 cap / (1 + e^(2 z / cap)): off by a few 2^-23 of the
+// cap, absolutely, and no further at either end.
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 capped2(const Attn& P, F2 x, F2 bias) {
+  float a, b;
+  take2(mul2(x, make2(P.cap_in, P.cap_in)), a, b);
+  take2(add2(make2(exp2_fast(a), exp2_fast(b)), make2(1.0f, 1.0f)), a, b);
+  const float m = -2.0f * P.cap_out;
+  return fma2(make2(rcp_fast(a), rcp_fast(b)), make2(m, m), add2(bias, make2(P.cap_out, P.cap_out)));
+}
+__device__ __forceinline__ F2 scored2(const Attn& P, F2 x, F2 bias) {
+  return P.cap_in != 0.0f ? capped2(P, x, bias) : fma2(x, make2(P.scale2, P.scale2), bias);
+}
+__device__ __forceinline__ float scored(const Attn& P, float x, float slope2, float ahead) {
+  float y, unused;
+  take2(scored2(P, make2(x, x), make2(slope2 * ahead, 0.0f)), y, unused);
+  return y;
+}
+
+// A query head's slope in log2 units.
+__device__ __forceinline__ float slope2_of(const Attn& P, uint32_t head) {
+  return P.a.d_slopes ? kLog2e * __ldg(P.a.d_slopes + head) : 0.0f;
+}
+
+// sum += x with what the addition lost kept in `rest`: beside one large term, a
+// long cache's small ones would be lost one by one (2^-25 of a row's largest
+// does not change a 1 at all).  Both are at least 0.
+__device__ __forceinline__ void add_kept(float& sum, float& rest, float x) {
+  const float t = sum + x;
+  rest += fminf(sum, x) - (t - fmaxf(sum, x));
+  sum = t;
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));

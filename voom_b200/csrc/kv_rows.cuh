@@ -216,20 +216,39 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
       const bool fresh = step >= cs;
       const uint32_t p0 = (w0 + step) * KT;  // of a cached tile: its first position
       if constexpr (SCORED) {
+        // a row's limit: the first key of the tile inside its window
+        const bool edge = P.a.window && (fresh || p0 < window_all(P, g.len));
 #pragma unroll
-        for (uint32_t j = 0; j < NT; j++)
+        for (int t = 0; t < MT; t++)
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const uint32_t k = 8 * j + 2 * quad + e;
-            const int32_t key = fresh ? depth_of(P, g.b, (step - cs) * KT + k) : int32_t(p0 + k) - int32_t(g.len);
+          for (int x = 0; x < 2; x++) {
+            if (16 * t + 8 * x >= nrows) continue;  // (the same for the whole block) no such rows
+            if (fresh && P.a.d_mask) {  // a tree's tokens stand at their depths
 #pragma unroll
-            for (int t = 0; t < MT; t++)
+              for (uint32_t j = 0; j < NT; j++)
 #pragma unroll
-              for (int x = 0; x < 2; x++) {
-                const int32_t ahead = key - behind[t][x];
-                float& y = z[t][j][2 * x + e];
-                y = in_window(P, ahead) ? scored(P, y, slope2[t][x], float(ahead)) : -INFINITY;
+                for (int e = 0; e < 2; e++) {
+                  const int32_t ahead = depth_of(P, g.b, (step - cs) * KT + 8 * j + 2 * quad + e) - behind[t][x];
+                  float& y = z[t][j][2 * x + e];
+                  y = in_window(P, ahead) ? scored(P, y, slope2[t][x], float(ahead)) : -INFINITY;
+                }
+              continue;
+            }
+            // of the lane's first key
+            const int32_t ahead = (fresh ? int32_t((step - cs) * KT) : int32_t(p0) - int32_t(g.len)) + int32_t(2 * quad) - behind[t][x];
+            const float first = slope2[t][x] * float(ahead);
+            const F2 from = make2(first, first), by = make2(slope2[t][x], slope2[t][x]);
+#pragma unroll
+            for (uint32_t j = 0; j < NT; j++) {
+              float a, b;
+              take2(scored2(P, make2(z[t][j][2 * x], z[t][j][2 * x + 1]), fma2(make2(float(8 * j), float(8 * j + 1)), by, from)), a, b);
+              if (edge) {
+                if (!in_window(P, ahead + int32_t(8 * j))) a = -INFINITY;
+                if (!in_window(P, ahead + int32_t(8 * j + 1))) b = -INFINITY;
               }
+              z[t][j][2 * x] = a;
+              z[t][j][2 * x + 1] = b;
+            }
           }
       }
       // masks: positions past the length, and the new tokens that a row does not see

@@ -202,10 +202,10 @@ __global__ void __launch_bounds__(Sums<DP>::THREADS, 1) attn_sums(const __grid_c
               float p, q;
               if constexpr (SCORED) {
                 const int32_t d0 = key - sh.behind[w][c + e], d1 = key - sh.behind[w][c + e + 1];
-                p = exp2_fast(scored(P, __uint_as_float(s[e]), sh.slope2[w][c + e], float(d0)) + x.x);
-                q = exp2_fast(scored(P, __uint_as_float(s[e + 1]), sh.slope2[w][c + e + 1], float(d1)) + x.z);
-                if (P.a.window && -int64_t(d0) >= int64_t(P.a.window)) p = 0.0f;
-                if (P.a.window && -int64_t(d1) >= int64_t(P.a.window)) q = 0.0f;
+                const F2 bias = make2(sh.slope2[w][c + e] * float(d0), sh.slope2[w][c + e + 1] * float(d1));
+                take2(add2(scored2(P, make2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), bias), make2(x.x, x.z)), p, q);
+                p = in_window(P, d0) ? exp2_fast(p) : 0.0f;
+                q = in_window(P, d1) ? exp2_fast(q) : 0.0f;
               } else {
                 p = exp2_fast(fmaf(__uint_as_float(s[e]), P.scale2, x.x));
                 q = exp2_fast(fmaf(__uint_as_float(s[e + 1]), P.scale2, x.z));

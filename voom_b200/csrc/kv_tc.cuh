@@ -457,14 +457,28 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
 #pragma unroll
         for (uint32_t c = 0; c < KT / 32; c++) tc::tmem_hold(s[c]);
         if constexpr (SCORED) {
+          auto pair = [&](uint32_t c, int e, F2 bias) {
+            float x, y;
+            take2(scored2(P, make2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), bias), x, y);
+            s[c][e] = __float_as_uint(x);
+            s[c][e + 1] = __float_as_uint(y);
+          };
+          if (fresh && P.a.d_mask && P.a.d_slopes) {  // a tree's tokens stand at their depths
 #pragma unroll
-          for (uint32_t c = 0; c < KT / 32; c++)
+            for (uint32_t c = 0; c < KT / 32; c++)
 #pragma unroll
-            for (int e = 0; e < 32; e++) {
-              const int32_t k = int32_t(32 * c) + e;
-              const int32_t d = fresh && P.a.d_mask && P.a.d_slopes ? depth_of(P, g.b, (step - cs) * KT + k) - behind : ahead + k;
-              s[c][e] = __float_as_uint(scored(P, __uint_as_float(s[c][e]), slope2, float(d)));
-            }
+              for (int e = 0; e < 32; e += 2) {
+                const uint32_t j = (step - cs) * KT + 32 * c + e;
+                pair(c, e, make2(slope2 * float(depth_of(P, g.b, j) - behind), slope2 * float(depth_of(P, g.b, j + 1) - behind)));
+              }
+          } else {
+            const float first = slope2 * float(ahead);
+            const F2 from = make2(first, first), by = make2(slope2, slope2);
+#pragma unroll
+            for (uint32_t c = 0; c < KT / 32; c++)
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) pair(c, e, fma2(make2(float(32 * c + e), float(32 * c + e + 1)), by, from));
+          }
         }
         if (masked) {
 #pragma unroll
