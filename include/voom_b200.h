@@ -751,7 +751,8 @@ typedef struct voom_kv_fork_args {
   int64_t k_layer, k_page, k_head, k_pos, v_layer, v_page, v_head, v_pos; /* strides, elements */
   uint32_t layers, n_pages, hk, page, D, rows, per, grow, add_missing, pad;
 } voom_kv_fork_args;
-uint64_t voom_kv_fork_scratch_bytes(const voom_kv_fork_args* a); /* 16-byte aligned, contents ignored */
+/* Scratch: 16-byte aligned, contents ignored; in_place: d_table_out is d_table. */
+uint64_t voom_kv_fork_scratch_bytes(uint32_t rows, uint32_t per, uint32_t n_pages, uint32_t in_place);
 int voom_kv_fork(const voom_kv_fork_args* a, void* d_scratch, uint64_t scratch_bytes, void* stream);
 
 /* The pages that the rows hold (the first ceil(length / page) entries of each)
@@ -769,7 +770,7 @@ typedef struct voom_kv_compact_args {
   int64_t k_layer, k_page, k_head, k_pos, v_layer, v_page, v_head, v_pos;
   uint32_t layers, n_pages, hk, page, D, rows, per, pad;
 } voom_kv_compact_args;
-uint64_t voom_kv_compact_scratch_bytes(const voom_kv_compact_args* a);
+uint64_t voom_kv_compact_scratch_bytes(uint32_t n_pages);
 int voom_kv_compact(const voom_kv_compact_args* a, void* d_scratch, uint64_t scratch_bytes, void* stream);
 
 /* ------------------------------------------------------------ beam selection */

@@ -197,9 +197,9 @@ SIGNATURES: dict[str, tuple] = {
     "voom_tree_attention": (_i32, [_vp, _vp, _vp, _u64, _vp]),
     "voom_kv_evict": (_i32, [_vp, _vp, _vp]),
     "voom_kv_append": (_i32, [_vp, _vp, _vp]),
-    "voom_kv_fork_scratch_bytes": (_u64, [_vp]),
+    "voom_kv_fork_scratch_bytes": (_u64, [_u32, _u32, _u32, _u32]),
     "voom_kv_fork": (_i32, [_vp, _vp, _u64, _vp]),
-    "voom_kv_compact_scratch_bytes": (_u64, [_vp]),
+    "voom_kv_compact_scratch_bytes": (_u64, [_u32]),
     "voom_kv_compact": (_i32, [_vp, _vp, _u64, _vp]),
     "voom_beam_select_scratch_bytes": (_u64, [_vp]),
     "voom_beam_select": (_i32, [_vp, _vp, _u64, _vp]),

@@ -1,6 +1,7 @@
 // Attention of drafted tokens over a KV cache, its weight sums, and the tree masks.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <initializer_list>
 #include <type_traits>
 
@@ -271,6 +272,9 @@ void map_cache(Attn& P) {
   if (one(P.k_map, c.d_k, c.k_pos, c.k_head, c.k_page) && one(P.v_map, c.d_v, c.v_pos, c.v_head, c.v_page)) P.box = box;
 }
 
+// The scores are more than products.
+bool scored(const Attn& P) { return P.a.cap > 0.0f || P.a.d_slopes || P.a.window; }
+
 // Tiles, grid and scratch of a call.  Returns the scratch bytes; sets the
 // pointers where `scratch` is given.
 uint64_t plan(Attn& P, void* scratch) {
@@ -282,6 +286,15 @@ uint64_t plan(Attn& P, void* scratch) {
   if (P.a.cap > 0.0f) {
     P.cap_in = 2.0f * P.scale2 / P.a.cap;
     P.cap_out = P.a.cap * voom::kv::kLog2e;
+    // cap tanh(z / cap) log2(e) = x P(x^2) for z = scale x, |z| <= 3/4 cap
+    const double r = double(P.a.scale) / P.a.cap;
+    double f = P.scale2;
+    bool fine = true;
+    for (int i = 0; i < 5; i++, f *= r * r) {
+      P.poly[i] = make_float2(float(voom::kv::kTanh[i] * f), float(voom::kv::kTanh[i] * f));
+      fine = fine && std::isfinite(P.poly[i].x);
+    }
+    P.cap_small = fine ? float(0.75 / r) : -1.0f;
   }
   P.ld_o = c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256;
   P.tc = -1;
@@ -294,7 +307,7 @@ uint64_t plan(Attn& P, void* scratch) {
     P.keys = P.tc == voom::kv::kSingle ? 64 : 128;
     P.rows = P.tc == voom::kv::kPair ? 256 : 128;
   } else {
-    P.keys = voom::kv::row_keys(P.ld_o);
+    P.keys = voom::kv::row_keys(P.ld_o, scored(P));
     P.rows = P.R > 16 ? 32 : 16;
   }
   P.mblocks = (P.R + P.rows - 1) / P.rows;
@@ -305,8 +318,8 @@ uint64_t plan(Attn& P, void* scratch) {
   const uint32_t steps = cached + (P.a.n + P.keys - 1) / P.keys;
   // a block takes at least two tiles for each of its warps (rows), or a few of
   // the larger ones (tensor cores), before the work is spread further
-  const uint32_t least = P.tc >= 0 ? 3 : 8;
-  P.ctas = steps <= (P.tc >= 0 ? 4u : 16u) ? 0u : uint32_t(min(uint64_t(sm_count()), (units * steps + least - 1) / least));
+  const uint32_t least = P.tc >= 0 ? 3 : 2 * voom::kv::row_warps(P.ld_o, scored(P));
+  P.ctas = steps <= (P.tc >= 0 ? 4u : 2 * least) ? 0u : uint32_t(min(uint64_t(sm_count()), (units * steps + least - 1) / least));
   uint64_t at = 0;
   auto take = [&](uint64_t bytes) {
     const uint64_t o = at;
@@ -350,9 +363,8 @@ int finish(const Attn& P, cudaStream_t s) {
 
 template <typename T>
 int run(Attn& P, cudaStream_t s) {
-  const bool scored = P.a.cap > 0.0f || P.a.d_slopes || P.a.window;
   if (P.tc >= 0) map_cache(P);
-  int rc = scored ? voom::kv::launch_attention<T, true>(P, s) : voom::kv::launch_attention<T, false>(P, s);
+  int rc = scored(P) ? voom::kv::launch_attention<T, true>(P, s) : voom::kv::launch_attention<T, false>(P, s);
   if (rc != VOOM_OK) return rc;
   if (P.ctas || P.scores) rc = finish<T>(P, s);
   if (rc != VOOM_OK || !P.a.d_weights || P.scores) return rc;
@@ -366,7 +378,7 @@ int run(Attn& P, cudaStream_t s) {
   const uint64_t steps = uint64_t(P.c.v.B) * P.c.v.hk * (cached + P.tails);
   P.ctas = uint32_t(min(uint64_t(sm_count()), steps));
   map_cache(P);
-  return scored ? voom::kv::launch_sums<T, true>(P, s) : voom::kv::launch_sums<T, false>(P, s);
+  return scored(P) ? voom::kv::launch_sums<T, true>(P, s) : voom::kv::launch_sums<T, false>(P, s);
 }
 
 }  // namespace

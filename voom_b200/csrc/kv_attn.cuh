@@ -37,6 +37,8 @@ struct alignas(64) Attn {
   uint32_t score_ld, score_new; // score row length; where the new tokens' scores start
   float scale2;              // scale * log2(e)
   float cap_in, cap_out;     // of capped scores: 2 scale log2(e) / cap, and cap log2(e); 0: not capped
+  float cap_small;           // products up to it take the polynomial: its coefficients, twice each
+  float2 poly[5];
   int32_t tc;                // tensor-core kernel's mode, or -1: attn_rows
 };
 
@@ -273,8 +275,17 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
 }
 // Products q . k as scores in log2 units, for calls whose scores are capped,
 // biased or windowed ("scored"): two at a time, whose biases are `bias`.
-// cap tanh(z / cap) as cap - 2 cap / (1 + e^(2 z / cap)): off by a few 2^-23 of the
-// cap, absolutely, and no further at either end.
+//   kPlain    not capped
+//   kSmall    capped, with |z| <= 3/4 cap: cap tanh(z / cap) = z P((z / cap)^2), off by
+//             2.6e-7 of the cap.  Six instructions for two scores, none of them on the
+//             special-function unit, which the softmax needs for its own exponentials
+//   kAny      capped: cap - 2 cap / (1 + e^(2 z / cap)), off by a few 2^-23 of the cap,
+//             absolutely, and no further at either end
+constexpr int kPlain = 0, kSmall = 1, kAny = 2;
+// w P(w^2) nearest to tanh w on [0, 3/4] (largest difference 1.9e-7, by reweighted
+// least squares; 2.6e-7 in fp32).
+constexpr double kTanh[5] = {0.9999971985816956, -0.33323076367378235, 0.13226091861724854, -0.049280449748039246,
+                             0.01231883279979229};
 __device__ __forceinline__ float rcp_fast(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -285,21 +296,30 @@ __device__ __forceinline__ F2 mul2(F2 a, F2 b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
   return r;
 }
-__device__ __forceinline__ F2 capped2(const Attn& P, F2 x, F2 bias) {
+template <int KIND>
+__device__ __forceinline__ F2 scored2(const Attn& P, F2 x, F2 bias) {
+  auto both = [](float c) { return make2(c, c); };
+  if (KIND == kPlain) return fma2(x, both(P.scale2), bias);
+  if (KIND == kSmall) {
+    auto c = [&](int i) { return make2(P.poly[i].x, P.poly[i].y); };
+    const F2 s = mul2(x, x);
+    return fma2(x, fma2(s, fma2(s, fma2(s, fma2(s, c(4), c(3)), c(2)), c(1)), c(0)), bias);
+  }
   float a, b;
-  take2(mul2(x, make2(P.cap_in, P.cap_in)), a, b);
-  take2(add2(make2(exp2_fast(a), exp2_fast(b)), make2(1.0f, 1.0f)), a, b);
-  const float m = -2.0f * P.cap_out;
-  return fma2(make2(rcp_fast(a), rcp_fast(b)), make2(m, m), add2(bias, make2(P.cap_out, P.cap_out)));
+  take2(mul2(x, both(P.cap_in)), a, b);
+  take2(add2(make2(exp2_fast(a), exp2_fast(b)), both(1.0f)), a, b);
+  return fma2(make2(rcp_fast(a), rcp_fast(b)), both(-2.0f * P.cap_out), add2(bias, both(P.cap_out)));
 }
 __device__ __forceinline__ F2 scored2(const Attn& P, F2 x, F2 bias) {
-  return P.cap_in != 0.0f ? capped2(P, x, bias) : fma2(x, make2(P.scale2, P.scale2), bias);
+  return P.cap_in != 0.0f ? scored2<kAny>(P, x, bias) : scored2<kPlain>(P, x, bias);
 }
 __device__ __forceinline__ float scored(const Attn& P, float x, float slope2, float ahead) {
   float y, unused;
   take2(scored2(P, make2(x, x), make2(slope2 * ahead, 0.0f)), y, unused);
   return y;
 }
+template <int KIND>
+using Kind = std::integral_constant<int, KIND>;
 
 // A query head's slope in log2 units.
 __device__ __forceinline__ float slope2_of(const Attn& P, uint32_t head) {

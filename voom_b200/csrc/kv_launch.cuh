@@ -27,11 +27,11 @@ inline bool allow_smem(const void* kernel, uint32_t bytes, std::atomic<uint64_t>
 
 template <typename T, int DP, int MT, bool SCORED>
 int launch_rows(const Attn& P, cudaStream_t s) {
-  constexpr uint32_t smem = row_smem(DP, MT);
+  constexpr uint32_t smem = row_smem(DP, MT, SCORED);
   static std::atomic<uint64_t> allowed{0};
   if (!allow_smem(reinterpret_cast<const void*>(attn_rows<T, DP, MT, SCORED>), smem, allowed)) return VOOM_E_CUDA;
   const uint64_t grid = P.ctas ? P.ctas : uint64_t(P.c.v.B) * P.c.v.hk * P.mblocks;
-  attn_rows<T, DP, MT, SCORED><<<uint32_t(grid), 32 * kRowWarps, smem, s>>>(P);
+  attn_rows<T, DP, MT, SCORED><<<uint32_t(grid), 32 * row_warps(DP, SCORED), smem, s>>>(P);
   return cudaGetLastError() == cudaSuccess ? VOOM_OK : VOOM_E_CUDA;
 }
 

@@ -10,11 +10,13 @@
 // their order does not matter) while it writes the new table; fork_plan, one
 // block, numbers the wanted pages by row and the free ones by index, so that the
 // k-th wanted meets the k-th free; fork_finish enters them and copies the open
-// pages.  Compaction is alike: kv_mark, compact_plan, compact_finish.
+// pages.  Compaction is alike: kv_mark, compact_plan, compact_finish.  For small
+// tables one block does the first two (fork_small, compact_small).
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "kv_view.cuh"
 #include "rows.h"
@@ -22,6 +24,11 @@
 namespace {
 
 constexpr uint32_t kMaxPage = 32768, kMaxRows = 65535;
+#ifndef SMALL_ENTRIES
+#define SMALL_ENTRIES 32768
+#endif
+constexpr uint32_t kSmallPages = 12288, kSmallRows = 4096, kSmallEntries = SMALL_ENTRIES;
+constexpr uint32_t kSmallBytes = 8 * kSmallPages + 8 * kSmallRows;
 
 __device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -134,27 +141,37 @@ __device__ __forceinline__ RowState row_state(const Fork& P, uint32_t r, uint32_
 
 __device__ __forceinline__ uint32_t claim_of(uint32_t fill, uint32_t r) { return fill << 16 | (0xFFFFu - r); }
 
-__global__ void __launch_bounds__(256) fork_tables(const __grid_constant__ Fork P) {
-  const uint32_t r = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
-  if (j >= P.a.per) return;
-  uint32_t p;
-  const bool live = parent_of(P, r, p);
-  const uint32_t len = live ? clamped_length(P.a.d_lengths, p, uint64_t(P.a.per) * P.a.page) : 0u;
+// The length that row r takes over.
+__device__ __forceinline__ uint32_t taken_length(const Fork& P, uint32_t r, uint32_t& p) {
+  return parent_of(P, r, p) ? clamped_length(P.a.d_lengths, p, uint64_t(P.a.per) * P.a.page) : 0u;
+}
+
+// Entry j of row r, which continues row p with `len` positions: written, and counted.
+__device__ __forceinline__ void take_entry(const Fork& P, uint32_t r, uint32_t j, uint32_t p, uint32_t len, uint32_t* count,
+                                           uint32_t* owner) {
   int32_t t = -1;
   if (uint64_t(j) * P.a.page < len) {
     t = P.a.d_table[uint64_t(p) * P.a.per + j];
     if (uint32_t(t) >= P.a.n_pages) t = -1;
   }
   P.table[uint64_t(r) * P.a.per + j] = t;
-  if (j == 0) P.lengths[r] = int32_t(len);
   if (t < 0) return;
   const uint32_t fill = len - j * P.a.page;
   if (fill >= P.a.page) {
-    atomicAdd(&P.count[t], 1u);
+    atomicAdd(&count[t], 1u);
   } else {
-    atomicAdd(&P.count[t], 1u << 16);
-    atomicMax(&P.owner[t], claim_of(fill, r));
+    atomicAdd(&count[t], 1u << 16);
+    atomicMax(&owner[t], claim_of(fill, r));
   }
+}
+
+__global__ void __launch_bounds__(256) fork_tables(const __grid_constant__ Fork P) {
+  const uint32_t r = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
+  if (j >= P.a.per) return;
+  uint32_t p;
+  const uint32_t len = taken_length(P, r, p);
+  if (j == 0) P.lengths[r] = int32_t(len);
+  take_entry(P, r, j, p, len, P.count, P.owner);
 }
 
 // Exclusive sum of x over the block's threads, and the total; all threads call it.
@@ -232,12 +249,12 @@ __device__ __forceinline__ uint32_t walk_pages(uint32_t n, uint32_t* s_sum, Load
 }
 static_assert(kPlanThreads / 32 * kPlanDeep == 256, "walk_pages sums 256 counts");
 
-__global__ void __launch_bounds__(kPlanThreads) fork_plan(const __grid_constant__ Fork P) {
+__device__ __forceinline__ void plan_fork(const Fork& P, uint32_t* count, const uint32_t* owner) {
   __shared__ uint64_t s_warp[32];
   __shared__ uint32_t s_sum[257];
   __shared__ uint32_t s_lost;
   if (threadIdx.x == 0) s_lost = 0;
-  wait_for_last();
+  __syncthreads();
   uint64_t all = 0;  // copies, then pages wanted (low half), of the rows so far
   for (uint32_t r0 = 0; r0 < P.a.rows; r0 += kPlanThreads) {
     const uint32_t r = r0 + threadIdx.x;
@@ -253,13 +270,13 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan(const __grid_constant_
         const int32_t t = P.table[uint64_t(r) * P.a.per + s.used - 1];
         if (t >= 0) {
           src = uint32_t(t);
-          copy = (P.count[src] & 0xFFFFu) || P.owner[src] != claim_of(fill, r);
+          copy = (count[src] & 0xFFFFu) || owner[src] != claim_of(fill, r);
         }
       }
       if (copy) {
         need++;
         first--;
-        atomicSub(&P.count[src], 1u << 16);  // (the full holders, which others read, stay)
+        atomicSub(&count[src], 1u << 16);  // (the full holders, which others read, stay)
       }
     }
     uint64_t total;
@@ -273,7 +290,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan(const __grid_constant_
   __syncthreads();
   const uint32_t wanted = uint32_t(all);
   const uint32_t free = walk_pages(
-      P.a.n_pages, s_sum, [&](uint32_t p) { return P.count[p]; }, [](uint32_t c) { return c == 0; },
+      P.a.n_pages, s_sum, [&](uint32_t p) { return count[p]; }, [](uint32_t c) { return c == 0; },
       [&](uint32_t p, uint32_t c, bool none, uint32_t rank) {
         if (none && rank < wanted) P.fresh[rank] = int32_t(p);
         P.a.d_refs[p] = none ? (rank < wanted ? 1 : 0) : int32_t((c & 0xFFFFu) + (c >> 16));
@@ -284,6 +301,31 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan(const __grid_constant_
     P.words[0] = free;
     P.words[1] = uint32_t(all >> 32);
   }
+}
+
+__global__ void __launch_bounds__(kPlanThreads) fork_plan(const __grid_constant__ Fork P) {
+  wait_for_last();
+  plan_fork(P, P.count, P.owner);
+}
+
+// Small tables: fork_tables and fork_plan in one block, the pages' counts in shared memory.
+__global__ void __launch_bounds__(kPlanThreads) fork_small(const __grid_constant__ Fork P) {
+  extern __shared__ uint32_t s_pages[];
+  uint32_t *count = s_pages, *owner = count + P.a.n_pages, *len = owner + P.a.n_pages, *parent = len + P.a.rows;
+  for (uint32_t i = threadIdx.x; i < 2 * P.a.n_pages; i += kPlanThreads) s_pages[i] = 0;
+  for (uint32_t r = threadIdx.x; r < P.a.rows; r += kPlanThreads) {
+    len[r] = taken_length(P, r, parent[r]);
+    P.lengths[r] = int32_t(len[r]);
+  }
+  __syncthreads();
+  const uint32_t entries = P.a.rows * P.a.per;
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < entries; i += kPlanThreads) {
+    const uint32_t r = i / P.a.per;
+    take_entry(P, r, i - r * P.a.per, parent[r], len[r], count, owner);
+  }
+  __syncthreads();
+  plan_fork(P, count, owner);
 }
 
 // n rows of `chunks` 16-byte pieces, kDeep of them a thread under way.
@@ -361,17 +403,16 @@ __global__ void __launch_bounds__(256) kv_mark(const __grid_constant__ Compact P
   if (t >= 0) P.held[t] = 1;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) compact_plan(const __grid_constant__ Compact P) {
+__device__ __forceinline__ void plan_compact(const Compact& P, const uint32_t* held) {
   __shared__ uint32_t s_sum[257];
-  wait_for_last();
-  auto load = [&](uint32_t p) { return P.held[p]; };
-  auto held = [](uint32_t c) { return c != 0; };
-  const uint32_t live = walk_pages(P.a.n_pages, s_sum, load, held, [](uint32_t, uint32_t, bool, uint32_t) {});
+  auto load = [&](uint32_t p) { return held[p]; };
+  auto marked = [](uint32_t c) { return c != 0; };
+  const uint32_t live = walk_pages(P.a.n_pages, s_sum, load, marked, [](uint32_t, uint32_t, bool, uint32_t) {});
   // below `live` the free pages are as many as the held ones past it
-  const uint32_t stay = walk_pages(live, s_sum, load, held, [&](uint32_t p, uint32_t, bool on, uint32_t rank) {
+  const uint32_t stay = walk_pages(live, s_sum, load, marked, [&](uint32_t p, uint32_t, bool on, uint32_t rank) {
     if (!on) P.to[p - rank] = int32_t(p);
   });
-  walk_pages(P.a.n_pages, s_sum, load, held, [&](uint32_t p, uint32_t, bool on, uint32_t rank) {
+  walk_pages(P.a.n_pages, s_sum, load, marked, [&](uint32_t p, uint32_t, bool on, uint32_t rank) {
     if (on && p >= live) P.from[rank - stay] = int32_t(p);
   });
   __syncthreads();
@@ -381,6 +422,27 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan(const __grid_consta
     P.words[0] = live;
     P.words[1] = live - stay;
   }
+}
+
+__global__ void __launch_bounds__(kPlanThreads) compact_plan(const __grid_constant__ Compact P) {
+  wait_for_last();
+  plan_compact(P, P.held);
+}
+
+// Small tables: kv_mark and compact_plan in one block.
+__global__ void __launch_bounds__(kPlanThreads) compact_small(const __grid_constant__ Compact P) {
+  extern __shared__ uint32_t s_pages[];
+  for (uint32_t i = threadIdx.x; i < P.a.n_pages; i += kPlanThreads) s_pages[i] = 0;
+  __syncthreads();
+  const uint32_t entries = P.a.rows * P.a.per;
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < entries; i += kPlanThreads) {
+    const uint32_t r = i / P.a.per;
+    const int32_t t = held_page(P, r, i - r * P.a.per);
+    if (t >= 0) s_pages[t] = 1;
+  }
+  __syncthreads();
+  plan_compact(P, s_pages);
 }
 
 __global__ void __launch_bounds__(256) compact_finish(const __grid_constant__ Compact P) {
@@ -470,6 +532,26 @@ int check(const voom_kv_fork_args* a) {
 
 int check(const voom_kv_compact_args* a) { return !a || !a->d_live ? VOOM_E_INVALID_ARG : check_pool(*a); }
 
+// One block does the table where that is quicker than counting in global memory
+// with a clear and two more launches.
+template <typename A>
+bool small(const A& a) {
+  return a.n_pages <= kSmallPages && a.rows <= kSmallRows && uint64_t(a.rows) * a.per <= kSmallEntries;
+}
+
+// Lets a kernel use kSmallBytes of shared memory on the current device, once per device.
+bool allow(const void* kernel, std::atomic<uint64_t>& devices) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  if (devices.load(std::memory_order_relaxed) >> (dev & 63) & 1u) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmallBytes)) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  devices.fetch_or(uint64_t(1) << (dev & 63), std::memory_order_relaxed);
+  return true;
+}
+
 bool scratch_ok(const void* p) { return p && !(reinterpret_cast<uintptr_t>(p) & 15u); }
 
 }  // namespace
@@ -507,10 +589,14 @@ VOOM_API int voom_kv_append(const voom_kv_view* c, const voom_kv_append_args* a,
   return cudaGetLastError() == cudaSuccess ? VOOM_OK : VOOM_E_CUDA;
 }
 
-VOOM_API uint64_t voom_kv_fork_scratch_bytes(const voom_kv_fork_args* a) {
+VOOM_API uint64_t voom_kv_fork_scratch_bytes(uint32_t rows, uint32_t per, uint32_t n_pages, uint32_t in_place) {
   Fork P{};
-  if (check(a) != VOOM_OK) return 0;
-  P.a = *a;
+  P.a.rows = rows;
+  P.a.per = per;
+  P.a.n_pages = n_pages;
+  int32_t any;
+  P.a.d_table = &any;
+  P.a.d_table_out = in_place ? &any : nullptr;
   return layout(P, nullptr);
 }
 
@@ -522,21 +608,28 @@ VOOM_API int voom_kv_fork(const voom_kv_fork_args* a, void* d_scratch, uint64_t 
   if (!scratch_ok(d_scratch)) return VOOM_E_INVALID_ARG;
   if (layout(P, d_scratch) > bytes) return VOOM_E_CAPACITY;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (cudaMemsetAsync(P.count, 0, 8 * uint64_t(a->n_pages), s) != cudaSuccess) return VOOM_E_CUDA;
-  if (a->rows) {
-    fork_tables<<<dim3((a->per + 255) / 256, a->rows), 256, 0, s>>>(P);
+  if (small(*a)) {
+    static std::atomic<uint64_t> allowed{0};
+    if (!allow(reinterpret_cast<const void*>(fork_small), allowed)) return VOOM_E_CUDA;
+    fork_small<<<1, kPlanThreads, 8 * (a->n_pages + a->rows), s>>>(P);
     if (cudaGetLastError() != cudaSuccess) return VOOM_E_CUDA;
+  } else {
+    if (cudaMemsetAsync(P.count, 0, 8 * uint64_t(a->n_pages), s) != cudaSuccess) return VOOM_E_CUDA;
+    if (a->rows) {
+      fork_tables<<<dim3((a->per + 255) / 256, a->rows), 256, 0, s>>>(P);
+      if (cudaGetLastError() != cudaSuccess) return VOOM_E_CUDA;
+    }
+    const int err = launch_early(fork_plan, dim3(1), kPlanThreads, s, P);
+    if (err != VOOM_OK) return err;
   }
-  const int err = launch_early(fork_plan, dim3(1), kPlanThreads, s, P);
-  if (err != VOOM_OK || !a->rows) return err;
+  if (!a->rows) return VOOM_OK;
   const uint64_t items = uint64_t(a->rows) * a->layers * a->hk;
   return launch_early(fork_finish, dim3(uint32_t(std::min<uint64_t>(items, 8ull * sm_count()))), 256, s, P);
 }
 
-VOOM_API uint64_t voom_kv_compact_scratch_bytes(const voom_kv_compact_args* a) {
+VOOM_API uint64_t voom_kv_compact_scratch_bytes(uint32_t n_pages) {
   Compact P{};
-  if (check(a) != VOOM_OK) return 0;
-  P.a = *a;
+  P.a.n_pages = n_pages;
   return layout(P, nullptr);
 }
 
@@ -548,12 +641,20 @@ VOOM_API int voom_kv_compact(const voom_kv_compact_args* a, void* d_scratch, uin
   if (!scratch_ok(d_scratch)) return VOOM_E_INVALID_ARG;
   if (layout(P, d_scratch) > bytes) return VOOM_E_CAPACITY;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (cudaMemsetAsync(P.held, 0, 4 * uint64_t(a->n_pages), s) != cudaSuccess) return VOOM_E_CUDA;
-  if (a->rows) {
-    kv_mark<<<dim3((a->per + 255) / 256, a->rows), 256, 0, s>>>(P);
+  if (small(*a)) {
+    static std::atomic<uint64_t> allowed{0};
+    if (!allow(reinterpret_cast<const void*>(compact_small), allowed)) return VOOM_E_CUDA;
+    compact_small<<<1, kPlanThreads, 4 * a->n_pages, s>>>(P);
     if (cudaGetLastError() != cudaSuccess) return VOOM_E_CUDA;
+  } else {
+    if (cudaMemsetAsync(P.held, 0, 4 * uint64_t(a->n_pages), s) != cudaSuccess) return VOOM_E_CUDA;
+    if (a->rows) {
+      kv_mark<<<dim3((a->per + 255) / 256, a->rows), 256, 0, s>>>(P);
+      if (cudaGetLastError() != cudaSuccess) return VOOM_E_CUDA;
+    }
+    const int err = launch_early(compact_plan, dim3(1), kPlanThreads, s, P);
+    if (err != VOOM_OK) return err;
   }
-  const int err = launch_early(compact_plan, dim3(1), kPlanThreads, s, P);
-  if (err != VOOM_OK || !a->rows) return err;
+  if (!a->rows) return VOOM_OK;
   return launch_early(compact_finish, dim3(8u * sm_count()), 256, s, P);
 }

@@ -21,16 +21,17 @@
 namespace voom {
 namespace kv {
 
-constexpr uint32_t kRowWarps = 4;
 constexpr uint32_t kRowStages = 3;
-constexpr uint32_t kJoin = 64;  // values of a head that the warps join at a time
 
+// Values of a head that the warps join at a time.
+__host__ __device__ constexpr uint32_t row_join(uint32_t dp, bool scored) { return row_wide(dp, scored) ? 32 : 64; }
 // Shared memory: the warps' stages, the joining buffer, the rows' maxima and
 // sums, and the queries.
-__host__ __device__ constexpr uint32_t row_smem(uint32_t dp, uint32_t mt) {
-  return kRowWarps * kRowStages * 16384u + kRowWarps * 16u * kJoin * 4u + 2u * kRowWarps * 16u * mt * 4u + 16u * mt * dp * 2u;
+__host__ __device__ constexpr uint32_t row_smem(uint32_t dp, uint32_t mt, bool scored) {
+  return row_warps(dp, scored) * (kRowStages * row_tile(dp, scored) + 16u * row_join(dp, scored) * 4u + 2u * 16u * mt * 4u) + 16u * mt * dp * 2u;
 }
-static_assert(row_smem(128, 2) <= 227 * 1024 && row_smem(256, 1) <= 227 * 1024, "shared memory of a block");
+static_assert(row_smem(128, 2, false) <= 227 * 1024 && row_smem(256, 1, false) <= 227 * 1024 && row_smem(128, 2, true) <= 227 * 1024,
+              "shared memory of a block");
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -68,11 +69,11 @@ __device__ __forceinline__ uint32_t row_off(uint32_t r, uint32_t c) {
   return r * (DP * 2u) + ((c ^ (r & 7u)) << 4);
 }
 
-// One tile's loads: K to dst, V to dst + 8 KB.  Rows past the valid ones, and
+// One tile's loads: K to dst, V behind it.  Rows past the valid ones, and
 // new tokens that are none, become zeros.
-template <typename T, int DP>
+template <typename T, int DP, bool SCORED>
 __device__ __forceinline__ void load_tile(const Attn& P, const Seg& g, uint32_t h, uint32_t step, uint32_t dst) {
-  constexpr uint32_t KT = row_keys(DP), CH = DP / 8, per = (KT + 31) / 32;
+  constexpr uint32_t KT = row_keys(DP, SCORED), CH = DP / 8, per = (KT + 31) / 32;
   const uint32_t lane = threadIdx.x & 31u, cs = cache_steps(P, g.len), w0 = first_tile(P, g.len),
                  none = window_none(P, g.len);
   // a lane finds the rows lane, lane + 32; the loads take them by shuffles
@@ -109,21 +110,22 @@ __device__ __forceinline__ void load_tile(const Attn& P, const Seg& g, uint32_t 
     const uint32_t off = row_off<DP>(r, c);
     const void* any = P.c.v.d_k;  // a readable address for the chunks that are zeros
     cp16(dst + off, in && k ? reinterpret_cast<const void*>(k + 16 * c) : any, in && k);
-    cp16(dst + 8192u + off, in && v ? reinterpret_cast<const void*>(v + 16 * c) : any, in && v);
+    cp16(dst + row_tile(DP, SCORED) / 2 + off, in && v ? reinterpret_cast<const void*>(v + 16 * c) : any, in && v);
   }
 }
 
 // DP: head size rounded up to 64, 128 or 256.  MT: blocks of 16 rows.
 template <typename T, int DP, int MT, bool SCORED>
-__global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_constant__ Attn P) {
-  constexpr uint32_t KT = row_keys(DP), CH = DP / 8, NT = KT / 8, DT = DP / 8, LDJ = kJoin, ROWS = 16 * MT;
+__global__ void __launch_bounds__(32 * row_warps(DP, SCORED), 1) attn_rows(const __grid_constant__ Attn P) {
+  constexpr uint32_t W = row_warps(DP, SCORED), TILE = row_tile(DP, SCORED), KT = row_keys(DP, SCORED), LDJ = row_join(DP, SCORED);
+  constexpr uint32_t CH = DP / 8, NT = KT / 8, DT = DP / 8, ROWS = 16 * MT;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, quad = lane & 3u, oct = lane >> 2;
-  const uint32_t stage0 = smem_addr(smem) + warp * kRowStages * 16384u;
-  float* s_join = reinterpret_cast<float*>(smem + kRowWarps * kRowStages * 16384u);  // [warp][16][LDJ]
-  float* s_m = s_join + kRowWarps * 16 * LDJ;                                        // [warp][ROWS]
-  float* s_l = s_m + kRowWarps * ROWS;
-  uint8_t* s_q = reinterpret_cast<uint8_t*>(s_l + kRowWarps * ROWS);
+  const uint32_t stage0 = smem_addr(smem) + warp * kRowStages * TILE;
+  float* s_join = reinterpret_cast<float*>(smem + W * kRowStages * TILE);  // [warp][16][LDJ]
+  float* s_m = s_join + W * 16 * LDJ;                                        // [warp][ROWS]
+  float* s_l = s_m + W * ROWS;
+  uint8_t* s_q = reinterpret_cast<uint8_t*>(s_l + W * ROWS);
   const uint32_t q_addr = smem_addr(s_q);
 
   Seg g;
@@ -137,8 +139,8 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
       ps = pg.s0 + warp;
     }
     if (more) {
-      load_tile<T, DP>(P, pg, pg.h, ps, stage0 + slot * 16384u);
-      ps += kRowWarps;
+      load_tile<T, DP, SCORED>(P, pg, pg.h, ps, stage0 + slot * TILE);
+      ps += W;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -162,7 +164,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
         }
     }
     // the unit's queries
-    for (uint32_t i = tid; i < ROWS * CH; i += 32 * kRowWarps) {
+    for (uint32_t i = tid; i < ROWS * CH; i += 32 * W) {
       const uint32_t r = i / CH, c = i % CH, row = row0 + r;
       uint4 x = make_uint4(0, 0, 0, 0);
       if (r < nrows && c * 8 < P.c.v.D && sees(P, g.b, row / P.g, row / P.g))
@@ -181,11 +183,11 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
       m[t][0] = m[t][1] = -INFINITY;
       l[t][0] = l[t][1] = rest[t][0] = rest[t][1] = 0.0f;
     }
-    for (uint32_t step = g.s0 + warp; step < g.s1; step += kRowWarps) {
+    for (uint32_t step = g.s0 + warp; step < g.s1; step += W) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kRowStages - 2) : "memory");
       __syncwarp();
       produce(slot == 0 ? kRowStages - 1 : slot - 1);
-      const uint32_t ks = stage0 + slot * 16384u, vs = ks + 8192u;
+      const uint32_t ks = stage0 + slot * TILE, vs = ks + TILE / 2;
       // z = q . k
       float z[MT][NT][4];
 #pragma unroll
@@ -238,16 +240,21 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
             const int32_t ahead = (fresh ? int32_t((step - cs) * KT) : int32_t(p0) - int32_t(g.len)) + int32_t(2 * quad) - behind[t][x];
             const float first = slope2[t][x] * float(ahead);
             const F2 from = make2(first, first), by = make2(slope2[t][x], slope2[t][x]);
+            auto all = [&](auto kind) {
 #pragma unroll
-            for (uint32_t j = 0; j < NT; j++) {
-              float a, b;
-              take2(scored2(P, make2(z[t][j][2 * x], z[t][j][2 * x + 1]), fma2(make2(float(8 * j), float(8 * j + 1)), by, from)), a, b);
-              if (edge) {
-                if (!in_window(P, ahead + int32_t(8 * j))) a = -INFINITY;
-                if (!in_window(P, ahead + int32_t(8 * j + 1))) b = -INFINITY;
-              }
-              z[t][j][2 * x] = a;
-              z[t][j][2 * x + 1] = b;
+              for (uint32_t j = 0; j < NT; j++)
+                take2(scored2<decltype(kind)::value>(P, make2(z[t][j][2 * x], z[t][j][2 * x + 1]),
+                                                     fma2(make2(float(8 * j), float(8 * j + 1)), by, from)),
+                      z[t][j][2 * x], z[t][j][2 * x + 1]);
+            };
+            if (P.cap_in != 0.0f) all(Kind<kAny>());
+            else all(Kind<kPlain>());
+            if (edge) {
+#pragma unroll
+              for (uint32_t j = 0; j < NT; j++)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                  if (!in_window(P, ahead + int32_t(8 * j + e))) z[t][j][2 * x + e] = -INFINITY;
             }
           }
       }
@@ -436,16 +443,16 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) attn_rows(const __grid_cons
             *reinterpret_cast<float2*>(s_join + (warp * 16 + oct + 8 * x) * LDJ + 8 * d + 2 * quad) =
                 make_float2(o[t][d0 / 8 + d][2 * x], o[t][d0 / 8 + d][2 * x + 1]);
         __syncthreads();
-        for (uint32_t i = tid; i < 16 * LDJ / 2; i += 32 * kRowWarps) {
+        for (uint32_t i = tid; i < 16 * LDJ / 2; i += 32 * W) {
           const uint32_t r = i / (LDJ / 2), d = 2 * (i % (LDJ / 2)), rr = 16 * t + r, row = row0 + rr;
           if (rr >= nrows || d0 + d >= P.c.v.D) continue;
-          float mm[kRowWarps], top = -INFINITY, sum = 0.0f;
+          float mm[W], top = -INFINITY, sum = 0.0f;
 #pragma unroll
-          for (uint32_t w = 0; w < kRowWarps; w++) top = fmaxf(top, mm[w] = s_m[w * ROWS + rr]);
+          for (uint32_t w = 0; w < W; w++) top = fmaxf(top, mm[w] = s_m[w * ROWS + rr]);
           const float base = top == -INFINITY ? 0.0f : top;
           float2 y = make_float2(0.0f, 0.0f);
 #pragma unroll
-          for (uint32_t w = 0; w < kRowWarps; w++) {
+          for (uint32_t w = 0; w < W; w++) {
             const float f = exp2_fast(mm[w] - base);
             const float2 v = *reinterpret_cast<const float2*>(s_join + (w * 16 + r) * LDJ + d);
             sum += f * s_l[w * ROWS + rr];

@@ -457,11 +457,32 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
 #pragma unroll
         for (uint32_t c = 0; c < KT / 32; c++) tc::tmem_hold(s[c]);
         if constexpr (SCORED) {
-          auto pair = [&](uint32_t c, int e, F2 bias) {
+          auto pair = [&](uint32_t c, int e) { return make2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])); };
+          auto put = [&](uint32_t c, int e, F2 v) {
             float x, y;
-            take2(scored2(P, make2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), bias), x, y);
+            take2(v, x, y);
             s[c][e] = __float_as_uint(x);
             s[c][e + 1] = __float_as_uint(y);
+          };
+          auto all = [&](auto kind, auto biased) {
+            const F2 by = make2(2.0f * slope2, 2.0f * slope2);
+            const float from = slope2 * float(ahead);
+#pragma unroll
+            for (uint32_t c = 0; c < KT / 32; c++)
+#pragma unroll
+              for (int q = 0; q < 32; q += 8) {  // a bias by steps: four of them from one that is made anew
+                const float first = fmaf(slope2, float(32 * c + q), from);
+                F2 bias = decltype(biased)::value ? make2(first, first + slope2) : make2(0.0f, 0.0f);
+#pragma unroll
+                for (int e = q; e < q + 8; e += 2) {
+                  put(c, e, scored2<decltype(kind)::value>(P, pair(c, e), bias));
+                  if (decltype(biased)::value) bias = add2(bias, by);
+                }
+              }
+          };
+          auto with_bias = [&](auto kind) {
+            if (P.a.d_slopes) all(kind, std::true_type());
+            else all(kind, std::false_type());
           };
           if (fresh && P.a.d_mask && P.a.d_slopes) {  // a tree's tokens stand at their depths
 #pragma unroll
@@ -469,15 +490,21 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
 #pragma unroll
               for (int e = 0; e < 32; e += 2) {
                 const uint32_t j = (step - cs) * KT + 32 * c + e;
-                pair(c, e, make2(slope2 * float(depth_of(P, g.b, j) - behind), slope2 * float(depth_of(P, g.b, j + 1) - behind)));
+                put(c, e, scored2(P, pair(c, e), make2(slope2 * float(depth_of(P, g.b, j) - behind),
+                                                       slope2 * float(depth_of(P, g.b, j + 1) - behind))));
               }
+          } else if (P.cap_in == 0.0f) {
+            with_bias(Kind<kPlain>());
           } else {
-            const float first = slope2 * float(ahead);
-            const F2 from = make2(first, first), by = make2(slope2, slope2);
+            float most[2] = {0.0f, 0.0f};
 #pragma unroll
             for (uint32_t c = 0; c < KT / 32; c++)
 #pragma unroll
-              for (int e = 0; e < 32; e += 2) pair(c, e, fma2(make2(float(32 * c + e), float(32 * c + e + 1)), by, from));
+              for (int e = 0; e < 32; e += 2)
+                most[e >> 1 & 1] = max3(most[e >> 1 & 1], fabsf(__uint_as_float(s[c][e])), fabsf(__uint_as_float(s[c][e + 1])));
+            const float m1 = fmaxf(most[0], most[1]);
+            if (__any_sync(0xFFFFFFFFu, m1 > P.cap_small)) with_bias(Kind<kAny>());
+            else with_bias(Kind<kSmall>());
           }
         }
         if (masked) {

@@ -20,6 +20,7 @@ and the paged pool of runtime/kv_cache.py:255-810 (outside its ported path).
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 from typing import NamedTuple
 
@@ -71,20 +72,20 @@ def kv_append(cache: KVView, k: torch.Tensor, v: torch.Tensor, *, index: torch.T
 
 
 def _pool(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor) -> tuple:
-    """Checks a pool, its table and lengths; device index, sizes."""
-    if k.dim() != 5 or v.shape != k.shape or k.dtype not in _CACHE_TYPES or v.dtype != k.dtype:
+    """Checks a pool, its table and lengths; device index, sizes, strides."""
+    size, kind, index = k.shape, k.dtype, k.get_device()
+    if len(size) != 5 or v.shape != size or kind not in _CACHE_TYPES or v.dtype is not kind:
         raise ValueError(f"k and v: (layers, pages, heads, positions, D) BF16 or FP16 wanted, got {tuple(k.shape)} {k.dtype} and "
                          f"{tuple(v.shape)} {v.dtype}")
-    L, N, H, P, D = k.shape
-    if not k.numel() or D % 8 or D > MAX_HEAD_DIM or P > MAX_PAGE:
-        raise ValueError(f"{tuple(k.shape)}: no dimension may be empty, D a multiple of 8 up to {MAX_HEAD_DIM}, pages of at most "
+    L, N, H, P, D = size
+    if not (L and N and H and P and D) or D % 8 or D > MAX_HEAD_DIM or P > MAX_PAGE:
+        raise ValueError(f"{tuple(size)}: no dimension may be empty, D a multiple of 8 up to {MAX_HEAD_DIM}, pages of at most "
                          f"{MAX_PAGE} positions")
-    for x, name in ((k, "k"), (v, "v")):
-        s = x.stride()
-        if s[4] != 1 or (s[0] | s[1] | s[2] | s[3]) & 7 or x.data_ptr() & 15:
-            raise ValueError(f"{name}: the values of a position must be adjacent and every row must start on 16 bytes")
-    index = k.get_device()
-    if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous() or not table.shape[1]:
+    ks, vs = k.stride(), v.stride()
+    if ks[4] != 1 or vs[4] != 1 or (ks[0] | ks[1] | ks[2] | ks[3] | vs[0] | vs[1] | vs[2] | vs[3]) & 7 or \
+            (k.data_ptr() | v.data_ptr()) & 15:
+        raise ValueError("k and v: the values of a position must be adjacent and every row must start on 16 bytes")
+    if table.dim() != 2 or table.dtype is not torch.int32 or not table.is_contiguous() or not table.shape[1]:
         raise ValueError(f"table: a contiguous int32 (rows, pages) tensor wanted, got {tuple(table.shape)} {table.dtype}")
     R, per = table.shape
     if R > MAX_ROWS or per * P >= 2 ** 31 or R * per >= 2 ** 31:
@@ -92,7 +93,7 @@ def _pool(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.
     _row_numbers(lengths, "lengths", R)
     if index < 0 or not index == v.get_device() == table.get_device() == lengths.get_device():
         raise ValueError("keys, values, table and lengths must be on one CUDA device")
-    return index, L, N, H, P, D, R, per
+    return index, L, N, H, P, D, R, per, (*ks[:4], *vs[:4])
 
 
 def _row_numbers(x: torch.Tensor, name: str, rows: int) -> None:
@@ -104,6 +105,34 @@ def _refused(rc: int, what: str) -> None:
     if rc == VOOM_E_OVERLAP:
         raise ValueError("positions of the pool overlap one another, or keys share memory with values")
     check(rc, what)
+
+
+@functools.lru_cache(maxsize=256)
+def _fork_words(rows: int, per: int, pages: int, in_place: bool) -> int:
+    return load().voom_kv_fork_scratch_bytes(rows, per, pages, in_place) // 4
+
+
+@functools.lru_cache(maxsize=256)
+def _compact_words(pages: int) -> int:
+    return load().voom_kv_compact_scratch_bytes(pages) // 4
+
+
+def _changes(parents: torch.Tensor | None, grow: int | torch.Tensor, rows: int, index: int) -> tuple[int, int, int]:
+    """Checks parents and grow: their addresses (0: none), and the one number that all rows grow by."""
+    at = each = 0
+    if parents is not None:
+        _row_numbers(parents, "parents", rows)
+        if parents.get_device() != index:
+            raise ValueError("parents must be on the pool's device")
+        at = parents.data_ptr()
+    if isinstance(grow, torch.Tensor):
+        _row_numbers(grow, "grow", rows)
+        if grow.get_device() != index:
+            raise ValueError("grow must be on the pool's device")
+        return at, grow.data_ptr(), 0
+    if not 0 <= grow < 2 ** 31:
+        raise ValueError(f"grow {grow}: not a number of positions")
+    return at, each, int(grow)
 
 
 class Forked(NamedTuple):
@@ -133,42 +162,28 @@ def fork_pages(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: t
 
     `out`: where the results go.  Its table and lengths may be `table` and
     `lengths` themselves (both); `missing` is then added to."""
-    index, L, N, H, P, D, R, per = _pool(k, v, table, lengths)
+    index, L, N, H, P, D, R, per, strides = _pool(k, v, table, lengths)
     if stream is not None or _device.current_index() != index:
         with _device.on_stream(k.device, stream):
             return fork_pages(k, v, table, lengths, parents, grow=grow, out=out)
-    rows = 0
-    if parents is not None:
-        _row_numbers(parents, "parents", R)
-        if parents.get_device() != index:
-            raise ValueError("parents must be on the pool's device")
-        rows = parents.data_ptr()
-    each = more = 0
-    if isinstance(grow, torch.Tensor):
-        _row_numbers(grow, "grow", R)
-        if grow.get_device() != index:
-            raise ValueError("grow must be on the pool's device")
-        each = grow.data_ptr()
-    elif not 0 <= grow < 2 ** 31:
-        raise ValueError(f"grow {grow}: not a number of positions")
-    else:
-        more = grow
-    same = False
+    rows, each, more = _changes(parents, grow, R, index)
     if out is None:
-        buf = table.new_empty(R * per + R + N + 1)
-        out = Forked(buf[:R * per].view(R, per), buf[R * per:R * per + R], buf[R * per + R:-1], buf[-1:])
+        # the workspace and the results in one piece
+        words = _fork_words(R, per, N, False)
+        ws, new, lens, refs, missing = table.new_empty(words + R * per + R + N + 1).split_with_sizes((words, R * per, R, N, 1))
+        out, same = Forked(new.view(R, per), lens, refs, missing), False
     else:
         same = out.table.data_ptr() == table.data_ptr()
         for x, name, shape in zip(out, Forked._fields, ((R, per), (R,), (N,), (1,))):
             if x.shape != shape or x.dtype != torch.int32 or not x.is_contiguous() or x.get_device() != index:
                 raise ValueError(f"out.{name}: contiguous int32 {shape} on the pool's device wanted, got {tuple(x.shape)} {x.dtype}")
         _apart(out, [table, lengths] + [x for x in (parents,) if x is not None], same)
+        words = _fork_words(R, per, N, same)
+        ws = table.new_empty(words)
     a = _FORK.pack(k.data_ptr(), v.data_ptr(), table.data_ptr(), lengths.data_ptr(), rows, each, out.table.data_ptr(),
-                   out.lengths.data_ptr(), out.refs.data_ptr(), out.missing.data_ptr(), *k.stride()[:4], *v.stride()[:4], L, N, H,
-                   P, D, R, per, more, same, 0)
-    lib = load()
-    ws = table.new_empty(lib.voom_kv_fork_scratch_bytes(a), dtype=torch.uint8)
-    _refused(lib.voom_kv_fork(a, ws.data_ptr(), ws.numel(), _device.raw_stream(index)), "voom_kv_fork")
+                   out.lengths.data_ptr(), out.refs.data_ptr(), out.missing.data_ptr(), *strides, L, N, H, P, D, R, per, more,
+                   same, 0)
+    _refused(load().voom_kv_fork(a, ws.data_ptr(), 4 * words, _device.raw_stream(index)), "voom_kv_fork")
     return out
 
 
@@ -205,24 +220,25 @@ def compact_pages(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths
     """Moves the pages that the rows hold to the front of the pool, in all layers:
     pages past their number go, in order, to the free ones below it.  `out.table`
     may be `table` itself."""
-    index, L, N, H, P, D, R, per = _pool(k, v, table, lengths)
+    index, L, N, H, P, D, R, per, strides = _pool(k, v, table, lengths)
     if stream is not None or _device.current_index() != index:
         with _device.on_stream(k.device, stream):
             return compact_pages(k, v, table, lengths, out=out)
+    words = _compact_words(N)
     if out is None:
-        buf = table.new_empty(R * per + 1)
-        out = Compacted(buf[:-1].view(R, per), buf[-1:])
+        ws, new, live = table.new_empty(words + R * per + 1).split_with_sizes((words, R * per, 1))
+        out = Compacted(new.view(R, per), live)
     else:
         for x, name, shape in zip(out, Compacted._fields, ((R, per), (1,))):
             if x.shape != shape or x.dtype != torch.int32 or not x.is_contiguous() or x.get_device() != index:
                 raise ValueError(f"out.{name}: contiguous int32 {shape} on the pool's device wanted, got {tuple(x.shape)} {x.dtype}")
-        _apart(out[:1], [table], out.table.data_ptr() == table.data_ptr())
-        _apart((out.live, out.table), [lengths] if out.table.data_ptr() == table.data_ptr() else [lengths, table], False)
+        same = out.table.data_ptr() == table.data_ptr()
+        _apart(out[:1], [table], same)
+        _apart((out.live, out.table), [lengths] if same else [lengths, table], False)
+        ws = table.new_empty(words)
     a = _COMPACT.pack(k.data_ptr(), v.data_ptr(), table.data_ptr(), lengths.data_ptr(), out.table.data_ptr(), out.live.data_ptr(),
-                      *k.stride()[:4], *v.stride()[:4], L, N, H, P, D, R, per, 0)
-    lib = load()
-    ws = table.new_empty(lib.voom_kv_compact_scratch_bytes(a), dtype=torch.uint8)
-    _refused(lib.voom_kv_compact(a, ws.data_ptr(), ws.numel(), _device.raw_stream(index)), "voom_kv_compact")
+                      *strides, L, N, H, P, D, R, per, 0)
+    _refused(load().voom_kv_compact(a, ws.data_ptr(), 4 * words, _device.raw_stream(index)), "voom_kv_compact")
     return out
 
 
@@ -245,7 +261,6 @@ class PagePool:
         self.missing = torch.zeros(1, dtype=torch.int32, device=dev)
         self.refs = torch.zeros(pages, dtype=torch.int32, device=dev)
         self._wait_status = torch.zeros(1, dtype=torch.int32, device=dev)
-        _pool(self.k, self.v, self.table, self.lengths)
         self._views: list[KVView] = []
         self._make_views()
 
@@ -254,6 +269,10 @@ class PagePool:
                        for k, v in zip(self.k.unbind(0), self.v.unbind(0))]
         for view in self._views:
             view.status, view.status_ptr = self._wait_status, self._wait_status.data_ptr()
+        # fork's arguments but for those that change from call to call
+        self._index, *sizes, strides = _pool(self.k, self.v, self.table, self.lengths)
+        at = [x.data_ptr() for x in (self.k, self.v, self.table, self.lengths, self.table, self.lengths, self.refs, self.missing)]
+        self._fork_to = (*at, *strides, *sizes)
 
     @property
     def pages(self) -> int:
@@ -266,8 +285,15 @@ class PagePool:
     def fork(self, parents: torch.Tensor | None = None, *, grow: int | torch.Tensor = 0,
              stream: torch.cuda.Stream | None = None) -> None:
         """fork_pages of the pool's own table, in place."""
-        fork_pages(self.k, self.v, self.table, self.lengths, parents, grow=grow, stream=stream,
-                   out=Forked(self.table, self.lengths, self.refs, self.missing))
+        index = self._index
+        if stream is not None or _device.current_index() != index:
+            with _device.on_stream(self.k.device, stream):
+                return self.fork(parents, grow=grow)
+        rows, each, more = _changes(parents, grow, self.rows, index)
+        words = _fork_words(*self.table.shape, self.pages, True)
+        ws = self.table.new_empty(words)
+        a = _FORK.pack(*self._fork_to[:4], rows, each, *self._fork_to[4:], more, True, 0)
+        _refused(load().voom_kv_fork(a, ws.data_ptr(), 4 * words, _device.raw_stream(index)), "voom_kv_fork")
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, *, index: torch.Tensor | None = None,
                stream: torch.cuda.Stream | None = None) -> None:
