@@ -297,7 +297,7 @@ uint64_t plan(Attn& P, void* scratch) {
     P.cap_small = fine ? float(0.75 / r) : -1.0f;
   }
   P.ld_o = c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256;
-  P.tc = -1;
+  P.tc = scored(P) && P.R <= voom::kv::kFewRows ? voom::kv::kFew : voom::kv::kRows;
   // attn_rows up to the rows whose output its registers hold in one block; it
   // takes a block of 32 (16 at head size 256) rows over the cache again for
   // each further one: 65 us against 27 at 104 rows over 8191 positions, 630
@@ -363,7 +363,8 @@ int finish(const Attn& P, cudaStream_t s) {
 
 template <typename T>
 int run(Attn& P, cudaStream_t s) {
-  if (P.tc >= 0) map_cache(P);
+  // (attn_few with few tiles: the maps cost the host more than they save)
+  if (P.tc >= 0 || (P.tc == voom::kv::kFew && P.ctas == uint32_t(sm_count()))) map_cache(P);
   int rc = scored(P) ? voom::kv::launch_attention<T, true>(P, s) : voom::kv::launch_attention<T, false>(P, s);
   if (rc != VOOM_OK) return rc;
   if (P.ctas || P.scores) rc = finish<T>(P, s);

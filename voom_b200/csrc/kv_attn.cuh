@@ -39,7 +39,7 @@ struct alignas(64) Attn {
   float cap_in, cap_out;     // of capped scores: 2 scale log2(e) / cap, and cap log2(e); 0: not capped
   float cap_small;           // products up to it take the polynomial: its coefficients, twice each
   float2 poly[5];
-  int32_t tc;                // tensor-core kernel's mode, or -1: attn_rows
+  int32_t tc;                // which kernel (kv_modes.cuh): at least 0 for attn_tc
 };
 
 struct Seg {
@@ -361,6 +361,12 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
 }
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+
+// Byte offset of 16-byte chunk c of row r in a tile of `rows` rows: blocks of
+// 64 values (128 bytes a row) one after another, the chunk turned by the row.
+__device__ __forceinline__ uint32_t sw128(uint32_t r, uint32_t c, uint32_t rows) {
+  return (c >> 3) * (rows * 128u) + r * 128u + (((c ^ r) & 7u) << 4);
+}
 
 // 16 bytes to shared memory without a register, or 16 zero bytes.
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {

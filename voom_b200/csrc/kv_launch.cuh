@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <atomic>
 
+#include "kv_few.cuh"
 #include "kv_rows.cuh"
 #include "kv_sums.cuh"
 #include "kv_tc.cuh"
@@ -54,12 +55,24 @@ int launch_sums_of(const Attn& P, cudaStream_t s) {
   return cudaGetLastError() == cudaSuccess ? VOOM_OK : VOOM_E_CUDA;
 }
 
+template <typename T, int DP>
+int launch_few(const Attn& P, cudaStream_t s) {
+  static std::atomic<uint64_t> allowed{0};
+  if (!allow_smem(reinterpret_cast<const void*>(attn_few<T, DP>), Few<DP>::SMEM, allowed)) return VOOM_E_CUDA;
+  const uint64_t grid = P.ctas ? P.ctas : uint64_t(P.c.v.B) * P.c.v.hk;
+  attn_few<T, DP><<<uint32_t(grid), 32 * Few<DP>::W, Few<DP>::SMEM, s>>>(P);
+  return cudaGetLastError() == cudaSuccess ? VOOM_OK : VOOM_E_CUDA;
+}
+
 template <typename T, bool SCORED>
 int launch_attention(const Attn& P, cudaStream_t s) {
   if (P.tc == kSingle) return launch_tc<T, 256, kSingle, SCORED>(P, s);
   if (P.tc == kPair) return P.ld_o == 64 ? launch_tc<T, 64, kPair, SCORED>(P, s) : launch_tc<T, 128, kPair, SCORED>(P, s);
   if (P.tc == kAlternate)
     return P.ld_o == 64 ? launch_tc<T, 64, kAlternate, SCORED>(P, s) : launch_tc<T, 128, kAlternate, SCORED>(P, s);
+  if constexpr (SCORED) {
+    if (P.tc == kFew) return P.ld_o == 64 ? launch_few<T, 64>(P, s) : P.ld_o == 128 ? launch_few<T, 128>(P, s) : launch_few<T, 256>(P, s);
+  }
   if (P.ld_o == 64) return P.rows == 16 ? launch_rows<T, 64, 1, SCORED>(P, s) : launch_rows<T, 64, 2, SCORED>(P, s);
   if (P.ld_o == 128) return P.rows == 16 ? launch_rows<T, 128, 1, SCORED>(P, s) : launch_rows<T, 128, 2, SCORED>(P, s);
   return launch_rows<T, 256, 1, SCORED>(P, s);

@@ -6,8 +6,9 @@
 namespace voom {
 namespace kv {
 
-// attn_tc's modes (kv_tc.cuh).
-constexpr int kPair = 0, kAlternate = 1, kSingle = 2;
+// Which kernel a call takes: attn_tc's modes (kv_tc.cuh), attn_rows, attn_few.
+constexpr int kPair = 0, kAlternate = 1, kSingle = 2, kRows = -1, kFew = -2;
+constexpr uint32_t kFewRows = 8;  // rows that attn_few takes
 
 // attn_rows: warps of a block, and bytes of a tile, half of them keys.  Scored
 // calls do more for a score, and a warp's tile is bound by its instructions'

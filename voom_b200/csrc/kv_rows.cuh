@@ -69,9 +69,10 @@ __device__ __forceinline__ uint32_t row_off(uint32_t r, uint32_t c) {
   return r * (DP * 2u) + ((c ^ (r & 7u)) << 4);
 }
 
-// One tile's loads: K to dst, V behind it.  Rows past the valid ones, and
-// new tokens that are none, become zeros.
-template <typename T, int DP, bool SCORED>
+// One tile's loads: K to dst, V behind it, in row_off's places, or (SW) in those
+// that TMA gives them.  Rows past the valid ones, and new tokens that are none,
+// become zeros.
+template <typename T, int DP, bool SCORED, bool SW = false>
 __device__ __forceinline__ void load_tile(const Attn& P, const Seg& g, uint32_t h, uint32_t step, uint32_t dst) {
   constexpr uint32_t KT = row_keys(DP, SCORED), CH = DP / 8, per = (KT + 31) / 32;
   const uint32_t lane = threadIdx.x & 31u, cs = cache_steps(P, g.len), w0 = first_tile(P, g.len),
@@ -101,13 +102,13 @@ __device__ __forceinline__ void load_tile(const Attn& P, const Seg& g, uint32_t 
       }
     }
   }
-#pragma unroll
+#pragma unroll(SW ? 2 : KT * CH / 32)
   for (uint32_t it = 0; it < KT * CH / 32; it++) {
     const uint32_t id = it * 32 + lane, r = id / CH, c = id % CH;
     const uint64_t k = __shfl_sync(0xFFFFFFFFu, ka[(it * 32 / CH) / 32], r & 31u);
     const uint64_t v = __shfl_sync(0xFFFFFFFFu, va[(it * 32 / CH) / 32], r & 31u);
     const bool in = c * 8 < P.c.v.D;
-    const uint32_t off = row_off<DP>(r, c);
+    const uint32_t off = SW ? sw128(r, c, KT) : row_off<DP>(r, c);
     const void* any = P.c.v.d_k;  // a readable address for the chunks that are zeros
     cp16(dst + off, in && k ? reinterpret_cast<const void*>(k + 16 * c) : any, in && k);
     cp16(dst + row_tile(DP, SCORED) / 2 + off, in && v ? reinterpret_cast<const void*>(v + 16 * c) : any, in && v);

@@ -66,12 +66,6 @@ constexpr uint32_t tc_smem() {
   return n;
 }
 
-// Byte offset of 16-byte chunk c of row r in a tile of `rows` rows: blocks of
-// 64 values (128 bytes a row) one after another, the chunk turned by the row.
-__device__ __forceinline__ uint32_t sw128(uint32_t r, uint32_t c, uint32_t rows) {
-  return (c >> 3) * (rows * 128u) + r * 128u + (((c ^ r) & 7u) << 4);
-}
-
 // Values of new tokens that are not finite were taken out of their tiles (a
 // probability of 0 must not meet them); this adds them back for a row that
 // sees them, one at a time: y[0..32) are the row's sums of values col ..
