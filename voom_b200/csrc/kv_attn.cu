@@ -47,13 +47,20 @@ __global__ void __launch_bounds__(256) tree_mask(const int32_t* __restrict__ par
 
 // ------------------------------------------------------------------- finish
 // Joins the partial sums of units that several blocks shared (blocks below
-// n_merge: one per unit and 8 rows), and adds the rows' weights at each
+// n_merge: one per unit and merge_rows of its rows), and adds the rows' weights at each
 // position to the running sums (the others: one per key head and kWeightSpan
 // positions), from the scores the attention kept and the rows' denominators.
 // The partial sums are joined in block order, the rows added in row order, so
 // that nothing depends on scheduling.
 constexpr uint32_t kWeightSpan = 1024;
-constexpr uint32_t kMergeRows = 8;
+constexpr uint32_t kMergeRows = 16;  // at most
+
+// (more blocks than the GPU holds at a time: the latency of one counts for 16 rows, 1000
+// tokens x 32 heads 188 us a call against 194; fewer: more of them at work, 26 drafts
+// x 32 heads 30 us against 34)
+__host__ __device__ __forceinline__ uint32_t merge_rows(const Attn& P) {
+  return uint64_t(P.c.v.B) * P.c.v.hk * P.mblocks * P.rows >= 16384u ? kMergeRows : 8u;
+}
 
 struct Split {
   uint32_t first, last;  // blocks that hold the unit's partial sums; first > last: none, it is whole
@@ -103,7 +110,7 @@ __global__ void __launch_bounds__(256) attn_finish(const __grid_constant__ Attn 
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
   __shared__ Split s_split;
   if (blockIdx.x < n_merge) {
-    const uint32_t groups = (P.rows + kMergeRows - 1) / kMergeRows, unit = blockIdx.x / groups, r0 = (blockIdx.x - unit * groups) * kMergeRows;
+    const uint32_t some = merge_rows(P), groups = (P.rows + some - 1) / some, unit = blockIdx.x / groups, r0 = (blockIdx.x - unit * groups) * some;
     const uint32_t m = unit % P.mblocks, head = unit / P.mblocks, b = head / P.c.v.hk, h = head - b * P.c.v.hk, row0 = m * P.rows;
     if (row0 + r0 >= P.R) return;
     if (warp == 0) {
@@ -113,7 +120,7 @@ __global__ void __launch_bounds__(256) attn_finish(const __grid_constant__ Attn 
     __syncthreads();
     const Split s = s_split;
     if (s.first > s.last) return;
-    const uint32_t rows = min(min(uint32_t(kMergeRows), P.rows - r0), P.R - row0 - r0);
+    const uint32_t rows = min(min(some, P.rows - r0), P.R - row0 - r0);
     for (uint32_t k = warp; k < rows; k += 8) {
       const float2 ml = joined(P, s, r0 + k);
       if (lane == 0) {
@@ -344,7 +351,7 @@ uint64_t plan(Attn& P, void* scratch) {
 template <typename T>
 int finish(const Attn& P, cudaStream_t s) {
   const uint64_t units = uint64_t(P.c.v.B) * P.c.v.hk * P.mblocks;
-  const uint32_t n_merge = P.ctas ? uint32_t(units * ((P.rows + kMergeRows - 1) / kMergeRows)) : 0u;
+  const uint32_t n_merge = P.ctas ? uint32_t(units * ((P.rows + merge_rows(P) - 1) / merge_rows(P))) : 0u;
   const uint64_t spans = P.scores ? uint64_t(P.c.v.B) * P.c.v.hk * ((P.score_ld + kWeightSpan - 1) / kWeightSpan) : 0;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(uint32_t(n_merge + spans));

@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
           is_v = x == 2 * n - 1 || (x >= 2 && !(x & 1u));
           j = is_v ? (x == 2 * n - 1 ? n - 1 : (x - 2) >> 1) : (x + 1) >> 1;
         }
-        const uint32_t step = g.s0 + j, place = it % RING;
+        const uint32_t step = SCORED ? g.s1 - 1 - j : g.s0 + j, place = it % RING;
         if (it >= RING && !(ok = warp_wait(sh.empty[place], (it / RING - 1) & 1u))) break;
         it++;
         if (load_tile_sw128<T, DP, KT>(P, g, step, cs, is_v, pw, lane, ring_s + place * C::TILE, bar(sh.full[place]),
@@ -412,7 +412,8 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
       const float slope2 = SCORED ? slope2_of(P, g.h * P.g + row % P.g) : 0.0f;
       const int32_t behind = SCORED ? depth_of(P, g.b, tok) : 0;  // how far behind the cache the row stands
       for (uint32_t i = MODE == kAlternate ? w : 0; i < n; i += MODE == kAlternate ? 2 : 1) {
-        const uint32_t slot = MODE == kSingle ? i & 1u : w, step = g.s0 + i;
+        // scored: the newest keys first, whose biases are the largest, so that the maximum is not raised tile by tile
+        const uint32_t slot = MODE == kSingle ? i & 1u : w, step = SCORED ? g.s1 - 1 - i : g.s0 + i;
         const uint32_t o_col = C::O_COL + (MODE == kSingle ? 0u : w * DP);
         if (!(ok = warp_wait(sh.s_full[slot], ns[slot]++ & 1u))) break;
         tc::tc_fence_after();
