@@ -53,6 +53,12 @@ def test_sizes_and_types(dtype, B, beams, V, width):
 
 
 @pytest.mark.gpu
+def test_long_rows_of_one_block():
+    """More rows than blocks at a time: a block reads a row alone and looks at its groups several times."""
+    compare(*made(150, 4, 70001, torch.float32, 11), 8)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("shift", [0, 1, 3, 7])
 def test_rows_anywhere(dtype, shift):

@@ -525,3 +525,23 @@ def test_a_pool_that_runs_out_says_so():
     pool.check_status()
     with pytest.raises(ValueError, match="in use"):
         pool.resize(1)
+
+
+@pytest.mark.gpu
+def test_a_row_that_is_full_says_so():
+    """max_len counts whole pages; what a row has no room for is reported, not written past its end."""
+    from voom_b200.runtime.kv_pool import PagePool
+
+    pool = PagePool(1, 1, 64, pages=8, rows=2, max_len=10, page=4)
+    assert pool.max_len == 12
+    pool.fork(grow=i32([12, 5]))
+    x = torch.ones((2, 13, 1, 64), dtype=torch.bfloat16, device="cuda")
+    pool.k.zero_()
+    pool.append(0, x, x)
+    pool.check_status()
+    pool.advance(i32([12, 5]))
+    pool.fork(grow=1)
+    assert pool.lengths.tolist() == [12, 5]
+    with pytest.raises(RuntimeError, match="1 too few"):
+        pool.check_status()
+    assert int(pool.k.sum()) == (12 + 8) * 64  # the rows' five pages and no other

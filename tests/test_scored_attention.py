@@ -7,7 +7,10 @@ the cap adds.  cap tanh(z / cap) is computed as cap (1 - 2 r), r = 1 / (1 + u), 
 2^t.  In units of 2^-24: u is off by 4 relative (ex2) and by ln 2 |t| (the rounding
 of t), of which r takes u / (1 + u)^2: 1 and 0.23 at most; the rounding of 1 + u
 gives r another 1, the reciprocal 2.  So cap 2 dr <= 8.5 cap 2^-24, and the
-rounding of the result in log2 units 1.5: 10 cap 2^-24 = 6e-7 cap.  A bias is
+rounding of the result in log2 units 1.5: 10 cap 2^-24 = 6e-7 cap.  That form is for
+|z| > 3/4 cap, where it is at most 8e-7 |z|; below, a polynomial is off by 7.8e-7 of z and
+the rounding of x P + bias, 9e-7 |z| in all.  So a capped score is off by 9e-7 min(cap, 20),
+as the scores here are below 20 (times `sharp`).  A bias is
 rounded to 2^-24 of itself, and of what it is added to: with biases b <= 16 scores
 apart from the row's largest counting (e^-16 of the weight past that), 3e-6."""
 
@@ -58,7 +61,7 @@ def run_case(B, n, hq, hk, D, lens, dtype, *, cap=0.0, bias=False, window=0, lay
     bare, bare_lse = kva.tree_attention(*args, **kw)
     torch.cuda.synchronize()
     view.check_status()
-    score = 3e-5 * max(1.0, sharp) + 6e-7 * cap + (3e-6 if bias else 0.0)
+    score = 3e-5 * max(1.0, sharp) + 9e-7 * min(cap, 20.0 * max(1.0, sharp)) + (3e-6 if bias else 0.0)
     for b, x in enumerate(lens):
         o, l, s = od.scored_attention(qkv[b, :, :hq], qkv[b, :, hq:hq + hk], qkv[b, :, hq + hk:], oa.tree_sees(par[b]),
                                       oa.tree_depth(par[b]), k[b, :, :x], v[b, :, :x], D ** -0.5, cap=cap, slopes=slopes,
@@ -131,6 +134,14 @@ def test_long_and_ragged():
 def test_saturated_caps(n, g, D):
     # scores far past the cap at either end, and maxima that move along the keys
     run_case(1, n, g, 1, D, [700], torch.bfloat16, cap=3.0, sharp=30.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [2e-3, 200.0, 1e4, 1e9, 1e30])
+@pytest.mark.parametrize("n,g,D", [(1, 4, 128), (4, 4, 64), (40, 4, 128), (20, 4, 256)])
+def test_caps_of_any_size(cap, n, g, D):
+    # far above the scores a cap changes nothing, and costs no precision; far below, it is all that is left
+    run_case(1, n, g, 1, D, [300], torch.bfloat16, cap=cap)
 
 
 @pytest.mark.gpu
@@ -233,7 +244,7 @@ def test_refusals():
     d = qkv.cuda()
     view = place(k, v, [10], "whole", 0)
     args = (d[:, :, :4], d[:, :, 4:6], d[:, :, 6:], kva.DraftTree.chain(1, 1, "cuda"), view)
-    for cap in (0.0, -1.0, math.nan, math.inf):
+    for cap in (0.0, -1.0, 1e-12, math.nan, math.inf):
         with pytest.raises(ValueError, match="cap"):
             kva.tree_attention(*args, cap=cap)
     for window in (0, -3):
@@ -272,7 +283,7 @@ def test_c_entry_refuses(built_lib):
 
     assert attn() == VOOM_E_CAPACITY  # goes on to its scratch
     assert attn(cap=1.0, window=3, slopes=1 << 25) == VOOM_E_CAPACITY
-    for bad in (dict(cap=-1.0), dict(cap=math.nan), dict(cap=math.inf), dict(mask=1 << 26, window=3),
+    for bad in (dict(cap=-1.0), dict(cap=1e-42), dict(cap=math.nan), dict(cap=math.inf), dict(mask=1 << 26, window=3),
                 dict(mask=1 << 26, slopes=1 << 25)):
         assert attn(**bad) == VOOM_E_INVALID_ARG, bad
     assert attn(mask=1 << 26, depth=1 << 27, window=3) == VOOM_E_CAPACITY

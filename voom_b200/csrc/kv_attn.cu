@@ -410,6 +410,7 @@ int check(const voom_kv_view* c, const voom_tree_attention_args* a, Attn& P) {
   if (rc != VOOM_OK) return rc;
   if (!a->hq || a->hq % c->hk || !(a->scale > 0.0f && a->scale <= 3.0e38f)) return VOOM_E_INVALID_ARG;
   if (!(a->cap >= 0.0f && a->cap <= 3.0e38f)) return VOOM_E_INVALID_ARG;
+  if (a->cap > 0.0f && !std::isfinite(4.0f * a->scale / a->cap)) return VOOM_E_INVALID_ARG;
   if (a->d_mask && (a->d_slopes || a->window) && !a->d_depth) return VOOM_E_INVALID_ARG;
   if (a->d_mask && a->n > kMaxTree) return VOOM_E_CAPACITY;
   if (uint64_t(c->max_len) + a->n > 0x7FFFFFFFu || uint64_t(c->B) * a->n * a->hq > 0x7FFFFFFFu) return VOOM_E_UNSUPPORTED;

@@ -107,7 +107,7 @@ struct Fork {
   uint32_t* count;  // n_pages, 0 at first
   uint32_t* owner;  // n_pages, 0 at first: (filled positions, then the first row) of its open holders, the largest
   uint32_t* words;  // free pages, copies
-  uint2* rows;      // rows: rank of the row's first fresh page, and its place in the row
+  uint4* rows;      // rows: rank of the row's first fresh page, its place in the row, and the place behind the last one
   CopyItem* copies; // rows
   int32_t* fresh;   // free pages in order, as many as are wanted
   int32_t* table;   // the new table and lengths: the caller's, or scratch where those are still read
@@ -265,12 +265,13 @@ __device__ __forceinline__ void plan_fork(const Fork& P, uint32_t* count, const 
   uint64_t all = 0;  // copies, then pages wanted (low half), of the rows so far
   for (uint32_t r0 = 0; r0 < P.a.rows; r0 += kPlanThreads) {
     const uint32_t r = r0 + threadIdx.x;
-    uint32_t src = 0, fill = 0, need = 0, first = 0;
+    uint32_t src = 0, fill = 0, need = 0, first = 0, want = 0;
     bool copy = false;
     if (r < P.a.rows) {
       const RowState s = row_state(P, r, length(r), live(r));
       need = s.want - s.used;
       first = s.used;
+      want = s.want;
       fill = s.fill;
       if (s.lost) atomicAdd(&s_lost, s.lost);
       if (s.grows && fill) {
@@ -289,7 +290,7 @@ __device__ __forceinline__ void plan_fork(const Fork& P, uint32_t* count, const 
     uint64_t total;
     const uint64_t at = all + block_before(uint64_t(copy) << 32 | need, s_warp, total);
     if (r < P.a.rows) {
-      P.rows[r] = make_uint2(uint32_t(at), first);
+      P.rows[r] = make_uint4(uint32_t(at), first, want, 0u);
       if (copy) P.copies[at >> 32] = CopyItem{src, uint32_t(at), fill};
     }
     all += total;
@@ -380,16 +381,15 @@ __global__ void __launch_bounds__(256) fork_finish(const __grid_constant__ Fork 
   const uint32_t free = P.words[0], parts = P.a.layers * P.a.hk;
   const bool back = P.table != P.a.d_table_out;
   for (uint32_t r = blockIdx.x; r < P.a.rows; r += gridDim.x) {
-    uint32_t p;
-    const uint32_t len = uint32_t(P.lengths[r]), want = row_state(P, r, len, parent_of(P, r, p)).want;
-    const uint2 fresh = P.rows[r];
+    const uint4 fresh = P.rows[r];
+    const uint32_t want = fresh.z;
     const int32_t* from = P.table + uint64_t(r) * P.a.per;
     int32_t* to = P.a.d_table_out + uint64_t(r) * P.a.per;
     for (uint32_t j = (back ? 0u : fresh.y) + threadIdx.x; j < (back ? P.a.per : want); j += 256) {
       const uint32_t rank = fresh.x + (j - fresh.y);
       to[j] = j < fresh.y || j >= want ? from[j] : rank < free ? P.fresh[rank] : -1;
     }
-    if (back && threadIdx.x == 0) P.a.d_lengths_out[r] = int32_t(len);
+    if (back && threadIdx.x == 0) P.a.d_lengths_out[r] = P.lengths[r];
   }
   const uint64_t items = uint64_t(P.words[1]) * parts;
   for (uint64_t i = blockIdx.x; i < items; i += gridDim.x) {
@@ -522,7 +522,7 @@ uint64_t layout(Fork& P, void* scratch) {
   P.count = take.get<uint32_t>(2 * uint64_t(a.n_pages));  // cleared together
   P.owner = P.count ? P.count + a.n_pages : nullptr;
   P.words = take.get<uint32_t>(2);
-  P.rows = take.get<uint2>(a.rows);
+  P.rows = take.get<uint4>(a.rows);
   P.copies = take.get<CopyItem>(a.rows);
   P.fresh = take.get<int32_t>(std::min<uint64_t>(entries, a.n_pages));
   const bool back = a.d_table_out == a.d_table;

@@ -302,8 +302,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: Draf
             raise ValueError(f"token_weight: contiguous fp32 ({B}, {n}) on {cache.device} wanted")
         tw = token_weight.data_ptr()
     sl = depth = 0
-    if cap is not None and not 0.0 < cap < 3e38:
-        raise ValueError(f"cap {cap}: a positive number wanted")
+    if cap is not None and not 1e-9 <= cap < 3e38:
+        raise ValueError(f"cap {cap}: a number from 1e-9 on wanted")
     if window is not None and window < 1:
         raise ValueError(f"a window of {window} positions: at least 1, the row itself")
     if slopes is not None:

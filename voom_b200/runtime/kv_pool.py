@@ -22,6 +22,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import struct
+import threading
 from typing import NamedTuple
 
 import torch
@@ -177,7 +178,7 @@ def fork_pages(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: t
         for x, name, shape in zip(out, Forked._fields, ((R, per), (R,), (N,), (1,))):
             if x.shape != shape or x.dtype != torch.int32 or not x.is_contiguous() or x.get_device() != index:
                 raise ValueError(f"out.{name}: contiguous int32 {shape} on the pool's device wanted, got {tuple(x.shape)} {x.dtype}")
-        _apart(out, [table, lengths] + [x for x in (parents,) if x is not None], same)
+        _apart(out, [table, lengths] + [x for x in (parents, grow) if isinstance(x, torch.Tensor)], same)
         words = _fork_words(R, per, N, same)
         ws = table.new_empty(words)
     a = _FORK.pack(k.data_ptr(), v.data_ptr(), table.data_ptr(), lengths.data_ptr(), rows, each, out.table.data_ptr(),
@@ -244,23 +245,27 @@ def compact_pages(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths
 
 class PagePool:
     """Keys and values of `rows` continuations over all layers, in pages that rows
-    share.  A step: fork(parents, grow=n) makes room, every layer attends over
-    view(layer) and append()s its new tokens, advance(n) counts them.  The table
-    and the lengths keep their addresses, so a captured step stays valid (but for
-    resize)."""
+    share; a row holds at most `max_len` positions, rounded up to whole pages.  A
+    step: fork(parents, grow=n) makes room, every layer attends over view(layer)
+    and append()s its new tokens, advance(n) counts them.  The table and the
+    lengths keep their addresses, so a captured step stays valid (but for resize).
+    Pages that a row does not hold (rows that never grew, or ended) read as zeros.
+    `refs` says how many rows held each page after the last fork."""
 
     def __init__(self, layers: int, heads: int, head_dim: int, *, pages: int, rows: int, max_len: int, page: int = 64,
                  dtype: torch.dtype = torch.bfloat16, device=None):
         dev = _device.require_cuda(device)
         if min(layers, heads, head_dim, pages, rows, max_len, page) < 1:
             raise ValueError("a pool of at least one layer, head, value, page, row and position wanted")
-        self.page, self.rows, self.max_len = int(page), int(rows), int(max_len)
+        per = -(-max_len // page)
+        self.page, self.rows, self.max_len = int(page), int(rows), int(per * page)
         self.k, self.v = (torch.empty((layers, pages, heads, page, head_dim), dtype=dtype, device=dev) for _ in range(2))
-        self.table = torch.full((rows, -(-max_len // page)), -1, dtype=torch.int32, device=dev)
+        self.table = torch.full((rows, per), -1, dtype=torch.int32, device=dev)
         self.lengths = torch.zeros(rows, dtype=torch.int32, device=dev)
         self.missing = torch.zeros(1, dtype=torch.int32, device=dev)
         self.refs = torch.zeros(pages, dtype=torch.int32, device=dev)
         self._wait_status = torch.zeros(1, dtype=torch.int32, device=dev)
+        self._lock = threading.Lock()
         self._views: list[KVView] = []
         self._make_views()
 
@@ -293,7 +298,9 @@ class PagePool:
         words = _fork_words(*self.table.shape, self.pages, True)
         ws = self.table.new_empty(words)
         a = _FORK.pack(*self._fork_to[:4], rows, each, *self._fork_to[4:], more, True, 0)
-        _refused(load().voom_kv_fork(a, ws.data_ptr(), 4 * words, _device.raw_stream(index)), "voom_kv_fork")
+        with self._lock:  # the launches of one call stay together
+            rc = load().voom_kv_fork(a, ws.data_ptr(), 4 * words, _device.raw_stream(index))
+        _refused(rc, "voom_kv_fork")
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, *, index: torch.Tensor | None = None,
                stream: torch.cuda.Stream | None = None) -> None:
@@ -308,8 +315,11 @@ class PagePool:
 
     def compact(self, *, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
         """compact_pages in place; the number of pages in use, on the device."""
-        return compact_pages(self.k, self.v, self.table, self.lengths, stream=stream,
-                             out=Compacted(self.table, self.table.new_empty(1))).live
+        if stream is not None or _device.current_index() != self._index:
+            with _device.on_stream(self.k.device, stream):
+                return self.compact()
+        with self._lock:
+            return compact_pages(self.k, self.v, self.table, self.lengths, out=Compacted(self.table, self.table.new_empty(1))).live
 
     def resize(self, pages: int) -> None:
         """Compacts the pool and gives it `pages` pages, those in use at least.
