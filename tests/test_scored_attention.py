@@ -130,6 +130,14 @@ def test_long_and_ragged():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("window", [1, 60, 129, 333, 900])
+@pytest.mark.parametrize("n,g,D,lens", [(500, 3, 64, [700]), (450, 4, 128, [300, 0]), (400, 2, 256, [130])])
+def test_windows_that_leave_tiles_behind(window, n, g, D, lens):
+    """Chunks longer than the window: later blocks of rows see neither the cache nor the first new tokens."""
+    run_case(len(lens), n, g, 1, D, lens, torch.bfloat16, kind="chain", window=window, weights=False, cap=30.0, bias=window == 60)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n,g,D", [(1, 4, 128), (40, 4, 128), (40, 2, 256)])
 def test_saturated_caps(n, g, D):
     # scores far past the cap at either end, and maxima that move along the keys
