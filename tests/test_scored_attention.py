@@ -122,6 +122,13 @@ def test_head_sizes(D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("rows", [8, 9, 16, 17, 24, 25, 32, 33])
+def test_rows_where_the_kernels_change(rows, D):
+    run_case(2, rows, 2, 2, D, [2500, 70], torch.float16, layout="pool", page=16, cap=15.0, bias=True, window=1500)
+
+
+@pytest.mark.gpu
 def test_long_and_ragged():
     run_case(4, 1, 4, 1, 64, [20000, 0, 777, 5], torch.bfloat16, layout="pool", page=16, cap=15.0, bias=True)
     run_case(4, 1, 4, 1, 64, [20000, 0, 777, 5], torch.bfloat16, layout="pool", page=16, window=3001)

@@ -309,7 +309,7 @@ uint64_t plan(Attn& P, void* scratch) {
   // takes a block of 32 (16 at head size 256) rows over the cache again for
   // each further one: 65 us against 27 at 104 rows over 8191 positions, 630
   // against 88 at 256 rows (8 requests of up to 16384)
-  if (P.R > (P.ld_o == 256 ? 16u : 32u)) {
+  if (P.R > voom::kv::row_most(P.ld_o, scored(P))) {
     P.tc = P.ld_o == 256 ? voom::kv::kSingle : P.R > 128 ? voom::kv::kPair : voom::kv::kAlternate;
     P.keys = P.tc == voom::kv::kSingle ? 64 : 128;
     P.rows = P.tc == voom::kv::kPair ? 256 : 128;
