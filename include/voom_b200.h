@@ -645,8 +645,8 @@ int voom_tree_mask(const int32_t* d_parents, uint32_t B, uint32_t n, uint32_t* d
  * another: out[b, i, h] = sum_j softmax_j(scale q . k_j) v_j over the cached
  * positions and the new tokens j that row i of the mask names (d_mask NULL: a
  * chain, j <= i).  With cap > 0 a score becomes cap tanh(score / cap); with
- * d_slopes, slopes[h] times (key's position - query's) is added to it (after
- * the cap); with window > 0 a row sees the positions less than `window` before
+ * d_slopes (finite), slopes[h] times (key's position - query's) is added to it
+ * (after the cap); with window > 0 a row sees the positions less than `window` before
  * its own only.  A cached position is its index, a new token's d_len[b] + its
  * depth (d_depth as voom_tree_mask gives it; NULL in a chain, where it is i).
  * Query head h reads key head h / (hq / hk).  A row that sees

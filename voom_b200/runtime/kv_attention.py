@@ -259,7 +259,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: Draf
     of no token gives zeros and lse -inf.  `out` must not share memory with q, k
     or v, nor rows of `out` or `weights` with one another.
 
-    With `cap` a score z becomes cap tanh(z / cap); with `slopes` (Hq) fp32,
+    With `cap` a score z becomes cap tanh(z / cap); with `slopes` (Hq) fp32, finite,
     slopes[h] (p_k - p_q) is added to it, after the cap; with `window` a row sees
     only positions with p_q - p_k < window, itself among them (its tiles before
     are not read).  A cached position is its index, a new token's lengths[b] + its
