@@ -51,22 +51,26 @@ __host__ __device__ __forceinline__ uint32_t ceil_div(uint32_t a, uint32_t b) { 
 
 // The first tile of cached positions that any of a request's rows sees: a window
 // ends `window` positions before the row, and no row stands before position len.
+// (SCORED false: the call is known to have no window; nothing is asked)
+template <bool SCORED = true>
 __device__ __forceinline__ uint32_t first_tile(const Attn& P, uint32_t len) {
-  return P.a.window && len >= P.a.window ? (len - P.a.window + 1) / P.keys : 0u;
+  return SCORED && P.a.window && len >= P.a.window ? (len - P.a.window + 1) / P.keys : 0u;
 }
 
 // A window's edge moves with the rows: no row sees a cached position below
 // `none`, all see those from `all` on (the last of n rows stands at len + n - 1 at
 // most).  Values between must not reach the rows that do not see them, not even
 // times 0: tiles below `all` are looked through for values that are not finite.
+template <bool SCORED = true>
 __device__ __forceinline__ uint32_t window_none(const Attn& P, uint32_t len) {
-  return P.a.window && len >= P.a.window ? len - P.a.window + 1 : 0u;
+  return SCORED && P.a.window && len >= P.a.window ? len - P.a.window + 1 : 0u;
 }
 __device__ __forceinline__ uint32_t window_all(const Attn& P, uint32_t len) {
   return P.a.window && len + P.a.n > P.a.window ? len + P.a.n - P.a.window : 0u;
 }
 
-__device__ __forceinline__ uint32_t cache_steps(const Attn& P, uint32_t len) { return ceil_div(len, P.keys) - first_tile(P, len); }
+template <bool SCORED = true>
+__device__ __forceinline__ uint32_t cache_steps(const Attn& P, uint32_t len) { return ceil_div(len, P.keys) - first_tile<SCORED>(P, len); }
 
 // Steps over the new tokens of the m-th block of rows: in a chain, up to its last token.
 __host__ __device__ __forceinline__ uint32_t tail_of(const Attn& P, uint32_t m) {
@@ -98,14 +102,16 @@ __host__ __device__ __forceinline__ uint64_t tails_before(const Attn& P, uint32_
 }
 
 // Steps of one key head of a request.
+template <bool SCORED = true>
 __device__ __forceinline__ uint64_t head_steps(const Attn& P, uint32_t len) {
-  return uint64_t(P.mblocks) * cache_steps(P, len) + P.tails;
+  return uint64_t(P.mblocks) * cache_steps<SCORED>(P, len) + P.tails;
 }
 
 // Steps of all units before request b (warp-collective); b = B: of all.
+template <bool SCORED = true>
 __device__ __forceinline__ uint64_t steps_before(const Attn& P, uint32_t b) {
   uint64_t sum = 0;
-  for (uint32_t i = threadIdx.x & 31u; i < b; i += 32) sum += head_steps(P, P.c.length(i));
+  for (uint32_t i = threadIdx.x & 31u; i < b; i += 32) sum += head_steps<SCORED>(P, P.c.length(i));
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
   return sum * P.c.v.hk;
 }
@@ -119,6 +125,7 @@ __device__ __forceinline__ uint32_t sharers(const Attn& P, uint64_t total) {
 }
 
 // First segment of grid block `cta` (warp-collective); false: it has none.
+template <bool SCORED>
 __device__ __forceinline__ bool first_seg(const Attn& P, uint32_t cta, Seg& s) {
   if (!P.ctas) {  // the units of a request with the most steps first
     const uint32_t hk = P.c.v.hk, U = hk * P.mblocks, r = cta % U;
@@ -126,13 +133,13 @@ __device__ __forceinline__ bool first_seg(const Attn& P, uint32_t cta, Seg& s) {
     s.h = r % hk;
     s.m = P.mblocks - 1 - r / hk;
     s.len = P.c.length(s.b);
-    s.steps = s.s1 = cache_steps(P, s.len) + tail_of(P, s.m);
+    s.steps = s.s1 = cache_steps<SCORED>(P, s.len) + tail_of(P, s.m);
     s.s0 = 0;
     s.at = 0;
     s.end = s.steps;
     return true;
   }
-  const uint64_t total = steps_before(P, P.c.v.B);
+  const uint64_t total = steps_before<SCORED>(P, P.c.v.B);
   const uint32_t ctas = sharers(P, total);
   if (cta >= ctas) return false;
   const uint64_t top = total * (cta + 1);
@@ -143,7 +150,7 @@ __device__ __forceinline__ bool first_seg(const Attn& P, uint32_t cta, Seg& s) {
   for (uint32_t b0 = 0;; b0 += 32) {
     if (b0 >= P.c.v.B) return false;  // not reached: at < total
     const uint32_t b = b0 + lane;
-    const uint64_t mine = b < P.c.v.B ? head_steps(P, P.c.length(b)) * P.c.v.hk : 0;
+    const uint64_t mine = b < P.c.v.B ? head_steps<SCORED>(P, P.c.length(b)) * P.c.v.hk : 0;
     uint64_t upto = mine;
     for (int o = 1; o < 32; o <<= 1) {
       const uint64_t x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
@@ -159,8 +166,8 @@ __device__ __forceinline__ bool first_seg(const Attn& P, uint32_t cta, Seg& s) {
     base += __shfl_sync(0xFFFFFFFFu, upto, 31);
   }
   s.len = P.c.length(s.b);
-  const uint32_t cs = cache_steps(P, s.len);
-  const uint64_t per = head_steps(P, s.len);
+  const uint32_t cs = cache_steps<SCORED>(P, s.len);
+  const uint64_t per = head_steps<SCORED>(P, s.len);
   uint64_t off = s.at - base;
   s.h = uint32_t(off / per);
   off -= s.h * per;
@@ -178,6 +185,7 @@ __device__ __forceinline__ bool first_seg(const Attn& P, uint32_t cta, Seg& s) {
   return true;
 }
 
+template <bool SCORED>
 __device__ __forceinline__ bool next_seg(const Attn& P, Seg& s) {
   s.at += s.s1 - s.s0;
   if (s.at >= s.end) return false;
@@ -188,7 +196,7 @@ __device__ __forceinline__ bool next_seg(const Attn& P, Seg& s) {
       s.len = P.c.length(++s.b);
     }
   }
-  s.steps = cache_steps(P, s.len) + tail_of(P, s.m);
+  s.steps = cache_steps<SCORED>(P, s.len) + tail_of(P, s.m);
   s.s0 = 0;
   s.s1 = uint32_t(min(uint64_t(s.steps), s.end - s.at));
   return true;

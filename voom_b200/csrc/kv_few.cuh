@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(32 * Few<DP>::W, 1) attn_few(const __grid_cons
   const uint32_t q_addr = smem_addr(s_q), bars = smem_addr(s_q + kFewRows * DP * 2) + warp * kRowStages * 8;
 
   Seg g;
-  if (!first_seg(P, blockIdx.x, g)) return;
+  if (!first_seg<true>(P, blockIdx.x, g)) return;
   if (lane == 0)
     for (uint32_t i = 0; i < kRowStages; i++) tc::mbar_init(bars + 8 * i, 1);
   __syncwarp();
@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(32 * Few<DP>::W, 1) attn_few(const __grid_cons
   look();
   auto produce = [&](uint32_t slot) {
     while (more && ps >= pg.s1) {
-      more = next_seg(P, pg);
+      more = next_seg<true>(P, pg);
       ps = pg.s0 + warp;
       if (more) look();
     }
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(32 * Few<DP>::W, 1) attn_few(const __grid_cons
       }
       __syncthreads();
     }
-  } while (next_seg(P, g));
+  } while (next_seg<true>(P, g));
   asm volatile("cp.async.wait_all;" ::: "memory");
   if (!ok && lane == 0 && P.a.d_status) atomicOr(P.a.d_status, 1u);
 }

@@ -78,8 +78,8 @@ __device__ __forceinline__ uint32_t row_off(uint32_t r, uint32_t c) {
 template <typename T, int DP, bool SCORED, bool SW = false>
 __device__ __forceinline__ void load_tile(const Attn& P, const Seg& g, uint32_t h, uint32_t step, uint32_t dst) {
   constexpr uint32_t KT = row_keys(DP, SCORED), CH = DP / 8, per = (KT + 31) / 32;
-  const uint32_t lane = threadIdx.x & 31u, cs = cache_steps(P, g.len), w0 = first_tile(P, g.len),
-                 none = window_none(P, g.len);
+  const uint32_t lane = threadIdx.x & 31u, cs = cache_steps<SCORED>(P, g.len), w0 = first_tile<SCORED>(P, g.len),
+                 none = window_none<SCORED>(P, g.len);
   // a lane finds the rows lane, lane + 32; the loads take them by shuffles
   uint64_t ka[per], va[per];
 #pragma unroll
@@ -105,8 +105,7 @@ __device__ __forceinline__ void load_tile(const Attn& P, const Seg& g, uint32_t 
       }
     }
   }
-#pragma unroll(SW ? 2 : KT * CH / 32)
-  for (uint32_t it = 0; it < KT * CH / 32; it++) {
+  auto copy = [&](uint32_t it) {
     const uint32_t id = it * 32 + lane, r = id / CH, c = id % CH;
     const uint64_t k = __shfl_sync(0xFFFFFFFFu, ka[(it * 32 / CH) / 32], r & 31u);
     const uint64_t v = __shfl_sync(0xFFFFFFFFu, va[(it * 32 / CH) / 32], r & 31u);
@@ -115,6 +114,13 @@ __device__ __forceinline__ void load_tile(const Attn& P, const Seg& g, uint32_t 
     const void* any = P.c.v.d_k;  // a readable address for the chunks that are zeros
     cp16(dst + off, in && k ? reinterpret_cast<const void*>(k + 16 * c) : any, in && k);
     cp16(dst + row_tile(DP, SCORED) / 2 + off, in && v ? reinterpret_cast<const void*>(v + 16 * c) : any, in && v);
+  };
+  if constexpr (SW) {
+#pragma unroll 2
+    for (uint32_t it = 0; it < KT * CH / 32; it++) copy(it);
+  } else {  // (a count given to the pragma, though the loop's own, made the unscored calls 2 % slower)
+#pragma unroll
+    for (uint32_t it = 0; it < KT * CH / 32; it++) copy(it);
   }
 }
 
@@ -133,13 +139,13 @@ __global__ void __launch_bounds__(32 * row_warps(DP, SCORED), 1) attn_rows(const
   const uint32_t q_addr = smem_addr(s_q);
 
   Seg g;
-  if (!first_seg(P, blockIdx.x, g)) return;
+  if (!first_seg<SCORED>(P, blockIdx.x, g)) return;
   Seg pg = g;  // where the loads are
   bool more = true;
   uint32_t ps = pg.s0 + warp;
   auto produce = [&](uint32_t slot) {
     while (more && ps >= pg.s1) {
-      more = next_seg(P, pg);
+      more = next_seg<SCORED>(P, pg);
       ps = pg.s0 + warp;
     }
     if (more) {
@@ -154,7 +160,7 @@ __global__ void __launch_bounds__(32 * row_warps(DP, SCORED), 1) attn_rows(const
   uint32_t slot = 0;
   do {
     const uint32_t h = g.h, row0 = g.m * ROWS, nrows = min(ROWS, P.R - row0);
-    const uint32_t cs = cache_steps(P, g.len), w0 = SCORED ? first_tile(P, g.len) : 0u;
+    const uint32_t cs = cache_steps<SCORED>(P, g.len), w0 = first_tile<SCORED>(P, g.len);
     float slope2[MT][2];  // of the lane's rows, and how far behind the cache they stand
     int32_t behind[MT][2];
     if constexpr (SCORED) {
@@ -264,6 +270,23 @@ __global__ void __launch_bounds__(32 * row_warps(DP, SCORED), 1) attn_rows(const
       }
       // masks: positions past the length, and the new tokens that a row does not see
       uint32_t odd = 0, odd_hi = 0;  // keys of the tile that some rows do not see and whose values are not all finite
+      auto look = [&] {  // a probability of 0 must not meet an infinite or NaN value: takes those out
+        bool found = false;
+        for (uint32_t id = lane; id < KT * CH; id += 32) {
+          const uint32_t r = id / CH, at = vs - smem_addr(smem) + row_off<DP>(r, id % CH);
+          if (odd_values<T>(*reinterpret_cast<const uint4*>(smem + at))) {
+            *reinterpret_cast<uint4*>(smem + at) = make_uint4(0, 0, 0, 0);
+            if (r < 32) odd |= 1u << r;
+            else odd_hi |= 1u << (r - 32);
+            found = true;
+          }
+        }
+        if (__any_sync(0xFFFFFFFFu, found)) {
+          odd = __reduce_or_sync(0xFFFFFFFFu, odd);
+          odd_hi = __reduce_or_sync(0xFFFFFFFFu, odd_hi);
+        }
+        __syncwarp();
+      };
       if (fresh || p0 + KT > g.len) {
         const uint32_t j0 = fresh ? (step - cs) * KT : 0u, valid = fresh ? 0u : g.len - p0;
 #pragma unroll
@@ -281,24 +304,10 @@ __global__ void __launch_bounds__(32 * row_warps(DP, SCORED), 1) attn_rows(const
                 if (!((k < 32 ? lo : hi) >> (k & 31u) & 1u)) z[t][j][2 * x + e] = -INFINITY;
               }
           }
+        if (!SCORED && fresh) look();
       }
-      const bool ragged = SCORED && !fresh && p0 < window_all(P, g.len) && P.a.n > 1;
-      if (fresh || ragged) {  // a probability of 0 must not meet an infinite or NaN value: take those out here
-        bool found = false;
-        for (uint32_t id = lane; id < KT * CH; id += 32) {
-          const uint32_t r = id / CH, at = vs - smem_addr(smem) + row_off<DP>(r, id % CH);
-          if (odd_values<T>(*reinterpret_cast<const uint4*>(smem + at))) {
-            *reinterpret_cast<uint4*>(smem + at) = make_uint4(0, 0, 0, 0);
-            if (r < 32) odd |= 1u << r;
-            else odd_hi |= 1u << (r - 32);
-            found = true;
-          }
-        }
-        if (__any_sync(0xFFFFFFFFu, found)) {
-          odd = __reduce_or_sync(0xFFFFFFFFu, odd);
-          odd_hi = __reduce_or_sync(0xFFFFFFFFu, odd_hi);
-        }
-        __syncwarp();
+      if constexpr (SCORED) {
+        if (fresh || (p0 < window_all(P, g.len) && P.a.n > 1)) look();
       }
 #pragma unroll
       for (int t = 0; t < MT; t++) {
@@ -482,7 +491,7 @@ __global__ void __launch_bounds__(32 * row_warps(DP, SCORED), 1) attn_rows(const
         }
         __syncthreads();
       }
-  } while (next_seg(P, g));
+  } while (next_seg<SCORED>(P, g));
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 

@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(Sums<DP>::THREADS, 1) attn_sums(const __grid_c
     return __all_sync(0xFFFFFFFFu, tc::mbar_wait(smem_addr(&b), parity)) != 0;
   };
   Seg g;
-  const bool any = first_seg(P, blockIdx.x, g) && (q_s & 1023u) == 0;
+  const bool any = first_seg<SCORED>(P, blockIdx.x, g) && (q_s & 1023u) == 0;
   if (tid == 0) {
     for (uint32_t i = 0; i < RING; i++) {
       tc::mbar_init(bar(sh.full[i]), 128);
@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(Sums<DP>::THREADS, 1) attn_sums(const __grid_c
     uint32_t it = 0, nq = 0;
     bool ok = true;
     do {
-      const uint32_t cs = cache_steps(P, g.len);
+      const uint32_t cs = cache_steps<SCORED>(P, g.len);
       for (uint32_t m = 0; m < blocks && ok; m++) {
         const uint32_t row0 = m * NB, rows = (min(NB, P.R - row0) + 31u) & ~31u;
         if (nq && !(ok = warp_wait(sh.q_empty, (nq - 1) & 1u))) break;
@@ -112,10 +112,10 @@ __global__ void __launch_bounds__(Sums<DP>::THREADS, 1) attn_sums(const __grid_c
         for (uint32_t step = g.s0; step < g.s1; step++, it++) {
           const uint32_t place = it % RING;
           if (it >= RING && !(ok = warp_wait(sh.empty[place], (it / RING - 1) & 1u))) break;
-          load_keys<T, DP, KT>(P, g, step, cs, pw, lane, ring_s + place * C::TILE, bar(sh.full[place]));
+          load_keys<T, DP, KT, SCORED>(P, g, step, cs, pw, lane, ring_s + place * C::TILE, bar(sh.full[place]));
         }
       }
-    } while (ok && next_seg(P, g));
+    } while (ok && next_seg<SCORED>(P, g));
     asm volatile("cp.async.wait_all;" ::: "memory");
     if (!ok) sh.failed = 1;
   } else if (any && warp == MMA_WARP) {
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(Sums<DP>::THREADS, 1) attn_sums(const __grid_c
           }
         }
       }
-    } while (ok && next_seg(P, g));
+    } while (ok && next_seg<SCORED>(P, g));
     if (one) tc::umma_commit(bar(sh.drained));
     if (!warp_wait(sh.drained, 0)) ok = false;
     if (!ok) sh.failed = 1;
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(Sums<DP>::THREADS, 1) attn_sums(const __grid_c
       return warp_wait(sh.ready[w], nr++ & 1u);
     };
     do {
-      const uint32_t cs = cache_steps(P, g.len), n = g.s1 - g.s0, w0 = SCORED ? first_tile(P, g.len) : 0u;
+      const uint32_t cs = cache_steps<SCORED>(P, g.len), n = g.s1 - g.s0, w0 = first_tile<SCORED>(P, g.len);
       float* sums = P.a.d_weights + int64_t(g.b) * P.a.w_b + int64_t(g.h) * P.a.w_h;
       for (uint32_t m = 0; m < blocks && ok; m++) {
         const uint32_t row0 = m * NB, nrows = min(NB, P.R - row0), cols = (nrows + 31u) & ~31u;
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(Sums<DP>::THREADS, 1) attn_sums(const __grid_c
           if (fresh ? j < P.a.n : j < g.len) sums[fresh ? g.len + j : j] += got;
         }
       }
-    } while (ok && next_seg(P, g));
+    } while (ok && next_seg<SCORED>(P, g));
     if (!ok) sh.failed = 1;
   }
   tc::tc_fence_before();

@@ -80,7 +80,7 @@ constexpr uint32_t tc_smem() {
 // sees them, one at a time: y[0..32) are the row's sums of values col ..
 template <typename T, bool SCORED>
 __device__ __forceinline__ void odd_fix(const Attn& P, const Seg& g, uint32_t row, float m2, uint32_t col, float* y) {
-  const uint32_t cs = cache_steps(P, g.len), i = row / P.g;
+  const uint32_t cs = cache_steps<SCORED>(P, g.len), i = row / P.g;
   const T* q = static_cast<const T*>(P.a.d_q) + int64_t(g.b) * P.a.q_b + int64_t(i) * P.a.q_t +
                int64_t(g.h * P.g + row % P.g) * P.a.q_h;
   // one key's part; `ahead`: from the row to it
@@ -100,9 +100,9 @@ __device__ __forceinline__ void odd_fix(const Attn& P, const Seg& g, uint32_t ro
   };
   const int32_t behind = SCORED ? depth_of(P, g.b, i) : 0;
   if constexpr (SCORED) {  // cached positions that the window's edge passes
-    const uint32_t w0 = first_tile(P, g.len);
+    const uint32_t w0 = first_tile<SCORED>(P, g.len);
     const uint32_t edge = ceil_div(window_all(P, g.len), P.keys) * P.keys;  // (whole tiles are looked through)
-    const uint32_t s0 = max(window_none(P, g.len), (w0 + g.s0) * P.keys), s1 = min(min(edge, g.len), (w0 + g.s1) * P.keys);
+    const uint32_t s0 = max(window_none<SCORED>(P, g.len), (w0 + g.s0) * P.keys), s1 = min(min(edge, g.len), (w0 + g.s1) * P.keys);
     if (P.a.n > 1)
       for (uint32_t s = s0; s < s1; s++) {
         const int32_t ahead = int32_t(s) - int32_t(g.len) - behind;
@@ -129,13 +129,13 @@ __device__ __forceinline__ void odd_fix(const Attn& P, const Seg& g, uint32_t ro
 // barrier hears of the copies as they land, and the issuing thread fences them
 // for the tensor cores.  With `hold` nothing is announced: the caller waits
 // for the copies, and arrives; true then.
-template <typename T, int DP, int KT>
+template <typename T, int DP, int KT, bool SCORED>
 __device__ __forceinline__ bool load_tile_sw128(const Attn& P, const Seg& g, uint32_t step, uint32_t cs, bool is_v, uint32_t pw,
                                                 uint32_t lane, uint32_t dst, uint32_t full, bool hold) {
   constexpr uint32_t CH = DP / 8, RW = KT / 4;
   const bool fresh = step >= cs;
-  const uint32_t p0 = (first_tile(P, g.len) + step) * KT;  // of a cached tile: its first position
-  const uint32_t none = window_none(P, g.len);  // what no row sees comes as zeros
+  const uint32_t p0 = (first_tile<SCORED>(P, g.len) + step) * KT;  // of a cached tile: its first position
+  const uint32_t none = window_none<SCORED>(P, g.len);  // what no row sees comes as zeros
   if (P.box && !fresh && p0 + KT <= g.len && p0 >= none && !hold) {
     if (pw == 0) {
       if (lane == 0) tc::mbar_arrive_expect(full, KT * DP * 2);
@@ -184,10 +184,10 @@ __device__ __forceinline__ bool load_tile_sw128(const Attn& P, const Seg& g, uin
   return hold;
 }
 
-template <typename T, int DP, int KT>
+template <typename T, int DP, int KT, bool SCORED>
 __device__ __forceinline__ void load_keys(const Attn& P, const Seg& g, uint32_t step, uint32_t cs, uint32_t pw, uint32_t lane,
                                           uint32_t dst, uint32_t full) {
-  load_tile_sw128<T, DP, KT>(P, g, step, cs, false, pw, lane, dst, full, false);
+  load_tile_sw128<T, DP, KT, SCORED>(P, g, step, cs, false, pw, lane, dst, full, false);
 }
 
 template <typename T, int DP, int MODE, bool SCORED>
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
   };
 
   Seg g;
-  const bool any = first_seg(P, blockIdx.x, g) && (q_s & 1023u) == 0;
+  const bool any = first_seg<SCORED>(P, blockIdx.x, g) && (q_s & 1023u) == 0;
   if (tid == 0) {
     for (uint32_t i = 0; i < RING; i++) {
       tc::mbar_init(bar(sh.full[i]), 128);
@@ -253,9 +253,9 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
       if (found) sh.odd = 1;
     };
     do {
-      const uint32_t row0 = g.m * ROWS, cs = cache_steps(P, g.len), n = g.s1 - g.s0;
+      const uint32_t row0 = g.m * ROWS, cs = cache_steps<SCORED>(P, g.len), n = g.s1 - g.s0;
       // tiles of values below it are looked through, as those of the new tokens are
-      const uint32_t edge = SCORED && P.a.n > 1 ? window_all(P, g.len) : 0u, w0 = SCORED ? first_tile(P, g.len) : 0u;
+      const uint32_t edge = SCORED && P.a.n > 1 ? window_all(P, g.len) : 0u, w0 = first_tile<SCORED>(P, g.len);
       if (nq) {  // the last segment's products of the queries must be done
         if (!(ok = warp_wait(sh.q_empty, (nq - 1) & 1u))) break;
       }
@@ -290,13 +290,13 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
         const uint32_t step = SCORED ? g.s1 - 1 - j : g.s0 + j, place = it % RING;
         if (it >= RING && !(ok = warp_wait(sh.empty[place], (it / RING - 1) & 1u))) break;
         it++;
-        if (load_tile_sw128<T, DP, KT>(P, g, step, cs, is_v, pw, lane, ring_s + place * C::TILE, bar(sh.full[place]),
+        if (load_tile_sw128<T, DP, KT, SCORED>(P, g, step, cs, is_v, pw, lane, ring_s + place * C::TILE, bar(sh.full[place]),
                                            is_v && (step >= cs || (SCORED && (w0 + step) * KT < edge)))) {
           look_through(place);
           tc::mbar_arrive(bar(sh.full[place]));
         }
       }
-    } while (ok && next_seg(P, g));
+    } while (ok && next_seg<SCORED>(P, g));
     asm volatile("cp.async.wait_all;" ::: "memory");
     if (!ok) sh.failed = 1;
   } else if (any && warp >= MMA_WARP) {
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
         }
       }
       it += 2 * n;
-    } while (ok && next_seg(P, g));
+    } while (ok && next_seg<SCORED>(P, g));
     commit(sh.drained);  // nothing may be under way when TMEM is given back
     if (!warp_wait(sh.drained, 0)) ok = false;
     if (!ok) sh.failed = 1;
@@ -414,8 +414,8 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
     uint32_t ns[2] = {0, 0}, no[2] = {0, 0}, done = 0, nj = 0;  // S tiles, finished outputs, steps, joins so far
     bool ok = true;
     do {
-      const uint32_t row = g.m * ROWS + (MODE == kPair ? w * 128 : 0) + tr, tok = row / P.g, cs = cache_steps(P, g.len);
-      const uint32_t n = g.s1 - g.s0, w0 = SCORED ? first_tile(P, g.len) : 0u;
+      const uint32_t row = g.m * ROWS + (MODE == kPair ? w * 128 : 0) + tr, tok = row / P.g, cs = cache_steps<SCORED>(P, g.len);
+      const uint32_t n = g.s1 - g.s0, w0 = first_tile<SCORED>(P, g.len);
       float m = -INFINITY, l = 0.0f, rest = 0.0f;  // l + rest: the denominator
       const float to_log2 = SCORED ? 1.0f : P.scale2;
       const float slope2 = SCORED ? slope2_of(P, g.h * P.g + row % P.g) : 0.0f;
@@ -654,7 +654,7 @@ __global__ void __launch_bounds__(Tc<DP, MODE>::THREADS, 1) attn_tc(const __grid
         tc::mbar_arrive(bar(sh.joined));
         if (!(ok = warp_wait(sh.joined, nj++ & 1u))) break;
       }
-    } while (next_seg(P, g));
+    } while (next_seg<SCORED>(P, g));
     if (!ok) sh.failed = 1;
   }
   tc::tc_fence_before();
