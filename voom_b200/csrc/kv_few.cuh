@@ -14,8 +14,8 @@
 // one vote stands for the lanes' exchange; until then probabilities are at most 2^8.
 //
 // Bound by the cache's bytes where requests are long.  Measured: 32 requests of up to
-// 16000 positions in pages of 16, 4 rows of 128, capped: 180 us a call, 177 of it here
-// under a profiler, 5.8 TB/s (88 % of what a copy reaches); the same in attn_rows
+// 16000 positions in pages of 16, 4 rows of 128, capped: 180 us a call, 177 of it here,
+// 5.8 TB/s (88 % of what a copy reaches); the same in attn_rows
 // 223.  One token over a window of 1000, heads of 64: 13 us, a block's chain of loads.
 // 168, 200 and 255 registers a thread (heads of 64, 128, 256), none spilled.
 #pragma once
