@@ -545,3 +545,37 @@ def test_a_row_that_is_full_says_so():
     with pytest.raises(RuntimeError, match="1 too few"):
         pool.check_status()
     assert int(pool.k.sum()) == (12 + 8) * 64  # the rows' five pages and no other
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 9])
+def test_pages_past_32_bits(n):
+    """A pool of more than 2^32 bytes and 2^31 values: its last pages are written, forked, read and moved as its first are."""
+    from voom_b200.runtime import kv_attention as kva
+    from voom_b200.runtime.kv_pool import compact_pages, fork_pages, kv_append
+
+    N, H, P, D, L = 34000, 8, 64, 128, 130
+    k, v = (torch.zeros((1, N, H, P, D), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    assert (N - 3) * H * P * D > 2 ** 31
+    g = torch.Generator(device="cuda").manual_seed(3)
+    new = [torch.randn((1, L, H, D), generator=g, device="cuda").bfloat16() for _ in range(2)]
+    q, kn, vn = (torch.randn((2, n, h, D), generator=g, device="cuda").bfloat16() for h in (2 * H, H, H))
+    tables = [torch.tensor([[a, a + 1, a + 2, -1]], dtype=torch.int32, device="cuda") for a in (0, N - 3)]
+    empty, full = (torch.full((1,), x, dtype=torch.int32, device="cuda") for x in (0, L))
+    for t in tables:
+        kv_append(kva.KVView.pool(k[0], v[0], t, empty, max_len=4 * P), *new)
+    assert torch.equal(k[0, N - 3:], k[0, :3]) and torch.equal(v[0, N - 3:], v[0, :3]) and bool(k[0, N - 1, :, 0].any())
+    both = torch.cat(tables)
+    view = kva.KVView.pool(k[0], v[0], both, torch.cat([full, full]), max_len=4 * P)
+    qs, ks, vs = (x[:1].expand(2, -1, -1, -1).contiguous() for x in (q, kn, vn))
+    out = kva.tree_attention(qs, ks, vs, kva.DraftTree.chain(2, n, "cuda"), view, cap=20.0, window=100)
+    view.check_status()
+    assert torch.equal(out[0], out[1]) and bool(out[0].any())
+    # the last row twice, both growing: its open page is copied for one of them
+    f = fork_pages(k, v, both, torch.cat([full, full]), torch.tensor([1, 1], dtype=torch.int32, device="cuda"), grow=1)
+    assert f.table.tolist() == [[N - 3, N - 2, N - 1, -1], [N - 3, N - 2, 0, -1]] and int(f.missing) == 0
+    assert torch.equal(k[0, 0, :, :L % P], k[0, N - 1, :, :L % P])
+    was = k[0, N - 3:].clone()
+    c = compact_pages(k, v, f.table, f.lengths)
+    assert c.table.tolist() == [[1, 2, 3, -1], [1, 2, 0, -1]] and int(c.live) == 4
+    assert torch.equal(k[0, 1:4], was) and torch.equal(v[0, 1:4], v[0, N - 3:])
