@@ -133,6 +133,37 @@ def test_peaked_and_shifted_rows():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 600])
+def test_long_rising_rows(rows):
+    """Rows that rise all along: a maximum that is raised a thousand times costs the sum nothing.  The terms' error
+    is 2^-22 (ex2) and 2^-25 (its argument); a group's 16 are added in eight steps of 2^-24 at most, one after
+    another; beyond, sums keep what they lose: 2^-22 + 2^-25 + 8 * 2^-24 < 7.5e-7."""
+    from voom_b200.runtime.beam import beam_select
+
+    V = 1 << 22
+    for rise in (4.0, 40.0, 4000.0):
+        row = (torch.arange(V, dtype=torch.float64) * (rise / V)).to(torch.float32).cuda()
+        x = row.expand(rows, 1, V)  # as many rows as make a block read each by itself
+        got = beam_select(x, torch.zeros((rows, 1), device="cuda"), 5)
+        want = row[-1].double() - torch.logsumexp(row.double(), 0)
+        top = torch.sort(row, descending=True, stable=True)[1][:5]
+        assert torch.equal(got.tokens, top.to(torch.int32).expand(rows, 5)), rise
+        err = (got.scores[:, 0].double() - want).abs().max()
+        assert float(err) <= 7.5e-7 + STEP * abs(float(want)), (rise, float(err))
+
+
+@pytest.mark.gpu
+def test_rows_of_values_past_two_to_the_twenty():
+    """Logits so large that fp32 holds no part of an exponent, at either end, and a row that is one value alone."""
+    for shift in (3e5, 1e7, -1e7, 1e30, -1e30):
+        x, s = made(2, 3, 5003, torch.float32, 16)
+        x[0, 1] = x[0, 1] * 4 + shift
+        x[1, 0] = shift
+        x[1, 2, 100:] = -torch.finfo(torch.float32).max
+        compare(x, s, 6)
+
+
+@pytest.mark.gpu
 def test_streams_graphs_and_repeats():
     from voom_b200.runtime.beam import beam_select
 

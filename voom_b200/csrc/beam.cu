@@ -48,6 +48,7 @@ constexpr uint32_t kFound = 512;     // groups, and entries, that a block holds
 constexpr uint32_t kMaxSort = 8192;  // entries that beam_join sorts
 constexpr uint32_t kMaxCount = 512;  // entries that it puts in order by counting instead
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kFarRef = 1048576.0f, kFar = kFarRef / 2;  // rows whose largest value is further from 0 are summed in fp64
 
 struct Beam {
   voom_beam_select_args a;
@@ -153,11 +154,14 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+
+// 2^-n of a whole number n of at least 1.
+__device__ __forceinline__ float down2(float n) { return n < 126.0f ? __int_as_float((127 - int(n)) << 23) : 0.0f; }
 
 struct Bar {
   float tops[kWarps][32];  // the warps' values, falling
@@ -268,7 +272,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm) beam_rows(const __grid_const
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  float top = -INFINITY, sum = 0.0f, rest = 0.0f;  // sum + rest: of exp(x - top)
+  // sum + rest: of 2^(x log2 e - ref).  `ref` is a whole number, so that raising it scales both
+  // exactly, however often a row rises, and x log2 e - ref is rounded once, as small as it is
+  float top = -INFINITY, ref = -INFINITY, sum = 0.0f, rest = 0.0f;
   bool many = false;
   uint32_t slot = 0;
 #pragma unroll
@@ -288,12 +294,16 @@ __global__ void __launch_bounds__(kThreads, kPerSm) beam_rows(const __grid_const
         slot = slot + 1 == kStages ? 0 : slot + 1;
         best = largest<T>(raw);
         if (best > top) {
-          const float f = exp2_fast((top - best) * kLog2e);
-          sum *= f;
-          rest *= f;
           top = best;
+          const float r = fminf(fmaxf(ceilf(best * kLog2e), -kFarRef), kFarRef);
+          if (r > ref) {
+            const float f = down2(r - ref);
+            sum *= f;
+            rest *= f;
+            ref = r;
+          }
         }
-        const float base = top == -INFINITY ? 0.0f : top;
+        const float base = ref == -INFINITY ? 0.0f : ref;
         const uint64_t nb = make2(-base, -base), l2 = make2(kLog2e, kLog2e);
         uint64_t acc[2] = {0, 0};
 #pragma unroll
@@ -303,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) beam_rows(const __grid_const
 #pragma unroll
           for (uint32_t e = 0; e < VEC; e += 2) {
             float p, q;
-            take2(mul2(add2(make2(x[e], x[e + 1]), nb), l2), p, q);
+            take2(fma2(make2(x[e], x[e + 1]), l2, nb), p, q);
             acc[e >> 1 & 1] = add2(acc[e >> 1 & 1], make2(exp2_fast(p), exp2_fast(q)));
           }
         }
@@ -338,20 +348,24 @@ __global__ void __launch_bounds__(kThreads, kPerSm) beam_rows(const __grid_const
     }
     __syncthreads();
   }
+  // the part's values, one after another
+  auto each = [&](auto f) {
+    const uint64_t t0 = uint64_t(first) * 32 * kChunks * VEC, t1 = uint64_t(last) * 32 * kChunks * VEC;
+    for (uint64_t at = t0 + tid; at < t1; at += kThreads) {
+      const uint32_t t = uint32_t(at) - skew;
+      if (t < V) f(t, value(x0[t]));
+    }
+  };
   many |= sh.n > kFound;
   if (many) {  // values that tie, or lie under few threads: one after another, each the best after the last
     uint64_t last_one = ~0ull;
     uint32_t k = 0;
-    const uint64_t t0 = uint64_t(first) * 32 * kChunks * VEC, t1 = uint64_t(last) * 32 * kChunks * VEC;
     for (; k < width; k++) {
       uint64_t mine = 0;
-      for (uint64_t at = t0 + tid; at < t1; at += kThreads) {
-        const uint32_t t = uint32_t(at) - skew;
-        if (t >= V) continue;
-        const float x = value(x0[t]);
+      each([&](uint32_t t, float x) {
         const uint64_t y = x > -INFINITY ? entry_of(x, t) : 0;
         if (y < last_one) mine = max(mine, y);
-      }
+      });
       last_one = block_max(sh, mine);
       if (!last_one) break;
       if (tid == 0) sh.found[k] = last_one;
@@ -362,14 +376,27 @@ __global__ void __launch_bounds__(kThreads, kPerSm) beam_rows(const __grid_const
   // the warps' sums
   float all = top;
   for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xFFFFFFFFu, all, o));
-  // (a NaN value is not a maximum, but it is in the sum)
-  double s = top == -INFINITY ? double(sum) : (double(sum) + double(rest)) * exp(double(top) - double(all));
+  // (a NaN value is not a maximum, but it is in the sum; far below the block's largest the sum is 0, far above made anew)
+  double s = fabsf(top) > kFar ? double(sum) : (double(sum) + double(rest)) * exp2(double(ref) - double(all) * double(kLog2e));
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
   if (lane == 0) {
     sh.top[warp] = all;
     sh.sum[warp] = s;
   }
   __syncthreads();
+  float most = -INFINITY;
+  for (uint32_t w = 0; w < kWarps; w++) most = fmaxf(most, sh.top[w]);
+  if (fabsf(most) > kFar && fabsf(most) < INFINITY) {  // fp32 holds little of such an exponent
+    double far = 0.0;
+    each([&](uint32_t, float x) { far += exp(double(x) - double(most)); });
+    for (int o = 16; o; o >>= 1) far += __shfl_xor_sync(0xFFFFFFFFu, far, o);
+    __syncthreads();
+    if (lane == 0) {
+      sh.top[warp] = most;
+      sh.sum[warp] = far;
+    }
+    __syncthreads();
+  }
   if (warp == 0) {
     const float t = lane < kWarps ? sh.top[lane] : -INFINITY;
     float m = t;
