@@ -777,11 +777,13 @@ int voom_kv_compact(const voom_kv_compact_args* a, void* d_scratch, uint64_t scr
 /* The `width` best continuations of each of B requests over its beams and the
  * vocabulary: candidates (beam i, token t) have the score
  *   d_scores[b, i] + x - log(sum over t' of exp(x_t')),   x = d_logits[b, i, t],
- * and come largest first, equal ones by beam, then token.  Scores that are NaN or
- * -inf are never chosen: a logit of -inf takes a token out, a score of -inf a
- * beam, and a row with a NaN or an infinite logit has none.  Candidates are
- * compared in 64 bits; the denominators' sums keep what fp32 addition rounds
- * away.  d_parents: b * beams + i, d_tokens: t, d_scores_out rounded to fp32; where
+ * and come largest first, equal ones by beam, within a beam by logit, then token.
+ * Scores that are NaN or -inf are never chosen: a logit of -inf takes a token out, a
+ * score of -inf a beam, and a row with a NaN or an infinite logit has none.  The
+ * scores are off by 1e-6 and their rounding at most, and in order as their 64-bit
+ * values are: beams with candidates that are closer than 2e-6 have their sums made
+ * again in 64 bits (two such beams of 200019 values: 38 us more).
+ * d_parents: b * beams + i, d_tokens: t, d_scores_out rounded to fp32; where
  * there are fewer candidates: -1, -1, -inf.  width <= 64, beams <= 64,
  * beams * V < 2^31. */
 typedef struct voom_beam_select_args {

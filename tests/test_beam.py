@@ -164,6 +164,46 @@ def test_rows_of_values_past_two_to_the_twenty():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,V", [(torch.float16, 50257), (torch.bfloat16, 50257), (torch.float32, 9001), (torch.float16, 200019)])
+@pytest.mark.parametrize("beams,width", [(8, 8), (3, 7)])
+def test_equal_beams_go_by_beam(dtype, V, beams, width):
+    """Beams with the same logits and the same score tie token by token, wherever in 16 bytes their rows start."""
+    x, _ = made(2, 1, V, dtype, 12)
+    x = x.expand(2, beams, V).contiguous()
+    got = compare(x, torch.full((2, beams), -1.5, device="cuda"), width)
+    best = x[:, 0].float().argmax(1)
+    assert got.parents[:, :min(beams, width)].tolist() == [[b * beams + i for i in range(min(beams, width))] for b in range(2)]
+    assert got.tokens[:, :min(beams, width)].tolist() == [[int(t)] * min(beams, width) for t in best]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,V", [(torch.float16, 50257), (torch.float32, 30011)])
+def test_candidates_a_few_2_to_the_minus_24_apart(dtype, V):
+    """Scores are compared in 64 bits: equal rows whose scores are one fp32 step apart, and rows whose sums
+    differ by 1e-8 of themselves."""
+    beams = 7
+    x, _ = made(3, 1, V, dtype, 13)
+    x = x.expand(3, beams, V).contiguous()
+    for b in range(3):
+        top = x[b, 0].float().amax()
+        for i in range(beams):  # of a sum of at least 1: e^-18 = 1.5e-8 for each step
+            x[b, i, 17] = (top - 17 - (i * 3 + b) % beams).to(dtype)
+    order = [3, 0, 6, 2, 5, 1, 4]
+    s = torch.tensor([[0.5 + k * 2.0 ** -24 for k in order]], device="cuda").expand(3, beams).contiguous()
+    s[1] = 0.5
+    compare(x, s, 9)
+
+
+@pytest.mark.gpu
+def test_more_candidates_than_are_put_in_order_by_counting():
+    """64 equal beams, 64 wanted: every beam's best tie."""
+    x, _ = made(2, 1, 300, torch.float32, 14)
+    compare(x.expand(2, 64, 300).contiguous(), torch.full((2, 64), -0.75, device="cuda"), 64)
+    x, s = made(2, 64, 300, torch.float32, 15, spread=0.01)
+    compare(x, s * 1e-3, 64)
+
+
+@pytest.mark.gpu
 def test_streams_graphs_and_repeats():
     from voom_b200.runtime.beam import beam_select
 

@@ -47,6 +47,8 @@ constexpr uint32_t kSlots = 148 * kPerSm;
 constexpr uint32_t kFound = 512;     // groups, and entries, that a block holds
 constexpr uint32_t kMaxSort = 8192;  // entries that beam_join sorts
 constexpr uint32_t kMaxCount = 512;  // entries that it puts in order by counting instead
+constexpr uint32_t kCandidate = 20;  // bytes of one there
+constexpr float kNear = 2e-6f;       // scores of two beams that are this close are made again
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFarRef = 1048576.0f, kFar = kFarRef / 2;  // rows whose largest value is further from 0 are summed in fp64
 
@@ -55,7 +57,10 @@ struct Beam {
   uint64_t* best;  // rows x parts x width entries, 0: none
   double* sums;    // rows x parts: sum of exp(x - top)
   float* tops;     // rows x parts
+  double* exact;   // rows x slices: beam_join's sums over a slice
+  uint32_t* came;  // B: blocks that have made theirs
   uint32_t parts;  // blocks of a row
+  uint32_t slices; // blocks of a request in beam_join
   uint32_t sorted; // entries that beam_join sorts: a power of two
 };
 
@@ -236,6 +241,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) beam_rows(const __grid_const
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, width = P.a.width, V = P.a.V;
   const uint32_t b = row / P.a.beams, i = row - b * P.a.beams;
   const uint64_t out = uint64_t(row) * P.parts + part;
+  if (i == 0 && part == 0 && tid == 0) P.came[b] = 0;
   if (!(P.a.d_scores[row] > -INFINITY)) {  // nothing of a beam that has no score is chosen
     for (uint32_t k = tid; k < width; k += kThreads) P.best[out * width + k] = 0;
     if (tid == 0) {
@@ -419,24 +425,120 @@ __global__ void __launch_bounds__(kThreads, kPerSm) beam_rows(const __grid_const
   for (uint32_t k = n + tid; k < width; k += kThreads) P.best[out * width + k] = 0;
 }
 
-__device__ __forceinline__ uint64_t ordered(double x) {
-  const uint64_t u = uint64_t(__double_as_longlong(x == 0.0 ? 0.0 : x));
-  return u >> 63 ? ~u : u | 0x8000000000000000ull;
-}
-__device__ __forceinline__ double unordered(uint64_t k) {
-  return __longlong_as_double(static_cast<long long>(k >> 63 ? k & 0x7FFFFFFFFFFFFFFFull : ~k));
+// y = e^y for -inf <= y <= 0, in fp64, N at a time step by step: one alone waits for each
+// result.  y = n ln 2 + r with ln 2 as its first 32 bits and the rest (Cody and Waite), and
+// Taylor's series of e^r, |r| <= 0.347: the 14th term is below 5e-18.
+template <int N>
+__device__ __forceinline__ void exp_down(double (&y)[N]) {
+  constexpr double whole = 6755399441055744.0;  // 1.5 * 2^52: what is added to it is rounded, and stands in the low word
+  constexpr double hi = 2977044472.0 / 4294967296.0, lo = -4.2009150726810846e-11;
+  constexpr double f[14] = {1.0,       1.0,        2.0,         6.0,          24.0,         120.0,         720.0,
+                            5040.0,    40320.0,    362880.0,    3628800.0,    39916800.0,   479001600.0,   6227020800.0};
+  double p[N];
+  int n[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const double t = fma(fmax(y[i], -700.0), 1.4426950408889634, whole);
+    n[i] = __double2loint(t);
+    y[i] = fma(whole - t, lo, fma(whole - t, hi, fmax(y[i], -700.0)));
+    p[i] = 1.0 / f[13];
+  }
+#pragma unroll
+  for (int k = 12; k >= 0; k--)
+#pragma unroll
+    for (int i = 0; i < N; i++) p[i] = fma(p[i], y[i], 1.0 / f[k]);
+#pragma unroll
+  for (int i = 0; i < N; i++) y[i] = __hiloint2double(__double2hiint(p[i]) + (n[i] << 20), __double2loint(p[i]));
 }
 
+struct JoinShared {
+  double lse[kMaxBeams];  // NaN: the beam has no candidates
+  double part[kWarps];
+  float score[kMaxBeams], top[kMaxBeams];
+  Bar bar;
+  uint32_t n;
+  unsigned long long near;  // beams whose candidates are too close to others'
+  uint32_t last;
+};
+
+// Sum of e^(x - top) over tokens [t0, t1) of a row, in fp64 and an order that only the
+// tokens decide; the whole block calls it, thread 0 gets it.
+template <typename T>
+__device__ __noinline__ double sum_exactly(JoinShared& sh, const T* row, double top, uint32_t t0, uint32_t t1) {
+  constexpr int kDeep = 8;
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+  double s = 0.0;
+  for (uint32_t at = t0 + tid; at - tid < t1; at += kDeep * kThreads) {
+    T x[kDeep];  // all under way together
+    double y[kDeep];
+#pragma unroll
+    for (int u = 0; u < kDeep; u++) x[u] = at + u * kThreads < t1 ? row[at + u * kThreads] : T(-INFINITY);
+#pragma unroll
+    for (int u = 0; u < kDeep; u++) y[u] = double(value(x[u])) - top;
+    exp_down(y);
+#pragma unroll
+    for (int u = 0; u < kDeep; u++) s += y[u];
+  }
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+  __syncthreads();  // the last row's parts are read
+  if (lane == 0) sh.part[warp] = s;
+  __syncthreads();
+  s = 0.0;
+  for (uint32_t w = 0; w < kWarps; w++) s += sh.part[w];
+  return s;
+}
+
+// Makes the denominators of the beams in `near` again; false: another block goes on.
+__device__ __noinline__ bool settle(const Beam& P, JoinShared& sh, uint32_t b, uint32_t slice, unsigned long long near) {
+  const uint32_t tid = threadIdx.x, beams = P.a.beams;
+  const uint32_t V = P.a.V, t0 = uint32_t(uint64_t(V) * slice / P.slices), t1 = uint32_t(uint64_t(V) * (slice + 1) / P.slices);
+  for (unsigned long long left = near; left; left &= left - 1) {
+    const uint32_t i = uint32_t(__ffsll(static_cast<long long>(left))) - 1;
+    const int64_t row = int64_t(b) * P.a.l_b + int64_t(i) * P.a.l_i;
+    const double top = double(sh.top[i]);
+    double s;
+    if (P.a.type == VOOM_BF16) s = sum_exactly(sh, static_cast<const __nv_bfloat16*>(P.a.d_logits) + row, top, t0, t1);
+    else if (P.a.type == VOOM_FP16) s = sum_exactly(sh, static_cast<const __half*>(P.a.d_logits) + row, top, t0, t1);
+    else s = sum_exactly(sh, static_cast<const float*>(P.a.d_logits) + row, top, t0, t1);
+    if (tid == 0) P.exact[(uint64_t(b) * beams + i) * P.slices + slice] = s;
+  }
+  if (tid == 0) {
+    __threadfence();
+    sh.last = atomicAdd(P.came + b, 1u) + 1 == P.slices;
+    __threadfence();
+  }
+  __syncthreads();
+  if (!sh.last) return false;
+  for (unsigned long long left = near; left; left &= left - 1) {
+    const uint32_t i = uint32_t(__ffsll(static_cast<long long>(left))) - 1;
+    if (tid != i) continue;
+    double s = 0.0;
+    for (uint32_t g = 0; g < P.slices; g++) s += __ldcg(P.exact + (uint64_t(b) * beams + i) * P.slices + g);
+    sh.lse[i] = double(sh.top[i]) + log(s);
+  }
+  __syncthreads();
+  return true;
+}
+
+// The candidates' scores come from beam_rows' sums, which are off by 8e-7 of themselves
+// at most (ex2 2^-22, a group's additions 9 * 2^-24): enough for all but candidates of
+// two beams that are closer than twice that.  Such beams' denominators are made again in
+// fp64 (settle).  That is rare (one of twelve calls of 32 requests of 8 beams over 200019
+// FP16 values, for one pair), but a row takes one block long: several blocks do the same
+// for a request, each sums a slice of the rows if that is called for, and the last to
+// come adds the slices up (nothing waits).  Without it the first block is done.  The pair
+// 38 us more, all 256 rows of equal beams 142; the blocks that are not needed 1 us.
 __global__ void __launch_bounds__(kThreads) beam_join(const __grid_constant__ Beam P) {
-  extern __shared__ uint64_t s_key[];  // the scores in unsigned order, 0: none; then the candidates' indexes
-  __shared__ double s_lse[kMaxBeams];  // NaN: the beam has no candidates
-  __shared__ float s_score[kMaxBeams];
-  __shared__ Bar s_bar;
-  __shared__ uint32_t s_n;
-  uint32_t* s_at = reinterpret_cast<uint32_t*>(s_key + P.sorted);
-  const uint32_t b = blockIdx.x, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+  extern __shared__ double s_z[];      // the candidates' scores; their entries, their beams
+  __shared__ JoinShared sh;
+  uint64_t* s_entry = reinterpret_cast<uint64_t*>(s_z + P.sorted);
+  uint32_t* s_beam = reinterpret_cast<uint32_t*>(s_entry + P.sorted);
+  const uint32_t b = blockIdx.x / P.slices, slice = blockIdx.x - b * P.slices, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
   const uint32_t beams = P.a.beams, width = P.a.width, parts = P.parts, per = parts * width, all = beams * per;
-  if (tid == 0) s_n = 0;
+  if (tid == 0) {
+    sh.n = 0;
+    sh.near = 0;
+  }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint64_t* best = P.best + uint64_t(b) * all;
   uint64_t ahead = tid < all ? best[tid] : 0;  // on its way while the denominators are made
@@ -460,76 +562,114 @@ __global__ void __launch_bounds__(kThreads) beam_join(const __grid_constant__ Be
     if (m > -INFINITY && m != top) s *= exp(double(m) - double(top));
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
     if (lane == 0) {
-      s_lse[i] = top > -INFINITY ? double(top) + log(s) : double(NAN);
-      s_score[i] = score;
+      sh.lse[i] = top > -INFINITY ? double(top) + log(s) : double(NAN);
+      sh.score[i] = score;
+      sh.top[i] = top;
     }
   }
   __syncthreads();
   // a candidate's score; NaN: it is none
-  auto score_of = [&](uint32_t k, uint64_t x) {
-    const uint32_t i = k / per;
-    return x ? double(s_score[i]) + (double(unordered(uint32_t(x >> 32))) - s_lse[i]) : double(NAN);
+  auto score_of = [&](uint32_t i, uint64_t x) {
+    return x ? double(sh.score[i]) + (double(unordered(uint32_t(x >> 32))) - sh.lse[i]) : double(NAN);
   };
   float most = -INFINITY;
-  for (uint32_t k = tid; k < all; k += kThreads) most = fmaxf(most, float(score_of(k, k == tid ? ahead : best[k])));
-  const float bar = find_bar(s_bar, most, width);  // `width` candidates reach it, if there are as many
+  for (uint32_t k = tid; k < all; k += kThreads) most = fmaxf(most, float(score_of(k / per, k == tid ? ahead : best[k])));
+  float bar = find_bar(sh.bar, most, width);  // `width` candidates reach it, if there are as many
+  // (and those that may be as good: what two scores are off, and the rounding to fp32)
+  if (fabsf(bar) < INFINITY) bar -= 1.25f * kNear + fabsf(bar) * 0x1p-22f;
   for (uint32_t k = tid; k < all; k += kThreads) {
     const uint64_t x = k == tid ? ahead : best[k];
-    const double z = score_of(k, x);
+    const double z = score_of(k / per, x);
     if (z > -INFINITY && float(z) >= bar) {
-      const uint32_t at = atomicAdd(&s_n, 1u);
-      s_key[at] = ordered(z);
-      s_at[at] = k / per * P.a.V + ~uint32_t(x);
+      const uint32_t at = atomicAdd(&sh.n, 1u);
+      s_z[at] = z;
+      s_entry[at] = x;
+      s_beam[at] = k / per;
     }
   }
-  auto put = [&](uint32_t k, uint64_t key, uint32_t at) {
-    const uint64_t out = uint64_t(b) * width + k;
-    const uint32_t i = key ? at / P.a.V : 0u;
-    P.a.d_scores_out[out] = key ? float(unordered(key)) : -INFINITY;
-    P.a.d_parents[out] = key ? int32_t(b * beams + i) : -1;
-    P.a.d_tokens[out] = key ? int32_t(at - i * P.a.V) : -1;
+  // equal scores: the lower beam, then the larger logit, then the lower token
+  auto first = [&](uint32_t q, uint32_t k) { return s_beam[q] != s_beam[k] ? s_beam[q] < s_beam[k] : s_entry[q] > s_entry[k]; };
+  auto put = [&](uint32_t rank, uint32_t k, bool some) {
+    const uint64_t out = uint64_t(b) * width + rank;
+    P.a.d_scores_out[out] = some ? float(s_z[k]) : -INFINITY;
+    P.a.d_parents[out] = some ? int32_t(b * beams + s_beam[k]) : -1;
+    P.a.d_tokens[out] = some ? int32_t(~uint32_t(s_entry[k])) : -1;
   };
   __syncthreads();
-  const uint32_t n = s_n;
-  if (n <= kMaxCount) {  // a candidate's place is the number of better ones
-    for (uint32_t k = tid; k < n; k += kThreads) {
-      const uint64_t key = s_key[k];
-      const uint32_t at = s_at[k];
-      uint32_t rank = 0;
-#pragma unroll 4
-      for (uint32_t q = 0; q < n; q++) {
-        const uint64_t x = s_key[q];
-        rank += (x > key) | ((x == key) & (s_at[q] < at));
-      }
-      if (rank < width) put(rank, key, at);
-    }
-    for (uint32_t k = n + tid; k < width; k += kThreads) put(k, 0, 0);
-    return;
-  }
+  const uint32_t n = sh.n;
   uint32_t sorted = 2;
   while (sorted < n) sorted *= 2;
-  for (uint32_t k = n + tid; k < sorted; k += kThreads) {
-    s_key[k] = 0;
-    s_at[k] = 0xFFFFFFFFu;
-  }
-  __syncthreads();
-  for (uint32_t k = 2; k <= sorted; k <<= 1)
-    for (uint32_t d = k >> 1; d; d >>= 1) {
-      for (uint32_t q = tid; q < sorted / 2; q += kThreads) {
-        const uint32_t lo = 2 * q - (q & (d - 1)), hi = lo + d;
-        const uint64_t x = s_key[lo], y = s_key[hi];
-        const uint32_t xa = s_at[lo], ya = s_at[hi];
-        const bool behind = x < y || (x == y && xa > ya);  // `lo` belongs behind `hi`
-        if (behind == ((lo & k) == 0) && (x != y || xa != ya)) {
-          s_key[lo] = y;
-          s_key[hi] = x;
-          s_at[lo] = ya;
-          s_at[hi] = xa;
+  for (bool again = false;; again = true) {
+    constexpr uint32_t kMine = kMaxCount / kThreads;
+    uint32_t rank[kMine];
+    if (n <= kMaxCount) {  // a candidate's place is the number of better ones
+#pragma unroll
+      for (uint32_t c = 0; c < kMine; c++) {
+        const uint32_t k = tid + c * kThreads;
+        rank[c] = width;
+        if (k >= n) continue;
+        const double z = s_z[k];
+        uint32_t r = 0;
+        unsigned long long near = 0;
+#pragma unroll 4
+        for (uint32_t q = 0; q < n; q++) {
+          const double d = s_z[q] - z;
+          r += d > 0.0;
+          if (!(fabs(d) > double(kNear)) && q != k) {  // seldom (infinite ones are equal)
+            if (!(fabs(d) > 0.0)) r += first(q, k);
+            if (s_beam[q] != s_beam[k]) near |= 1ull << s_beam[q] | 1ull << s_beam[k];
+          }
         }
+        if (near && r < width && !again) atomicOr(&sh.near, near);
+        rank[c] = r;
+      }
+    } else {
+      for (uint32_t k = n + tid; k < sorted; k += kThreads) {
+        s_z[k] = -INFINITY;
+        s_beam[k] = kMaxBeams;
+        s_entry[k] = sorted - k;
       }
       __syncthreads();
+      for (uint32_t k = 2; k <= sorted; k <<= 1)
+        for (uint32_t d = k >> 1; d; d >>= 1) {
+          for (uint32_t q = tid; q < sorted / 2; q += kThreads) {
+            const uint32_t lo = 2 * q - (q & (d - 1)), hi = lo + d;
+            const double z = s_z[lo], y = s_z[hi];
+            if ((z != y ? z < y : first(hi, lo)) == ((lo & k) == 0)) {  // (no two are equal)
+              const uint64_t x = s_entry[lo];
+              const uint32_t i = s_beam[lo];
+              s_z[lo] = y;
+              s_entry[lo] = s_entry[hi];
+              s_beam[lo] = s_beam[hi];
+              s_z[hi] = z;
+              s_entry[hi] = x;
+              s_beam[hi] = i;
+            }
+          }
+          __syncthreads();
+        }
+      if (!again)  // (of two beams with close candidates, some are neighbours)
+        for (uint32_t k = tid; k + 1 < n; k += kThreads)
+          if (s_beam[k] != s_beam[k + 1] && !(s_z[k] - s_z[k + 1] > double(kNear))) atomicOr(&sh.near, 1ull << s_beam[k] | 1ull << s_beam[k + 1]);
     }
-  for (uint32_t k = tid; k < width; k += kThreads) put(k, s_key[k], s_at[k]);  // (n > kMaxCount >= width)
+    __syncthreads();
+    const unsigned long long near = again ? 0ull : sh.near;
+    if (!near) {
+      if (!again && slice) return;
+      if (n <= kMaxCount) {
+#pragma unroll
+        for (uint32_t c = 0; c < kMine; c++)
+          if (rank[c] < width) put(rank[c], tid + c * kThreads, true);
+        for (uint32_t k = n + tid; k < width; k += kThreads) put(k, 0, false);
+      } else {
+        for (uint32_t k = tid; k < width; k += kThreads) put(k, k, true);  // (n > kMaxCount >= width)
+      }
+      return;
+    }
+    if (!settle(P, sh, b, slice, near)) return;
+    for (uint32_t k = tid; k < n; k += kThreads) s_z[k] = score_of(s_beam[k], s_entry[k]);
+    __syncthreads();
+  }
 }
 
 int check(const voom_beam_select_args* a) {
@@ -553,12 +693,21 @@ uint64_t plan(Beam& P, void* scratch) {
   P.parts = uint32_t(std::max<uint64_t>(parts, 1));
   P.sorted = 2;
   while (P.sorted < a.beams * P.parts * a.width) P.sorted *= 2;
+  // a slice of 4096 values at least, and no more blocks than two to an SM
+  P.slices = uint32_t(std::max<uint64_t>(1, std::min<uint64_t>({32, 296 / std::max(a.B, 1u), (a.V + 4095) / 4096})));
   uint8_t* base = static_cast<uint8_t*>(scratch);
   const uint64_t n = rows * P.parts;
-  P.best = reinterpret_cast<uint64_t*>(base);
-  P.sums = reinterpret_cast<double*>(base + 8 * n * a.width);
-  P.tops = reinterpret_cast<float*>(base + 8 * n * (a.width + 1));
-  return 8 * n * (a.width + 1) + 4 * n;
+  uint64_t at = 0;
+  auto take = [&](uint64_t bytes) {
+    at += bytes;
+    return base + (at - bytes);
+  };
+  P.best = reinterpret_cast<uint64_t*>(take(8 * n * a.width));
+  P.sums = reinterpret_cast<double*>(take(8 * n));
+  P.exact = reinterpret_cast<double*>(take(8 * rows * P.slices));
+  P.tops = reinterpret_cast<float*>(take(4 * n));
+  P.came = reinterpret_cast<uint32_t*>(take(4 * uint64_t(a.B)));
+  return at;
 }
 
 }  // namespace
@@ -584,7 +733,7 @@ VOOM_API int voom_beam_select(const voom_beam_select_args* a, void* d_scratch, u
   if (cudaGetDevice(&dev) != cudaSuccess) return VOOM_E_CUDA;
   if (!(allowed.load(std::memory_order_relaxed) >> (dev & 63) & 1u)) {
     const auto allow = [](const void* kernel, int n) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, n) == cudaSuccess; };
-    if (!allow(reinterpret_cast<const void*>(beam_join), kMaxSort * 12) ||
+    if (!allow(reinterpret_cast<const void*>(beam_join), kMaxSort * kCandidate) ||
         !allow(reinterpret_cast<const void*>(beam_rows<__nv_bfloat16>), sizeof(RowShared)) ||
         !allow(reinterpret_cast<const void*>(beam_rows<__half>), sizeof(RowShared)) ||
         !allow(reinterpret_cast<const void*>(beam_rows<float>), sizeof(RowShared))) {
@@ -599,9 +748,9 @@ VOOM_API int voom_beam_select(const voom_beam_select_args* a, void* d_scratch, u
   if (cudaGetLastError() != cudaSuccess) return VOOM_E_CUDA;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute early{};
-  cfg.gridDim = dim3(a->B);
+  cfg.gridDim = dim3(a->B * P.slices);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = P.sorted * 12;
+  cfg.dynamicSmemBytes = P.sorted * kCandidate;
   cfg.stream = s;
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;

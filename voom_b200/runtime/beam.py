@@ -42,9 +42,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: int, *,
                 stream: torch.cuda.Stream | None = None) -> BeamChoice:
     """The `width` candidates with the largest score + log_softmax(logits) of each
     request.  logits: (B, beams, V) BF16, FP16 or FP32, a row's values adjacent,
-    any alignment; scores: (B, beams) fp32, the beams' sums so far.  Equal
-    candidates: the lower beam, then the lower token; compared in 64 bits.  A
-    logit of -inf is never chosen, nor is anything of a beam whose score is -inf
+    any alignment; scores: (B, beams) fp32, the beams' sums so far.  Compared in
+    64 bits; equal candidates: the lower beam, within one the larger logit, then
+    the lower token.  A logit of -inf is never chosen, nor is anything of a beam whose score is -inf
     (a first step has one beam alive; an ended one none) or that has a NaN or
     an infinite logit.  width <= 64: twice the beams, to set ended ones aside."""
     index = logits.get_device()
