@@ -782,7 +782,8 @@ int voom_kv_compact(const voom_kv_compact_args* a, void* d_scratch, uint64_t scr
  * score of -inf a beam, and a row with a NaN or an infinite logit has none.  The
  * scores are off by 1e-6 and their rounding at most, and in order as their 64-bit
  * values are: beams with candidates that are closer than 2e-6 have their sums made
- * again in 64 bits (two such beams of 200019 values: 38 us more).
+ * again in 64 bits (two such beams of 200019 values: 38 us more).  Tokens are best
+ * masked with -inf: a finite mask ties all along a row, which is read three times then.
  * d_parents: b * beams + i, d_tokens: t, d_scores_out rounded to fp32; where
  * there are fewer candidates: -1, -1, -inf.  width <= 64, beams <= 64,
  * beams * V < 2^31. */

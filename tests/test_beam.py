@@ -204,6 +204,43 @@ def test_more_candidates_than_are_put_in_order_by_counting():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows", [4, 592])
+def test_vocabularies_masked_with_the_lowest_value(dtype, rows):
+    """Fewer tokens allowed than wanted, the others at the type's lowest value: a tie as long as the row."""
+    from voom_b200.runtime.beam import beam_select
+
+    V, width = 128000, 16
+    r = torch.Generator().manual_seed(3)
+    row = torch.full((V,), torch.finfo(dtype).min, dtype=dtype)
+    allowed = torch.randperm(V, generator=r)[:5]
+    row[allowed] = torch.randn(5, generator=r).to(dtype)
+    want, parents, tokens = od.beam_select(row[None, None], torch.zeros((1, 1)), width)
+    got = beam_select(row.cuda().expand(rows, 1, V), torch.zeros((rows, 1), device="cuda"), width)
+    assert torch.equal(got.tokens.cpu(), tokens.expand(rows, width))
+    err = (got.scores.cpu().double() - want).abs() - STEP * want.abs()
+    assert bool((err <= 6e-7).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [1, 17, 64])
+def test_best_values_under_one_thread(width):
+    """More of a row's best than a block holds lie 256 apart: the last resort, one after another."""
+    from voom_b200.runtime.beam import beam_select
+
+    V = 400000
+    row = torch.zeros(V, dtype=torch.float32)
+    at = torch.arange(5, V, 256)
+    row[at] = 1.0 + torch.arange(at.numel()).float() / 2048
+    x = torch.stack((row, row.flip(0)))[:, None].contiguous().cuda()
+    compare(x, torch.full((2, 1), -0.5, device="cuda"), width)
+    big = row.cuda().expand(600, 1, V)  # a block to each row
+    got = beam_select(big, torch.zeros((600, 1), device="cuda"), width)
+    want = at.flip(0)[:width].to(torch.int32)
+    assert torch.equal(got.tokens.cpu(), want.expand(600, width))
+
+
+@pytest.mark.gpu
 def test_streams_graphs_and_repeats():
     from voom_b200.runtime.beam import beam_select
 

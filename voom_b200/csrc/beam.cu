@@ -168,15 +168,16 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 // 2^-n of a whole number n of at least 1.
 __device__ __forceinline__ float down2(float n) { return n < 126.0f ? __int_as_float((127 - int(n)) << 23) : 0.0f; }
 
+template <typename X>
 struct Bar {
-  float tops[kWarps][32];  // the warps' values, falling
-  float at;
+  X tops[kWarps][32];  // the warps' values, falling
+  X at;
 };
 
 struct RowShared {
   uint4 raw[kStages][kChunks][kThreads];  // a thread's values on their way; it reads its own alone
   float best[kSteps][kThreads];  // the groups' largest values
-  Bar bar;
+  Bar<float> bar;
   uint64_t found[kFound];        // entries that reached the bar
   uint32_t groups[kFound];       // step, thread
   uint64_t most[kWarps];
@@ -185,9 +186,14 @@ struct RowShared {
   uint32_t n_groups, n;
 };
 
+__device__ __forceinline__ float lane_xor(float x, uint32_t d) { return __shfl_xor_sync(0xFFFFFFFFu, x, d); }
+__device__ __forceinline__ uint64_t lane_xor(uint64_t x, uint32_t d) {
+  return uint64_t(__shfl_xor_sync(0xFFFFFFFFu, static_cast<unsigned long long>(x), d));
+}
+
 // The largest of the block's x; all threads call it.
 __device__ __forceinline__ uint64_t block_max(RowShared& sh, uint64_t x) {
-  for (int o = 16; o; o >>= 1) x = max(x, uint64_t(__shfl_xor_sync(0xFFFFFFFFu, static_cast<unsigned long long>(x), o)));
+  for (uint32_t o = 16; o; o >>= 1) x = max(x, lane_xor(x, o));
   __syncthreads();
   if ((threadIdx.x & 31u) == 0) sh.most[threadIdx.x >> 5] = x;
   __syncthreads();
@@ -197,15 +203,16 @@ __device__ __forceinline__ uint64_t block_max(RowShared& sh, uint64_t x) {
 
 // The width-th largest of the threads' values (of equal ones, each counts).  Every warp sorts its own; a value's rank among the others' is
 // found by halving.
-__device__ __forceinline__ float find_bar(Bar& sh, float y, uint32_t width) {
+template <typename X>
+__device__ __forceinline__ X find_bar(Bar<X>& sh, X y, uint32_t width) {
   const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
 #pragma unroll
   for (uint32_t k = 2; k <= 32; k <<= 1)
 #pragma unroll
     for (uint32_t d = k >> 1; d; d >>= 1) {
-      const float o = __shfl_xor_sync(0xFFFFFFFFu, y, d);
+      const X o = lane_xor(y, d);
       const bool up = (lane & k) != 0, low = (lane & d) == 0;  // falling where not up
-      y = low != up ? fmaxf(y, o) : fminf(y, o);
+      y = (low != up) == (y < o) ? o : y;
     }
   sh.tops[warp][lane] = y;
   __syncthreads();
@@ -216,11 +223,11 @@ __device__ __forceinline__ float find_bar(Bar& sh, float y, uint32_t width) {
     uint32_t at = 0;  // values of warp v that come before y
 #pragma unroll
     for (uint32_t d = 16; d; d >>= 1) {
-      const float o = sh.tops[v][at + d - 1];
+      const X o = sh.tops[v][at + d - 1];
       if (o > y || (o == y && v < warp)) at += d;
     }
     if (at == 31) {
-      const float o = sh.tops[v][31];
+      const X o = sh.tops[v][31];
       at += o > y || (o == y && v < warp);
     }
     rank += at;
@@ -354,30 +361,59 @@ __global__ void __launch_bounds__(kThreads, kPerSm) beam_rows(const __grid_const
     }
     __syncthreads();
   }
-  // the part's values, one after another
+  // the part's values once more (-inf for what is not the row's)
   auto each = [&](auto f) {
+    constexpr uint32_t kDeep = 8;
     const uint64_t t0 = uint64_t(first) * 32 * kChunks * VEC, t1 = uint64_t(last) * 32 * kChunks * VEC;
-    for (uint64_t at = t0 + tid; at < t1; at += kThreads) {
-      const uint32_t t = uint32_t(at) - skew;
-      if (t < V) f(t, value(x0[t]));
+    for (uint64_t at = t0 + tid; at < t1; at += kDeep * kThreads) {
+      float x[kDeep];
+#pragma unroll
+      for (uint32_t u = 0; u < kDeep; u++) {
+        const uint32_t t = uint32_t(at) + u * kThreads - skew;
+        x[u] = at + u * kThreads < t1 && t < V ? value(x0[t]) : -INFINITY;
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < kDeep; u++) f(uint32_t(at) + u * kThreads - skew, x[u]);
     }
   };
   many |= sh.n > kFound;
-  if (many) {  // values that tie, or lie under few threads: one after another, each the best after the last
-    uint64_t last_one = ~0ull;
-    uint32_t k = 0;
-    for (; k < width; k++) {
-      uint64_t mine = 0;
-      each([&](uint32_t t, float x) {
-        const uint64_t y = x > -INFINITY ? entry_of(x, t) : 0;
-        if (y < last_one) mine = max(mine, y);
-      });
-      last_one = block_max(sh, mine);
-      if (!last_one) break;
-      if (tid == 0) sh.found[k] = last_one;
-    }
-    if (tid == 0) sh.n = k;
+  if (many) {
+    // Values that tie, as a mask of the type's lowest value does wherever fewer than
+    // `width` tokens are left, or that lie under few threads.  The threads' best entries,
+    // every 256th token to one, give a bar that ties cannot crowd: 32 requests of 8 such
+    // beams over 200019 values, 16 wanted, 248 us a call (2390 one after another; without
+    // the mask 48, L2 flushed).
+    Bar<uint64_t>& bar = *reinterpret_cast<Bar<uint64_t>*>(sh.raw);
+    static_assert(sizeof(Bar<uint64_t>) <= sizeof(sh.raw), "nothing is on its way there any more");
+    auto entry = [&](uint32_t t, float x) { return x > -INFINITY ? entry_of(x, t) : 0; };
+    uint64_t most = 0;
+    each([&](uint32_t t, float x) { most = max(most, entry(t, x)); });
+    __syncthreads();  // sh.n and sh.raw are read
+    if (tid == 0) sh.n = 0;
+    const uint64_t reach = max(find_bar(bar, most, width), uint64_t(1));
+    each([&](uint32_t t, float x) {
+      const uint64_t y = entry(t, x);
+      if (y < reach) return;
+      const uint32_t at = atomicAdd(&sh.n, 1u);
+      if (at < kFound) sh.found[at] = y;
+    });
     __syncthreads();
+    if (sh.n > kFound) {  // the best under few threads again: one after another, each the best after the last
+      uint64_t last_one = ~0ull;
+      uint32_t k = 0;
+      for (; k < width; k++) {
+        uint64_t mine = 0;
+        each([&](uint32_t t, float x) {
+          const uint64_t y = entry(t, x);
+          if (y < last_one) mine = max(mine, y);
+        });
+        last_one = block_max(sh, mine);
+        if (!last_one) break;
+        if (tid == 0) sh.found[k] = last_one;
+      }
+      if (tid == 0) sh.n = k;
+      __syncthreads();
+    }
   }
   // the warps' sums
   float all = top;
@@ -455,7 +491,7 @@ struct JoinShared {
   double lse[kMaxBeams];  // NaN: the beam has no candidates
   double part[kWarps];
   float score[kMaxBeams], top[kMaxBeams];
-  Bar bar;
+  Bar<float> bar;
   uint32_t n;
   unsigned long long near;  // beams whose candidates are too close to others'
   uint32_t last;
