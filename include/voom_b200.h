@@ -704,8 +704,8 @@ int voom_kv_evict(const voom_kv_view* c, const voom_kv_evict_args* a, void* stre
 
 /* New tokens enter the cache: position d_len[b] + j of request b takes the keys
  * and values of its new token j, or d_index[b * m + j] if given (an entry outside
- * [0, n): nothing is written), j < m.  Positions past the view's pages, and
- * pages that are none, take nothing.  The lengths stay.  The view's keys and
+ * [0, n): nothing is written), j < m; max_len does not matter.  Positions past the
+ * view's pages, and pages that are none, take nothing.  The lengths stay.  The view's keys and
  * values are written although the view names them const; a cache whose rows
  * overlap one another, or the new tokens, is refused (VOOM_E_OVERLAP; pages
  * anywhere are checked page by page, not against one another).

@@ -103,6 +103,34 @@ def test_append_past_pages_and_bad_entries():
     assert torch.equal(k, want)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["whole", "pool"])
+def test_append_behind_a_view_s_bound(kind):
+    """lengths[b] + j is where a token goes, whatever the view's max_len: what is cached already stays."""
+    from voom_b200.runtime.kv_attention import KVView
+    from voom_b200.runtime.kv_pool import kv_append
+
+    k, v = (torch.zeros((2, 2, 40, 64), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    if kind == "whole":
+        view = KVView.contiguous(k, v, i32([10, 25]), max_len=10)
+    else:
+        k, v = (x.view(10, 2, 8, 64) for x in (k, v))
+        view = KVView.pool(k, v, i32([[0, 1, 2, 3, 4], [5, 6, 7, 8, 9]]), i32([10, 25]), max_len=10)
+
+    def rows():
+        y = k if kind == "whole" else k.view(2, 5, 2, 8, 64).transpose(1, 2).reshape(2, 2, 40, 64)
+        return y[:, 0, :, 0].float().cpu()
+
+    want = torch.zeros(2, 40)
+    for step in range(5):
+        x = torch.full((2, 4, 2, 64), step + 1.0, dtype=torch.bfloat16, device="cuda")
+        kv_append(view, x, x)
+        for b, at in ((0, 10 + 4 * step), (1, 25 + 4 * step)):
+            want[b, at:at + 4] = step + 1.0
+        assert torch.equal(rows(), want), step
+        view.lengths.add_(4)
+
+
 # ----------------------------------------------------------------------- fork
 
 def state(seed, *, rows, page, per, n_pages, ended=True):

@@ -71,7 +71,8 @@ __global__ void __launch_bounds__(256) kv_append(const __grid_constant__ Append 
   const uint32_t b = uint32_t(token / P.a.m), j = uint32_t(token - uint64_t(b) * P.a.m);
   if (b >= P.c.v.B || e >= chunks) return;
   const int32_t i = P.a.d_index ? P.a.d_index[token] : int32_t(j);
-  const uint64_t s = uint64_t(P.c.length(b)) + j;
+  // (not length(b): a view's max_len bounds what is read, and must not turn a write back to what is cached)
+  const uint64_t s = uint64_t(max(P.c.v.d_len[b], 0)) + j;
   int64_t ko, vo;
   if (uint32_t(i) >= P.a.n || s >= P.capacity || !P.c.row_at(b, 0, uint32_t(s), ko, vo)) return;
   const uint16_t* kn = static_cast<const uint16_t*>(P.a.d_kn) + int64_t(b) * P.a.kn_b + int64_t(i) * P.a.kn_t + 8 * e;

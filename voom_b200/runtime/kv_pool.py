@@ -46,8 +46,8 @@ def kv_append(cache: KVView, k: torch.Tensor, v: torch.Tensor, *, index: torch.T
     """Writes new tokens' k and v (B, n, heads, D) into the cache behind each
     request's positions: lengths[b] + j gets token j or, with `index` (B, m)
     int32, token index[b, j] (an accepted path of a drafted tree; an entry
-    outside [0, n) writes nothing).  Positions that the cache has no page for are
-    not written.  The lengths stay: every layer is written before they grow.
+    outside [0, n) writes nothing), whatever the view's max_len.  Positions that
+    the cache has no page for are not written.  The lengths stay: every layer is written before they grow.
     Rows that share the page they would write to must be forked first
     (fork_pages makes it theirs)."""
     if stream is not None or _device.current_index() != cache.index:
