@@ -160,3 +160,26 @@ def test_view_of_resident_pages_does_not_wait(tmp_path):
         tree_attention(q, k[:, :, :1].transpose(1, 2), k[:, :, :1].transpose(1, 2), tree, kv.view(0))
     finally:
         torch.cuda.set_sync_debug_mode(mode)
+
+
+@pytest.mark.gpu
+def test_a_view_that_holds_copies_is_not_written_to(tmp_path):
+    """kv_append to a cache's view would go into a copy of its open page: it is refused, and the cache stays as it is."""
+    from voom_b200.runtime.kv_attention import KVView
+    from voom_b200.runtime.kv_paged import PagedKVCache
+    from voom_b200.runtime.kv_pool import kv_append
+
+    k, v = (torch.randn((1, 2, 37, 64), device="cuda").bfloat16() for _ in range(2))
+    x = torch.randn((1, 3, 2, 64), device="cuda").bfloat16()
+    for n in (5, 32, 37):  # an open page alone, none, and both kinds
+        kv = PagedKVCache(1, 1 << 40, tmp_path, page_positions=16)
+        kv.append(0, k[:, :, :n], v[:, :, :n])
+        with pytest.raises(ValueError, match="append"):
+            kv_append(kv.view(0), x, x)
+        K, V = kv.update(0, x.transpose(1, 2), x.transpose(1, 2))
+        assert torch.equal(K[:, :, :n], k[:, :, :n]) and torch.equal(K[:, :, n:], x.transpose(1, 2))
+    # pages of the caller's own are written to
+    pages = [[(k[:, :, :16].clone(), v[:, :, :16].clone())]]
+    view = KVView.pages(pages, torch.tensor([4], dtype=torch.int32, device="cuda"))
+    kv_append(view, x, x)
+    assert torch.equal(pages[0][0][0][:, :, 4:7], x.transpose(1, 2))

@@ -62,12 +62,14 @@ class KVView:
     """Keys and values of B requests as the attention reads them; holds the
     tensors.  `lengths` is an int32 device tensor of the B requests' cached
     positions, read by the kernels when they run (it may change between
-    calls, and a captured graph sees the change); `max_len` bounds them."""
+    calls, and a captured graph sees the change); `max_len` bounds them.
+    `writable`: False where positions are copies that their owner does not look at
+    again (PagedKVCache.view): kv_append refuses such a view."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, *, batch: int, heads: int,
                  head_dim: int, page: int, strides: tuple, max_len: int, table: torch.Tensor | None = None,
                  offsets: torch.Tensor | None = None, table_stride: int = 0, n_pages: int = 0, keep: object = None,
-                 status: torch.Tensor | None = None):
+                 status: torch.Tensor | None = None, writable: bool = True):
         if k.dtype not in _CACHE_TYPES or v.dtype != k.dtype:
             raise ValueError(f"cached keys and values must both be BF16 or FP16, got {k.dtype} and {v.dtype}")
         if head_dim % 8 or not 0 < head_dim <= MAX_HEAD_DIM:
@@ -82,7 +84,7 @@ class KVView:
             raise ValueError(f"max_len {max_len} of a cache that holds {capacity} positions")
         self.k, self.v, self.lengths, self.table, self.offsets, self.keep = k, v, lengths, table, offsets, keep
         self.batch, self.heads, self.head_dim, self.max_len = batch, heads, head_dim, max_len
-        self.dtype = k.dtype
+        self.dtype, self.writable = k.dtype, writable
         self.struct = KvViewStruct(k.data_ptr(), v.data_ptr(), lengths.data_ptr(),
                                    None if table is None else table.data_ptr(),
                                    None if offsets is None else offsets.data_ptr(), *strides, batch, heads, head_dim,
@@ -126,7 +128,7 @@ class KVView:
 
     @classmethod
     def pages(cls, pages: list[list[tuple[torch.Tensor, torch.Tensor]]], lengths: torch.Tensor,
-              max_len: int | None = None, status: torch.Tensor | None = None) -> "KVView":
+              max_len: int | None = None, status: torch.Tensor | None = None, writable: bool = True) -> "KVView":
         """One list of (k, v) pages per request, each (1, heads, positions, D)
         or (heads, positions, D) with the same strides, anywhere on the device.
         Positions past a request's own pages read as zero keys and values.
@@ -157,7 +159,7 @@ class KVView:
         offsets = torch.from_numpy(off).pin_memory().to(k0.device, non_blocking=True)
         return cls(k0, v0, lengths, batch=len(pages), heads=H, head_dim=D, page=P, offsets=offsets, table_stride=per,
                    max_len=P * per if max_len is None else max_len, strides=(0, ks[0], ks[1], 0, vs[0], vs[1]),
-                   keep=flat, status=status)
+                   keep=flat, status=status, writable=writable)
 
     def check_status(self) -> None:
         """Raises RuntimeError if a wait inside an attention kernel ran out since

@@ -328,7 +328,9 @@ class PagedKVCache:
         """The layer's positions for kv_attention.tree_attention: pages are read
         where they are (spilled ones reloaded for the view's life), only the
         open page is copied, into a page of its own; update() would copy every
-        position instead.  The host waits for the device only to reload pages."""
+        position instead.  The host waits for the device only to reload pages.
+        For reading: kv_append refuses it, as the cache would not see what is
+        written to a copy; append() stores new positions."""
         from .kv_attention import KVView
 
         tail = self._tail_k[layer]
@@ -345,7 +347,7 @@ class PagedKVCache:
         if self._status is None or self._status.device != tail.device:
             self._status = torch.zeros(1, dtype=torch.int32, device=tail.device)
         length = torch.full((1,), n, dtype=torch.int32, device=tail.device)  # (a tensor from a list waits for the device)
-        return KVView.pages([pages], length, max_len=n, status=self._status)
+        return KVView.pages([pages], length, max_len=n, status=self._status, writable=False)
 
     def check_status(self) -> None:
         """Raises RuntimeError if a wait inside an attention kernel ran out, over

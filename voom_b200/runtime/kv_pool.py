@@ -49,7 +49,10 @@ def kv_append(cache: KVView, k: torch.Tensor, v: torch.Tensor, *, index: torch.T
     outside [0, n) writes nothing), whatever the view's max_len.  Positions that
     the cache has no page for are not written.  The lengths stay: every layer is written before they grow.
     Rows that share the page they would write to must be forked first
-    (fork_pages makes it theirs)."""
+    (fork_pages makes it theirs).  A PagedKVCache's view holds copies and is
+    refused: its own append() stores positions."""
+    if not cache.writable:
+        raise ValueError("this view holds copies of its cache's positions: what is written there would be lost; use the cache's append()")
     if stream is not None or _device.current_index() != cache.index:
         with _device.on_stream(cache.device, stream):
             return kv_append(cache, k, v, index=index)
