@@ -183,3 +183,40 @@ def test_a_view_that_holds_copies_is_not_written_to(tmp_path):
     view = KVView.pages(pages, torch.tensor([4], dtype=torch.int32, device="cuda"))
     kv_append(view, x, x)
     assert torch.equal(pages[0][0][0][:, :, 4:7], x.transpose(1, 2))
+
+
+@pytest.mark.gpu
+def test_slopes_and_windows_are_refused_after_an_eviction(tmp_path):
+    """An index is no position any more, and its distance would be wrong in silence; a cap does not ask for it."""
+    from voom_b200.runtime.kv_attention import DraftTree, KVView, kv_evict, tree_attention
+    from voom_b200.runtime.kv_paged import PagedKVCache
+
+    k, v = (torch.randn((1, 2, 40, 64), device="cuda").bfloat16() for _ in range(2))
+    x = torch.randn((1, 3, 8, 64), device="cuda").bfloat16()
+    args = (x[:, :, :4], x[:, :, 4:6], x[:, :, 6:])
+    tree = DraftTree.chain(1, 3, "cuda")
+    slopes = torch.rand(4, device="cuda")
+    kv = PagedKVCache(2, 1 << 40, tmp_path, page_positions=16)
+    for layer in range(2):
+        kv.append(layer, k, v)
+    w = torch.rand((1, 2, 40), device="cuda")
+    kv.evict(0, w, budget=64)  # keeps all: nothing moves
+    whole = KVView.contiguous(k, v, torch.tensor([40], dtype=torch.int32, device="cuda"))
+    for layer in range(2):
+        for kw in (dict(window=9), dict(slopes=slopes), dict(cap=9.0)):
+            assert torch.equal(tree_attention(*args, tree, kv.view(layer), **kw), tree_attention(*args, tree, whole, **kw))
+    kv.evict(0, w, budget=30, sinks=2, recent=4)
+    e = kv_evict(whole, w, budget=30, sinks=2, recent=4)
+    kept = KVView.contiguous(e.k, e.v, e.lengths, displaced=True)
+    for view in (kv.view(0), kept):
+        for kw in (dict(window=9), dict(slopes=slopes), dict(window=9, cap=5.0)):
+            with pytest.raises(ValueError, match="eviction"):
+                tree_attention(*args, tree, view, **kw)
+    assert torch.equal(tree_attention(*args, tree, kv.view(0), cap=9.0), tree_attention(*args, tree, kept, cap=9.0))
+    tree_attention(*args, tree, kv.view(1), window=9)  # the other layer has not been cut
+    kv.append(0, k, v)
+    with pytest.raises(ValueError, match="eviction"):
+        tree_attention(*args, tree, kv.view(0), window=9)
+    kv.release()
+    kv.append(0, k, v)
+    tree_attention(*args, tree, kv.view(0), window=9)

@@ -64,12 +64,14 @@ class KVView:
     positions, read by the kernels when they run (it may change between
     calls, and a captured graph sees the change); `max_len` bounds them.
     `writable`: False where positions are copies that their owner does not look at
-    again (PagedKVCache.view): kv_append refuses such a view."""
+    again (PagedKVCache.view): kv_append refuses such a view.  `displaced`: True where
+    a cached position's index is not its place in the sequence, as after an
+    eviction: tree_attention refuses slopes and windows there."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, *, batch: int, heads: int,
                  head_dim: int, page: int, strides: tuple, max_len: int, table: torch.Tensor | None = None,
                  offsets: torch.Tensor | None = None, table_stride: int = 0, n_pages: int = 0, keep: object = None,
-                 status: torch.Tensor | None = None, writable: bool = True):
+                 status: torch.Tensor | None = None, writable: bool = True, displaced: bool = False):
         if k.dtype not in _CACHE_TYPES or v.dtype != k.dtype:
             raise ValueError(f"cached keys and values must both be BF16 or FP16, got {k.dtype} and {v.dtype}")
         if head_dim % 8 or not 0 < head_dim <= MAX_HEAD_DIM:
@@ -84,7 +86,7 @@ class KVView:
             raise ValueError(f"max_len {max_len} of a cache that holds {capacity} positions")
         self.k, self.v, self.lengths, self.table, self.offsets, self.keep = k, v, lengths, table, offsets, keep
         self.batch, self.heads, self.head_dim, self.max_len = batch, heads, head_dim, max_len
-        self.dtype, self.writable = k.dtype, writable
+        self.dtype, self.writable, self.displaced = k.dtype, writable, displaced
         self.struct = KvViewStruct(k.data_ptr(), v.data_ptr(), lengths.data_ptr(),
                                    None if table is None else table.data_ptr(),
                                    None if offsets is None else offsets.data_ptr(), *strides, batch, heads, head_dim,
@@ -99,15 +101,17 @@ class KVView:
         self.lock = threading.Lock()  # a call's launches share the stream's workspace: they stay together
 
     @classmethod
-    def contiguous(cls, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, max_len: int | None = None) -> "KVView":
-        """k, v: (B, heads, capacity, D), any strides that keep rows on 16 bytes."""
+    def contiguous(cls, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, max_len: int | None = None, *,
+                   displaced: bool = False) -> "KVView":
+        """k, v: (B, heads, capacity, D), any strides that keep rows on 16 bytes.
+        `displaced`: True over what kv_evict has kept."""
         if k.dim() != 4 or v.shape != k.shape:
             raise ValueError(f"k and v: (B, heads, capacity, D) wanted, got {tuple(k.shape)} and {tuple(v.shape)}")
         _rows(k, "k")
         _rows(v, "v")
         B, H, cap, D = k.shape
         return cls(k, v, lengths, batch=B, heads=H, head_dim=D, page=cap, max_len=cap if max_len is None else max_len,
-                   strides=(*k.stride()[:3], *v.stride()[:3]))
+                   strides=(*k.stride()[:3], *v.stride()[:3]), displaced=displaced)
 
     @classmethod
     def pool(cls, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
@@ -128,7 +132,8 @@ class KVView:
 
     @classmethod
     def pages(cls, pages: list[list[tuple[torch.Tensor, torch.Tensor]]], lengths: torch.Tensor,
-              max_len: int | None = None, status: torch.Tensor | None = None, writable: bool = True) -> "KVView":
+              max_len: int | None = None, status: torch.Tensor | None = None, writable: bool = True,
+              displaced: bool = False) -> "KVView":
         """One list of (k, v) pages per request, each (1, heads, positions, D)
         or (heads, positions, D) with the same strides, anywhere on the device.
         Positions past a request's own pages read as zero keys and values.
@@ -159,7 +164,7 @@ class KVView:
         offsets = torch.from_numpy(off).pin_memory().to(k0.device, non_blocking=True)
         return cls(k0, v0, lengths, batch=len(pages), heads=H, head_dim=D, page=P, offsets=offsets, table_stride=per,
                    max_len=P * per if max_len is None else max_len, strides=(0, ks[0], ks[1], 0, vs[0], vs[1]),
-                   keep=flat, status=status, writable=writable)
+                   keep=flat, status=status, writable=writable, displaced=displaced)
 
     def check_status(self) -> None:
         """Raises RuntimeError if a wait inside an attention kernel ran out since
@@ -265,7 +270,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: Draf
     slopes[h] (p_k - p_q) is added to it, after the cap; with `window` a row sees
     only positions with p_q - p_k < window, itself among them (its tiles before
     are not read).  A cached position is its index, a new token's lengths[b] + its
-    depth in the tree.
+    depth in the tree: after an eviction that is not their distance, and a view that
+    says so (KVView.displaced, PagedKVCache.view) is refused with slopes or a window.
 
     `weights` (B, heads, >= max_len + n) fp32: each position's softmax weight,
     summed over the rows that share its head (each times `token_weight` (B, n)
@@ -312,8 +318,11 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: Draf
         if slopes.shape != (hq,) or slopes.dtype != torch.float32 or not slopes.is_contiguous() or slopes.get_device() != cache.index:
             raise ValueError(f"slopes: contiguous fp32 ({hq},) on {cache.device} wanted, got {tuple(slopes.shape)} {slopes.dtype}")
         sl = slopes.data_ptr()
-    if tree.mask_ptr and (slopes is not None or window is not None):
-        depth = tree.depth.data_ptr()
+    if slopes is not None or window is not None:
+        if cache.displaced:
+            raise ValueError("slopes and windows go by positions, and an eviction has moved this cache's")
+        if tree.mask_ptr:
+            depth = tree.depth.data_ptr()
     if out is None:
         out = q.new_empty((B, n, hq, D))
     os = _new(out, "out", B, n, hq, cache)

@@ -347,7 +347,8 @@ class PagedKVCache:
         if self._status is None or self._status.device != tail.device:
             self._status = torch.zeros(1, dtype=torch.int32, device=tail.device)
         length = torch.full((1,), n, dtype=torch.int32, device=tail.device)  # (a tensor from a list waits for the device)
-        return KVView.pages([pages], length, max_len=n, status=self._status, writable=False)
+        return KVView.pages([pages], length, max_len=n, status=self._status, writable=False,
+                             displaced=self._cut[layer])
 
     def check_status(self) -> None:
         """Raises RuntimeError if a wait inside an attention kernel ran out, over
@@ -374,6 +375,7 @@ class PagedKVCache:
         self._pages[layer] = []
         self._tail_k[layer] = self._tail_v[layer] = None
         m = min(n, budget)
+        self._cut[layer] |= m < n  # positions are not their indexes any more
         # closed pages are copies already; a tail alone must be one too, as the caller has e
         k, v = (x[:, :, :m] if m >= self.page_positions else _piece(x, 0, m) for x in (e.k, e.v))
         self._extend(layer, k, v)
@@ -417,6 +419,7 @@ class PagedKVCache:
     def _reset(self) -> None:
         self._pages = [[] for _ in range(self.num_layers)]
         self._tail_k = [None] * self.num_layers
+        self._cut = [False] * self.num_layers
         self._tail_v = [None] * self.num_layers
         self._offset = 0
 
