@@ -576,6 +576,68 @@ def test_a_row_that_is_full_says_so():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("pages,fail_at", [(40, 0), (40, 1), (40, 2), (9, 0), (9, 1), (9, 2)])
+def test_a_resize_that_runs_out_leaves_the_pool_usable(pages, fail_at, monkeypatch):
+    from voom_b200.runtime.kv_pool import PagePool
+
+    def fill(pool, n, x):
+        pool.fork(grow=n)
+        for layer in range(2):
+            pool.append(layer, x, 2 * x)
+        pool.advance(n)
+
+    def read(pool):
+        t = pool.table[:, :2].long()
+        return [y[:, t].transpose(2, 3).reshape(2, 2, 2, 16, 64)[..., :11, :].clone() for y in (pool.k, pool.v)]
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    pool = PagePool(2, 2, 64, pages=20, rows=2, max_len=32, page=8)
+    fill(pool, 11, torch.randn((2, 11, 2, 64), device="cuda", generator=g).bfloat16())
+    want = read(pool)
+    plain, calls = torch.Tensor.new_empty, []
+
+    def new_empty(self, size, *a, **kw):  # only what resize asks for
+        if isinstance(size, tuple) and len(size) == 5:
+            calls.append(tuple(size))
+            if len(calls) == fail_at + 1:
+                raise torch.OutOfMemoryError("no memory for a test")
+        return plain(self, size, *a, **kw)
+
+    monkeypatch.setattr(torch.Tensor, "new_empty", new_empty)
+    if fail_at < 2:
+        with pytest.raises(torch.OutOfMemoryError):
+            pool.resize(pages)
+    else:
+        pool.resize(pages)
+    monkeypatch.undo()
+    assert pool.k.shape == pool.v.shape and pool.refs.shape == (pool.pages,) and pool.pages >= 4
+    assert all(pool.view(i).k.data_ptr() == pool.k[i].data_ptr() and pool.view(i).v.data_ptr() == pool.v[i].data_ptr() for i in range(2))
+    assert all(torch.equal(a, b) for a, b in zip(read(pool), want))
+    x = torch.randn((2, 3, 2, 64), device="cuda", generator=g).bfloat16()
+    fill(pool, 3, x)
+    pool.check_status()
+    assert pool.lengths.tolist() == [14, 14]
+    assert all(torch.equal(a, b) for a, b in zip(read(pool), want))
+    pool.resize(12)
+    assert pool.pages == 12 and all(torch.equal(a, b) for a, b in zip(read(pool), want))
+
+
+@pytest.mark.gpu
+def test_resize_holds_one_old_and_one_new_piece_at_a_time():
+    from voom_b200.runtime.kv_pool import PagePool
+
+    pool = PagePool(1, 8, 128, pages=4000, rows=2, max_len=128, page=64)  # 524 MB of keys, as much of values
+    pool.fork(grow=70)
+    one = pool.k.numel() * 2
+    torch.cuda.synchronize()
+    was = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    pool.resize(3600)
+    assert torch.cuda.max_memory_allocated() - was < one
+    assert torch.cuda.memory_allocated() - was < -0.15 * one
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [1, 9])
 def test_pages_past_32_bits(n):
     """A pool of more than 2^32 bytes and 2^31 values: its last pages are written, forked, read and moved as its first are."""

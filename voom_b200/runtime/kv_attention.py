@@ -115,10 +115,10 @@ class KVView:
 
     @classmethod
     def pool(cls, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
-             max_len: int | None = None) -> "KVView":
+             max_len: int | None = None, status: torch.Tensor | None = None) -> "KVView":
         """k, v: (pages, heads, positions, D); table: (B, pages per request)
         int32, the pool page of each run of positions.  A table entry outside
-        the pool reads as zero keys and values."""
+        the pool reads as zero keys and values.  `status`: as in `pages`."""
         if k.dim() != 4 or v.shape != k.shape:
             raise ValueError(f"k and v: (pages, heads, positions, D) wanted, got {tuple(k.shape)} and {tuple(v.shape)}")
         if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous() or table.device != k.device:
@@ -128,7 +128,7 @@ class KVView:
         N, H, P, D = k.shape
         B, per = table.shape
         return cls(k, v, lengths, batch=B, heads=H, head_dim=D, page=P, table=table, table_stride=per, n_pages=N,
-                   max_len=P * per if max_len is None else max_len, strides=(*k.stride()[:3], *v.stride()[:3]))
+                   max_len=P * per if max_len is None else max_len, strides=(*k.stride()[:3], *v.stride()[:3]), status=status)
 
     @classmethod
     def pages(cls, pages: list[list[tuple[torch.Tensor, torch.Tensor]]], lengths: torch.Tensor,

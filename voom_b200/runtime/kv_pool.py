@@ -253,7 +253,8 @@ class PagePool:
     and append()s its new tokens, advance(n) counts them.  The table and the
     lengths keep their addresses, so a captured step stays valid (but for resize).
     Pages that a row does not hold (rows that never grew, or ended) read as zeros.
-    `refs` says how many rows held each page after the last fork."""
+    `refs` says how many rows held each page after the last fork, by the page
+    numbers of that time: compact and resize change them, the next fork counts anew."""
 
     def __init__(self, layers: int, heads: int, head_dim: int, *, pages: int, rows: int, max_len: int, page: int = 64,
                  dtype: torch.dtype = torch.bfloat16, device=None):
@@ -273,10 +274,8 @@ class PagePool:
         self._make_views()
 
     def _make_views(self) -> None:
-        self._views = [KVView.pool(k, v, self.table, self.lengths, max_len=self.max_len)
+        self._views = [KVView.pool(k, v, self.table, self.lengths, max_len=self.max_len, status=self._wait_status)
                        for k, v in zip(self.k.unbind(0), self.v.unbind(0))]
-        for view in self._views:
-            view.status, view.status_ptr = self._wait_status, self._wait_status.data_ptr()
         # fork's arguments but for those that change from call to call
         self._index, *sizes, strides = _pool(self.k, self.v, self.table, self.lengths)
         at = [x.data_ptr() for x in (self.k, self.v, self.table, self.lengths, self.table, self.lengths, self.refs, self.missing)]
@@ -326,21 +325,32 @@ class PagePool:
 
     def resize(self, pages: int) -> None:
         """Compacts the pool and gives it `pages` pages, those in use at least.
-        Synchronises; views taken before are not valid any more."""
+        Synchronises; views taken before are not valid any more, and hold the old
+        memory for as long as they live.  Beside the pool it needs room for the new
+        keys, then for the new values.  Where that is not to be had the error goes
+        on to the caller and the pool stays usable: it keeps its pages, or (where
+        the values of a smaller one had no room) the fewer that were asked for."""
         live = int(self.compact().item())
         if pages < max(live, 1):
             raise ValueError(f"{live} pages are in use, {pages} do not hold them")
-        keep = min(live, pages)
+        refs = self.refs.new_zeros(pages)
 
         def moved(x):
             y = x.new_empty((x.shape[0], pages, *x.shape[2:]))
-            y[:, :keep] = x[:, :keep]
+            y[:, :live] = x[:, :live]
             return y
 
-        self.k = moved(self.k)  # one at a time: the old keys are given back before the values are copied
-        self.v = moved(self.v)
-        self.refs = self.refs.new_zeros(pages)
-        self._make_views()
+        with self._lock:
+            self._views = []  # they hold the old keys and values: these are given back one after the other
+            try:
+                self.k = moved(self.k)
+                self.v = moved(self.v)
+            finally:
+                if self.k.shape != self.v.shape:  # the values had no room: both hold this many
+                    n = min(self.k.shape[1], self.v.shape[1])
+                    self.k, self.v = self.k[:, :n], self.v[:, :n]
+                self.refs = refs if self.pages == pages else self.refs[:self.pages]
+                self._make_views()
 
     def check_status(self) -> None:
         """Raises RuntimeError if pages were missing in a fork since the last
