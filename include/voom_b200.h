@@ -759,7 +759,8 @@ int voom_kv_fork(const voom_kv_fork_args* a, void* d_scratch, uint64_t scratch_b
  * move to the front of the pool: with L of them, the i-th one past L, in the
  * pool's order, goes to the i-th page below L that no row holds, in all layers.
  * The table follows (entries past a row's pages, and outside the pool: -1);
- * d_live = L.  d_table_out may be d_table. */
+ * d_live = L.  d_table_out may be d_table.  room: not 0 where a row also holds the
+ * pages that its other entries name, as a fork leaves them for positions to come. */
 typedef struct voom_kv_compact_args {
   void* d_k; /* as above */
   void* d_v;
@@ -768,7 +769,7 @@ typedef struct voom_kv_compact_args {
   int32_t* d_table_out;
   int32_t* d_live;
   int64_t k_layer, k_page, k_head, k_pos, v_layer, v_page, v_head, v_pos;
-  uint32_t layers, n_pages, hk, page, D, rows, per, pad;
+  uint32_t layers, n_pages, hk, page, D, rows, per, room;
 } voom_kv_compact_args;
 uint64_t voom_kv_compact_scratch_bytes(uint32_t n_pages);
 int voom_kv_compact(const voom_kv_compact_args* a, void* d_scratch, uint64_t scratch_bytes, void* stream);

@@ -638,6 +638,39 @@ def test_resize_holds_one_old_and_one_new_piece_at_a_time():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("how", ["compact", "resize"])
+def test_room_outlasts_compaction(how):
+    """Room that a fork made and nothing has filled yet is still there afterwards: what is appended then is written."""
+    from voom_b200.runtime.kv_pool import PagePool
+
+    pool = PagePool(2, 1, 64, pages=30, rows=4, max_len=64, page=8)
+    pool.fork(grow=i32([20, 3, 9, 8]))
+    x = torch.randn((4, 20, 1, 64), device="cuda").bfloat16()
+    for layer in range(2):
+        pool.append(layer, x, x)
+    pool.advance(i32([20, 3, 9, 8]))
+    pool.fork(i32([-1, 1, 2, 3]), grow=13)  # row 0's pages are free: there are holes
+    live = -(-16 // 8) + -(-22 // 8) + -(-21 // 8)
+    if how == "compact":
+        assert pool.compact().tolist() == [live]
+    else:
+        with pytest.raises(ValueError, match="in use"):
+            pool.resize(live - 1)
+        pool.resize(live)
+    y = torch.randn((4, 13, 1, 64), device="cuda").bfloat16()
+    for layer in range(2):
+        pool.append(layer, y, 2 * y)
+    pool.advance(i32([0, 13, 13, 13]))
+    pool.check_status()
+    for r, n in ((1, 3), (2, 9), (3, 8)):
+        t = pool.table[r, :-(-(n + 13) // 8)].long()
+        assert bool((t >= 0).all()) and bool((t < live).all())
+        for layer in range(2):
+            k, v = (p[layer, t, 0].reshape(-1, 64)[:n + 13] for p in (pool.k, pool.v))
+            assert torch.equal(k[:n], x[r, :n, 0]) and torch.equal(k[n:], y[r, :, 0]) and torch.equal(v[n:], 2 * y[r, :, 0])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [1, 9])
 def test_pages_past_32_bits(n):
     """A pool of more than 2^32 bytes and 2^31 values: its last pages are written, forked, read and moved as its first are."""

@@ -119,7 +119,7 @@ class KvForkArgs(ctypes.Structure):
 
 class KvCompactArgs(ctypes.Structure):
     _fields_ = _fields("p: k v table lengths table_out live", "i64: k_layer k_page k_head k_pos v_layer v_page v_head v_pos",
-                       "u32: layers n_pages hk page D rows per pad")
+                       "u32: layers n_pages hk page D rows per room")
 
 
 class BeamSelectArgs(ctypes.Structure):

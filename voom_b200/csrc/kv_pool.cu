@@ -412,7 +412,7 @@ struct Compact {
 
 __device__ __forceinline__ int32_t held_page(const Compact& P, uint32_t r, uint32_t j) {
   const uint32_t len = clamped_length(P.a.d_lengths, r, uint64_t(P.a.per) * P.a.page);
-  if (uint64_t(j) * P.a.page >= len) return -1;
+  if (uint64_t(j) * P.a.page >= len && !P.a.room) return -1;
   const int32_t t = P.a.d_table[uint64_t(r) * P.a.per + j];
   return uint32_t(t) < P.a.n_pages ? t : -1;
 }

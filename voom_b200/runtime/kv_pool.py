@@ -219,15 +219,16 @@ class Compacted(NamedTuple):
     live: torch.Tensor
 
 
-def compact_pages(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *, out: Compacted | None = None,
-                  stream: torch.cuda.Stream | None = None) -> Compacted:
+def compact_pages(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *, room: bool = False,
+                  out: Compacted | None = None, stream: torch.cuda.Stream | None = None) -> Compacted:
     """Moves the pages that the rows hold to the front of the pool, in all layers:
-    pages past their number go, in order, to the free ones below it.  `out.table`
-    may be `table` itself."""
+    pages past their number go, in order, to the free ones below it.  `room`: a row
+    holds the pages past its length too, which a fork has made ready; else they are
+    let go.  `out.table` may be `table` itself."""
     index, L, N, H, P, D, R, per, strides = _pool(k, v, table, lengths)
     if stream is not None or _device.current_index() != index:
         with _device.on_stream(k.device, stream):
-            return compact_pages(k, v, table, lengths, out=out)
+            return compact_pages(k, v, table, lengths, room=room, out=out)
     words = _compact_words(N)
     if out is None:
         ws, new, live = table.new_empty(words + R * per + 1).split_with_sizes((words, R * per, 1))
@@ -241,7 +242,7 @@ def compact_pages(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths
         _apart((out.live, out.table), [lengths] if same else [lengths, table], False)
         ws = table.new_empty(words)
     a = _COMPACT.pack(k.data_ptr(), v.data_ptr(), table.data_ptr(), lengths.data_ptr(), out.table.data_ptr(), out.live.data_ptr(),
-                      *strides, L, N, H, P, D, R, per, 0)
+                      *strides, L, N, H, P, D, R, per, room)
     _refused(load().voom_kv_compact(a, ws.data_ptr(), 4 * words, _device.raw_stream(index)), "voom_kv_compact")
     return out
 
@@ -306,7 +307,8 @@ class PagePool:
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, *, index: torch.Tensor | None = None,
                stream: torch.cuda.Stream | None = None) -> None:
-        """kv_append to one layer, into room that fork(grow=..) has made."""
+        """kv_append to one layer, into room that the last fork has made with grow=..;
+        what there is no room for is not written."""
         kv_append(self._views[layer], k, v, index=index, stream=stream)
 
     def advance(self, n: int | torch.Tensor) -> None:
@@ -316,12 +318,14 @@ class PagePool:
         self.lengths.add_(n).clamp_(0, self.max_len)
 
     def compact(self, *, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
-        """compact_pages in place; the number of pages in use, on the device."""
+        """compact_pages in place; the number of pages in use, on the device.  Room
+        that the last fork made and nothing has filled yet stays."""
         if stream is not None or _device.current_index() != self._index:
             with _device.on_stream(self.k.device, stream):
                 return self.compact()
         with self._lock:
-            return compact_pages(self.k, self.v, self.table, self.lengths, out=Compacted(self.table, self.table.new_empty(1))).live
+            return compact_pages(self.k, self.v, self.table, self.lengths, room=True,
+                                 out=Compacted(self.table, self.table.new_empty(1))).live
 
     def resize(self, pages: int) -> None:
         """Compacts the pool and gives it `pages` pages, those in use at least.
