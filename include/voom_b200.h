@@ -730,8 +730,10 @@ int voom_kv_append(const voom_kv_view* c, const voom_kv_append_args* a, void* st
  *   - fresh pages for the positions past the open page.
  * Fresh pages are those that no row holds any more, the lowest first, given out in
  * the order of rows and positions; those that are not to be had, or that a table
- * row has no room for, are counted in d_missing and their entries are -1.  Entries
- * past the pages of length + grow are -1, and so are entries outside the pool.
+ * row has no room for, are counted in d_missing and their entries are -1.  An open
+ * page that found no copy stays the row's, as page - 2^31: no page to whoever reads or
+ * appends, but the next fork takes it for the page that it is, and copies it then.
+ * Entries past the pages of length + grow are -1, and so are entries outside the pool.
  * d_refs counts each page's rows in the new table.  d_table_out / d_lengths_out
  * may be d_table / d_lengths (both or neither).  A row names a page once.
  * page <= 32768, rows <= 65535.  Nothing depends on scheduling.

@@ -62,12 +62,18 @@ def beam_select(logits, scores, width):
     return best, parents, tokens
 
 
+def page_in(x, n_pages):
+    """The page that an entry names; as page - 2^31 its row holds it, but cannot use it.  -1: none."""
+    x &= 2 ** 31 - 1
+    return x if x < n_pages else -1
+
+
 def held(table, lengths, page, n_pages):
     """Each row's pages: the first ceil(length / page) entries, -1 where an entry is no page."""
     rows = []
     for t, n in zip(table, lengths):
         n = max(0, min(n, len(t) * page))
-        rows.append([x if 0 <= x < n_pages else -1 for x in t[:-(-n // page)]])
+        rows.append([page_in(x, n_pages) for x in t[:-(-n // page)]])
     return rows
 
 
@@ -108,12 +114,12 @@ def fork(table, lengths, parents, grow, page, n_pages):
     missing += sum(x < 0 for x in given)
     out = [t + [-1] * (per - len(t)) for t in rows]
     for (r, j), x in zip(wanted, given):
-        out[r][j] = x
+        out[r][j] = x if x >= 0 or out[r][j] < 0 else out[r][j] - 2 ** 31  # (an open page that found no copy)
     refs = [0] * n_pages
     for t in out:
         for x in t:
-            if x >= 0:
-                refs[x] += 1
+            if page_in(x, n_pages) >= 0:
+                refs[page_in(x, n_pages)] += 1
     return out, new_len, refs, missing, [(a, given[i], m) for a, _, m, i in copies if given[i] >= 0]
 
 
@@ -124,4 +130,6 @@ def compact(table, lengths, page, n_pages):
     live = sorted({x for t in rows for x in t if x >= 0})
     count = len(live)
     moves = dict(zip([x for x in live if x >= count], [x for x in range(count) if x not in set(live)]))
-    return [[moves.get(x, x) for x in t] + [-1] * (per - len(t)) for t in rows], count, sorted(moves.items())
+    new = [[moves.get(x, x) - (2 ** 31 if x >= 0 and was < 0 else 0) for x, was in zip(t, old)] + [-1] * (per - len(t))
+           for t, old in zip(rows, table)]
+    return new, count, sorted(moves.items())

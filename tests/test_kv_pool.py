@@ -218,6 +218,94 @@ def test_fork_finds_every_case():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("in_place", [False, True])
+def test_an_open_page_that_finds_no_copy_is_kept(in_place):
+    """Too few pages for the copies: the rows hold their open pages still, marked, until a fork has pages for them."""
+    P, N = 4, 5
+    shared = [[0, 1, -1]] * 4  # four rows with an open page, two pages left for three copies
+    t, n, missing, copies = check_fork(shared, [6] * 4, [0, 1, 2, 3], [1] * 4, P, N, in_place=in_place)
+    assert t == [[0, 1, -1], [0, 2, -1], [0, 3, -1], [0, 4, -1]] and not missing
+    t, n, missing, copies = check_fork(shared, [6] * 4, [0, 1, 2, 3], [3] * 4, P, N, in_place=in_place)
+    assert t == [[0, 1, 2], [0, 3, 4], [0, 1 - 2 ** 31, -1], [0, 1 - 2 ** 31, -1]] and missing == 4 and len(copies) == 1
+    again, _, missing, copies = check_fork(t, n, [0, 1, 2, 3], [1] * 4, P, 8, in_place=in_place)  # three pages more
+    assert again == [[0, 1, -1], [0, 3, -1], [0, 2, -1], [0, 4, -1]] and not missing and len(copies) == 2
+    # the others end: the page is the row's own, nothing is copied
+    again, _, missing, copies = check_fork(t, n, [-1, -1, -1, 3], [1] * 4, P, N, in_place=in_place)
+    assert again[3] == [0, 1, -1] and not missing and not copies
+    # no growth: it reads as the page that it is
+    again, _, missing, copies = check_fork(t, n, [0, 1, 2, 3], [0] * 4, P, N, in_place=in_place)
+    assert again[2] == again[3] == [0, 1, -1]
+    check_fork([[0, -2 ** 31 + 9, 2], [-2 ** 31, 3, -1]], [9, 5], [0, 1], [1, 1], P, N, in_place=in_place)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(6))
+def test_forks_with_too_few_pages(seed):
+    """Rows that all share and all grow over pools of a few pages, then forks and compactions of what that leaves."""
+    from voom_b200.runtime import kv_pool
+
+    rows, page, per = ((4, 16, 6), (9, 5, 11), (33, 4, 9))[seed % 3]
+    table, lengths, r = state(seed, rows=rows, page=page, per=per, n_pages=rows * per)
+    n_pages = max(max(x for t in table for x in t) + 1, 1)
+    for again in range(4):
+        parents = [r.randrange(-1, rows) for _ in range(rows)]
+        grow = [r.choice((0, 1, 1, page)) for _ in range(rows)]
+        table, lengths, _, _ = check_fork(table, lengths, parents, grow, page, n_pages, in_place=bool(seed & 1))
+        k, v = (torch.zeros((1, n_pages, 1, page, 8), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        for room in (False, True):
+            counted = [per * page] * rows if room else lengths
+            want, live, _ = od.compact(table, counted, page, n_pages)
+            got = kv_pool.compact_pages(k, v, i32(table), i32(lengths), room=room)
+            assert got.table.tolist() == want and got.live.tolist() == [live]
+
+
+@pytest.mark.gpu
+def test_a_large_table_with_too_few_pages():
+    """More entries than one block forks: rows in fives share two pages, and two copies of every three wanted are to be had."""
+    rows, page, per = 1000, 4, 9
+    table = [[2 * (i // 5), 2 * (i // 5) + 1] + [-1] * 7 for i in range(rows)]
+    n_pages = 400 + 500
+    t, n, missing, _ = check_fork(table, [6] * rows, list(range(rows)), [1] * rows, page, n_pages, layers=1, H=1, D=8)
+    assert missing == 300 and sum(x < -1 for r in t for x in r) == 300
+    check_fork(t, n, list(range(rows)), [1] * rows, page, n_pages + 300, layers=1, H=1, D=8, in_place=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("compact", [False, True])
+def test_a_pool_that_ran_out_goes_on_after_a_resize(compact):
+    from voom_b200.runtime.kv_pool import PagePool
+
+    pool = PagePool(2, 1, 64, pages=4, rows=3, max_len=32, page=8)
+    pool.fork(grow=i32([12, 0, 0]))
+    x = torch.randn((1, 12, 1, 64), device="cuda").bfloat16().expand(3, -1, -1, -1)
+    for layer in range(2):
+        pool.append(layer, x, 2 * x)
+    pool.advance(i32([12, 0, 0]))
+    pool.fork(i32([0, 0, 0]))
+    pool.fork(grow=6)  # the first row's next page, then two copies and two pages behind them: two are left
+    with pytest.raises(RuntimeError, match="3 too few"):
+        pool.check_status()
+    held = pool.refs.tolist()
+    assert held[:2] == [3, 2] and pool.lengths.tolist() == [12] * 3
+    if compact:
+        pool.compact()
+    pool.resize(8)
+    pool.fork(grow=6)
+    y = torch.randn((3, 6, 1, 64), device="cuda").bfloat16()
+    for layer in range(2):
+        pool.append(layer, y, 2 * y)
+    pool.advance(6)
+    pool.check_status()
+    for r in range(3):
+        t = pool.table[r, :3].long()
+        assert bool((t >= 0).all())
+        for layer in range(2):
+            k, v = (p[layer, t, 0].reshape(-1, 64)[:18] for p in (pool.k, pool.v))
+            want = torch.cat((x[r, :, 0], y[r, :, 0]))
+            assert torch.equal(k, want) and torch.equal(v, 2 * want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,per,page,n_pages", [(1, 1, 32768, 3), (700, 3, 2, 2500), (5, 600, 16, 9000), (1500, 40, 16, 70001)])
 def test_fork_large(rows, per, page, n_pages):
     r = random.Random(rows)

@@ -55,6 +55,15 @@ int launch_early(void (*kernel)(A...), dim3 grid, uint32_t threads, cudaStream_t
   return VOOM_E_CUDA;
 }
 
+// A table entry may be a page that its row holds but cannot use: an open one whose copy
+// found no fresh page.  It stands as page - 2^31, which no reader or writer takes for a
+// page; the next fork takes it for the page that it is.
+constexpr uint32_t kUnusable = 0x80000000u;
+__device__ __forceinline__ int32_t page_in(int32_t entry, uint32_t n_pages) {
+  const uint32_t t = uint32_t(entry) & ~kUnusable;
+  return t < n_pages ? int32_t(t) : -1;
+}
+
 // ------------------------------------------------------------------- append
 struct Append {
   voom::kv::View c;
@@ -108,7 +117,8 @@ struct Fork {
   uint32_t* count;  // n_pages, 0 at first
   uint32_t* owner;  // n_pages, 0 at first: (filled positions, then the first row) of its open holders, the largest
   uint32_t* words;  // free pages, copies
-  uint4* rows;      // rows: rank of the row's first fresh page, its place in the row, and the place behind the last one
+  uint4* rows;      // rows: rank of the row's first fresh page, its place in the row, the place behind the last one, and
+                    // whether the first replaces an open page
   CopyItem* copies; // rows
   int32_t* fresh;   // free pages in order, as many as are wanted
   int32_t* table;   // the new table and lengths: the caller's, or scratch where those are still read
@@ -155,10 +165,7 @@ __device__ __forceinline__ uint32_t taken_length(const Fork& P, uint32_t r, uint
 __device__ __forceinline__ int32_t take_entry(const Fork& P, uint32_t r, uint32_t j, uint32_t p, uint32_t len, uint32_t* count,
                                            uint32_t* owner) {
   int32_t t = -1;
-  if (uint64_t(j) * P.a.page < len) {
-    t = P.a.d_table[uint64_t(p) * P.a.per + j];
-    if (uint32_t(t) >= P.a.n_pages) t = -1;
-  }
+  if (uint64_t(j) * P.a.page < len) t = page_in(P.a.d_table[uint64_t(p) * P.a.per + j], P.a.n_pages);
   P.table[uint64_t(r) * P.a.per + j] = t;
   if (t < 0) return t;
   const uint32_t fill = len - j * P.a.page;
@@ -291,7 +298,7 @@ __device__ __forceinline__ void plan_fork(const Fork& P, uint32_t* count, const 
     uint64_t total;
     const uint64_t at = all + block_before(uint64_t(copy) << 32 | need, s_warp, total);
     if (r < P.a.rows) {
-      P.rows[r] = make_uint4(uint32_t(at), first, want, 0u);
+      P.rows[r] = make_uint4(uint32_t(at), first, want, uint32_t(copy));
       if (copy) P.copies[at >> 32] = CopyItem{src, uint32_t(at), fill};
     }
     all += total;
@@ -304,6 +311,11 @@ __device__ __forceinline__ void plan_fork(const Fork& P, uint32_t* count, const 
         if (none && rank < wanted) P.fresh[rank] = int32_t(p);
         P.a.d_refs[p] = none ? (rank < wanted ? 1 : 0) : int32_t((c & 0xFFFFu) + (c >> 16));
       });
+  if (free < wanted) {  // rows whose open page has no copy hold it still
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < uint32_t(all >> 32); i += kPlanThreads)
+      if (P.copies[i].rank >= free) atomicAdd(&P.a.d_refs[P.copies[i].src], 1);
+  }
   if (threadIdx.x == 0) {
     const uint32_t lost = s_lost + (wanted > free ? wanted - free : 0u);
     *P.a.d_missing = int32_t(lost + (P.a.add_missing ? uint32_t(*P.a.d_missing) : 0u));
@@ -388,7 +400,10 @@ __global__ void __launch_bounds__(256) fork_finish(const __grid_constant__ Fork 
     int32_t* to = P.a.d_table_out + uint64_t(r) * P.a.per;
     for (uint32_t j = (back ? 0u : fresh.y) + threadIdx.x; j < (back ? P.a.per : want); j += 256) {
       const uint32_t rank = fresh.x + (j - fresh.y);
-      to[j] = j < fresh.y || j >= want ? from[j] : rank < free ? P.fresh[rank] : -1;
+      to[j] = j < fresh.y || j >= want ? from[j]
+              : rank < free            ? P.fresh[rank]
+              : fresh.w && j == fresh.y ? int32_t(uint32_t(from[j]) | kUnusable)
+                                        : -1;
     }
     if (back && threadIdx.x == 0) P.a.d_lengths_out[r] = P.lengths[r];
   }
@@ -413,8 +428,7 @@ struct Compact {
 __device__ __forceinline__ int32_t held_page(const Compact& P, uint32_t r, uint32_t j) {
   const uint32_t len = clamped_length(P.a.d_lengths, r, uint64_t(P.a.per) * P.a.page);
   if (uint64_t(j) * P.a.page >= len && !P.a.room) return -1;
-  const int32_t t = P.a.d_table[uint64_t(r) * P.a.per + j];
-  return uint32_t(t) < P.a.n_pages ? t : -1;
+  return page_in(P.a.d_table[uint64_t(r) * P.a.per + j], P.a.n_pages);
 }
 
 __global__ void __launch_bounds__(256) kv_mark(const __grid_constant__ Compact P) {
@@ -471,8 +485,8 @@ __global__ void __launch_bounds__(256) compact_finish(const __grid_constant__ Co
   const uint64_t entries = uint64_t(P.a.rows) * P.a.per;
   for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < entries; i += uint64_t(gridDim.x) * 256) {
     const uint32_t r = uint32_t(i / P.a.per);
-    const int32_t t = held_page(P, r, uint32_t(i - uint64_t(r) * P.a.per));
-    P.a.d_table_out[i] = t < int32_t(live) ? t : P.place[t];
+    const int32_t t = held_page(P, r, uint32_t(i - uint64_t(r) * P.a.per)), to = t < int32_t(live) ? t : P.place[t];
+    P.a.d_table_out[i] = int32_t(uint32_t(to) | (uint32_t(P.a.d_table[i]) & (t < 0 ? 0u : kUnusable)));
   }
   const uint64_t items = uint64_t(moves) * parts;
   for (uint64_t i = blockIdx.x; i < items; i += gridDim.x) {

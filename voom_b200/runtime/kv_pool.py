@@ -162,7 +162,8 @@ def fork_pages(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: t
     rows that hold a page, the longest may (equal ones: the first), unless one
     holds it full.  Fresh pages are the lowest that no row holds any more, in
     the order of the rows; where there are none left, entries are -1 and `missing`
-    says how many.
+    says how many.  An open page that found no copy is not lost: its entry is page
+    - 2^31, which reads as zeros and takes nothing, until a later fork has a page.
 
     `out`: where the results go.  Its table and lengths may be `table` and
     `lengths` themselves (both); `missing` is then added to."""
@@ -360,7 +361,8 @@ class PagePool:
         """Raises RuntimeError if pages were missing in a fork since the last
         check (positions past the pool's room were not written), or a wait inside an
         attention kernel over view() ran out.  Synchronises; call it where results
-        are read."""
+        are read.  Right after a fork that lacked pages nothing is lost yet: resize,
+        then fork(grow=..) again, and go on."""
         from .kv_attention import check_wait_status
 
         check_wait_status(self._wait_status)
