@@ -669,14 +669,14 @@ typedef struct voom_tree_attention_args {
   float* d_weights; /* or NULL */
   const float* d_token_weight; /* B x n contiguous, or NULL */
   uint32_t* d_status; /* bit 0 set if a wait inside the kernel ran out (reported, never observed); or NULL */
-  const float* d_slopes;  /* hq, or NULL */
-  const int32_t* d_depth; /* B x n contiguous: wanted with d_mask and (d_slopes or window); else ignored */
   int64_t q_b, q_t, q_h, kn_b, kn_t, kn_h, vn_b, vn_t, vn_h, o_b, o_t, o_h, w_b, w_h; /* strides, elements */
   uint32_t n, hq;
   float scale;
+  uint32_t size; /* sizeof(voom_tree_attention_args); else what follows is not read, and 0 (callers built without it) */
+  const float* d_slopes;  /* hq, or NULL */
+  const int32_t* d_depth; /* B x n contiguous: wanted with d_mask and (d_slopes or window); else ignored */
   float cap;       /* 0: scores are not capped */
   uint32_t window; /* 0: none */
-  uint32_t pad;
 } voom_tree_attention_args;
 /* Scratch (16-byte aligned, contents ignored) of a call; with less of it the
  * call returns VOOM_E_CAPACITY and launches nothing.  scale > 0, cap >= 0. */

@@ -302,3 +302,70 @@ def test_c_entry_refuses(built_lib):
                 dict(mask=1 << 26, slopes=1 << 25)):
         assert attn(**bad) == VOOM_E_INVALID_ARG, bad
     assert attn(mask=1 << 26, depth=1 << 27, window=3) == VOOM_E_CAPACITY
+
+
+def old_layout(a):
+    """The fields that callers built before slopes, caps and windows pass, and what may lie behind them in memory."""
+    from voom_b200._lib import TreeAttentionArgs
+
+    n = TreeAttentionArgs.slopes.offset
+    raw = bytearray(bytes(a)[:n]) + bytearray(b"\xff" * 64)
+    raw[TreeAttentionArgs.size.offset:n] = bytes(4)  # padding then
+    return bytes(raw)
+
+
+def test_callers_of_the_shorter_structure(built_lib):
+    import ctypes
+
+    from voom_b200._lib import VOOM_E_CAPACITY, VOOM_E_INVALID_ARG, KvViewStruct, TreeAttentionArgs
+
+    names = [f[0] for f in TreeAttentionArgs._fields_]
+    assert names[:10] == "q kn vn out lse mask weights token_weight status q_b".split() and names[-5:] == "size slopes depth cap window".split()
+    assert TreeAttentionArgs.slopes.offset == 9 * 8 + 14 * 8 + 16
+    c = KvViewStruct()
+    c.k = c.v = c.len = 1 << 30
+    c.k_page = c.k_head = c.v_page = c.v_head = 64 * 64
+    c.k_pos = c.v_pos = 64
+    c.B, c.hk, c.D, c.page, c.max_len = 2, 2, 64, 64, 64
+    a = TreeAttentionArgs()
+    a.q, a.kn, a.vn, a.out, a.mask, a.weights = 1 << 20, 1 << 21, 1 << 22, 1 << 23, 1 << 26, 1 << 24
+    a.n, a.hq, a.scale = 3, 4, 0.125
+    a.q_h = a.kn_h = a.vn_h = a.o_h = 64
+    a.q_t = a.o_t = 4 * 64
+    a.kn_t = a.vn_t = 2 * 64
+    a.q_b = a.o_b = 3 * 4 * 64
+    a.kn_b = a.vn_b = 3 * 2 * 64
+    a.w_b, a.w_h = 2 * 80, 80
+    raw = old_layout(a)
+    assert built_lib.voom_tree_attention(ctypes.byref(c), raw, None, 0, None) == VOOM_E_CAPACITY
+    assert built_lib.voom_tree_attention_scratch_bytes(ctypes.byref(c), raw) == \
+        built_lib.voom_tree_attention_scratch_bytes(ctypes.byref(c), ctypes.byref(a)) > 0
+    a.window = 3  # the longer one: its window is seen, and wants depths beside the mask
+    assert built_lib.voom_tree_attention(ctypes.byref(c), ctypes.byref(a), None, 0, None) == VOOM_E_INVALID_ARG
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 40])
+def test_a_call_with_the_shorter_structure(n):
+    from voom_b200 import _device
+    from voom_b200._lib import TreeAttentionArgs, load
+    from voom_b200.runtime import kv_attention as kva
+
+    qkv, k, v = inputs(1, n, 4, 2, 64, [300], torch.float16)
+    d = qkv.cuda()
+    view = place(k, v, [300], "pool", 16)
+    q, kn, vn = d[:, :, :4], d[:, :, 4:6], d[:, :, 6:]
+    want = kva.tree_attention(q, kn, vn, kva.DraftTree.chain(1, n, "cuda"), view)
+    out = torch.zeros_like(want)
+    a = TreeAttentionArgs()
+    a.q, a.kn, a.vn, a.out = (x.data_ptr() for x in (q, kn, vn, out))
+    for name, x in (("q", q), ("kn", kn), ("vn", vn), ("o", out)):
+        for i, s in enumerate("bth"):
+            setattr(a, f"{name}_{s}", x.stride(i))
+    a.n, a.hq, a.scale = n, 4, 64 ** -0.5
+    raw = old_layout(a)
+    lib = load()
+    ws = torch.empty(lib.voom_tree_attention_scratch_bytes(view.packed, raw), dtype=torch.uint8, device="cuda")
+    rc = lib.voom_tree_attention(view.packed, raw, ws.data_ptr(), ws.numel(), _device.raw_stream(view.index))
+    torch.cuda.synchronize()
+    assert rc == 0 and torch.equal(out, want)

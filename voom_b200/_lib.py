@@ -97,9 +97,13 @@ class KvViewStruct(ctypes.Structure):
 
 
 class TreeAttentionArgs(ctypes.Structure):
-    _fields_ = _fields("p: q kn vn out lse mask weights token_weight status slopes depth",
-                       "i64: q_b q_t q_h kn_b kn_t kn_h vn_b vn_t vn_h o_b o_t o_h w_b w_h", "u32: n hq", "f32: scale cap",
-                       "u32: window pad")
+    _fields_ = _fields("p: q kn vn out lse mask weights token_weight status",
+                       "i64: q_b q_t q_h kn_b kn_t kn_h vn_b vn_t vn_h o_b o_t o_h w_b w_h", "u32: n hq", "f32: scale",
+                       "u32: size", "p: slopes depth", "f32: cap", "u32: window")
+
+    def __init__(self, *args, **kw):
+        super().__init__(*args, **kw)
+        self.size = ctypes.sizeof(self)
 
 
 class KvEvictArgs(ctypes.Structure):

@@ -2,6 +2,8 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <cstddef>
+#include <cstring>
 #include <initializer_list>
 #include <type_traits>
 
@@ -404,8 +406,15 @@ VOOM_API int voom_tree_mask(const int32_t* d_parents, uint32_t B, uint32_t n, ui
 
 namespace {
 
+// The arguments, without what a caller built before slopes, caps and windows does not have.
+voom_tree_attention_args known(const voom_tree_attention_args* a) {
+  voom_tree_attention_args x{};
+  if (a) std::memcpy(&x, a, a->size == sizeof x ? sizeof x : offsetof(voom_tree_attention_args, d_slopes));
+  return x;
+}
+
 int check(const voom_kv_view* c, const voom_tree_attention_args* a, Attn& P) {
-  if (!a || !a->d_q || !a->d_kn || !a->d_vn || !a->d_out) return VOOM_E_INVALID_ARG;
+  if (!a->d_q || !a->d_kn || !a->d_vn || !a->d_out) return VOOM_E_INVALID_ARG;
   const int rc = voom::kv::make_view(c, P.c);
   if (rc != VOOM_OK) return rc;
   if (!a->hq || a->hq % c->hk || !(a->scale > 0.0f && a->scale <= 3.0e38f)) return VOOM_E_INVALID_ARG;
@@ -432,14 +441,16 @@ int check(const voom_kv_view* c, const voom_tree_attention_args* a, Attn& P) {
 
 }  // namespace
 
-VOOM_API uint64_t voom_tree_attention_scratch_bytes(const voom_kv_view* c, const voom_tree_attention_args* a) {
+VOOM_API uint64_t voom_tree_attention_scratch_bytes(const voom_kv_view* c, const voom_tree_attention_args* args) {
+  const voom_tree_attention_args x = known(args), *a = &x;
   Attn P{};
   if (check(c, a, P) != VOOM_OK || !a->n) return 0;
   return plan(P, nullptr);
 }
 
-VOOM_API int voom_tree_attention(const voom_kv_view* c, const voom_tree_attention_args* a, void* d_scratch,
+VOOM_API int voom_tree_attention(const voom_kv_view* c, const voom_tree_attention_args* args, void* d_scratch,
                                  uint64_t bytes, void* stream) {
+  const voom_tree_attention_args x = known(args), *a = &x;
   Attn P{};
   const int rc = check(c, a, P);
   if (rc != VOOM_OK) return rc;

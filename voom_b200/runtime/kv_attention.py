@@ -227,7 +227,7 @@ class DraftTree:
 
 # voom_tree_attention_args and voom_kv_evict_args as bytes: cheaper to make than
 # ctypes structures, and one-token calls are bound by the host
-_ATTN = struct.Struct("11Q14q2I2fI4x")
+_ATTN = struct.Struct("9Q14q2IfI2QfI")
 _EVICT = struct.Struct("Q2q5Q4I")
 assert _ATTN.size == ctypes.sizeof(TreeAttentionArgs) and _EVICT.size == ctypes.sizeof(KvEvictArgs)
 
@@ -329,9 +329,9 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: Draf
     lse = q.new_empty((B, n, hq), dtype=torch.float32) if return_lse else None
     if n:
         a = _ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-                       tree.mask_ptr, wp, tw, cache.status_ptr, sl, depth, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0],
-                       vs[1], vs[2], os[0], os[1], os[2], wb, wh, n, hq, cache.scale if scale is None else scale, cap or 0.0,
-                       0 if window is None or window >= 2 ** 31 else window)
+                       tree.mask_ptr, wp, tw, cache.status_ptr, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+                       os[0], os[1], os[2], wb, wh, n, hq, cache.scale if scale is None else scale, _ATTN.size, sl, depth,
+                       cap or 0.0, 0 if window is None or window >= 2 ** 31 else window)
         lib, sp = load(), _device.raw_stream(cache.index)
         if _device.capturing():
             # a workspace from the graph's own pool, which no tensor outside the graph gets for as long as it lives
