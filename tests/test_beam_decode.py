@@ -51,3 +51,29 @@ def test_example_runs():
     assert bool((s[:, :-1] >= s[:, 1:]).all())  # the best first
     assert len({tuple(x) for x in r["tokens"].view(6, 9).tolist()[:3]}) == 3  # a request's beams differ
     assert r["pages"] < r["unshared"]
+
+
+def test_example_reads_a_prompt_once_and_leaves_empty_rows_empty(monkeypatch):
+    """The pool's contract: only rows that were written to are advanced; a prompt is one row's work."""
+    from examples import beam_decode as bd
+    from voom_b200.runtime.kv_pool import PagePool
+
+    asked, lengths = [], []
+    attend, fork = bd.tree_attention, PagePool.fork
+    monkeypatch.setattr(bd, "tree_attention", lambda q, *a, **kw: (asked.append(tuple(q.shape[:2])), attend(q, *a, **kw))[1])
+    monkeypatch.setattr(PagePool, "fork", lambda self, *a, **kw: (lengths.append(self.lengths.tolist()), fork(self, *a, **kw))[1])
+    r = bd.run(batch=2, beams=3, layers=2, prompt=37, steps=4, window=20)
+    assert asked == [(2, 37)] * 2 + [(6, 1)] * 6
+    assert lengths[1] == [37, 0, 0, 37, 0, 0] and r["pool"].lengths.tolist() == [40] * 6
+
+
+@pytest.mark.parametrize("vocab,alive", [(1, 1), (2, 3)])
+def test_example_with_fewer_candidates_than_beams(monkeypatch, vocab, alive):
+    from examples import beam_decode as bd
+
+    monkeypatch.setattr(bd, "SMOLLM2_135M", dict(bd.SMOLLM2_135M, vocab=vocab))
+    r = bd.run(batch=2, beams=3, layers=2, prompt=9, steps=4, window=5)
+    t, s = r["tokens"], r["scores"]
+    assert bool((t[:, :alive] >= 0).all()) and bool((t[:, alive:] == -1).all())
+    assert bool(torch.isfinite(s[:, :alive]).all()) and bool((s[:, alive:] == -float("inf")).all())
+    assert r["pool"].lengths.tolist() == [12 if i % 3 < alive else 0 for i in range(6)]
