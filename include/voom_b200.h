@@ -789,7 +789,7 @@ int voom_kv_compact(const voom_kv_compact_args* a, void* d_scratch, uint64_t scr
  * masked with -inf: a finite mask ties all along a row, which is read three times then.
  * d_parents: b * beams + i, d_tokens: t, d_scores_out rounded to fp32; where
  * there are fewer candidates: -1, -1, -inf.  width <= 64, beams <= 64,
- * beams * V < 2^31. */
+ * beams * V < 2^31, B * beams < 2^27. */
 typedef struct voom_beam_select_args {
   const void* d_logits;  /* B x beams x V, l_b and l_i strides (elements), any alignment */
   const float* d_scores; /* B x beams contiguous */

@@ -286,6 +286,17 @@ def test_refusals():
         beam_select(x[:, :, :0], s, 2)
 
 
+@pytest.mark.gpu
+def test_sizes_past_the_limits_are_refused_in_words():
+    from voom_b200.runtime.beam import beam_select
+
+    x = torch.zeros((1, 1, 1), dtype=torch.bfloat16, device="cuda")
+    for shape in ((2 ** 27, 1, 1), (2 ** 21, 64, 1)):
+        y = x.expand(shape)
+        with pytest.raises(ValueError, match="2\\^31|2\\^27"):
+            beam_select(y, torch.zeros((1, 1), device="cuda").expand(shape[:2]).contiguous(), 1)
+
+
 def test_refusals_without_a_device(built_lib):
     from voom_b200._lib import VOOM_E_CAPACITY, VOOM_E_INVALID_ARG, VOOM_E_UNSUPPORTED, BeamSelectArgs
     from voom_b200.runtime.beam import beam_select

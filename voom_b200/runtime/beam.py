@@ -23,6 +23,7 @@ from .._lib import ELEMENT_TYPES, BeamSelectArgs, check, load
 
 MAX_BEAMS = 64
 MAX_WIDTH = 64
+MAX_ROWS = 2 ** 27  # beams of all requests, fewer
 
 _ARGS = struct.Struct("5Q2q6I")
 assert _ARGS.size == ctypes.sizeof(BeamSelectArgs)
@@ -64,8 +65,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: int, *,
     if not 0 < beams <= MAX_BEAMS or not 0 < width <= MAX_WIDTH or not V:
         raise ValueError(f"{beams} beams, {width} continuations of {V} tokens: 1 to {MAX_BEAMS} beams and 1 to {MAX_WIDTH} "
                          "continuations, one token at least")
-    if beams * V >= 2 ** 31 or B * beams >= 2 ** 31:
-        raise ValueError(f"{B} requests of {beams} beams over {V} tokens: fewer than 2^31 candidates each wanted")
+    if beams * V >= 2 ** 31 or B * beams >= MAX_ROWS:
+        raise ValueError(f"{B} requests of {beams} beams over {V} tokens: fewer than 2^31 candidates each, and 2^27 beams, wanted")
     best = scores.new_empty((B, width))
     parents, tokens = scores.new_empty((2, B, width), dtype=torch.int32).unbind(0)
     if B:
