@@ -418,6 +418,18 @@ def test_refusals():
         kv_pool.PagePool(1, 2, 60, pages=2, rows=1, max_len=8)
 
 
+@pytest.mark.gpu
+def test_tables_without_rows_are_refused_in_words():
+    from voom_b200.runtime import kv_pool
+
+    k, v = (torch.zeros((1, 6, 2, 8, 64), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    for shape in ((0, 3), (3, 0)):
+        t = torch.zeros(shape, dtype=torch.int32, device="cuda")
+        for call in (kv_pool.fork_pages, kv_pool.compact_pages):
+            with pytest.raises(ValueError, match="table"):
+                call(k, v, t, torch.zeros(shape[0], dtype=torch.int32, device="cuda"))
+
+
 def test_c_entries_refuse(built_lib):
     from voom_b200._lib import (VOOM_E_CAPACITY, VOOM_E_INVALID_ARG, VOOM_E_OVERLAP, VOOM_E_UNSUPPORTED, KvAppendArgs,
                                 KvCompactArgs, KvForkArgs, KvViewStruct)

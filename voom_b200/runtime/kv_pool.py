@@ -89,8 +89,9 @@ def _pool(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.
     if ks[4] != 1 or vs[4] != 1 or (ks[0] | ks[1] | ks[2] | ks[3] | vs[0] | vs[1] | vs[2] | vs[3]) & 7 or \
             (k.data_ptr() | v.data_ptr()) & 15:
         raise ValueError("k and v: the values of a position must be adjacent and every row must start on 16 bytes")
-    if table.dim() != 2 or table.dtype is not torch.int32 or not table.is_contiguous() or not table.shape[1]:
-        raise ValueError(f"table: a contiguous int32 (rows, pages) tensor wanted, got {tuple(table.shape)} {table.dtype}")
+    if table.dim() != 2 or table.dtype is not torch.int32 or not table.is_contiguous() or not table.numel():
+        raise ValueError(f"table: a contiguous int32 (rows, pages) tensor wanted, one of each at least, got {tuple(table.shape)} "
+                         f"{table.dtype}")
     R, per = table.shape
     if R > MAX_ROWS or per * P >= 2 ** 31 or R * per >= 2 ** 31:
         raise ValueError(f"{R} rows of {per} pages of {P} positions: at most {MAX_ROWS} rows, fewer than 2^31 positions and entries")
