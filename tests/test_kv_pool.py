@@ -131,6 +131,34 @@ def test_append_behind_a_view_s_bound(kind):
         view.lengths.add_(4)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n,cap", [(1, None), (1, 9.0), (8, 9.0), (12, None), (20, 9.0), (60, None), (60, 9.0), (150, None), (150, 9.0)])
+def test_entries_that_are_no_pages_read_as_zeros(n, cap, D):
+    """By every kernel, however far outside the pool, an open page without a copy among them."""
+    from voom_b200.runtime.kv_attention import DraftTree, KVView, tree_attention
+
+    B, H, P, per = 2, 2, 64, 40  # tiles that TMA reads, requests that several blocks share
+    g = torch.Generator(device="cuda").manual_seed(7)
+    k, v = (torch.randn((B * per, H, P, D), device="cuda", generator=g).bfloat16() for _ in range(2))
+    table = torch.randperm(B * per, generator=torch.Generator().manual_seed(1)).reshape(B, per)
+    k2, v2 = (x[table.reshape(-1).cuda()].reshape(B, per, H, P, D).clone() for x in (k, v))
+    for b, j, x in ((0, 0, -1), (0, 3, B * per), (0, 4, 2 ** 31 - 1), (0, 39, 3 - 2 ** 31), (1, 1, -2 ** 31), (1, 2, 10 ** 6), (1, 38, -7)):
+        table[b, j] = x
+        k2[b, j], v2[b, j] = 0, 0
+    k2, v2 = (x.transpose(1, 2).reshape(B, H, per * P, D).contiguous() for x in (k2, v2))
+    lengths = i32([per * P - 3, per * P - 70])
+    x = torch.randn((B, n, 3 * H, D), device="cuda", generator=g).bfloat16()
+    args = (x[:, :, :H], x[:, :, H:2 * H], x[:, :, 2 * H:], DraftTree.chain(B, n, "cuda"))
+    got = []
+    for view in (KVView.pool(k, v, table.to(torch.int32).cuda(), lengths), KVView.contiguous(k2, v2, lengths)):
+        w = torch.zeros((B, H, per * P + n), device="cuda")
+        out, lse = tree_attention(*args, view, cap=cap, return_lse=True, weights=w)
+        view.check_status()
+        got.append((out, lse, w, tree_attention(*args, view, cap=cap)))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 # ----------------------------------------------------------------------- fork
 
 def state(seed, *, rows, page, per, n_pages, ended=True):

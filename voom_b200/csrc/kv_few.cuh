@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(32 * Few<DP>::W, 1) attn_few(const __grid_cons
         __syncwarp();
         if (lane < KT / P.box) {
           const uint32_t s = p0 + lane * P.box, at = P.c.page_of(s);
-          const int32_t w = P.c.v.d_table ? __ldg(P.c.v.d_table + uint64_t(pg.b) * P.c.v.table_stride + at) : int32_t(pg.b);
+          const int32_t w = P.c.page_box(pg.b, at);
           const uint32_t y = P.c.v.d_table ? s - at * P.c.v.page : s;
 #pragma unroll
           for (uint32_t x = 0; x < DP; x += 64) {

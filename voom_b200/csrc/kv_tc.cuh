@@ -143,7 +143,7 @@ __device__ __forceinline__ bool load_tile_sw128(const Attn& P, const Seg& g, uin
       __syncwarp();
       if (lane < KT / P.box) {
         const uint32_t s = p0 + lane * P.box, pg = P.c.page_of(s);
-        const int32_t w = P.c.v.d_table ? __ldg(P.c.v.d_table + uint64_t(g.b) * P.c.v.table_stride + pg) : int32_t(g.b);
+        const int32_t w = P.c.page_box(g.b, pg);
         const uint32_t y = P.c.v.d_table ? s - pg * P.c.v.page : s;
         const void* map = is_v ? &P.v_map : &P.k_map;
 #pragma unroll

@@ -26,6 +26,13 @@ struct View {
     const int32_t n = v.d_len[b];
     return n <= 0 ? 0u : min(uint32_t(n), v.max_len);
   }
+  // The page as TMA's coordinate: of a pool -1 for an entry that is no page, whatever it
+  // is (its box comes as zeros), without a table the request.
+  __device__ __forceinline__ int32_t page_box(uint32_t b, uint32_t p) const {
+    if (!v.d_table) return int32_t(b);
+    const int32_t i = __ldg(v.d_table + uint64_t(b) * v.table_stride + p);
+    return uint32_t(i) < v.n_pages ? i : -1;
+  }
   // Element offsets (from d_k, d_v) of the page that holds position s of
   // request b, head 0, position 0 of the page; false for a page that is none.
   __device__ __forceinline__ bool page_at(uint32_t b, uint32_t p, int64_t& k, int64_t& w) const {
