@@ -406,14 +406,12 @@ VOOM_API int voom_tree_mask(const int32_t* d_parents, uint32_t B, uint32_t n, ui
 
 namespace {
 
-// The arguments, without what a caller built before slopes, caps and windows does not have.
-voom_tree_attention_args known(const voom_tree_attention_args* a) {
-  voom_tree_attention_args x{};
-  if (a) std::memcpy(&x, a, a->size == sizeof x ? sizeof x : offsetof(voom_tree_attention_args, d_slopes));
-  return x;
-}
-
-int check(const voom_kv_view* c, const voom_tree_attention_args* a, Attn& P) {
+int check(const voom_kv_view* c, const voom_tree_attention_args* args, Attn& P) {
+  if (!args) return VOOM_E_INVALID_ARG;
+  // (P is zeros: so is what a caller built before slopes, caps and windows does not have)
+  if (args->size == sizeof *args) P.a = *args;
+  else std::memcpy(&P.a, args, offsetof(voom_tree_attention_args, d_slopes));
+  const voom_tree_attention_args* a = &P.a;
   if (!a->d_q || !a->d_kn || !a->d_vn || !a->d_out) return VOOM_E_INVALID_ARG;
   const int rc = voom::kv::make_view(c, P.c);
   if (rc != VOOM_OK) return rc;
@@ -435,22 +433,19 @@ int check(const voom_kv_view* c, const voom_tree_attention_args* a, Attn& P) {
     return VOOM_E_OVERLAP;
   if (a->d_weights && !voom::separate({a->d_weights, {B, hk, 1}, {a->w_b, a->w_h, 0}, int64_t(c->max_len) + n, 4}))
     return VOOM_E_OVERLAP;
-  P.a = *a;
   return VOOM_OK;
 }
 
 }  // namespace
 
-VOOM_API uint64_t voom_tree_attention_scratch_bytes(const voom_kv_view* c, const voom_tree_attention_args* args) {
-  const voom_tree_attention_args x = known(args), *a = &x;
+VOOM_API uint64_t voom_tree_attention_scratch_bytes(const voom_kv_view* c, const voom_tree_attention_args* a) {
   Attn P{};
   if (check(c, a, P) != VOOM_OK || !a->n) return 0;
   return plan(P, nullptr);
 }
 
-VOOM_API int voom_tree_attention(const voom_kv_view* c, const voom_tree_attention_args* args, void* d_scratch,
+VOOM_API int voom_tree_attention(const voom_kv_view* c, const voom_tree_attention_args* a, void* d_scratch,
                                  uint64_t bytes, void* stream) {
-  const voom_tree_attention_args x = known(args), *a = &x;
   Attn P{};
   const int rc = check(c, a, P);
   if (rc != VOOM_OK) return rc;

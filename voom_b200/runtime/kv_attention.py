@@ -229,7 +229,8 @@ class DraftTree:
 # ctypes structures, and one-token calls are bound by the host
 _ATTN = struct.Struct("9Q14q2IfI2QfI")
 _EVICT = struct.Struct("Q2q5Q4I")
-assert _ATTN.size == ctypes.sizeof(TreeAttentionArgs) and _EVICT.size == ctypes.sizeof(KvEvictArgs)
+_ATTN_SIZE = _ATTN.size
+assert _ATTN_SIZE == ctypes.sizeof(TreeAttentionArgs) and _EVICT.size == ctypes.sizeof(KvEvictArgs)
 
 
 def _new(x: torch.Tensor, name: str, B: int, n: int, heads: int, cache: KVView) -> tuple:
@@ -330,7 +331,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: Draf
     if n:
         a = _ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
                        tree.mask_ptr, wp, tw, cache.status_ptr, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-                       os[0], os[1], os[2], wb, wh, n, hq, cache.scale if scale is None else scale, _ATTN.size, sl, depth,
+                       os[0], os[1], os[2], wb, wh, n, hq, cache.scale if scale is None else scale, _ATTN_SIZE, sl, depth,
                        cap or 0.0, 0 if window is None or window >= 2 ** 31 else window)
         lib, sp = load(), _device.raw_stream(cache.index)
         if _device.capturing():
