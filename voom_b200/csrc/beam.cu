@@ -237,6 +237,78 @@ __device__ __forceinline__ X find_bar(Bar<X>& sh, X y, uint32_t width) {
   return sh.at;
 }
 
+// A part's values once more, for what is rare: out of the way of beam_rows' registers.
+template <typename T>
+struct Part {
+  const T* x0;
+  uint64_t t0, t1;  // of the row's chunks
+  uint32_t skew, V;
+
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {  // (-inf for what is not the row's)
+    constexpr uint32_t kDeep = 8;
+    for (uint64_t at = t0 + threadIdx.x; at < t1; at += kDeep * kThreads) {
+      float x[kDeep];
+#pragma unroll
+      for (uint32_t u = 0; u < kDeep; u++) {
+        const uint32_t t = uint32_t(at) + u * kThreads - skew;
+        x[u] = at + u * kThreads < t1 && t < V ? value(x0[t]) : -INFINITY;
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < kDeep; u++) f(uint32_t(at) + u * kThreads - skew, x[u]);
+    }
+  }
+};
+
+// A thread's part of the sum of e^(x - top).
+template <typename T>
+__device__ __noinline__ double sum_far(const Part<T>& p, float top) {
+  double s = 0.0;
+  p.each([&](uint32_t, float x) { s += exp(double(x) - double(top)); });
+  return s;
+}
+
+// The part's best entries where more reached the bar than a block holds: values that
+// tie, as a mask of the type's lowest value does wherever fewer than `width` tokens are
+// left, or that lie under few threads.  The threads' best entries, every 256th token to
+// one, give a bar that ties cannot crowd: 32 requests of 8 such beams over 200019 values,
+// 16 wanted, 248 us a call (2390 one after another; without the mask 48, L2 flushed).
+template <typename T>
+__device__ __noinline__ void best_again(RowShared& sh, const Part<T>& p, uint32_t width) {
+  const uint32_t tid = threadIdx.x;
+  Bar<uint64_t>& bar = *reinterpret_cast<Bar<uint64_t>*>(sh.raw);
+  static_assert(sizeof(Bar<uint64_t>) <= sizeof(sh.raw), "nothing is on its way there any more");
+  auto entry = [&](uint32_t t, float x) { return x > -INFINITY ? entry_of(x, t) : 0; };
+  uint64_t most = 0;
+  p.each([&](uint32_t t, float x) { most = max(most, entry(t, x)); });
+  __syncthreads();  // sh.n and sh.raw are read
+  if (tid == 0) sh.n = 0;
+  const uint64_t reach = max(find_bar(bar, most, width), uint64_t(1));
+  p.each([&](uint32_t t, float x) {
+    const uint64_t y = entry(t, x);
+    if (y < reach) return;
+    const uint32_t at = atomicAdd(&sh.n, 1u);
+    if (at < kFound) sh.found[at] = y;
+  });
+  __syncthreads();
+  if (sh.n <= kFound) return;
+  // under few threads again: one after another, each the best after the last
+  uint64_t last_one = ~0ull;
+  uint32_t k = 0;
+  for (; k < width; k++) {
+    uint64_t mine = 0;
+    p.each([&](uint32_t t, float x) {
+      const uint64_t y = entry(t, x);
+      if (y < last_one) mine = max(mine, y);
+    });
+    last_one = block_max(sh, mine);
+    if (!last_one) break;
+    if (tid == 0) sh.found[k] = last_one;
+  }
+  if (tid == 0) sh.n = k;
+  __syncthreads();
+}
+
 // Block: part `part` of a row.  The row's 16-byte chunks are counted from the
 // aligned address at or before its start; those at its ends are read value by value.
 template <typename T>
@@ -361,60 +433,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) beam_rows(const __grid_const
     }
     __syncthreads();
   }
-  // the part's values once more (-inf for what is not the row's)
-  auto each = [&](auto f) {
-    constexpr uint32_t kDeep = 8;
-    const uint64_t t0 = uint64_t(first) * 32 * kChunks * VEC, t1 = uint64_t(last) * 32 * kChunks * VEC;
-    for (uint64_t at = t0 + tid; at < t1; at += kDeep * kThreads) {
-      float x[kDeep];
-#pragma unroll
-      for (uint32_t u = 0; u < kDeep; u++) {
-        const uint32_t t = uint32_t(at) + u * kThreads - skew;
-        x[u] = at + u * kThreads < t1 && t < V ? value(x0[t]) : -INFINITY;
-      }
-#pragma unroll
-      for (uint32_t u = 0; u < kDeep; u++) f(uint32_t(at) + u * kThreads - skew, x[u]);
-    }
-  };
-  many |= sh.n > kFound;
-  if (many) {
-    // Values that tie, as a mask of the type's lowest value does wherever fewer than
-    // `width` tokens are left, or that lie under few threads.  The threads' best entries,
-    // every 256th token to one, give a bar that ties cannot crowd: 32 requests of 8 such
-    // beams over 200019 values, 16 wanted, 248 us a call (2390 one after another; without
-    // the mask 48, L2 flushed).
-    Bar<uint64_t>& bar = *reinterpret_cast<Bar<uint64_t>*>(sh.raw);
-    static_assert(sizeof(Bar<uint64_t>) <= sizeof(sh.raw), "nothing is on its way there any more");
-    auto entry = [&](uint32_t t, float x) { return x > -INFINITY ? entry_of(x, t) : 0; };
-    uint64_t most = 0;
-    each([&](uint32_t t, float x) { most = max(most, entry(t, x)); });
-    __syncthreads();  // sh.n and sh.raw are read
-    if (tid == 0) sh.n = 0;
-    const uint64_t reach = max(find_bar(bar, most, width), uint64_t(1));
-    each([&](uint32_t t, float x) {
-      const uint64_t y = entry(t, x);
-      if (y < reach) return;
-      const uint32_t at = atomicAdd(&sh.n, 1u);
-      if (at < kFound) sh.found[at] = y;
-    });
-    __syncthreads();
-    if (sh.n > kFound) {  // the best under few threads again: one after another, each the best after the last
-      uint64_t last_one = ~0ull;
-      uint32_t k = 0;
-      for (; k < width; k++) {
-        uint64_t mine = 0;
-        each([&](uint32_t t, float x) {
-          const uint64_t y = entry(t, x);
-          if (y < last_one) mine = max(mine, y);
-        });
-        last_one = block_max(sh, mine);
-        if (!last_one) break;
-        if (tid == 0) sh.found[k] = last_one;
-      }
-      if (tid == 0) sh.n = k;
-      __syncthreads();
-    }
-  }
+  const Part<T> part_of{x0, uint64_t(first) * 32 * kChunks * VEC, uint64_t(last) * 32 * kChunks * VEC, skew, V};
+  if (many || sh.n > kFound) best_again(sh, part_of, width);
   // the warps' sums
   float all = top;
   for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xFFFFFFFFu, all, o));
@@ -429,8 +449,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) beam_rows(const __grid_const
   float most = -INFINITY;
   for (uint32_t w = 0; w < kWarps; w++) most = fmaxf(most, sh.top[w]);
   if (fabsf(most) > kFar && fabsf(most) < INFINITY) {  // fp32 holds little of such an exponent
-    double far = 0.0;
-    each([&](uint32_t, float x) { far += exp(double(x) - double(most)); });
+    double far = sum_far(part_of, most);
     for (int o = 16; o; o >>= 1) far += __shfl_xor_sync(0xFFFFFFFFu, far, o);
     __syncthreads();
     if (lane == 0) {
