@@ -647,7 +647,8 @@ int voom_tree_mask(const int32_t* d_parents, uint32_t B, uint32_t n, uint32_t* d
  * chain, j <= i).  With cap > 0 a score becomes cap tanh(score / cap); with
  * d_slopes (finite), slopes[h] times (key's position - query's) is added to it
  * (after the cap); with window > 0 a row sees the positions less than `window` before
- * its own only.  A cached position is its index, a new token's d_len[b] + its
+ * its own only (whole tiles of cached positions that no row of the request sees are not
+ * read; what some rows see, and the new tokens, are read and masked).  A cached position is its index, a new token's d_len[b] + its
  * depth (d_depth as voom_tree_mask gives it; NULL in a chain, where it is i).
  * Query head h reads key head h / (hq / hk).  A row that sees
  * nothing (a -2 token, which sees no cached position either) gives 0 and lse

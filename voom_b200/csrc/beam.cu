@@ -8,17 +8,18 @@
 // values.  The width-th largest of the block's 256 running maxima is a bar that
 // `width` values reach at least, and hardly more do; only the groups whose largest
 // reaches it are read again, and what reaches it there is put in order by
-// counting.  beam_join, a block per request, makes the beams' denominators and
-// finds the best of what their rows kept in the same way.
+// counting.  beam_join makes the beams' denominators and finds the best of what their
+// rows kept in the same way; where two beams come too close for fp32 sums, it makes
+// theirs again in fp64.
 //
 // The logits are read once: HBM would be the bound.  Measured: 32 requests of 8 beams
-// over 200019 FP16 tokens, 16 wanted: 32 us a call, 28 of it beam_rows (3.6 TB/s, 56 %
+// over 200019 FP16 tokens, 16 wanted: 36 us a call, 28 of it beam_rows (3.6 TB/s, 56 %
 // of what a copy reaches).  A block of one row over 100010 values is bound by its own
 // instructions, exponentials and maxima, with 512 of 592 places taken, then by the
 // last look at its groups (4.5 us).  More blocks to a row make the joining cost more
 // (39 to 54 us a call), lists kept by warps as they read cost the reading (75 us).  One
-// request of 4 beams over 49152: 9.6 us, two launches' latency; FP32, 8 requests'
-// first step over 131072 and 5 beams: 13.1 us.
+// request of 4 beams over 49152: 11.4 us, two launches' latency; FP32, 8 requests'
+// first step over 131072 and 5 beams: 15.7 us.
 //
 // An entry is one number: the value's bits in unsigned order, then the token
 // counted from the end, so that no two are equal and the larger one is the better.

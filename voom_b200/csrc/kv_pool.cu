@@ -17,7 +17,9 @@
 // Measured: 3 heads of 64 in 4 layers, 4 rows: 7.5 us a fork, 8.9 a compaction; 256
 // rows in 2 layers, 28 MB of open pages copied: 19 us, 12 of it the copies (4.8 TB/s
 // read and written); 1426 of 3001 pages of 256 KB moved: 128 us, 5.8 TB/s (89 % of
-// what a copy reaches).  16376 new tokens of 8 heads of 128 written: 20.5 us, 6.5 TB/s.
+// what a copy reaches).  One block numbers the pages, whatever their number: 256 rows in
+// a pool of 10^4, 10^5 and 10^6 pages take 13, 31 and 239 us to fork, 14, 39 and 283 to
+// compact.  16376 new tokens of 8 heads of 128 written: 20.5 us, 6.5 TB/s.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -31,7 +33,8 @@ namespace {
 
 constexpr uint32_t kMaxPage = 32768, kMaxRows = 65535;
 // Tables that one block does.  Entries: 4000 take 9.6 us forked by one block, 10.1 by
-// many; 8000 12.2 and 10.4, but for 5 us that the host saves; 16000 17.1 and 11.4.
+// many; 8000 12.2 and 10.4, but for 5 us that the host saves (a captured call has no
+// host to save, and would want the limit at 4000); 16000 17.1 and 11.4.
 // Pages and rows: what its shared memory holds.
 constexpr uint32_t kSmallPages = 12288, kSmallRows = 4096, kSmallEntries = 8192;
 constexpr uint32_t kSmallBytes = 8 * kSmallPages + 12 * kSmallRows;

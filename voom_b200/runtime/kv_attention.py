@@ -269,8 +269,9 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: Draf
 
     With `cap` a score z becomes cap tanh(z / cap); with `slopes` (Hq) fp32, finite,
     slopes[h] (p_k - p_q) is added to it, after the cap; with `window` a row sees
-    only positions with p_q - p_k < window, itself among them (its tiles before
-    are not read).  A cached position is its index, a new token's lengths[b] + its
+    only positions with p_q - p_k < window, itself among them (tiles of cached
+    positions that no row of the request sees are not read; what some of its rows
+    see, and the new tokens, are read and masked).  A cached position is its index, a new token's lengths[b] + its
     depth in the tree: after an eviction that is not their distance, and a view that
     says so (KVView.displaced, PagedKVCache.view) is refused with slopes or a window.
 

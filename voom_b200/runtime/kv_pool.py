@@ -316,7 +316,8 @@ class PagePool:
     def advance(self, n: int | torch.Tensor) -> None:
         """Counts n (one number, or int32 for each row) appended positions: after
         the last layer's append.  An ended or empty row that was not written to
-        must get 0."""
+        must get 0, and no row more than the last fork made room for: nothing else
+        says that a position was not written."""
         self.lengths.add_(n).clamp_(0, self.max_len)
 
     def compact(self, *, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
