@@ -799,6 +799,60 @@ def test_room_outlasts_compaction(how):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(40))
+def test_lives_of_a_pool(seed):
+    """Forks, ends, growth, rollbacks, compactions, resizes and shortages in any order: every row holds its own history."""
+    from voom_b200.runtime.kv_pool import PagePool
+
+    r = random.Random(seed)
+    rows, page, layers = r.choice((1, 2, 5, 9, 40)), r.choice((1, 2, 4, 8, 16)), 2
+    pool = PagePool(layers, 1, 8, pages=r.choice((1, 3, rows, 3 * rows)), rows=rows, max_len=r.choice((10, 40, 100)), page=page)
+    history, token = [[] for _ in range(rows)], 0
+    for step in range(20):
+        parents = [-1 if r.random() < 0.1 else r.choice((i, i, r.randrange(rows))) for i in range(rows)]
+        history = [list(history[p]) if p >= 0 else [] for p in parents]
+        grow = [min(r.choice((0, 1, 1, 2, page, 2 * page + 1)), pool.max_len - len(h)) for h in history]
+        pool.fork(i32(parents), grow=i32(grow))
+        grow = [g if p >= 0 else 0 for g, p in zip(grow, parents)]
+        for _ in range(100):
+            try:
+                pool.check_status()
+                break
+            except RuntimeError:
+                pool.resize(int(pool.compact().item()) + r.choice((1, 5, 2 * rows)))
+                pool.fork(grow=i32(grow))
+        if r.random() < 0.3:
+            live = int(pool.compact().item())
+            if r.random() < 0.5:
+                pool.resize(max(1, live + r.choice((0, 1, 4))))
+        n = max(grow + [1])
+        ids, index = torch.zeros((rows, n)), torch.full((rows, n), -1, dtype=torch.int32)
+        new = [r.randrange(g + 1) for g in grow]
+        for i, m in enumerate(new):
+            for j in range(m):
+                token = token % 200 + 1
+                ids[i, j], index[i, j] = token, j
+                history[i].append(token)
+        x = ids[:, :, None, None].expand(rows, n, 1, 8).to(torch.bfloat16).cuda()
+        for layer in range(layers):
+            pool.append(layer, x * (layer + 1), -x, index=index.cuda())
+        pool.advance(i32(new))
+        if r.random() < 0.2:
+            back = [min(r.randrange(page + 2), len(h)) if r.random() < 0.4 else 0 for h in history]
+            pool.advance(i32([-b for b in back]))
+            history = [h[:len(h) - b] for h, b in zip(history, back)]
+        assert pool.lengths.tolist() == [len(h) for h in history], step
+        table = pool.table.cpu().long()
+        for layer in range(layers):
+            k, v = pool.k[layer, :, 0, :, 0].float().cpu(), pool.v[layer, :, 0, :, 7].float().cpu()
+            for i, h in enumerate(history):
+                at = table[i, :-(-len(h) // page)]
+                assert bool(((at >= 0) & (at < pool.pages)).all()), (step, i)
+                assert k[at].reshape(-1)[:len(h)].tolist() == [float(y * (layer + 1)) for y in h], (step, i)
+                assert v[at].reshape(-1)[:len(h)].tolist() == [-float(y) for y in h], (step, i)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [1, 9])
 def test_pages_past_32_bits(n):
     """A pool of more than 2^32 bytes and 2^31 values: its last pages are written, forked, read and moved as its first are."""
